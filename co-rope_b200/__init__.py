@@ -8,6 +8,7 @@ from .fused_rope_attn import attention as fused_rope_attention  # noqa: F401
 from .fused_rope_attn import attention_theta as fused_rope_attention_theta  # noqa: F401
 from .flash_attn_v2_triton import attention as flash_attention  # noqa: F401
 from .flash_attn_co_rope_gqa_triton import attention as corope_gqa_attention  # noqa: F401
+from .kv_cache import KVCache, cache_append, cache_attention, cache_evict  # noqa: F401
 from .sharding import shard_units, unit_range  # noqa: F401
 from .host_pipeline import attention_fwd_bwd_host  # noqa: F401
 from ._ext import build, check_status  # noqa: F401

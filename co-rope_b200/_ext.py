@@ -25,7 +25,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "corope_b200.h")
 DEBUG_HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "corope_b200_debug.h")
 
 SOURCES = ["abi.cu", "rope_general.cu", "rope_fp32.cu", "rope_split.cu", "rope_split_fwd_sm100.cu", "rope_split_bwd_sm100.cu", "rope_split_prepass.cu", "rope_prepass.cu", "rope_fwd_sm100.cu", "rope_bwd_sm100.cu", "corope_general.cu", "corope_fwd_mma.cu", "corope_fwd_split.cu", "corope_bwd_mma.cu", "noalloc.cu",
-           "debug.cu"]
+           "debug.cu", "cache_abi.cu", "cache_append.cu", "cache_attn.cu", "cache_evict.cu"]
 
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 OP_ROPE_FWD, OP_ROPE_BWD, OP_GQA_FWD, OP_GQA_BWD = 0, 1, 2, 3
@@ -72,7 +72,7 @@ def _build_native(force):
 def build(force=False, verbose=False):
     """Compile csrc/*.cu into libcorope_b200.so for sm_100a (cross-compiles without a GPU) and the extension module beside it."""
     srcs = [os.path.join(_CSRC, s) for s in SOURCES]
-    deps = srcs + [os.path.join(_CSRC, "common.cuh"), os.path.join(_CSRC, "corope_mma.cuh"), os.path.join(_CSRC, "rope_split.cuh"), HEADER_PATH, DEBUG_HEADER_PATH]
+    deps = srcs + [os.path.join(_CSRC, "common.cuh"), os.path.join(_CSRC, "corope_mma.cuh"), os.path.join(_CSRC, "rope_split.cuh"), os.path.join(_CSRC, "cache.cuh"), HEADER_PATH, DEBUG_HEADER_PATH]
     if not force and _newer(LIB_PATH, deps):
         _build_native(force)
         return LIB_PATH
@@ -196,6 +196,15 @@ def lib():
             L.corope_gqa_fwd_strided.argtypes = L.corope_gqa_fwd.argtypes + [ctypes.POINTER(Strides)]
             L.corope_gqa_bwd_strided.restype = i32
             L.corope_gqa_bwd_strided.argtypes = L.corope_gqa_bwd.argtypes + [ctypes.POINTER(Strides)]
+            cp, qp, s3 = ctypes.POINTER(KVCacheView), ctypes.POINTER(CacheSeqs), ctypes.c_int64 * 3
+            L.corope_cache_append.restype = i32
+            L.corope_cache_append.argtypes = [cp, qp, vp, vp, s3, s3, i32, i32, vp, vp]
+            L.corope_cache_attn_workspace_bytes.restype = sz
+            L.corope_cache_attn_workspace_bytes.argtypes = [cp, qp, i32, i32, i32, i32]
+            L.corope_cache_attn.restype = i32
+            L.corope_cache_attn.argtypes = [cp, qp, vp, vp, s3, s3, i32, i32, i32, i32, f32, i32, vp, sz, vp, vp]
+            L.corope_cache_evict.restype = i32
+            L.corope_cache_evict.argtypes = [cp, qp, vp, i64, i32, i32, i32, vp, vp, vp, vp]
             _lib = L
         return _lib
 
@@ -203,6 +212,18 @@ def lib():
 class Strides(ctypes.Structure):
     """corope_strides_t of the C header: {batch, head, row} strides in elements of q, k, v, o, d_o, dq, dk, dv."""
     _fields_ = [(name, ctypes.c_int64 * 3) for name in ("q", "k", "v", "o", "d_o", "dq", "dk", "dv")]
+
+
+class KVCacheView(ctypes.Structure):
+    """corope_kv_cache_t of the C header."""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("k", "v", "k_scale", "v_scale", "weight")] + \
+               [(name, ctypes.c_int64 * 3) for name in ("k_stride", "v_stride")] + [(name, ctypes.c_int) for name in ("num_blocks", "Hkv", "block_size", "D", "code")]
+
+
+class CacheSeqs(ctypes.Structure):
+    """corope_cache_seqs_t of the C header."""
+    _fields_ = [("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("B", ctypes.c_int), ("max_blocks", ctypes.c_int)] + \
+               [(name, ctypes.c_void_p) for name in ("seq_lens", "new_lens", "positions", "cos", "sin")] + [("rope_stride", ctypes.c_int64), ("table_rows", ctypes.c_int)]
 
 
 def strides_of(**tensors):
@@ -240,6 +261,8 @@ def status_word(device):
 
 
 def _status_message(v):
+    if v == 0x4000:
+        return "a block table entry, length or position of a cache operator pointed outside its tensor (it was not followed; the tokens concerned were left out)"
     if v & 0x2000:
         return "a gradient term left the value range of the 16-bit Co-RoPE backward and was clamped (results of that call are inaccurate)"
     return "a bounded device-side wait expired (results of that call and of later calls are undefined)"

@@ -223,6 +223,7 @@ const char* corope_status_string(int status) {
         case COROPE_ERR_NO_DEVICE: return "no usable CUDA device or driver entry point";
         case COROPE_ERR_TOO_LARGE: return "size beyond the supported maximum";
         case COROPE_ERR_BAD_STRIDE: return "row stride smaller than the head dimension, or a negative stride";
+        case COROPE_ERR_BAD_CACHE: return "cache: codes are e4m3 or int8, blocks of 16, 32, 64, 128 or 256 tokens, rows aligned to 16 bytes";
         default: break;
     }
     if (status > 0) return cudaGetErrorString((cudaError_t)status);

@@ -1,0 +1,160 @@
+// The 8-bit paged key / value cache: what its kernels share.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace corope {
+
+struct CacheView {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale, *weight;
+    Strides sk, sv;              // block (b), head (h), row (n); bytes, as codes have one
+    int num_blocks, Hkv, bs_log2;
+};
+struct SeqView {
+    const int* table;
+    int64_t table_stride;
+    int B, max_blocks;
+    const int *lens, *new_lens, *positions;
+    const float *cos, *sin;
+    int64_t rope_stride;
+    int table_rows;
+};
+struct CacheAppendParams {
+    CacheView c;
+    SeqView s;
+    const void *k, *v;
+    Strides sk, sv;
+    int T, D, code, dtype;
+    int *status, *mirror;
+};
+struct CacheAttnParams {
+    CacheView c;
+    SeqView s;
+    const void* q;
+    void* o;
+    Strides sq, so;
+    int Hq, G, T, D, code, dtype, causal, accumulate;
+    int row_tiles;               // tiles of query rows per K / V head (row = t * G + head of the group)
+    float scale;                 // sm_scale * log2(e)
+    bool vec_o;                  // rows of o take stores of four elements
+    float* part;                 // partial results: two slots per block of the main kernel
+    float* part_ml;              // their maxima and sums
+    float* lse;                  // [B, Hkv, T * G] log2 of each row's sum (accumulate only)
+    int *status, *mirror;
+};
+struct CacheEvictParams {
+    CacheView c;
+    SeqView s;
+    const int* out_table;
+    int64_t out_stride;
+    int out_blocks, budget, recent, D, code;
+    int *new_lens, *kept;
+    int *status, *mirror;
+};
+
+int launch_cache_append(const CacheAppendParams& p, cudaStream_t s);
+size_t cache_attn_workspace_bytes(int B, int Hkv, int G, int T, int D, int max_blocks, int block_size, int dtype, int accumulate);
+int launch_cache_attn(CacheAttnParams p, void* ws, cudaStream_t s);
+int launch_cache_evict(const CacheEvictParams& p, cudaStream_t s);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void report_bad_index(int* status, int* mirror) {
+    if (status == nullptr) return;
+    atomicCAS(status, 0, COROPE_DEV_BAD_INDEX);
+    report_to_mirror(COROPE_DEV_BAD_INDEX, mirror);
+}
+// A sequence's length and its new tokens, brought into range.  A new token count above the length is one whose first tokens have no
+// slot: not an error (an empty place in a padded batch).
+__device__ __forceinline__ int cache_len(const SeqView& s, int bs_log2, int b, bool& bad) {
+    const int len = s.lens[b], most = s.max_blocks << bs_log2;
+    bad |= len < 0 || len > most;
+    return min(max(len, 0), most);
+}
+__device__ __forceinline__ int cache_new(const SeqView& s, int T, int b, bool& bad) {
+    if (s.new_lens == nullptr) return T;
+    const int n = s.new_lens[b];
+    bad |= n < 0 || n > T;
+    return min(max(n, 0), T);
+}
+// the block that holds slot `slot` of sequence b, or -1
+__device__ __forceinline__ int cache_page(const SeqView& s, int bs_log2, int num_blocks, int b, int slot, bool& bad) {
+    const int page = s.table[(int64_t)b * s.table_stride + (slot >> bs_log2)];
+    const bool ok = (unsigned)page < (unsigned)num_blocks;
+    bad |= !ok;
+    return ok ? page : -1;
+}
+// row of the cos / sin tables for token t of this call, whose slot is `slot`
+__device__ __forceinline__ int cache_position(const SeqView& s, int b, int t, int slot, bool& bad) {
+    const int64_t pos = s.positions == nullptr ? (int64_t)slot : (int64_t)s.positions[b] + t;
+    bad |= pos < 0 || pos >= s.table_rows;
+    return (int)min(max(pos, (int64_t)0), (int64_t)s.table_rows - 1);
+}
+
+// ---- codes.  Every step is an fp32 operation of its own (no contraction), so that codes do not depend on how a compiler joins them.
+template <int CODE> constexpr float kPerCode = 1.f / (CODE == COROPE_CODE_E4M3 ? 448.f : 127.f);   // scale of a block per unit of its largest element
+
+template <int CODE>
+__device__ __forceinline__ uint32_t to_code(float x, float scale) {
+    const float y = scale == 0.f ? 0.f : __fdiv_rn(x, scale);
+    if constexpr (CODE == COROPE_CODE_E4M3) return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+    else return (uint32_t)(int)fminf(fmaxf(rintf(y != y ? 0.f : y), -127.f), 127.f) & 0xffu;
+}
+template <int CODE>
+__device__ __forceinline__ float from_code(uint32_t byte) {
+    if constexpr (CODE == COROPE_CODE_E4M3) return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+    else return (float)(int)(int8_t)byte;
+}
+// four codes of scale `old` written for `scale` (different ones)
+template <int CODE>
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float old, float scale) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r |= to_code<CODE>(__fmul_rn(from_code<CODE>((w >> (8 * i)) & 0xffu), old), scale) << (8 * i);
+    return r;
+}
+// max(a, b), NaN if one of them is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// elements i .. i + 3 of a row, of any of the three types; `vec`: aligned to four elements
+__device__ __forceinline__ float load1(const void* base, int64_t i, int dtype) {
+    if (dtype == COROPE_DTYPE_F32) return static_cast<const float*>(base)[i];
+    if (dtype == COROPE_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
+    return __half2float(static_cast<const __half*>(base)[i]);
+}
+__device__ __forceinline__ float4 load4(const void* base, int64_t i, int dtype, bool vec) {
+    if (!vec) return make_float4(load1(base, i, dtype), load1(base, i + 1, dtype), load1(base, i + 2, dtype), load1(base, i + 3, dtype));
+    if (dtype == COROPE_DTYPE_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + i);
+    const float2 a = dtype == COROPE_DTYPE_BF16 ? unpack_bf162(u.x) : unpack_half2(u.x), b = dtype == COROPE_DTYPE_BF16 ? unpack_bf162(u.y) : unpack_half2(u.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void store1(void* base, int64_t i, int dtype, float x) {
+    if (dtype == COROPE_DTYPE_F32) static_cast<float*>(base)[i] = x;
+    else if (dtype == COROPE_DTYPE_BF16) static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
+    else static_cast<__half*>(base)[i] = __float2half_rn(x);
+}
+__device__ __forceinline__ void store4(void* base, int64_t i, int dtype, bool vec, float4 x) {
+    if (!vec) {
+        store1(base, i, dtype, x.x); store1(base, i + 1, dtype, x.y); store1(base, i + 2, dtype, x.z); store1(base, i + 3, dtype, x.w);
+    } else if (dtype == COROPE_DTYPE_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(base) + i) = x;
+    } else if (dtype == COROPE_DTYPE_BF16) {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + i) = make_uint2(pack_bf162(x.x, x.y), pack_bf162(x.z, x.w));
+    } else {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + i) = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
+    }
+}
+#endif  // __CUDACC__
+
+// rows whose groups of four elements start at multiples of their size
+inline bool rows_in_fours(const void* ptr, const Strides& st, int dtype) {
+    return (uintptr_t)ptr % (4 * dtype_bytes(dtype)) == 0 && st.b % 4 == 0 && st.h % 4 == 0 && st.n % 4 == 0;
+}
+
+}  // namespace corope

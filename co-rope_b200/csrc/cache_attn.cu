@@ -1,0 +1,796 @@
+// corope_cache_attn: attention of a few query rows per K / V head over the 8-bit cache.
+//
+// With R = G * T query rows a head, 2 D bytes of cache are read per slot for 4 R D operations: memory bound up to R of about 100.  So the kernel is built
+// around the reads:
+//   * Work is counted in units of 64 slots of one (sequence, K / V head, tile of query rows) and cut into equal contiguous ranges, one per resident
+//     block, from the lengths on the device: a batch of unequal lengths loads every SM alike.  A range that starts or ends inside an item leaves
+//     its part (fp32 sums, maximum, total) in the workspace, and a second kernel joins the parts in a fixed order.
+//   * Each warp streams its own 16-slot pieces (a piece lies in one block, so one scale) through its own ring in shared memory with
+//     cp.async, without block-wide barriers.
+//   * Products on mma.sync with slots as the M extent and query rows as N = 8: S^T = K Q^T, O^T = V^T P^T.  Codes become fp16 in registers,
+//     exactly.  Which elements a lane takes is chosen so that it reads whole 16-byte runs: the order of the sum over d is free, and so is the
+//     order of the rows of O^T.
+//   * Rotated queries are scaled by a power of two per row and split into two fp16 numbers (22 bits), so scores have fp32 accuracy.
+//     exp2(s + log2(v scale) - M) is rounded to fp16 (11 bits) for 16-bit outputs, whose own rounding is coarser or equal, and split in two for
+//     fp32 ones; the sum of the probabilities stays fp32.
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "cache.cuh"
+
+namespace corope {
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kPiece = 16;                    // slots per step of a warp; a block of the cache holds a whole number of them
+constexpr int kUnit = kWarps * kPiece;        // slots per unit of work
+constexpr float kLowest = -1e30f;             // running maximum before any score: finite, so that differences from it are no NaN
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool real) {   // zeros where not real
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4_async(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// two codes (the low 16 bits of `pair`) as fp16
+template <int CODE>
+__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint32_t& hi) {   // four codes: (0, 1), (2, 3)
+    if constexpr (CODE == COROPE_CODE_E4M3) {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(word));
+    } else {   // the byte c + 128 behind the fp16 exponent of 1024 reads as 1024 + 128 + c
+        const uint32_t u = word ^ 0x80808080u, bias = 0x64806480u;
+        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
+        const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&bias));
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ division of the work
+// Sequence b contributes items(b) = Hkv * (row tiles in use) items of units(b) units each.
+struct Load {
+    int len, n, units, items;
+};
+__device__ __forceinline__ Load load_of(const CacheAttnParams& p, int rows_per_tile, int b, bool& bad) {
+    Load l;
+    l.len = cache_len(p.s, p.c.bs_log2, b, bad);
+    l.n = cache_new(p.s, p.T, b, bad);
+    l.units = (l.len + kUnit - 1) / kUnit;
+    l.items = p.c.Hkv * ((l.n * p.G + rows_per_tile - 1) / rows_per_tile);
+    return l;
+}
+// Units of the sequences before each thread's share of the batch (thread t has [t * per, (t + 1) * per)) and of all together.
+struct Prefix {
+    int64_t before, total;
+};
+__device__ __forceinline__ Prefix prefix_units(const CacheAttnParams& p, int rows_per_tile, int per, int64_t* words, bool& bad) {
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    int64_t mine = 0;
+    for (int b = threadIdx.x * per; b < min(p.s.B, (int)(threadIdx.x + 1) * per); ++b) {
+        const Load l = load_of(p, rows_per_tile, b, bad);
+        mine += (int64_t)l.units * l.items;
+    }
+    int64_t sum = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, sum, m);
+        if (lane >= m) sum += up;
+    }
+    if (lane == 31) words[warp] = sum;
+    __syncthreads();
+    Prefix r{sum - mine, 0};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) r.before += words[w];
+        r.total += words[w];
+    }
+    return r;
+}
+
+// ------------------------------------------------------------------------------------------------ queries
+// Shared-memory form of a tile of query rows: for k-step w, row group nt and lane, {hi b0, b1, lo b0, b1} of the B operand.
+// Lane (g, c) of the MMA holds row g and the columns c * D / 4 + 4 w .. + 3.
+template <int D, int NT>
+__device__ __forceinline__ void pack_queries(const CacheAttnParams& p, int b, int h, int row0, int len, int n, uint32_t* packed, float* factor,
+                                             bool& bad) {
+    constexpr int kHalf = D / 2, kPairLanes = kHalf / 2;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    for (int r = warp; r < 8 * NT; r += kWarps) {
+        const int row = row0 + r, t = row / p.G;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};   // columns 2 lane, + 1, and their partners D / 2 further on
+        if (t < n && lane < kPairLanes) {
+            const int64_t at = (int64_t)b * p.sq.b + (int64_t)(h * p.G + row - t * p.G) * p.sq.h + (int64_t)t * p.sq.n + 2 * lane;
+            x[0] = load1(p.q, at, p.dtype); x[1] = load1(p.q, at + 1, p.dtype);
+            x[2] = load1(p.q, at + kHalf, p.dtype); x[3] = load1(p.q, at + kHalf + 1, p.dtype);
+            if (p.s.cos != nullptr) {
+                const int64_t tr = (int64_t)cache_position(p.s, b, t, len - n + t, bad) * p.s.rope_stride + 2 * lane;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float c = p.s.cos[tr + i], s = p.s.sin[tr + i], u = x[i], v = x[i + 2];
+                    x[i] = u * c - v * s;
+                    x[i + 2] = v * c + u * s;
+                }
+            }
+        }
+        float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+        for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+        // brings the row's largest element to [2^10, 2^11): then the second part is a normal fp16 number too
+        const bool usual = m >= 1e-30f && m <= 1e30f;
+        const int e = usual ? (int)(__float_as_uint(m) >> 23) - 127 - 10 : 0;
+        const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
+        if (lane == 0) factor[r] = down * p.scale;
+        if (lane < kPairLanes) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int d = 2 * lane + i * kHalf, c = d / (D / 4), w = d % (D / 4) / 4, j = d % 4 / 2;
+                const float u = x[2 * i] * up, v = x[2 * i + 1] * up;
+                const uint32_t hi = pack_half2(u, v);
+                const float2 back = unpack_half2(hi);
+                uint32_t* to = packed + ((w * NT + r / 8) * 32 + r % 8 * 4 + c) * 4 + j;
+                to[0] = hi;
+                to[2] = pack_half2(u - back.x, v - back.y);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ main kernel
+template <int D, int NT>
+struct Shape {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kStages = D == 128 ? 3 : D == 64 ? 6 : 8;
+    static constexpr int kStageBytes = 2 * kPiece * D;
+    static constexpr int kRing = kWarps * kStages * kStageBytes;
+    static constexpr int kJoin = kWarps * kRows * D * 4;                    // the warps' sums, in the place of the rings
+    static constexpr int kBig = kRing > kJoin ? kRing : kJoin;
+    static constexpr int kPacked = D / 16 * NT * 32 * 16;
+    static constexpr int kMeta = kWarps * kStages * 16;                     // {k scale, v scale, block found} of each stage
+    static constexpr int kSmem = kBig + kPacked + kMeta + kRows * 4 + 2 * kWarps * kRows * 4 + 64;
+    static constexpr int kBlocks = NT == 1 ? 4 : 2;                         // resident per SM
+};
+
+struct Piece {   // what a block does next: units [u0, u1) of an item
+    int b, h, tile, u0, u1;
+};
+
+template <int D, int CODE, int NT, bool EXACT_P>
+__global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_kernel(const CacheAttnParams p, int per) {
+    using S = Shape<D, NT>;
+    constexpr int kRows = S::kRows, kKSteps = D / 16, kVWords = D / 32, kStages = S::kStages;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint32_t* packed = reinterpret_cast<uint32_t*>(smem + S::kBig);
+    float* meta = reinterpret_cast<float*>(smem + S::kBig + S::kPacked);
+    float* factor = meta + S::kMeta / 4;
+    float* warp_max = factor + kRows;
+    float* warp_sum = warp_max + kWarps * kRows;
+    int64_t* words = reinterpret_cast<int64_t*>(smem + S::kSmem - 64);
+    __shared__ int64_t start_off;
+    __shared__ int start_b;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
+    bool bad = false;
+
+    // this block's range of units
+    const Prefix pre = prefix_units(p, kRows, per, words, bad);
+    const int64_t total = pre.total;
+    const int64_t ranges = min((int64_t)gridDim.x, total);
+    pdl_trigger();
+    if (blockIdx.x >= ranges) {
+        if (bad) report_bad_index(p.status, p.mirror);
+        return;
+    }
+    const int64_t lo = total * blockIdx.x / ranges, hi = total * (blockIdx.x + 1) / ranges;
+    {
+        int64_t at = pre.before;
+        for (int b = threadIdx.x * per; b < min(p.s.B, (int)(threadIdx.x + 1) * per); ++b) {
+            const Load l = load_of(p, kRows, b, bad);
+            const int64_t u = (int64_t)l.units * l.items;
+            if (lo >= at && lo < at + u) start_b = b, start_off = lo - at;
+            at += u;
+        }
+    }
+    __syncthreads();
+    int b = start_b;
+    int64_t off = start_off, left = hi - lo;   // position in sequence b's units, units left
+    Load l = load_of(p, kRows, b, bad);
+
+    uint8_t* ring = smem + warp * (kStages * S::kStageBytes);
+    float* my_meta = meta + warp * kStages * 4;
+    const uint32_t ring_at = smem_u32(ring), meta_at = smem_u32(my_meta);
+
+    while (left > 0) {
+        while (off >= (int64_t)l.units * l.items) {
+            off -= (int64_t)l.units * l.items;
+            l = load_of(p, kRows, ++b, bad);
+        }
+        const int item = (int)(off / l.units), tiles = l.items / p.c.Hkv;
+        const int h = item / tiles, tile = item % tiles, u0 = (int)(off - (int64_t)item * l.units);
+        const int u1 = (int)min((int64_t)l.units, u0 + left);
+        off += u1 - u0;
+        left -= u1 - u0;
+        const int row0 = tile * kRows, len = l.len, n = l.n;
+        const int least_seen = p.causal ? len - n + row0 / p.G + 1 : len;   // slots below this are seen by every row of the tile that has a query
+
+        __syncthreads();   // the tile before is written out
+        pack_queries<D, NT>(p, b, h, row0, len, n, packed, factor, bad);
+        __syncthreads();
+
+        // columns 2 c, 2 c + 1 of each group of eight rows are this lane's
+        float fac[NT][2];
+        int sees[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 8 * nt + 2 * c + i, t = (row0 + r) / p.G;
+                fac[nt][i] = factor[r];
+                sees[nt][i] = t >= n ? 0 : p.causal ? len - n + t + 1 : len;
+            }
+        uint4 qf[NT == 1 ? kKSteps : 1];
+        if constexpr (NT == 1) {
+#pragma unroll
+            for (int w = 0; w < kKSteps; ++w) qf[w] = reinterpret_cast<const uint4*>(packed)[w * 32 + lane];
+        }
+
+        float o[NT][D / 16][4], m[NT][2], sum[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nt][x][i] = 0.f;
+            m[nt][0] = m[nt][1] = kLowest;
+            sum[nt][0] = sum[nt][1] = 0.f;
+        }
+
+        // pieces first, first + 4, .. of this warp
+        const int first = u0 * kWarps + warp, end = min(u1 * kWarps, (len + kPiece - 1) / kPiece);
+        const int count = end > first ? (end - first + kWarps - 1) / kWarps : 0;
+        const int* table = p.s.table + (int64_t)b * p.s.table_stride;
+        const int shift = p.c.bs_log2 - 4;
+        int next_page = count > 0 ? table[first >> shift] : 0;
+        auto issue = [&](int j) {
+            if (j < count) {
+                const int piece = first + j * kWarps, stage = j % kStages;
+                const bool found = (unsigned)next_page < (unsigned)p.c.num_blocks;
+                const int page = found ? next_page : 0;
+                bad |= !found;
+                if (j + 1 < count) next_page = table[(piece + kWarps) >> shift];
+                const int in_block = (piece << 4) & ((1 << p.c.bs_log2) - 1), rows = found ? min(len - (piece << 4), kPiece) : 0;
+                const uint8_t* kb = p.c.k + (int64_t)page * p.c.sk.b + (int64_t)h * p.c.sk.h + (int64_t)in_block * p.c.sk.n;
+                const uint8_t* vb = p.c.v + (int64_t)page * p.c.sv.b + (int64_t)h * p.c.sv.h + (int64_t)in_block * p.c.sv.n;
+                const uint32_t dst = ring_at + stage * S::kStageBytes;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const int x = lane + 32 * i, row = x / (D / 16), col = x % (D / 16) * 16;
+                    const uint32_t to = (uint32_t)(x ^ ((x >> 3) & 7)) * 16;
+                    const bool real = row < rows;
+                    copy16_async(dst + to, kb + (real ? (int64_t)row * p.c.sk.n + col : 0), real);
+                    copy16_async(dst + kPiece * D + to, vb + (real ? (int64_t)row * p.c.sv.n + col : 0), real);
+                }
+                if (lane < 2) copy4_async(meta_at + stage * 16 + lane * 4, (lane ? p.c.v_scale : p.c.k_scale) + (int64_t)page * p.c.Hkv + h);
+                if (lane == 2) my_meta[stage * 4 + 2] = found ? 1.f : 0.f;
+            }
+            commit_copies();
+        };
+#pragma unroll
+        for (int j = 0; j < kStages - 1; ++j) issue(j);
+
+        for (int j = 0; j < count; ++j) {
+            issue(j + kStages - 1);   // into the stage that step j - 1 has read
+            wait_copies<kStages - 1>();
+            __syncwarp();
+            const int stage = j % kStages, slot0 = (first + j * kWarps) * kPiece;
+            const uint8_t* kt = ring + stage * S::kStageBytes;
+            const uint8_t* vt = kt + kPiece * D;
+            const float k_scale = my_meta[stage * 4], v_scale = my_meta[stage * 4 + 1];
+            const bool found = my_meta[stage * 4 + 2] != 0.f;
+
+            // S^T: slots g and g + 8 by rows 2 c and 2 c + 1
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            float rest[NT][4];   // the second parts' products apart: their sum's truncations are 2^-11 of those of the first
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) rest[nt][0] = rest[nt][1] = rest[nt][2] = rest[nt][3] = 0.f;
+            uint32_t k0[D / 16], k1[D / 16];
+            auto k_words = [&](int row, uint32_t (&w)[D / 16]) {
+                if constexpr (D == 32) {
+                    const int x = row * 2 + c / 2;
+                    const uint2 u = *reinterpret_cast<const uint2*>(kt + (x ^ ((x >> 3) & 7)) * 16 + c % 2 * 8);
+                    w[0] = u.x; w[1] = u.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i) {
+                        const int x = row * (D / 16) + c * (D / 64) + i;
+                        const uint4 u = *reinterpret_cast<const uint4*>(kt + (x ^ ((x >> 3) & 7)) * 16);
+                        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+                    }
+                }
+            };
+            k_words(g, k0);
+            k_words(g + 8, k1);
+#pragma unroll
+            for (int w = 0; w < kKSteps; ++w) {
+                uint32_t a[4];
+                codes_to_half<CODE>(k0[w], a[0], a[2]);
+                codes_to_half<CODE>(k1[w], a[1], a[3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint4 q = NT == 1 ? qf[NT == 1 ? w : 0] : reinterpret_cast<const uint4*>(packed)[(w * NT + nt) * 32 + lane];
+                    mma16816(s[nt], a, q.x, q.y);
+                    mma16816(rest[nt], a, q.z, q.w);
+                }
+            }
+
+            // scores in units of log2, the scale of V folded into the exponent: O = sum of exp2(s + log2 v_scale - M) * code
+            // (a scale of 0 is left out of the exponent, and its slots out of O)
+            const float v_size = v_scale == 0.f ? 1.f : max_nan(v_scale, 1e-30f), lift = __log2f(v_size), drop = 1.f / v_size, live = v_scale == 0.f ? 0.f : 1.f;
+            bool higher = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int slot = slot0 + g + 8 * (i / 2);
+                    const float x = fmaf(s[nt][i] + rest[nt][i], fac[nt][i % 2] * k_scale, lift);
+                    s[nt][i] = found && slot < sees[nt][i % 2] ? x : -INFINITY;
+                    higher |= s[nt][i] > m[nt][i % 2] + 8.f;
+                }
+            if (__any_sync(0xffffffffu, higher)) {   // exp2 of up to 8 above M fits fp16: M moves only when a score is beyond that
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float top = fmaxf(s[nt][i], s[nt][i + 2]);
+#pragma unroll
+                        for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                        top = fmaxf(top, m[nt][i]);
+                        const float shrink = fast_exp2(m[nt][i] - top);
+                        m[nt][i] = top;
+                        sum[nt][i] *= shrink;
+#pragma unroll
+                        for (int x = 0; x < D / 16; ++x) o[nt][x][i] *= shrink, o[nt][x][i + 2] *= shrink;
+                    }
+            }
+            uint32_t pb[NT][2], pl[EXACT_P ? NT : 1][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = fast_exp2(s[nt][i] - m[nt][i % 2]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float both = w[i] + w[i + 2];
+                    sum[nt][i] = both == 0.f ? sum[nt][i] : fmaf(both, drop, sum[nt][i]);   // hidden slots of a block whose scale is NaN count nothing
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    w[2 * i] *= live;
+                    w[2 * i + 1] *= live;
+                    const uint32_t hi = pack_half2(w[2 * i], w[2 * i + 1]);
+                    pb[nt][i] = transpose8x8(hi);
+                    if constexpr (EXACT_P) {
+                        const float2 back = unpack_half2(hi);
+                        pl[nt][i] = transpose8x8(pack_half2(w[2 * i] - back.x, w[2 * i + 1] - back.y));
+                    }
+                }
+            }
+
+            // O^T: columns g * D / 8 + 2 x and + 1 of V by rows 2 c and 2 c + 1
+            uint32_t v[4][kVWords];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 2 * c + i % 2 + 8 * (i / 2);
+                if constexpr (D == 128) {
+                    const int x = row * 8 + g;
+                    const uint4 u = *reinterpret_cast<const uint4*>(vt + (x ^ ((x >> 3) & 7)) * 16);
+                    v[i][0] = u.x; v[i][1] = u.y; v[i][2] = u.z; v[i][3] = u.w;
+                } else if constexpr (D == 64) {
+                    const int x = row * 4 + g / 2;
+                    const uint2 u = *reinterpret_cast<const uint2*>(vt + (x ^ ((x >> 3) & 7)) * 16 + g % 2 * 8);
+                    v[i][0] = u.x; v[i][1] = u.y;
+                } else {
+                    const int x = row * 2 + g / 4;
+                    v[i][0] = *reinterpret_cast<const uint32_t*>(vt + (x ^ ((x >> 3) & 7)) * 16 + g % 4 * 4);
+                }
+            }
+            auto add_values = [&](auto per_slot, int only) {   // only: the one slot of the piece to add, to the rows that see it
+                constexpr bool kPerSlot = decltype(per_slot)::value;
+#pragma unroll
+                for (int w = 0; w < kVWords; ++w) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = !kPerSlot || only == 2 * c + i % 2 + 8 * (i / 2) ? v[i][w] : 0u;
+                    uint32_t a[2][4];
+                    codes_to_half<CODE>(__byte_perm(x[0], x[1], 0x5140), a[0][0], a[0][1]);
+                    codes_to_half<CODE>(__byte_perm(x[2], x[3], 0x5140), a[0][2], a[0][3]);
+                    codes_to_half<CODE>(__byte_perm(x[0], x[1], 0x7362), a[1][0], a[1][1]);
+                    codes_to_half<CODE>(__byte_perm(x[2], x[3], 0x7362), a[1][2], a[1][3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            if constexpr (EXACT_P || kPerSlot) {   // EXACT_P: the long sum in fp32 additions, as MMA accumulation truncates
+                                float t[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma16816(t, a[y], pb[nt][0], pb[nt][1]);
+                                if constexpr (EXACT_P) mma16816(t, a[y], pl[nt][0], pl[nt][1]);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (!kPerSlot || slot0 + only < sees[nt][i % 2]) o[nt][2 * w + y][i] += t[i];
+                            } else {
+                                mma16816(o[nt][2 * w + y], a[y], pb[nt][0], pb[nt][1]);
+                            }
+                        }
+                }
+            };
+            // A NaN in V reaches the rows that see its slot, and 0 * NaN would bring it to the others: such a piece goes slot by slot
+            bool nan = false;
+            if (CODE == COROPE_CODE_E4M3 && slot0 + kPiece > least_seen) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int w = 0; w < kVWords; ++w) nan |= __vcmpeq4(v[i][w] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
+                nan = __any_sync(0xffffffffu, nan);
+            }
+            if (CODE == COROPE_CODE_E4M3 && nan) {
+#pragma unroll 1
+                for (int only = 0; only < kPiece; ++only) add_values(std::true_type{}, only);
+            } else {
+                add_values(std::false_type{}, 0);
+            }
+            __syncwarp();   // the stage has been read
+        }
+        wait_copies<0>();
+
+        // join the four warps
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int k = 4; k < 32; k *= 2) sum[nt][i] += __shfl_xor_sync(0xffffffffu, sum[nt][i], k);
+                if (g == 0) {
+                    warp_max[warp * kRows + 8 * nt + 2 * c + i] = m[nt][i];
+                    warp_sum[warp * kRows + 8 * nt + 2 * c + i] = sum[nt][i];
+                }
+            }
+        __syncthreads();
+        float* join = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 8 * nt + 2 * c + i;
+                float top = warp_max[r];
+#pragma unroll
+                for (int k = 1; k < kWarps; ++k) top = fmaxf(top, warp_max[k * kRows + r]);
+                const float shrink = fast_exp2(m[nt][i] - top);
+                float2* to = reinterpret_cast<float2*>(join + (warp * kRows + r) * D + g * (D / 8));
+#pragma unroll
+                for (int x = 0; x < D / 16; ++x) to[x] = make_float2(o[nt][x][i] * shrink, o[nt][x][i + 2] * shrink);
+            }
+        __syncthreads();
+        const bool whole = u0 == 0 && u1 == l.units;
+        const int64_t part = 2 * (int64_t)blockIdx.x + (u0 == 0 ? 1 : 0);
+        for (int x = threadIdx.x; x < kRows * (D / 4); x += kThreads) {
+            const int r = x / (D / 4), d = x % (D / 4) * 4, row = row0 + r, t = row / p.G;
+            float top = warp_max[r], all = 0.f;
+#pragma unroll
+            for (int k = 1; k < kWarps; ++k) top = fmaxf(top, warp_max[k * kRows + r]);
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) all = fmaf(warp_sum[k * kRows + r], fast_exp2(warp_max[k * kRows + r] - top), all);
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                const float4 z = *reinterpret_cast<const float4*>(join + (k * kRows + r) * D + d);
+                y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+            }
+            if (!whole) {
+                *reinterpret_cast<float4*>(p.part + (part * kRows + r) * D + d) = y;
+                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (part * kRows + r) * 2) = make_float2(top, all);
+            } else if (t < p.T) {
+                const float f = 1.f / all;
+                y = all == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+                store4(p.o, (int64_t)b * p.so.b + (int64_t)(h * p.G + row - t * p.G) * p.so.h + (int64_t)t * p.so.n + d, p.dtype, p.vec_o, y);
+                if (p.lse != nullptr && d == 0) p.lse[((int64_t)b * p.c.Hkv + h) * p.T * p.G + row] = all == 0.f ? INFINITY : top + log2f(all);
+            }
+        }
+    }
+    if (bad) report_bad_index(p.status, p.mirror);
+}
+
+// ------------------------------------------------------------------------------------------------ joining parts
+// One block per item, a warp per query row.  An item that one block of the main kernel did alone is finished; the parts of the others are
+// added in the order of their ranges.  Rows that no unit stands for are written here: 0.
+constexpr int kJoinThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const CacheAttnParams p, int rows_per_tile, int main_blocks) {
+    __shared__ int64_t words[2][kJoinThreads / 32];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int tile = (int)(blockIdx.x % (unsigned)p.row_tiles), bh = (int)(blockIdx.x / (unsigned)p.row_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
+    bool bad = false;
+    int64_t before = 0, total = 0;
+    for (int i = threadIdx.x; i < p.s.B; i += kJoinThreads) {
+        const Load l = load_of(p, rows_per_tile, i, bad);
+        const int64_t u = (int64_t)l.units * l.items;
+        total += u;
+        if (i < b) before += u;
+    }
+#pragma unroll
+    for (int m = 16; m; m >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, m);
+        total += __shfl_xor_sync(0xffffffffu, total, m);
+    }
+    if (lane == 0) words[0][warp] = before, words[1][warp] = total;
+    __syncthreads();
+    before = total = 0;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) before += words[0][w], total += words[1][w];
+
+    const Load l = load_of(p, rows_per_tile, b, bad);
+    const int tiles = l.items / p.c.Hkv;
+    const bool empty = l.units == 0 || tile >= tiles;
+    const int64_t ranges = min((int64_t)main_blocks, total);
+    int64_t r0 = 0, r1 = 0;
+    if (!empty) {
+        const int64_t u0 = before + (int64_t)(h * tiles + tile) * l.units, u1 = u0 + l.units - 1;
+        r0 = ((u0 + 1) * ranges - 1) / total;   // the range that holds a unit
+        r1 = ((u1 + 1) * ranges - 1) / total;
+    }
+    pdl_wait();   // by every block: the end of this kernel has to stand for the end of the one before
+    if (!empty && r0 == r1) return;
+    for (int r = warp; r < rows_per_tile; r += kJoinThreads / 32) {
+        const int row = tile * rows_per_tile + r, t = row / p.G;
+        if (t >= p.T) break;
+        float top = kLowest, all = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!empty) {
+            // a part that starts its item is in the second slot of its block, the others are in the first
+#pragma unroll 4
+            for (int64_t i = r0; i <= r1; ++i) top = fmaxf(top, p.part_ml[((2 * i + (i == r0 ? 1 : 0)) * rows_per_tile + r) * 2]);
+#pragma unroll 4
+            for (int64_t i = r0; i <= r1; ++i) {
+                const int64_t at = (2 * i + (i == r0 ? 1 : 0)) * rows_per_tile + r;
+                const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+                const float f = fast_exp2(ml.x - top);
+                all = fmaf(ml.y, f, all);
+                if (lane < D / 4) {
+                    const float4 z = *reinterpret_cast<const float4*>(p.part + at * D + 4 * lane);
+                    y.x = fmaf(z.x, f, y.x); y.y = fmaf(z.y, f, y.y); y.z = fmaf(z.z, f, y.z); y.w = fmaf(z.w, f, y.w);
+                }
+            }
+        }
+        const float f = 1.f / all;
+        if (lane < D / 4)
+            store4(p.o, (int64_t)b * p.so.b + (int64_t)(h * p.G + row - t * p.G) * p.so.h + (int64_t)t * p.so.n + 4 * lane, p.dtype, p.vec_o,
+                   all == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+        if (p.lse != nullptr && lane == 0) p.lse[((int64_t)b * p.c.Hkv + h) * p.T * p.G + row] = all == 0.f ? INFINITY : top + log2f(all);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ accumulated weights
+// weight[slot] += sum over rows of exp2(s - lse).  The scores are formed again, K being read once more: the same division into units, but a
+// unit's block goes through all tiles of query rows, so that each slot's sum is one addition in a fixed order.
+template <int D, int CODE, int NT>
+__global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const CacheAttnParams p, int per) {
+    constexpr int kRows = 8 * NT, kKSteps = D / 16;
+    __shared__ __align__(16) uint32_t packed[Shape<D, NT>::kPacked / 4];
+    __shared__ float factor[kRows], lse[kRows];
+    __shared__ int64_t words[kWarps], start_off;
+    __shared__ int start_b;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
+    bool bad = false;
+    auto load = [&](int b) {
+        Load l = load_of(p, kRows, b, bad);
+        l.items = l.n > 0 ? p.c.Hkv : 0;
+        return l;
+    };   // items of this kernel: K / V heads
+    int64_t mine = 0;
+    for (int b = threadIdx.x * per; b < min(p.s.B, (int)(threadIdx.x + 1) * per); ++b) {
+        const Load l = load(b);
+        mine += (int64_t)l.units * l.items;
+    }
+    int64_t sum = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, sum, m);
+        if (lane >= m) sum += up;
+    }
+    if (lane == 31) words[warp] = sum;
+    __syncthreads();
+    int64_t at = sum - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) at += words[w];
+        total += words[w];
+    }
+    const int64_t ranges = min((int64_t)gridDim.x, total);
+    if (blockIdx.x >= ranges) return;
+    const int64_t lo = total * blockIdx.x / ranges, hi = total * (blockIdx.x + 1) / ranges;
+    for (int b = threadIdx.x * per; b < min(p.s.B, (int)(threadIdx.x + 1) * per); ++b) {
+        const Load l = load(b);
+        const int64_t u = (int64_t)l.units * l.items;
+        if (lo >= at && lo < at + u) start_b = b, start_off = lo - at;
+        at += u;
+    }
+    __syncthreads();
+    int b = start_b, had = -1;
+    int64_t off = start_off;
+    Load l = load(b);
+    for (int64_t left = hi - lo; left > 0; --left, ++off) {
+        while (off >= (int64_t)l.units * l.items) {
+            off -= (int64_t)l.units * l.items;
+            l = load(++b);
+            had = -1;
+        }
+        const int h = (int)(off / l.units), slot0 = (int)(off - (int64_t)h * l.units) * kUnit + warp * kPiece;
+        const int page = slot0 < l.len ? cache_page(p.s, p.c.bs_log2, p.c.num_blocks, b, slot0, bad) : -1;
+        const int in_block = slot0 & ((1 << p.c.bs_log2) - 1);
+        uint32_t k[2][D / 16];
+        float k_scale = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int w = 0; w < D / 16; ++w) k[i][w] = 0u;
+        if (page >= 0) {
+            k_scale = p.c.k_scale[(int64_t)page * p.c.Hkv + h];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (slot0 + g + 8 * i >= l.len) continue;
+                const uint8_t* from = p.c.k + (int64_t)page * p.c.sk.b + (int64_t)h * p.c.sk.h + (int64_t)(in_block + g + 8 * i) * p.c.sk.n + c * (D / 4);
+                if constexpr (D == 32) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(from);
+                    k[i][0] = u.x; k[i][1] = u.y;
+                } else {
+#pragma unroll
+                    for (int x = 0; x < D / 64; ++x) {
+                        const uint4 u = reinterpret_cast<const uint4*>(from)[x];
+                        k[i][4 * x] = u.x; k[i][4 * x + 1] = u.y; k[i][4 * x + 2] = u.z; k[i][4 * x + 3] = u.w;
+                    }
+                }
+            }
+        }
+        float w0 = 0.f, w1 = 0.f;
+        const int tiles = (l.n * p.G + kRows - 1) / kRows;
+        for (int tile = 0; tile < tiles; ++tile) {
+            if (tiles > 1 || had != h) {
+                __syncthreads();
+                pack_queries<D, NT>(p, b, h, tile * kRows, l.len, l.n, packed, factor, bad);
+                for (int r = threadIdx.x; r < kRows; r += kThreads) {
+                    const int row = tile * kRows + r;
+                    lse[r] = row < l.n * p.G ? p.lse[((int64_t)b * p.c.Hkv + h) * p.T * p.G + row] : INFINITY;
+                }
+                __syncthreads();
+                had = h;
+            }
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kKSteps; ++w) {
+                uint32_t a[4];
+                codes_to_half<CODE>(k[0][w], a[0], a[2]);
+                codes_to_half<CODE>(k[1][w], a[1], a[3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint4 qf = reinterpret_cast<const uint4*>(packed)[(w * NT + nt) * 32 + lane];
+                    mma16816(s[nt], a, qf.x, qf.y);
+                    mma16816(s[nt], a, qf.z, qf.w);
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 8 * nt + 2 * c + i, t = (tile * kRows + r) / p.G;
+                    const int sees = t >= l.n ? 0 : p.causal ? l.len - l.n + t + 1 : l.len;
+                    const float f = factor[r] * k_scale, z = lse[r];
+                    if (slot0 + g < sees) w0 += fast_exp2(fmaf(s[nt][i], f, -z));
+                    if (slot0 + g + 8 < sees) w1 += fast_exp2(fmaf(s[nt][i + 2], f, -z));
+                }
+        }
+#pragma unroll
+        for (int m = 1; m < 4; m *= 2) {
+            w0 += __shfl_xor_sync(0xffffffffu, w0, m);
+            w1 += __shfl_xor_sync(0xffffffffu, w1, m);
+        }
+        // one addition per slot and call; atomic because sequences may share blocks
+        if (page >= 0 && c == 0) {
+            float* to = p.c.weight + (((int64_t)page * p.c.Hkv + h) << p.c.bs_log2) + in_block;
+            if (slot0 + g < l.len) atomicAdd(to + g, w0);
+            if (slot0 + g + 8 < l.len) atomicAdd(to + g + 8, w1);
+        }
+    }
+    if (bad) report_bad_index(p.status, p.mirror);
+}
+
+// rows of a tile by the number of query rows: 8 (one N extent of the MMA), 16 or 32
+int row_groups(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+int resident_blocks(int groups) { return groups == 1 ? 4 : 2; }
+unsigned main_blocks(int B, int Hkv, int row_tiles, int max_blocks, int block_size, int groups) {
+    const uint64_t units = (uint64_t)B * Hkv * row_tiles * (((uint64_t)max_blocks * block_size + kUnit - 1) / kUnit);
+    const uint64_t most = (uint64_t)sm_count() * resident_blocks(groups);
+    return (unsigned)(units < most ? units : most);
+}
+
+template <int D, int CODE, int NT, bool EXACT_P>
+int launch_main(const CacheAttnParams& p, unsigned blocks, int per, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    if (int e = allow_smem(cache_attn_kernel<D, CODE, NT, EXACT_P>, Shape<D, NT>::kSmem, done)) return e;
+    count_launch();
+    cache_attn_kernel<D, CODE, NT, EXACT_P><<<blocks, kThreads, Shape<D, NT>::kSmem, s>>>(p, per);
+    return (int)cudaGetLastError();
+}
+template <int D, int CODE, int NT>
+int launch_all(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
+    const int per = (p.s.B + kThreads - 1) / kThreads;
+    if (int e = p.dtype == COROPE_DTYPE_F32 ? launch_main<D, CODE, NT, true>(p, blocks, per, s) : launch_main<D, CODE, NT, false>(p, blocks, per, s)) return e;
+    count_launch();
+    if (int e = launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles), kJoinThreads, 0, s, p, 8 * NT, (int)blocks)) return e;
+    if (!p.accumulate) return COROPE_OK;
+    count_launch();
+    const uint64_t units = (uint64_t)p.s.B * p.c.Hkv * ((((uint64_t)p.s.max_blocks << p.c.bs_log2) + kUnit - 1) / kUnit);
+    const uint64_t most = (uint64_t)sm_count() * 8;
+    cache_attn_weight_kernel<D, CODE, NT><<<(unsigned)(units < most ? units : most), kThreads, 0, s>>>(p, per);
+    return (int)cudaGetLastError();
+}
+template <int D, int CODE>
+int by_rows(const CacheAttnParams& p, int groups, unsigned blocks, cudaStream_t s) {
+    return groups == 1 ? launch_all<D, CODE, 1>(p, blocks, s) : groups == 2 ? launch_all<D, CODE, 2>(p, blocks, s) : launch_all<D, CODE, 4>(p, blocks, s);
+}
+template <int D>
+int by_code(const CacheAttnParams& p, int groups, unsigned blocks, cudaStream_t s) {
+    return p.code == COROPE_CODE_E4M3 ? by_rows<D, COROPE_CODE_E4M3>(p, groups, blocks, s) : by_rows<D, COROPE_CODE_INT8>(p, groups, blocks, s);
+}
+
+struct Layout {
+    int groups, row_tiles;
+    unsigned blocks;
+    size_t part_ml, lse, total;   // the parts themselves come first
+};
+Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_size, int accumulate) {
+    Layout l{};
+    const int rows = G * T;
+    l.groups = row_groups(rows);
+    l.row_tiles = (rows + 8 * l.groups - 1) / (8 * l.groups);
+    l.blocks = main_blocks(B, Hkv, l.row_tiles, max_blocks, block_size, l.groups);
+    const size_t part_rows = (size_t)2 * l.blocks * 8 * l.groups;
+    l.part_ml = align_up(part_rows * D * 4, 256);
+    l.lse = l.part_ml + align_up(part_rows * 8, 256);
+    l.total = l.lse + (accumulate ? align_up((size_t)B * Hkv * rows * 4, 256) : 0);
+    return l;
+}
+
+}  // namespace
+
+size_t cache_attn_workspace_bytes(int B, int Hkv, int G, int T, int D, int max_blocks, int block_size, int dtype, int accumulate) {
+    (void)dtype;
+    return layout_of(B, Hkv, G, T, D, max_blocks, block_size, accumulate).total;
+}
+
+int launch_cache_attn(CacheAttnParams p, void* ws, cudaStream_t s) {
+    const Layout l = layout_of(p.s.B, p.c.Hkv, p.G, p.T, p.D, p.s.max_blocks, 1 << p.c.bs_log2, p.accumulate);
+    p.row_tiles = l.row_tiles;
+    p.part = static_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + l.part_ml);
+    p.lse = p.accumulate ? reinterpret_cast<float*>(static_cast<char*>(ws) + l.lse) : nullptr;
+    p.vec_o = rows_in_fours(p.o, p.so, p.dtype);
+    return p.D == 128 ? by_code<128>(p, l.groups, l.blocks, s) : p.D == 64 ? by_code<64>(p, l.groups, l.blocks, s) : by_code<32>(p, l.groups, l.blocks, s);
+}
+
+}  // namespace corope

@@ -60,6 +60,8 @@ DeviceStatus& device_status(int index) {
 }
 
 std::string status_message(int v) {
+    if (v == COROPE_DEV_BAD_INDEX)
+        return "a block table entry, length or position of a cache operator pointed outside its tensor (it was not followed; the tokens concerned were left out)";
     if (v & 0x2000)
         return "a gradient term left the value range of the 16-bit Co-RoPE backward and was clamped (results of that call are inaccurate)";
     return "a bounded device-side wait expired (results of that call and of later calls are undefined)";
@@ -337,6 +339,170 @@ Grads gqa_backward(const GqaSaved& s, const Tensor& d_out, double sm_scale, doub
     return g;
 }
 
+// ------------------------------------------------------------------------------------------------ 8-bit paged cache
+using Optional = c10::optional<Tensor>;
+
+struct CacheTensors {   // the attributes of a cache object (kv_cache.py)
+    Tensor k, v, k_scale, v_scale;
+    Optional weight;
+};
+
+void require_shape(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, const Tensor& like, const char* name) {
+    require_cuda(t);
+    if (t.sizes() != shape || t.scalar_type() != type || t.device() != like.device()) {
+        std::ostringstream os;
+        os << name << " must be a " << type << " tensor of shape " << shape << " on " << like.device() << ", got " << t.scalar_type() << " " << t.sizes() << " on "
+           << t.device();
+        throw ValueError(os.str());
+    }
+}
+// no gradient flows through the cache: a caller who expects one learns it here
+void require_no_grad(std::initializer_list<const Tensor*> ts) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const Tensor* t : ts)
+        if (t->requires_grad()) throw std::runtime_error("corope_b200: the cache operators have no backward pass; call them under torch.no_grad()");
+}
+
+corope_kv_cache_t cache_view(const CacheTensors& c) {
+    for (const Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale}) require_cuda(*t);
+    require_value(c.k.dim() == 4 && c.k.sizes() == c.v.sizes() && c.k.scalar_type() == c.v.scalar_type() && c.k.device() == c.v.device(),
+                  "cache.k and cache.v must be [num_blocks, Hkv, block_size, D] tensors of one shape, type and device");
+    require_value(c.k.scalar_type() == at::kFloat8_e4m3fn || c.k.scalar_type() == at::kChar, "cache.k and cache.v must be float8_e4m3fn or int8");
+    const int64_t N = c.k.size(0), H = c.k.size(1), bs = c.k.size(2), D = c.k.size(3);
+    require(D == 32 || D == 64 || D == 128, "corope_b200 supports head dims (32, 64, 128)");
+    require_value(bs >= 16 && bs <= 256 && (bs & (bs - 1)) == 0, "block_size must be 16, 32, 64, 128 or 256, got " + std::to_string(bs));
+    require_value(N > 0 && N < (1ll << 31) && H > 0 && H < (1ll << 24), "the cache must have blocks and heads");
+    require_shape(c.k_scale, {N, H}, at::kFloat, c.k, "cache.k_scale");
+    require_shape(c.v_scale, {N, H}, at::kFloat, c.k, "cache.v_scale");
+    require_value(c.k_scale.is_contiguous() && c.v_scale.is_contiguous(), "cache.k_scale and cache.v_scale must be contiguous");
+    corope_kv_cache_t r{};
+    if (c.weight.has_value()) {
+        require_shape(*c.weight, {N, H, bs}, at::kFloat, c.k, "cache.weight");
+        require_value(c.weight->is_contiguous(), "cache.weight must be contiguous");
+        r.weight = c.weight->data_ptr<float>();
+    }
+    for (const Tensor* t : {&c.k, &c.v}) {
+        const auto st = t->strides();
+        bool ok = st[3] == 1 && st[2] >= D && (uintptr_t)t->data_ptr() % 16 == 0;
+        for (int i = 0; i < 3; ++i) ok = ok && st[i] >= 0 && st[i] % 16 == 0;
+        require_value(ok, "rows of cache.k and cache.v must be contiguous and start at multiples of 16 bytes");
+    }
+    r.k = c.k.data_ptr(); r.v = c.v.data_ptr();
+    r.k_scale = c.k_scale.data_ptr<float>(); r.v_scale = c.v_scale.data_ptr<float>();
+    set_strides(r.k_stride, c.k);
+    set_strides(r.v_stride, c.v);
+    r.num_blocks = (int)N; r.Hkv = (int)H; r.block_size = (int)bs; r.D = (int)D;
+    r.code = c.k.scalar_type() == at::kChar ? COROPE_CODE_INT8 : COROPE_CODE_E4M3;
+    return r;
+}
+
+const int* index_ptr(const Tensor& t, int64_t B, const Tensor& like, const char* name) {
+    require_shape(t, {B}, at::kInt, like, name);
+    require_value(t.is_contiguous(), std::string(name) + " must be contiguous");
+    return t.data_ptr<int>();
+}
+void table_checks(const Tensor& t, int64_t B, const Tensor& like, const char* name) {
+    require_cuda(t);
+    require_value(t.dim() == 2 && t.size(0) == B && t.size(1) > 0 && t.scalar_type() == at::kInt && t.device() == like.device(),
+                  std::string(name) + " must be an int32 tensor [B, blocks] on the cache's device");
+    require_value((t.size(1) == 1 || t.stride(1) == 1) && (B == 1 || t.stride(0) >= t.size(1)), std::string(name) + " must have rows without gaps that do not overlap");
+}
+// `keep` holds what the tables were converted to
+corope_cache_seqs_t seqs_view(const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, const Optional& cos, const Optional& sin,
+                              const Optional& positions, const Optional& new_lens, Tables& keep) {
+    require_value(seq_lens.dim() == 1 && seq_lens.size(0) > 0, "seq_lens must be a tensor [B]");
+    const int64_t B = seq_lens.size(0), D = c.k.size(3);
+    corope_cache_seqs_t r{};
+    table_checks(block_table, B, c.k, "block_table");
+    r.block_table = block_table.data_ptr<int>();
+    r.table_stride = block_table.stride(0);
+    r.B = (int)B;
+    r.max_blocks = (int)block_table.size(1);
+    r.seq_lens = index_ptr(seq_lens, B, c.k, "seq_lens");
+    if (new_lens.has_value()) r.new_lens = index_ptr(*new_lens, B, c.k, "new_lens");
+    if (positions.has_value()) r.positions = index_ptr(*positions, B, c.k, "positions");
+    require_value(cos.has_value() == sin.has_value(), "give both freqs_cos and freqs_sin, or neither");
+    if (cos.has_value()) {
+        keep = tables(*cos, *sin, 1, D);
+        require_value(keep.cos.device() == c.k.device() && keep.sin.device() == c.k.device(), "freqs_cos and freqs_sin must be on the cache's device");
+        require_value(keep.cos.size(0) < (1ll << 31) && (keep.cos.size(0) == 1 || keep.stride >= D / 2), "rows of freqs_cos and freqs_sin must not overlap");
+        r.cos = keep.cos.data_ptr<float>();
+        r.sin = keep.sin.data_ptr<float>();
+        r.rope_stride = keep.stride;
+        r.table_rows = (int)keep.cos.size(0);
+    }
+    return r;
+}
+// rows as the cache kernels read them: any strides that are not negative, unit stride along the head dimension
+Tensor readable_rows(const Tensor& t) { return t.stride(3) == 1 ? t : t.contiguous(); }
+void check_tokens(const Tensor& t, const CacheTensors& c, int64_t B, const char* name) {
+    require_cuda(t);
+    require_value(t.dim() == 4 && t.size(0) == B && t.size(2) > 0 && t.size(3) == c.k.size(3) && t.device() == c.k.device() && dtype_code(t) >= 0,
+                  std::string(name) + " must be a [B, H, T, D] tensor in float32, bfloat16 or float16 with the cache's head dimension, on its device");
+    require_value(t.size(2) <= (1 << 20), "at most 2^20 tokens a call");
+}
+
+void cache_append(const Tensor& k_in, const Tensor& v_in, const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, const Optional& cos,
+                  const Optional& sin, const Optional& positions, const Optional& new_lens) {
+    require_no_grad({&k_in, &v_in});
+    const corope_kv_cache_t cache = cache_view(c);
+    Call call(c.k);
+    Tables keep;
+    const corope_cache_seqs_t seqs = seqs_view(c, block_table, seq_lens, cos, sin, positions, new_lens, keep);
+    check_tokens(k_in, c, seqs.B, "k");
+    require_value(k_in.size(1) == cache.Hkv && k_in.sizes() == v_in.sizes() && k_in.scalar_type() == v_in.scalar_type() && v_in.device() == c.k.device(),
+                  "k and v must share one shape, type and device and have the cache's heads");
+    const Tensor k = readable_rows(k_in), v = readable_rows(v_in);
+    int64_t sk[3], sv[3];
+    set_strides(sk, k);
+    set_strides(sv, v);
+    raise_for_status(corope_cache_append(&cache, &seqs, k.data_ptr(), v.data_ptr(), sk, sv, (int)k.size(2), dtype_code(k), call.status.word_ptr, call.stream),
+                     "corope_cache_append");
+}
+
+Tensor cache_attention(const Tensor& q_in, const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, bool causal, double sm_scale,
+                       const Optional& cos, const Optional& sin, const Optional& positions, const Optional& new_lens, bool accumulate) {
+    require_no_grad({&q_in});
+    const corope_kv_cache_t cache = cache_view(c);
+    Call call(c.k);
+    Tables keep;
+    const corope_cache_seqs_t seqs = seqs_view(c, block_table, seq_lens, cos, sin, positions, new_lens, keep);
+    check_tokens(q_in, c, seqs.B, "q");
+    require_value(q_in.size(1) > 0 && q_in.size(1) % cache.Hkv == 0, "Number of query heads must be divisible by KV heads.");
+    require_value(!accumulate || cache.weight != nullptr, "accumulate needs a cache with weights");
+    const Tensor q = readable_rows(q_in);
+    // o is laid out like q, whose heads or batch entries may share memory; o's may not
+    Tensor o = at::empty_like(q);
+    const int Hq = (int)q.size(1), T = (int)q.size(2), dt = dtype_code(q);
+    const size_t bytes = corope_cache_attn_workspace_bytes(&cache, &seqs, Hq, T, dt, accumulate ? 1 : 0);
+    const Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 256)}, q.options().dtype(at::kByte));
+    int64_t sq[3], so[3];
+    set_strides(sq, q);
+    set_strides(so, o);
+    raise_for_status(corope_cache_attn(&cache, &seqs, q.data_ptr(), o.data_ptr(), sq, so, Hq, T, dt, causal ? 1 : 0, (float)sm_scale, accumulate ? 1 : 0,
+                                       ws.data_ptr(), bytes, call.status.word_ptr, call.stream),
+                     "corope_cache_attn");
+    return o;
+}
+
+std::tuple<Tensor, Tensor> cache_evict(const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, const Tensor& out_table, int64_t budget,
+                                       int64_t recent) {
+    const corope_kv_cache_t cache = cache_view(c);
+    require_value(cache.weight != nullptr, "eviction needs a cache with weights");
+    Call call(c.k);
+    Tables keep;
+    const corope_cache_seqs_t seqs = seqs_view(c, block_table, seq_lens, {}, {}, {}, {}, keep);
+    table_checks(out_table, seqs.B, c.k, "out_table");
+    require_value(budget > 0 && recent >= 0 && recent <= budget, "budget must be positive and recent between 0 and budget");
+    require_value(out_table.size(1) * cache.block_size >= budget, "out_table's blocks must hold budget tokens");
+    const auto ints = seq_lens.options();
+    Tensor lens = at::empty({seqs.B}, ints), kept = at::empty({seqs.B, cache.Hkv, budget}, ints);
+    raise_for_status(corope_cache_evict(&cache, &seqs, out_table.data_ptr<int>(), out_table.stride(0), (int)out_table.size(1), (int)budget, (int)recent,
+                                        lens.data_ptr<int>(), kept.data_ptr<int>(), call.status.word_ptr, call.stream),
+                     "corope_cache_evict");
+    return {lens, kept};
+}
+
 // ------------------------------------------------------------------------------------------------ autograd nodes
 Tensor save(AutogradContext* ctx, Kind kind, const Saved& s, bool causal, double sm_scale, double theta) {
     variable_list t{s.q, s.k, s.v, s.o, s.m};
@@ -438,6 +604,20 @@ PYBIND11_MODULE(_corope_torch, m) {
                              double sm_scale, double theta) {
         Grads g = gqa_backward(GqaSaved{q, k, v, o, lse2, a_diag}, d_o, sm_scale, theta);
         return std::make_tuple(g.dq, g.dk, g.dv);
+    }, NoGil());
+    // the 8-bit cache: (k, v, k_scale, v_scale, weight) stand for the cache object
+    m.def("cache_append", [](const Tensor& k, const Tensor& v, const Tensor& ck, const Tensor& cv, const Tensor& ks, const Tensor& vs, const Optional& w,
+                             const Tensor& table, const Tensor& lens, const Optional& cos, const Optional& sin, const Optional& positions, const Optional& new_lens) {
+        cache_append(k, v, CacheTensors{ck, cv, ks, vs, w}, table, lens, cos, sin, positions, new_lens);
+    }, NoGil());
+    m.def("cache_attention", [](const Tensor& q, const Tensor& ck, const Tensor& cv, const Tensor& ks, const Tensor& vs, const Optional& w, const Tensor& table,
+                                const Tensor& lens, bool causal, double sm_scale, const Optional& cos, const Optional& sin, const Optional& positions,
+                                const Optional& new_lens, bool accumulate) {
+        return cache_attention(q, CacheTensors{ck, cv, ks, vs, w}, table, lens, causal, sm_scale, cos, sin, positions, new_lens, accumulate);
+    }, NoGil());
+    m.def("cache_evict", [](const Tensor& ck, const Tensor& cv, const Tensor& ks, const Tensor& vs, const Optional& w, const Tensor& table, const Tensor& lens,
+                            const Tensor& out_table, int64_t budget, int64_t recent) {
+        return cache_evict(CacheTensors{ck, cv, ks, vs, w}, table, lens, out_table, budget, recent);
     }, NoGil());
     // (status word tensor, pinned mirror tensor) of a device, created on first use
     m.def("device_status", [](int index) {

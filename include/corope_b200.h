@@ -61,11 +61,13 @@ extern "C" {
 #define COROPE_ERR_NO_DEVICE (-9)      /* no sm_100 device / driver entry point */
 #define COROPE_ERR_TOO_LARGE (-10)     /* size beyond what the entry point supports */
 #define COROPE_ERR_BAD_STRIDE (-11)    /* row stride below D, or a negative stride */
+#define COROPE_ERR_BAD_CACHE (-12)     /* code type, block size or strides that the cache operators do not take */
 
 /* device-side status codes written to *status_word */
 #define COROPE_DEV_OK 0
 #define COROPE_DEV_WAIT_EXPIRED 0x1000 /* | barrier id: a bounded mbarrier wait ran out */
 #define COROPE_DEV_RANGE 0x2000        /* a gradient term left the range of the 16-bit Co-RoPE backward and was clamped */
+#define COROPE_DEV_BAD_INDEX 0x4000    /* a block table entry, length or position of a cache operator pointed outside its tensor */
 
 int corope_abi_version(void);
 
@@ -283,6 +285,76 @@ int corope_gqa_bwd_strided(const void* q, const void* k, const void* v, const vo
                            int B, int Hq, int Hkv, int N, int D, int dtype, float sm_scale, float theta,
                            void* workspace, size_t workspace_bytes,
                            int* status_word, void* stream, const corope_strides_t* strides);
+
+/*
+ * ---- Paged key / value cache with 8-bit codes -----------------------------------------------------------------------------
+ *
+ * What generation needs next to the attention above: keys and values of the tokens so far, one byte per element, in blocks of
+ * `block_size` tokens that sequences own through a block table; a code c of block p and head h stands for c * scale[p][h].
+ * No counterpart in the reference, which has no cache; the rotation is that of the fused-RoPE attention (half layout, tables with
+ * columns [0, D/2) read), applied to keys before they are stored and to queries when they are read.
+ *
+ * All index arrays are device memory and are never read on the host.  An entry that points outside its tensor (a block id outside
+ * [0, num_blocks), a length beyond the block table or below 0, a position beyond the tables) is not followed: the tokens concerned are
+ * left out (a position is clamped) and COROPE_DEV_BAD_INDEX is written to the status word.  These kernels run on whatever an earlier kernel left in
+ * the word.  They take fp32 / bf16 / fp16 tensors, hold scores, sums and scales in fp32 and have no backward pass.
+ */
+#define COROPE_CODE_E4M3 0   /* 8-bit floats, largest finite value 448 */
+#define COROPE_CODE_INT8 1   /* whole numbers -127 .. 127 */
+
+typedef struct corope_kv_cache_t {
+    void *k, *v;                   /* codes [num_blocks, Hkv, block_size, D], 16-byte aligned */
+    float *k_scale, *v_scale;      /* [num_blocks, Hkv] contiguous */
+    float* weight;                 /* [num_blocks, Hkv, block_size] contiguous, accumulated attention weight of each slot, or NULL */
+    int64_t k_stride[3], v_stride[3];   /* {block, head, row} in elements, multiples of 16 */
+    int num_blocks, Hkv, block_size, D; /* block_size 16, 32, 64, 128 or 256; D 32, 64 or 128 */
+    int code;                      /* COROPE_CODE_* */
+} corope_kv_cache_t;
+
+typedef struct corope_cache_seqs_t {
+    const int* block_table;        /* [B, max_blocks]: block_table[b * table_stride + i] holds slots i * block_size .. of sequence b */
+    int64_t table_stride;
+    int B, max_blocks;
+    const int* seq_lens;           /* [B] tokens in the cache, those of this call included */
+    const int* new_lens;           /* [B] tokens of this call, at most T, or NULL = T each */
+    const int* positions;          /* [B] position of the first token of this call, or NULL = its slot */
+    const float *cos, *sin;        /* [table_rows, D/2 or more], or NULL = no rotation */
+    int64_t rope_stride;
+    int table_rows;
+} corope_cache_seqs_t;
+
+/*
+ * Stores n = new_lens[b] tokens of k, v [B, Hkv, T, D] (strides {batch, head, row} in elements) in slots seq_lens[b] - n .. of each
+ * sequence, keys rotated; a token whose slot would be negative is left out, slots behind and blocks without a new token stay as they were.
+ *   scale of a block: max(its scale so far, if it holds older tokens; largest |finite new element| * r), r = the fp32 number next to 1/448 or 1/127
+ *   code = x / scale rounded to nearest even, saturated; NaN stays NaN (e4m3) or becomes 0 (int8); a scale of 0 has codes 0
+ * Older codes of a block whose scale grows are written again for the new one.  weight (if any) of the new slots becomes 0.
+ * A block that a token is written to must belong to one sequence only.
+ */
+int corope_cache_append(const corope_kv_cache_t* cache, const corope_cache_seqs_t* seqs, const void* k, const void* v, const int64_t k_strides[3],
+                        const int64_t v_strides[3], int T, int dtype, int* status_word, void* stream);
+
+/*
+ * Attention of q [B, Hq, T, D] over the cache: query t < n of sequence b (its last n tokens) sees slots below
+ * seq_lens[b] - n + t + 1 (causal) or all seq_lens[b].  Query head h reads K / V head h / (Hq / Hkv), any group size.  o [B, Hq, T, D] in
+ * `dtype`; rows without a visible slot and rows t >= n are 0.  accumulate: weight[slot] += the slot's probabilities summed over
+ * the queries and the heads of its group.
+ */
+size_t corope_cache_attn_workspace_bytes(const corope_kv_cache_t* cache, const corope_cache_seqs_t* seqs, int Hq, int T, int dtype, int accumulate);
+int corope_cache_attn(const corope_kv_cache_t* cache, const corope_cache_seqs_t* seqs, const void* q, void* o, const int64_t q_strides[3],
+                      const int64_t o_strides[3], int Hq, int T, int dtype, int causal, float sm_scale, int accumulate, void* workspace,
+                      size_t workspace_bytes, int* status_word, void* stream);
+
+/*
+ * Thins each head's cache to `budget` slots: the last `recent` ones and, of the others, those of largest weight (equal weights: the
+ * lowest slot; NaN counts as the largest).  The slots kept move in order to slots 0 .. of the blocks in out_table [B, out_blocks], weights
+ * too; sequences of at most `budget` tokens move whole.  A new block's scale is the largest scale of the blocks its slots come from: codes of
+ * that scale move bit for bit, the others become code * scale / new scale, rounded.  Reads seq_lens and block_table of `seqs` only;
+ * out_table's blocks belong to one sequence each and to no block_table row of the call; source blocks are not written, they may be shared.
+ *   new_lens [B] = min(seq_lens, budget);  kept [B, Hkv, budget] = the slots kept, ascending, -1 behind them.
+ */
+int corope_cache_evict(const corope_kv_cache_t* cache, const corope_cache_seqs_t* seqs, const int* out_table, int64_t out_table_stride, int out_blocks,
+                       int budget, int recent, int* new_lens, int* kept, int* status_word, void* stream);
 
 #ifdef __cplusplus
 }
