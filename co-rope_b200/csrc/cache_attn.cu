@@ -37,6 +37,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool real) {   // zeros where not real
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
@@ -46,7 +49,13 @@ __device__ __forceinline__ void copy4_async(uint32_t dst, const void* src) {
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// two codes (the low 16 bits of `pair`) as fp16
+template <int WORDS> __device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], int at, uint32_t addr) {   // 1, 2 or 4 words to w[at ..]
+    static_assert(WORDS == 1 || WORDS == 2 || WORDS % 4 == 0, "");
+    if constexpr (WORDS == 1) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[at]) : "r"(addr));
+    else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[at]), "=r"(w[at + 1]) : "r"(addr));
+    else asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[at]), "=r"(w[at + 1]), "=r"(w[at + 2]), "=r"(w[at + 3]) : "r"(addr));
+}
+
 template <int CODE>
 __device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint32_t& hi) {   // four codes: (0, 1), (2, 3)
     if constexpr (CODE == COROPE_CODE_E4M3) {
@@ -212,6 +221,15 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     uint8_t* ring = smem + warp * (kStages * S::kStageBytes);
     float* my_meta = meta + warp * kStages * 4;
     const uint32_t ring_at = smem_u32(ring), meta_at = smem_u32(my_meta);
+    // A stage holds 16 rows of K, then of V; the 16-byte run x of a tile sits at run x ^ (x / 8 % 8), which keeps the reads below off one
+    // another's banks.  Lane's share of a copy: runs lane + 32 i, rows copy_row + kCopyRows i.
+    constexpr int kCopyRows = 512 / D;
+    const int copy_row = lane / (D / 16), copy_col = lane % (D / 16) * 16;
+    const uint32_t copy_to = (uint32_t)(lane ^ (lane >> 3)) * 16;
+    // K: row g, its c-th quarter.  V: row 2 c, its g-th eighth; the row after it and the rows 8 further on are one XOR and one addition away.
+    constexpr uint32_t kNext8Xor = D == 128 ? 0 : D == 64 ? 64 : 32, kNextXor = D == 128 ? 16 : D == 64 ? 64 : 32, kNextAdd = D == 128 ? 128 : 0;
+    const uint32_t k_run = (g * D + c * (D / 4)) / 16, v_run = (2 * c * D + g * (D / 8)) / 16;
+    const uint32_t k_from = (k_run ^ (k_run >> 3 & 7)) * 16 + c * (D / 4) % 16, v_from = (v_run ^ (v_run >> 3 & 7)) * 16 + g * (D / 8) % 16;
 
     while (left > 0) {
         while (off >= (int64_t)l.units * l.items) {
@@ -224,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
         off += u1 - u0;
         left -= u1 - u0;
         const int row0 = tile * kRows, len = l.len, n = l.n;
-        const int least_seen = p.causal ? len - n + row0 / p.G + 1 : len;   // slots below this are seen by every row of the tile that has a query
+        const int least_seen = p.causal ? len - n + row0 / p.G + 1 : len;
 
         __syncthreads();   // the tile before is written out
         pack_queries<D, NT>(p, b, h, row0, len, n, packed, factor, bad);
@@ -232,15 +250,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 
         // columns 2 c, 2 c + 1 of each group of eight rows are this lane's
         float fac[NT][2];
-        int sees[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = 8 * nt + 2 * c + i, t = (row0 + r) / p.G;
-                fac[nt][i] = factor[r];
-                sees[nt][i] = t >= n ? 0 : p.causal ? len - n + t + 1 : len;
-            }
+            for (int i = 0; i < 2; ++i) fac[nt][i] = factor[8 * nt + 2 * c + i];
+        // slots below this are seen by the row, those below least_seen by every row of the tile (rows without a query see what they like)
+        auto sees = [&](int nt, int i) { return p.causal ? len - n + (row0 + 8 * nt + 2 * c + i) / p.G + 1 : len; };
         uint4 qf[NT == 1 ? kKSteps : 1];
         if constexpr (NT == 1) {
 #pragma unroll
@@ -262,42 +277,58 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
         const int first = u0 * kWarps + warp, end = min(u1 * kWarps, (len + kPiece - 1) / kPiece);
         const int count = end > first ? (end - first + kWarps - 1) / kWarps : 0;
         const int* table = p.s.table + (int64_t)b * p.s.table_stride;
-        const int shift = p.c.bs_log2 - 4;
+        const int shift = p.c.bs_log2 - 4, in_block_mask = (1 << p.c.bs_log2) - 1;
+        const uint8_t* k_lane = p.c.k + (int64_t)h * p.c.sk.h + (int64_t)copy_row * p.c.sk.n + copy_col;
+        const uint8_t* v_lane = p.c.v + (int64_t)h * p.c.sv.h + (int64_t)copy_row * p.c.sv.n + copy_col;
+        const float* scale_lane = (lane ? p.c.v_scale : p.c.k_scale) + h;
         int next_page = count > 0 ? table[first >> shift] : 0;
+        uint32_t fill = ring_at;         // stage that the next piece is copied to
+        int fill_stage = 0;
         auto issue = [&](int j) {
             if (j < count) {
-                const int piece = first + j * kWarps, stage = j % kStages;
+                const int piece = first + j * kWarps;
                 const bool found = (unsigned)next_page < (unsigned)p.c.num_blocks;
                 const int page = found ? next_page : 0;
                 bad |= !found;
                 if (j + 1 < count) next_page = table[(piece + kWarps) >> shift];
-                const int in_block = (piece << 4) & ((1 << p.c.bs_log2) - 1), rows = found ? min(len - (piece << 4), kPiece) : 0;
-                const uint8_t* kb = p.c.k + (int64_t)page * p.c.sk.b + (int64_t)h * p.c.sk.h + (int64_t)in_block * p.c.sk.n;
-                const uint8_t* vb = p.c.v + (int64_t)page * p.c.sv.b + (int64_t)h * p.c.sv.h + (int64_t)in_block * p.c.sv.n;
-                const uint32_t dst = ring_at + stage * S::kStageBytes;
+                const int in_block = (piece << 4) & in_block_mask, rows = found ? len - (piece << 4) : 0;
+                const uint8_t* kb = k_lane + (int64_t)page * p.c.sk.b + (int64_t)in_block * p.c.sk.n;
+                const uint8_t* vb = v_lane + (int64_t)page * p.c.sv.b + (int64_t)in_block * p.c.sv.n;
+                const uint32_t dst = fill + copy_to;
+                if (rows >= kPiece) {
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const int x = lane + 32 * i, row = x / (D / 16), col = x % (D / 16) * 16;
-                    const uint32_t to = (uint32_t)(x ^ ((x >> 3) & 7)) * 16;
-                    const bool real = row < rows;
-                    copy16_async(dst + to, kb + (real ? (int64_t)row * p.c.sk.n + col : 0), real);
-                    copy16_async(dst + kPiece * D + to, vb + (real ? (int64_t)row * p.c.sv.n + col : 0), real);
+                    for (int i = 0; i < D / 32; ++i) {
+                        const uint32_t to = (dst ^ (i % 2 * 64)) + 512 * i;
+                        copy16_async(to, kb + (int64_t)i * kCopyRows * p.c.sk.n);
+                        copy16_async(to + kPiece * D, vb + (int64_t)i * kCopyRows * p.c.sv.n);
+                    }
+                } else {   // slots behind the last one become zeros
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const uint32_t to = (dst ^ (i % 2 * 64)) + 512 * i;
+                        const bool real = copy_row + i * kCopyRows < rows;
+                        copy16_async(to, real ? kb + (int64_t)i * kCopyRows * p.c.sk.n : p.c.k, real);
+                        copy16_async(to + kPiece * D, real ? vb + (int64_t)i * kCopyRows * p.c.sv.n : p.c.v, real);
+                    }
                 }
-                if (lane < 2) copy4_async(meta_at + stage * 16 + lane * 4, (lane ? p.c.v_scale : p.c.k_scale) + (int64_t)page * p.c.Hkv + h);
-                if (lane == 2) my_meta[stage * 4 + 2] = found ? 1.f : 0.f;
+                if (lane < 2) copy4_async(meta_at + fill_stage * 16 + lane * 4, scale_lane + (int64_t)page * p.c.Hkv);
+                if (lane == 2) my_meta[fill_stage * 4 + 2] = found ? 1.f : 0.f;
             }
             commit_copies();
+            fill += S::kStageBytes;
+            if (++fill_stage == kStages) fill_stage = 0, fill = ring_at;
         };
 #pragma unroll
         for (int j = 0; j < kStages - 1; ++j) issue(j);
 
+        uint32_t stage_at = ring_at;
+        int stage = 0;
         for (int j = 0; j < count; ++j) {
             issue(j + kStages - 1);   // into the stage that step j - 1 has read
             wait_copies<kStages - 1>();
             __syncwarp();
-            const int stage = j % kStages, slot0 = (first + j * kWarps) * kPiece;
-            const uint8_t* kt = ring + stage * S::kStageBytes;
-            const uint8_t* vt = kt + kPiece * D;
+            const int slot0 = (first + j * kWarps) * kPiece;
+            const uint32_t k_at = stage_at + k_from, v_at = stage_at + kPiece * D + v_from;
             const float k_scale = my_meta[stage * 4], v_scale = my_meta[stage * 4 + 1];
             const bool found = my_meta[stage * 4 + 2] != 0.f;
 
@@ -309,22 +340,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) rest[nt][0] = rest[nt][1] = rest[nt][2] = rest[nt][3] = 0.f;
             uint32_t k0[D / 16], k1[D / 16];
-            auto k_words = [&](int row, uint32_t (&w)[D / 16]) {
-                if constexpr (D == 32) {
-                    const int x = row * 2 + c / 2;
-                    const uint2 u = *reinterpret_cast<const uint2*>(kt + (x ^ ((x >> 3) & 7)) * 16 + c % 2 * 8);
-                    w[0] = u.x; w[1] = u.y;
-                } else {
 #pragma unroll
-                    for (int i = 0; i < D / 64; ++i) {
-                        const int x = row * (D / 16) + c * (D / 64) + i;
-                        const uint4 u = *reinterpret_cast<const uint4*>(kt + (x ^ ((x >> 3) & 7)) * 16);
-                        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
-                    }
-                }
-            };
-            k_words(g, k0);
-            k_words(g + 8, k1);
+            for (int i = 0; i < (D + 63) / 64; ++i) {
+                load_words(k0, 4 * i, k_at ^ (16 * i));
+                load_words(k1, 4 * i, (k_at ^ (16 * i) ^ kNext8Xor) + kPiece * D / 2);
+            }
 #pragma unroll
             for (int w = 0; w < kKSteps; ++w) {
                 uint32_t a[4];
@@ -340,17 +360,24 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 
             // scores in units of log2, the scale of V folded into the exponent: O = sum of exp2(s + log2 v_scale - M) * code
             // (a scale of 0 is left out of the exponent, and its slots out of O)
-            const float v_size = v_scale == 0.f ? 1.f : max_nan(v_scale, 1e-30f), lift = __log2f(v_size), drop = 1.f / v_size, live = v_scale == 0.f ? 0.f : 1.f;
+            const float v_size = v_scale == 0.f ? 1.f : max_nan(v_scale, 1e-30f), lift = __log2f(v_size), drop = __fdividef(1.f, v_size);
             bool higher = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float f0 = fac[nt][0] * k_scale, f1 = fac[nt][1] * k_scale;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[nt][i] = fmaf(s[nt][i] + rest[nt][i], i % 2 ? f1 : f0, lift);
+            }
+            if (!found || slot0 + kPiece > least_seen) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nt][i] = found && slot0 + g + 8 * (i / 2) < sees(nt, i % 2) ? s[nt][i] : -INFINITY;
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int slot = slot0 + g + 8 * (i / 2);
-                    const float x = fmaf(s[nt][i] + rest[nt][i], fac[nt][i % 2] * k_scale, lift);
-                    s[nt][i] = found && slot < sees[nt][i % 2] ? x : -INFINITY;
-                    higher |= s[nt][i] > m[nt][i % 2] + 8.f;
-                }
+                for (int i = 0; i < 2; ++i) higher |= fmaxf(s[nt][i], s[nt][i + 2]) > m[nt][i] + 8.f;
             if (__any_sync(0xffffffffu, higher)) {   // exp2 of up to 8 above M fits fp16: M moves only when a score is beyond that
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -380,13 +407,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    w[2 * i] *= live;
-                    w[2 * i + 1] *= live;
-                    const uint32_t hi = pack_half2(w[2 * i], w[2 * i + 1]);
+                    const uint32_t hi = v_scale == 0.f ? 0u : pack_half2(w[2 * i], w[2 * i + 1]);
                     pb[nt][i] = transpose8x8(hi);
                     if constexpr (EXACT_P) {
                         const float2 back = unpack_half2(hi);
-                        pl[nt][i] = transpose8x8(pack_half2(w[2 * i] - back.x, w[2 * i + 1] - back.y));
+                        pl[nt][i] = transpose8x8(v_scale == 0.f ? 0u : pack_half2(w[2 * i] - back.x, w[2 * i + 1] - back.y));
                     }
                 }
             }
@@ -394,21 +419,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             // O^T: columns g * D / 8 + 2 x and + 1 of V by rows 2 c and 2 c + 1
             uint32_t v[4][kVWords];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 2 * c + i % 2 + 8 * (i / 2);
-                if constexpr (D == 128) {
-                    const int x = row * 8 + g;
-                    const uint4 u = *reinterpret_cast<const uint4*>(vt + (x ^ ((x >> 3) & 7)) * 16);
-                    v[i][0] = u.x; v[i][1] = u.y; v[i][2] = u.z; v[i][3] = u.w;
-                } else if constexpr (D == 64) {
-                    const int x = row * 4 + g / 2;
-                    const uint2 u = *reinterpret_cast<const uint2*>(vt + (x ^ ((x >> 3) & 7)) * 16 + g % 2 * 8);
-                    v[i][0] = u.x; v[i][1] = u.y;
-                } else {
-                    const int x = row * 2 + g / 4;
-                    v[i][0] = *reinterpret_cast<const uint32_t*>(vt + (x ^ ((x >> 3) & 7)) * 16 + g % 4 * 4);
-                }
-            }
+            for (int i = 0; i < 4; ++i)   // slots 2 c, 2 c + 1, and 8 further on
+                load_words(v[i], 0, (v_at ^ (i % 2 * kNextXor) ^ (i / 2 * kNext8Xor)) + i % 2 * kNextAdd + i / 2 * (kPiece * D / 2));
             auto add_values = [&](auto per_slot, int only) {   // only: the one slot of the piece to add, to the rows that see it
                 constexpr bool kPerSlot = decltype(per_slot)::value;
 #pragma unroll
@@ -431,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                                 if constexpr (EXACT_P) mma16816(t, a[y], pl[nt][0], pl[nt][1]);
 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
-                                    if (!kPerSlot || slot0 + only < sees[nt][i % 2]) o[nt][2 * w + y][i] += t[i];
+                                    if (!kPerSlot || slot0 + only < sees(nt, i % 2)) o[nt][2 * w + y][i] += t[i];
                             } else {
                                 mma16816(o[nt][2 * w + y], a[y], pb[nt][0], pb[nt][1]);
                             }
@@ -453,6 +465,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             } else {
                 add_values(std::false_type{}, 0);
             }
+            stage_at += S::kStageBytes;
+            if (++stage == kStages) stage = 0, stage_at = ring_at;
             __syncwarp();   // the stage has been read
         }
         wait_copies<0>();
@@ -505,9 +519,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                 if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (part * kRows + r) * 2) = make_float2(top, all);
             } else if (t < p.T) {
                 const float f = 1.f / all;
-                y = all == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+                y = t >= n || all == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
                 store4(p.o, (int64_t)b * p.so.b + (int64_t)(h * p.G + row - t * p.G) * p.so.h + (int64_t)t * p.so.n + d, p.dtype, p.vec_o, y);
-                if (p.lse != nullptr && d == 0) p.lse[((int64_t)b * p.c.Hkv + h) * p.T * p.G + row] = all == 0.f ? INFINITY : top + log2f(all);
+                if (p.lse != nullptr && d == 0) p.lse[((int64_t)b * p.c.Hkv + h) * p.T * p.G + row] = t >= n || all == 0.f ? INFINITY : top + log2f(all);
             }
         }
     }
@@ -559,7 +573,7 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const Cac
         if (t >= p.T) break;
         float top = kLowest, all = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!empty) {
+        if (!empty && t < l.n) {
             // a part that starts its item is in the second slot of its block, the others are in the first
 #pragma unroll 4
             for (int64_t i = r0; i <= r1; ++i) top = fmaxf(top, p.part_ml[((2 * i + (i == r0 ? 1 : 0)) * rows_per_tile + r) * 2]);
