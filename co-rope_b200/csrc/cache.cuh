@@ -42,6 +42,8 @@ struct CacheAttnParams {
     float* part;                 // partial results: two slots per block of the main kernel
     float* part_ml;              // their maxima and sums
     float* lse;                  // [B, Hkv, T * G] log2 of each row's sum (accumulate only)
+    float* scores;               // [B, Hkv, capacity, score_rows] scores in units of log2, or null (accumulate only)
+    int capacity, score_rows;    // slots of a block table; rows a K / V head, rounded up to even
     int *status, *mirror;
 };
 struct CacheEvictParams {
@@ -101,18 +103,68 @@ __device__ __forceinline__ uint32_t to_code(float x, float scale) {
     if constexpr (CODE == COROPE_CODE_E4M3) return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
     else return (uint32_t)(int)fminf(fmaxf(rintf(y != y ? 0.f : y), -127.f), 127.f) & 0xffu;
 }
+// Four codes of x / scale without a division: x times a reciprocal is within 4 units of 2^-24 of the fp32 quotient; where the numbers 2^-20 below and
+// above it have the same code, that is the quotient's.  The rest (a quotient next to a tie, one in 10^4 numbers; NaN; scales without a usable
+// reciprocal) is divided.  `near` = reciprocal(scale).
+__device__ __forceinline__ float reciprocal(float scale) { return scale > 1e-30f && scale < 1e30f ? __frcp_rn(scale) : __int_as_float(0x7fffffff); }
 template <int CODE>
-__device__ __forceinline__ float from_code(uint32_t byte) {
-    if constexpr (CODE == COROPE_CODE_E4M3) return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
-    else return (float)(int)(int8_t)byte;
+__device__ __forceinline__ bool codes4_near(const float (&y)[4], uint32_t& w) {
+    constexpr float kBelow = 1.f - 0x1p-20f, kAbove = 1.f + 0x1p-20f;
+    if constexpr (CODE == COROPE_CODE_E4M3) {
+        uint16_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float f = i % 2 ? kAbove : kBelow;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r[i]) : "f"(y[i / 2 * 2 + 1] * f), "f"(y[i / 2 * 2] * f));
+        }
+        w = (uint32_t)r[0] | (uint32_t)r[2] << 16;
+        // NaN times anything is NaN: the same code twice, as it should be (a NaN reciprocal is not)
+        return r[0] == r[1] && r[2] == r[3];
+    } else {
+        uint32_t lo[4], off = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {   // rounded to whole numbers by the addition of 1.5 * 2^23
+            lo[i] = __float_as_uint(fminf(fmaxf(y[i] * kBelow, -127.f), 127.f) + 12582912.f);
+            off |= lo[i] ^ __float_as_uint(fminf(fmaxf(y[i] * kAbove, -127.f), 127.f) + 12582912.f);
+            off |= y[i] == y[i] ? 0u : 1u;
+        }
+        w = __byte_perm(__byte_perm(lo[0], lo[1], 0x0040), __byte_perm(lo[2], lo[3], 0x0040), 0x5410);
+        return off == 0;
+    }
+}
+template <int CODE>
+__device__ __forceinline__ uint32_t codes4(const float4& x, float scale, float near) {
+    uint32_t w;
+    const float y[4] = {x.x * near, x.y * near, x.z * near, x.w * near};
+    if (near == near && codes4_near<CODE>(y, w)) return w;
+    return to_code<CODE>(x.x, scale) | to_code<CODE>(x.y, scale) << 8 | to_code<CODE>(x.z, scale) << 16 | to_code<CODE>(x.w, scale) << 24;
+}
+template <int CODE>
+__device__ __forceinline__ void from_codes4(uint32_t w, float (&x)[4]) {
+    if constexpr (CODE == COROPE_CODE_E4M3) {
+        uint32_t a, b;
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
+        const float2 u = unpack_half2(a), v = unpack_half2(b);
+        x[0] = u.x; x[1] = u.y; x[2] = v.x; x[3] = v.y;
+    } else {   // the byte c + 128 as the last digits of 2^23 + 128 + c
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7540 + i)) - 8388736.f;
+    }
 }
 // four codes of scale `old` written for `scale` (different ones)
 template <int CODE>
-__device__ __forceinline__ uint32_t rescale4(uint32_t w, float old, float scale) {
-    uint32_t r = 0;
+__device__ __forceinline__ uint32_t rescale4(uint32_t codes, float old, float scale, float near) {
+    uint32_t w;
+    float x[4], y[4];
+    from_codes4<CODE>(codes, x);
+    const float ratio = old * near;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r |= to_code<CODE>(__fmul_rn(from_code<CODE>((w >> (8 * i)) & 0xffu), old), scale) << (8 * i);
-    return r;
+    for (int i = 0; i < 4; ++i) y[i] = x[i] * ratio;
+    if (near == near && ratio == ratio && codes4_near<CODE>(y, w)) return w;
+    w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= to_code<CODE>(__fmul_rn(x[i], old), scale) << (8 * i);
+    return w;
 }
 // max(a, b), NaN if one of them is
 __device__ __forceinline__ float max_nan(float a, float b) {

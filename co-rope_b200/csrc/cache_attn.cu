@@ -83,15 +83,21 @@ __device__ __forceinline__ Load load_of(const CacheAttnParams& p, int rows_per_t
     l.items = p.c.Hkv * ((l.n * p.G + rows_per_tile - 1) / rows_per_tile);
     return l;
 }
-// Units of the sequences before each thread's share of the batch (thread t has [t * per, (t + 1) * per)) and of all together.
-struct Prefix {
-    int64_t before, total;
+// The range of units that a block of kThreads has, as a place to start (sequence b, `off` units into its own) and a number of units; 0 of
+// them: the block is not needed.  `load(b)` tells a sequence's load.
+struct Range {
+    int b;
+    int64_t off, left;
 };
-__device__ __forceinline__ Prefix prefix_units(const CacheAttnParams& p, int rows_per_tile, int per, int64_t* words, bool& bad) {
+template <typename LoadFn>
+__device__ __forceinline__ Range take_range(int B, const LoadFn& load) {
+    __shared__ int64_t words[kWarps], start_off;
+    __shared__ int start_b;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int per = (B + kThreads - 1) / kThreads, b0 = min((int)threadIdx.x * per, B), b1 = min(b0 + per, B);
     int64_t mine = 0;
-    for (int b = threadIdx.x * per; b < min(p.s.B, (int)(threadIdx.x + 1) * per); ++b) {
-        const Load l = load_of(p, rows_per_tile, b, bad);
+    for (int b = b0; b < b1; ++b) {
+        const Load l = load(b);
         mine += (int64_t)l.units * l.items;
     }
     int64_t sum = mine;
@@ -102,13 +108,24 @@ __device__ __forceinline__ Prefix prefix_units(const CacheAttnParams& p, int row
     }
     if (lane == 31) words[warp] = sum;
     __syncthreads();
-    Prefix r{sum - mine, 0};
+    int64_t at = sum - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) r.before += words[w];
-        r.total += words[w];
+        if (w < warp) at += words[w];
+        total += words[w];
     }
-    return r;
+    const int64_t ranges = min((int64_t)gridDim.x, total);
+    if (blockIdx.x >= ranges) return Range{0, 0, 0};
+    const int64_t lo = total * blockIdx.x / ranges, hi = total * (blockIdx.x + 1) / ranges;
+    if (lo >= at && lo < at + mine)
+        for (int b = b0; b < b1; ++b) {
+            const Load l = load(b);
+            const int64_t u = (int64_t)l.units * l.items;
+            if (lo >= at && lo < at + u) start_b = b, start_off = lo - at;
+            at += u;
+        }
+    __syncthreads();
+    return Range{start_b, start_off, hi - lo};
 }
 
 // ------------------------------------------------------------------------------------------------ queries
@@ -170,7 +187,7 @@ struct Shape {
     static constexpr int kBig = kRing > kJoin ? kRing : kJoin;
     static constexpr int kPacked = D / 16 * NT * 32 * 16;
     static constexpr int kMeta = kWarps * kStages * 16;                     // {k scale, v scale, block found} of each stage
-    static constexpr int kSmem = kBig + kPacked + kMeta + kRows * 4 + 2 * kWarps * kRows * 4 + 64;
+    static constexpr int kSmem = kBig + kPacked + kMeta + kRows * 4 + 2 * kWarps * kRows * 4;
     static constexpr int kBlocks = NT == 1 ? 4 : 2;                         // resident per SM
 };
 
@@ -179,7 +196,7 @@ struct Piece {   // what a block does next: units [u0, u1) of an item
 };
 
 template <int D, int CODE, int NT, bool EXACT_P>
-__global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_kernel(const CacheAttnParams p, int per) {
+__global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_kernel(const CacheAttnParams p) {
     using S = Shape<D, NT>;
     constexpr int kRows = S::kRows, kKSteps = D / 16, kVWords = D / 32, kStages = S::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -188,35 +205,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     float* factor = meta + S::kMeta / 4;
     float* warp_max = factor + kRows;
     float* warp_sum = warp_max + kWarps * kRows;
-    int64_t* words = reinterpret_cast<int64_t*>(smem + S::kSmem - 64);
-    __shared__ int64_t start_off;
-    __shared__ int start_b;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
     bool bad = false;
 
-    // this block's range of units
-    const Prefix pre = prefix_units(p, kRows, per, words, bad);
-    const int64_t total = pre.total;
-    const int64_t ranges = min((int64_t)gridDim.x, total);
+    auto load = [&](int b) { return load_of(p, kRows, b, bad); };
+    Range range = take_range(p.s.B, load);
     pdl_trigger();
-    if (blockIdx.x >= ranges) {
+    if (range.left == 0) {
         if (bad) report_bad_index(p.status, p.mirror);
         return;
     }
-    const int64_t lo = total * blockIdx.x / ranges, hi = total * (blockIdx.x + 1) / ranges;
-    {
-        int64_t at = pre.before;
-        for (int b = threadIdx.x * per; b < min(p.s.B, (int)(threadIdx.x + 1) * per); ++b) {
-            const Load l = load_of(p, kRows, b, bad);
-            const int64_t u = (int64_t)l.units * l.items;
-            if (lo >= at && lo < at + u) start_b = b, start_off = lo - at;
-            at += u;
-        }
-    }
-    __syncthreads();
-    int b = start_b;
-    int64_t off = start_off, left = hi - lo;   // position in sequence b's units, units left
-    Load l = load_of(p, kRows, b, bad);
+    int b = range.b;
+    int64_t off = range.off, left = range.left;   // position in sequence b's units, units left
+    Load l = load(b);
 
     uint8_t* ring = smem + warp * (kStages * S::kStageBytes);
     float* my_meta = meta + warp * kStages * 4;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     while (left > 0) {
         while (off >= (int64_t)l.units * l.items) {
             off -= (int64_t)l.units * l.items;
-            l = load_of(p, kRows, ++b, bad);
+            l = load(++b);
         }
         const int item = (int)(off / l.units), tiles = l.items / p.c.Hkv;
         const int h = item / tiles, tile = item % tiles, u0 = (int)(off - (int64_t)item * l.units);
@@ -242,37 +243,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
         off += u1 - u0;
         left -= u1 - u0;
         const int row0 = tile * kRows, len = l.len, n = l.n;
+        // slots below least_seen are seen by every row of the tile (rows without a query see what they like)
         const int least_seen = p.causal ? len - n + row0 / p.G + 1 : len;
-
         __syncthreads();   // the tile before is written out
-        pack_queries<D, NT>(p, b, h, row0, len, n, packed, factor, bad);
-        __syncthreads();
-
-        // columns 2 c, 2 c + 1 of each group of eight rows are this lane's
-        float fac[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) fac[nt][i] = factor[8 * nt + 2 * c + i];
-        // slots below this are seen by the row, those below least_seen by every row of the tile (rows without a query see what they like)
-        auto sees = [&](int nt, int i) { return p.causal ? len - n + (row0 + 8 * nt + 2 * c + i) / p.G + 1 : len; };
-        uint4 qf[NT == 1 ? kKSteps : 1];
-        if constexpr (NT == 1) {
-#pragma unroll
-            for (int w = 0; w < kKSteps; ++w) qf[w] = reinterpret_cast<const uint4*>(packed)[w * 32 + lane];
-        }
-
-        float o[NT][D / 16][4], m[NT][2], sum[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int x = 0; x < D / 16; ++x)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[nt][x][i] = 0.f;
-            m[nt][0] = m[nt][1] = kLowest;
-            sum[nt][0] = sum[nt][1] = 0.f;
-        }
-
         // pieces first, first + 4, .. of this warp
         const int first = u0 * kWarps + warp, end = min(u1 * kWarps, (len + kPiece - 1) / kPiece);
         const int count = end > first ? (end - first + kWarps - 1) / kWarps : 0;
@@ -319,7 +292,34 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             if (++fill_stage == kStages) fill_stage = 0, fill = ring_at;
         };
 #pragma unroll
-        for (int j = 0; j < kStages - 1; ++j) issue(j);
+        for (int j = 0; j < kStages - 1; ++j) issue(j);   // on their way while the queries are made ready
+
+        pack_queries<D, NT>(p, b, h, row0, len, n, packed, factor, bad);
+        __syncthreads();
+
+        float fac[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) fac[nt][i] = factor[8 * nt + 2 * c + i];
+        // slots below this are seen by the row
+        auto sees = [&](int nt, int i) { return p.causal ? len - n + (row0 + 8 * nt + 2 * c + i) / p.G + 1 : len; };
+        uint4 qf[NT == 1 ? kKSteps : 1];
+        if constexpr (NT == 1) {
+#pragma unroll
+            for (int w = 0; w < kKSteps; ++w) qf[w] = reinterpret_cast<const uint4*>(packed)[w * 32 + lane];
+        }
+
+        float o[NT][D / 16][4], m[NT][2], sum[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nt][x][i] = 0.f;
+            m[nt][0] = m[nt][1] = kLowest;
+            sum[nt][0] = sum[nt][1] = 0.f;
+        }
 
         uint32_t stage_at = ring_at;
         int stage = 0;
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             for (int nt = 0; nt < NT; ++nt) {
                 const float f0 = fac[nt][0] * k_scale, f1 = fac[nt][1] * k_scale;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[nt][i] = fmaf(s[nt][i] + rest[nt][i], i % 2 ? f1 : f0, lift);
+                for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + rest[nt][i]) * (i % 2 ? f1 : f0);
             }
             if (!found || slot0 + kPiece > least_seen) {
 #pragma unroll
@@ -374,6 +374,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[nt][i] = found && slot0 + g + 8 * (i / 2) < sees(nt, i % 2) ? s[nt][i] : -INFINITY;
             }
+            if (p.scores != nullptr) {   // for the weights: whole rows of `score_rows` numbers a slot
+                float* to = p.scores + (((int64_t)b * p.c.Hkv + h) * p.capacity + slot0 + g) * p.score_rows + 2 * c;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    if (8 * nt + 2 * c < p.score_rows) {
+                        if (slot0 + g < len) *reinterpret_cast<float2*>(to + 8 * nt) = make_float2(s[nt][0], s[nt][1]);
+                        if (slot0 + g + 8 < len) *reinterpret_cast<float2*>(to + 8 * p.score_rows + 8 * nt) = make_float2(s[nt][2], s[nt][3]);
+                    }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[nt][i] += lift;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -574,18 +587,29 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const Cac
         float top = kLowest, all = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         if (!empty && t < l.n) {
-            // a part that starts its item is in the second slot of its block, the others are in the first
-#pragma unroll 4
-            for (int64_t i = r0; i <= r1; ++i) top = fmaxf(top, p.part_ml[((2 * i + (i == r0 ? 1 : 0)) * rows_per_tile + r) * 2]);
-#pragma unroll 4
-            for (int64_t i = r0; i <= r1; ++i) {
-                const int64_t at = (2 * i + (i == r0 ? 1 : 0)) * rows_per_tile + r;
-                const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-                const float f = fast_exp2(ml.x - top);
-                all = fmaf(ml.y, f, all);
-                if (lane < D / 4) {
-                    const float4 z = *reinterpret_cast<const float4*>(p.part + at * D + 4 * lane);
-                    y.x = fmaf(z.x, f, y.x); y.y = fmaf(z.y, f, y.y); y.z = fmaf(z.z, f, y.z); y.w = fmaf(z.w, f, y.w);
+            // a part that starts its item is in the second slot of its block, the others are in the first; 32 parts at a time, a lane each
+            for (int64_t base = r0; base <= r1; base += 32) {
+                const int here = (int)min(r1 - base + 1, (int64_t)32);
+                auto row_of = [&](int k) { return (2 * (base + k) + (base + k == r0 ? 1 : 0)) * rows_per_tile + r; };
+                const float2 ml = lane < here ? *reinterpret_cast<const float2*>(p.part_ml + row_of(lane) * 2) : make_float2(kLowest, 0.f);
+                float best = ml.x;
+#pragma unroll
+                for (int m = 16; m; m >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, m));
+                best = fmaxf(best, top);
+                const float shrink = fast_exp2(top - best), f = lane < here ? fast_exp2(ml.x - best) : 0.f;
+                top = best;
+                float add = ml.y * f;
+#pragma unroll
+                for (int m = 16; m; m >>= 1) add += __shfl_xor_sync(0xffffffffu, add, m);
+                all = fmaf(all, shrink, add);
+                y = make_float4(y.x * shrink, y.y * shrink, y.z * shrink, y.w * shrink);
+#pragma unroll 8
+                for (int k = 0; k < here; ++k) {
+                    const float fk = __shfl_sync(0xffffffffu, f, k);
+                    if (lane < D / 4) {
+                        const float4 z = *reinterpret_cast<const float4*>(p.part + row_of(k) * D + 4 * lane);
+                        y.x = fmaf(z.x, fk, y.x); y.y = fmaf(z.y, fk, y.y); y.z = fmaf(z.z, fk, y.z); y.w = fmaf(z.w, fk, y.w);
+                    }
                 }
             }
         }
@@ -598,15 +622,65 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const Cac
 }
 
 // ------------------------------------------------------------------------------------------------ accumulated weights
-// weight[slot] += sum over rows of exp2(s - lse).  The scores are formed again, K being read once more: the same division into units, but a
+// Few query rows (one tile): the main kernel has left the scores, 4 bytes a row and slot, and a thread sums a slot's exp2(s - lse).  K is not read
+// again, which would be D bytes a slot and all of its products.
+constexpr int kSumUnit = kThreads;
+template <bool FOURS>
+__global__ void __launch_bounds__(kThreads) cache_attn_sum_kernel(const CacheAttnParams p) {
+    bool bad = false;
+    auto load = [&](int b) {
+        Load l = load_of(p, 1, b, bad);
+        l.units = (l.len + kSumUnit - 1) / kSumUnit;
+        l.items = l.n > 0 ? p.c.Hkv : 0;
+        return l;
+    };
+    const Range range = take_range(p.s.B, load);
+    pdl_wait();
+    if (range.left == 0) return;
+    int b = range.b;
+    int64_t off = range.off;
+    Load l = load(b);
+    for (int64_t left = range.left; left > 0; --left, ++off) {
+        while (off >= (int64_t)l.units * l.items) {
+            off -= (int64_t)l.units * l.items;
+            l = load(++b);
+        }
+        const int h = (int)(off / l.units), slot = (int)(off - (int64_t)h * l.units) * kSumUnit + threadIdx.x;
+        if (slot >= l.len) continue;
+        const int page = cache_page(p.s, p.c.bs_log2, p.c.num_blocks, b, slot, bad), rows = l.n * p.G;
+        const int64_t bh = (int64_t)b * p.c.Hkv + h;
+        const float* s = p.scores + (bh * p.capacity + slot) * p.score_rows;
+        const float* lse = p.lse + bh * p.T * p.G;
+        float w = 0.f;
+        if constexpr (FOURS) {
+#pragma unroll 2
+            for (int r = 0; r < rows; r += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(s + r);
+                w += fast_exp2(x.x - lse[r]);
+                if (r + 1 < rows) w += fast_exp2(x.y - lse[r + 1]);
+                if (r + 2 < rows) w += fast_exp2(x.z - lse[r + 2]);
+                if (r + 3 < rows) w += fast_exp2(x.w - lse[r + 3]);
+            }
+        } else {
+            for (int r = 0; r < rows; r += 2) {
+                const float2 x = *reinterpret_cast<const float2*>(s + r);
+                w += fast_exp2(x.x - lse[r]);
+                if (r + 1 < rows) w += fast_exp2(x.y - lse[r + 1]);
+            }
+        }
+        // one addition per slot and call; atomic because sequences may share blocks
+        if (page >= 0) atomicAdd(p.c.weight + (((int64_t)page * p.c.Hkv + h) << p.c.bs_log2) + (slot & ((1 << p.c.bs_log2) - 1)), w);
+    }
+    if (bad) report_bad_index(p.status, p.mirror);
+}
+
+// Many rows, or no room for the scores: weight[slot] += sum over rows of exp2(s - lse).  The scores are formed again, K being read once more: the same division into units, but a
 // unit's block goes through all tiles of query rows, so that each slot's sum is one addition in a fixed order.
 template <int D, int CODE, int NT>
-__global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const CacheAttnParams p, int per) {
+__global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const CacheAttnParams p) {
     constexpr int kRows = 8 * NT, kKSteps = D / 16;
     __shared__ __align__(16) uint32_t packed[Shape<D, NT>::kPacked / 4];
     __shared__ float factor[kRows], lse[kRows];
-    __shared__ int64_t words[kWarps], start_off;
-    __shared__ int start_b;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
     bool bad = false;
     auto load = [&](int b) {
@@ -614,39 +688,12 @@ __global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const Cache
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     };   // items of this kernel: K / V heads
-    int64_t mine = 0;
-    for (int b = threadIdx.x * per; b < min(p.s.B, (int)(threadIdx.x + 1) * per); ++b) {
-        const Load l = load(b);
-        mine += (int64_t)l.units * l.items;
-    }
-    int64_t sum = mine;
-#pragma unroll
-    for (int m = 1; m < 32; m *= 2) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, sum, m);
-        if (lane >= m) sum += up;
-    }
-    if (lane == 31) words[warp] = sum;
-    __syncthreads();
-    int64_t at = sum - mine, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) at += words[w];
-        total += words[w];
-    }
-    const int64_t ranges = min((int64_t)gridDim.x, total);
-    if (blockIdx.x >= ranges) return;
-    const int64_t lo = total * blockIdx.x / ranges, hi = total * (blockIdx.x + 1) / ranges;
-    for (int b = threadIdx.x * per; b < min(p.s.B, (int)(threadIdx.x + 1) * per); ++b) {
-        const Load l = load(b);
-        const int64_t u = (int64_t)l.units * l.items;
-        if (lo >= at && lo < at + u) start_b = b, start_off = lo - at;
-        at += u;
-    }
-    __syncthreads();
-    int b = start_b, had = -1;
-    int64_t off = start_off;
+    const Range range = take_range(p.s.B, load);
+    if (range.left == 0) return;
+    int b = range.b, had = -1;
+    int64_t off = range.off;
     Load l = load(b);
-    for (int64_t left = hi - lo; left > 0; --left, ++off) {
+    for (int64_t left = range.left; left > 0; --left, ++off) {
         while (off >= (int64_t)l.units * l.items) {
             off -= (int64_t)l.units * l.items;
             l = load(++b);
@@ -743,24 +790,24 @@ unsigned main_blocks(int B, int Hkv, int row_tiles, int max_blocks, int block_si
 }
 
 template <int D, int CODE, int NT, bool EXACT_P>
-int launch_main(const CacheAttnParams& p, unsigned blocks, int per, cudaStream_t s) {
+int launch_main(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     if (int e = allow_smem(cache_attn_kernel<D, CODE, NT, EXACT_P>, Shape<D, NT>::kSmem, done)) return e;
     count_launch();
-    cache_attn_kernel<D, CODE, NT, EXACT_P><<<blocks, kThreads, Shape<D, NT>::kSmem, s>>>(p, per);
+    cache_attn_kernel<D, CODE, NT, EXACT_P><<<blocks, kThreads, Shape<D, NT>::kSmem, s>>>(p);
     return (int)cudaGetLastError();
 }
 template <int D, int CODE, int NT>
 int launch_all(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
-    const int per = (p.s.B + kThreads - 1) / kThreads;
-    if (int e = p.dtype == COROPE_DTYPE_F32 ? launch_main<D, CODE, NT, true>(p, blocks, per, s) : launch_main<D, CODE, NT, false>(p, blocks, per, s)) return e;
+    if (int e = p.dtype == COROPE_DTYPE_F32 ? launch_main<D, CODE, NT, true>(p, blocks, s) : launch_main<D, CODE, NT, false>(p, blocks, s)) return e;
     count_launch();
     if (int e = launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles), kJoinThreads, 0, s, p, 8 * NT, (int)blocks)) return e;
     if (!p.accumulate) return COROPE_OK;
     count_launch();
-    const uint64_t units = (uint64_t)p.s.B * p.c.Hkv * ((((uint64_t)p.s.max_blocks << p.c.bs_log2) + kUnit - 1) / kUnit);
-    const uint64_t most = (uint64_t)sm_count() * 8;
-    cache_attn_weight_kernel<D, CODE, NT><<<(unsigned)(units < most ? units : most), kThreads, 0, s>>>(p, per);
+    const uint64_t units = (uint64_t)p.s.B * p.c.Hkv * ((uint64_t)(p.capacity + kUnit - 1) / kUnit), most = (uint64_t)sm_count() * 8;
+    const unsigned grid = (unsigned)(units < most ? units : most);
+    if (p.scores != nullptr) return launch_dependent(p.score_rows % 4 == 0 ? cache_attn_sum_kernel<true> : cache_attn_sum_kernel<false>, grid, kThreads, 0, s, p);
+    cache_attn_weight_kernel<D, CODE, NT><<<grid, kThreads, 0, s>>>(p);
     return (int)cudaGetLastError();
 }
 template <int D, int CODE>
@@ -775,7 +822,8 @@ int by_code(const CacheAttnParams& p, int groups, unsigned blocks, cudaStream_t 
 struct Layout {
     int groups, row_tiles;
     unsigned blocks;
-    size_t part_ml, lse, total;   // the parts themselves come first
+    int score_rows;               // numbers a slot in `scores`, 0 = the scores are formed again
+    size_t part_ml, lse, scores, total;   // the parts themselves come first
 };
 Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_size, int accumulate) {
     Layout l{};
@@ -786,7 +834,12 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     const size_t part_rows = (size_t)2 * l.blocks * 8 * l.groups;
     l.part_ml = align_up(part_rows * D * 4, 256);
     l.lse = l.part_ml + align_up(part_rows * 8, 256);
-    l.total = l.lse + (accumulate ? align_up((size_t)B * Hkv * rows * 4, 256) : 0);
+    l.scores = l.lse + (accumulate ? align_up((size_t)B * Hkv * rows * 4, 256) : 0);
+    // Room for the scores of every slot that the block tables could hold.  Beyond half a gigabyte (long tables that the sequences may not fill) K is
+    // read again instead: 32 sequences of up to 8192 tokens, 4 rows a head, take SUMUS us with the scores, 148 without.
+    const size_t bytes = (size_t)B * Hkv * max_blocks * block_size * ((rows + 1) / 2 * 2) * 4;
+    l.score_rows = accumulate && l.row_tiles == 1 && bytes <= (512u << 20) ? (rows + 1) / 2 * 2 : 0;
+    l.total = l.scores + (l.score_rows ? align_up(bytes, 256) : 0);
     return l;
 }
 
@@ -803,6 +856,9 @@ int launch_cache_attn(CacheAttnParams p, void* ws, cudaStream_t s) {
     p.part = static_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + l.part_ml);
     p.lse = p.accumulate ? reinterpret_cast<float*>(static_cast<char*>(ws) + l.lse) : nullptr;
+    p.capacity = p.s.max_blocks << p.c.bs_log2;
+    p.score_rows = l.score_rows;
+    p.scores = l.score_rows ? reinterpret_cast<float*>(static_cast<char*>(ws) + l.scores) : nullptr;
     p.vec_o = rows_in_fours(p.o, p.so, p.dtype);
     return p.D == 128 ? by_code<128>(p, l.groups, l.blocks, s) : p.D == 64 ? by_code<64>(p, l.groups, l.blocks, s) : by_code<32>(p, l.groups, l.blocks, s);
 }
