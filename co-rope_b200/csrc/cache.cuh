@@ -103,41 +103,44 @@ __device__ __forceinline__ uint32_t to_code(float x, float scale) {
     if constexpr (CODE == COROPE_CODE_E4M3) return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
     else return (uint32_t)(int)fminf(fmaxf(rintf(y != y ? 0.f : y), -127.f), 127.f) & 0xffu;
 }
-// Four codes of x / scale without a division: x times a reciprocal is within 4 units of 2^-24 of the fp32 quotient; where the numbers 2^-20 below and
-// above it have the same code, that is the quotient's.  The rest (a quotient next to a tie, one in 10^4 numbers; NaN; scales without a usable
-// reciprocal) is divided.  `near` = reciprocal(scale).
+// Four codes of x / scale without a division.  x times a reciprocal is within 4 units of 2^-24 of the fp32 quotient, so it has the quotient's code
+// unless a tie lies that near (one number in 10^4): then, and where the scale has no usable reciprocal, all four are divided.
+// `near` = reciprocal(scale); |x| <= (1 + 2^-22) * scale * largest code, or `plain` is false.
 __device__ __forceinline__ float reciprocal(float scale) { return scale > 1e-30f && scale < 1e30f ? __frcp_rn(scale) : __int_as_float(0x7fffffff); }
 template <int CODE>
+__device__ __noinline__ uint32_t divided4(float a, float b, float c, float d, float scale) {
+    return to_code<CODE>(a, scale) | to_code<CODE>(b, scale) << 8 | to_code<CODE>(c, scale) << 16 | to_code<CODE>(d, scale) << 24;
+}
+template <int CODE>
 __device__ __forceinline__ bool codes4_near(const float (&y)[4], uint32_t& w) {
-    constexpr float kBelow = 1.f - 0x1p-20f, kAbove = 1.f + 0x1p-20f;
-    if constexpr (CODE == COROPE_CODE_E4M3) {
+    if constexpr (CODE == COROPE_CODE_E4M3) {   // the numbers 2^-20 below and above have the same code
+        constexpr float kBelow = 1.f - 0x1p-20f, kAbove = 1.f + 0x1p-20f;
         uint16_t r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float f = i % 2 ? kAbove : kBelow;
             asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r[i]) : "f"(y[i / 2 * 2 + 1] * f), "f"(y[i / 2 * 2] * f));
         }
-        w = (uint32_t)r[0] | (uint32_t)r[2] << 16;
-        // NaN times anything is NaN: the same code twice, as it should be (a NaN reciprocal is not)
-        return r[0] == r[1] && r[2] == r[3];
-    } else {
-        uint32_t lo[4], off = 0;
+        const uint32_t lo = (uint32_t)r[0] | (uint32_t)r[2] << 16, hi = (uint32_t)r[1] | (uint32_t)r[3] << 16;
+        w = lo;
+        return lo == hi;
+    } else {   // rounded by the addition of 1.5 * 2^23, and not within 2^-12 of a tie (2^-24 * 4 * 127 = 2^-15)
+        float r[4], off = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {   // rounded to whole numbers by the addition of 1.5 * 2^23
-            lo[i] = __float_as_uint(fminf(fmaxf(y[i] * kBelow, -127.f), 127.f) + 12582912.f);
-            off |= lo[i] ^ __float_as_uint(fminf(fmaxf(y[i] * kAbove, -127.f), 127.f) + 12582912.f);
-            off |= y[i] == y[i] ? 0u : 1u;
+        for (int i = 0; i < 4; ++i) {
+            r[i] = y[i] + 12582912.f;
+            off = fmaxf(off, fabsf(y[i] - (r[i] - 12582912.f)));
         }
-        w = __byte_perm(__byte_perm(lo[0], lo[1], 0x0040), __byte_perm(lo[2], lo[3], 0x0040), 0x5410);
-        return off == 0;
+        w = __byte_perm(__byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040), __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040), 0x5410);
+        return off < 0.5f - 0x1p-12f;
     }
 }
 template <int CODE>
-__device__ __forceinline__ uint32_t codes4(const float4& x, float scale, float near) {
+__device__ __forceinline__ uint32_t codes4(const float4& x, float scale, float near, bool plain) {
     uint32_t w;
     const float y[4] = {x.x * near, x.y * near, x.z * near, x.w * near};
-    if (near == near && codes4_near<CODE>(y, w)) return w;
-    return to_code<CODE>(x.x, scale) | to_code<CODE>(x.y, scale) << 8 | to_code<CODE>(x.z, scale) << 16 | to_code<CODE>(x.w, scale) << 24;
+    if (codes4_near<CODE>(y, w) && plain) return w;
+    return divided4<CODE>(x.x, x.y, x.z, x.w, scale);
 }
 template <int CODE>
 __device__ __forceinline__ void from_codes4(uint32_t w, float (&x)[4]) {
@@ -151,20 +154,18 @@ __device__ __forceinline__ void from_codes4(uint32_t w, float (&x)[4]) {
         for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7540 + i)) - 8388736.f;
     }
 }
-// four codes of scale `old` written for `scale` (different ones)
+// four codes of scale `old` written for a larger `scale`
 template <int CODE>
 __device__ __forceinline__ uint32_t rescale4(uint32_t codes, float old, float scale, float near) {
+    const bool plain = near == near && old < scale;   // not NaN, either
     uint32_t w;
     float x[4], y[4];
     from_codes4<CODE>(codes, x);
     const float ratio = old * near;
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = x[i] * ratio;
-    if (near == near && ratio == ratio && codes4_near<CODE>(y, w)) return w;
-    w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w |= to_code<CODE>(__fmul_rn(x[i], old), scale) << (8 * i);
-    return w;
+    if (codes4_near<CODE>(y, w) && plain) return w;
+    return divided4<CODE>(__fmul_rn(x[0], old), __fmul_rn(x[1], old), __fmul_rn(x[2], old), __fmul_rn(x[3], old), scale);
 }
 // max(a, b), NaN if one of them is
 __device__ __forceinline__ float max_nan(float a, float b) {

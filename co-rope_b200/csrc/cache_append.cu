@@ -8,7 +8,6 @@ namespace corope {
 namespace {
 
 constexpr int kSteps = 4;        // rows a thread holds
-constexpr int kMostThreads = 1024;
 
 // x1' = x1 c - x2 s, x2' = x2 c + x1 s, each operation rounded by itself: the codes are those of that formula in fp32
 __device__ __forceinline__ void rotate4(float4& a, float4& b, const float4& c, const float4& s) {
@@ -19,7 +18,29 @@ __device__ __forceinline__ void rotate4(float4& a, float4& b, const float4& c, c
                     __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w)));
 }
 __device__ __forceinline__ float finite_abs(float x) { return fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.f; }
-__device__ __forceinline__ float amax4(const float4& a) { return fmaxf(fmaxf(finite_abs(a.x), finite_abs(a.y)), fmaxf(finite_abs(a.z), finite_abs(a.w))); }
+__device__ __forceinline__ float finite_amax4(const float4& a) { return fmaxf(fmaxf(finite_abs(a.x), finite_abs(a.y)), fmaxf(finite_abs(a.z), finite_abs(a.w))); }
+// max(top, |a|), infinite or NaN if an element is
+__device__ __forceinline__ float amax4(float top, const float4& a) { return fmax3_nan(fmax3_nan(top, fabsf(a.x), fabsf(a.y)), fabsf(a.z), fabsf(a.w)); }
+
+// four elements as they are stored
+template <bool WIDE> struct Raw;
+template <> struct Raw<true> {
+    float4 x;
+    __device__ __forceinline__ void load(const void* base, int64_t i, int dtype, bool vec) { x = load4(base, i, dtype, vec); }
+    __device__ __forceinline__ float4 get(int) const { return x; }
+};
+template <> struct Raw<false> {
+    uint2 x;
+    __device__ __forceinline__ void load(const void* base, int64_t i, int, bool vec) {
+        const uint16_t* from = static_cast<const uint16_t*>(base) + i;
+        if (vec) x = *reinterpret_cast<const uint2*>(from);
+        else x = make_uint2((uint32_t)from[0] | (uint32_t)from[1] << 16, (uint32_t)from[2] | (uint32_t)from[3] << 16);
+    }
+    __device__ __forceinline__ float4 get(int dtype) const {
+        const float2 a = dtype == COROPE_DTYPE_BF16 ? unpack_bf162(x.x) : unpack_half2(x.x), b = dtype == COROPE_DTYPE_BF16 ? unpack_bf162(x.y) : unpack_half2(x.y);
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+};
 
 // largest value of the thread block, in every thread; `words`: 32 floats, a different array for each use
 __device__ __forceinline__ float block_max(float x, float* words) {
@@ -33,8 +54,9 @@ __device__ __forceinline__ float block_max(float x, float* words) {
     return x;
 }
 
-template <int CODE>
-__global__ void __launch_bounds__(kMostThreads) cache_append_kernel(const CacheAppendParams p, int touched, int per_row_log2, bool vec_k, bool vec_v, bool vec_t) {
+// WIDE: fp32 rows.  MOST: threads of the largest block launched.
+template <int CODE, bool WIDE, int MOST>
+__global__ void __launch_bounds__(MOST) cache_append_kernel(const CacheAppendParams p, int touched, int per_row_log2, bool vec_k, bool vec_v, bool vec_t) {
     __shared__ float words[2][32];
     const unsigned item = blockIdx.x / (unsigned)touched;
     const int j = (int)(blockIdx.x - item * (unsigned)touched), b = (int)(item / (unsigned)p.c.Hkv), h = (int)(item - (unsigned)b * (unsigned)p.c.Hkv);
@@ -51,39 +73,51 @@ __global__ void __launch_bounds__(kMostThreads) cache_append_kernel(const CacheA
     if (page < 0) return;
     bad = false;
 
+    // all of the thread's rows are on their way before the first is looked at
+    Raw<WIDE> raw[2][kSteps][2];
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int slot = lo + g + i * groups;
+            if (slot >= hi) continue;
+            const Strides st = part ? p.sv : p.sk;
+            const int64_t from = (int64_t)b * st.b + (int64_t)h * st.h + (int64_t)(slot - first) * st.n + d;
+            raw[part][i][0].load(part ? p.v : p.k, from, p.dtype, part ? vec_v : vec_k);
+            raw[part][i][1].load(part ? p.v : p.k, from + half, p.dtype, part ? vec_v : vec_k);
+        }
     const int64_t at = (int64_t)page * p.c.Hkv + h;
     const int held = lo - base;                                       // older tokens of the block
 #pragma unroll
     for (int part = 0; part < 2; ++part) {                            // keys, values
-        const void* src = part ? p.v : p.k;
-        const Strides st = part ? p.sv : p.sk;
         const Strides sc = part ? p.c.sv : p.c.sk;
-        const bool vec = part ? vec_v : vec_k;
         uint8_t* to = (part ? p.c.v : p.c.k) + (int64_t)page * sc.b + (int64_t)h * sc.h + d;
         float* scale_at = (part ? p.c.v_scale : p.c.k_scale) + at;
         const float old = held ? *scale_at : 0.f;
-        const int64_t from = (int64_t)b * st.b + (int64_t)h * st.h + d;
         float4 x1[kSteps], x2[kSteps];
         float top = 0.f;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const int slot = lo + g + i * groups;
-            if (slot >= hi) break;
-            x1[i] = load4(src, from + (int64_t)(slot - first) * st.n, p.dtype, vec);
-            x2[i] = load4(src, from + (int64_t)(slot - first) * st.n + half, p.dtype, vec);
-        }
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const int slot = lo + g + i * groups;
-            if (slot >= hi) break;
+            if (slot >= hi) continue;
+            x1[i] = raw[part][i][0].get(p.dtype);
+            x2[i] = raw[part][i][1].get(p.dtype);
             if (part == 0 && p.s.cos != nullptr) {
                 const int64_t row = (int64_t)cache_position(p.s, b, slot - first, slot, bad) * p.s.rope_stride + d;
                 rotate4(x1[i], x2[i], load4(p.s.cos, row, COROPE_DTYPE_F32, vec_t), load4(p.s.sin, row, COROPE_DTYPE_F32, vec_t));
             }
-            top = fmaxf(top, fmaxf(amax4(x1[i]), amax4(x2[i])));
+            top = amax4(amax4(top, x1[i]), x2[i]);
+        }
+        const bool finite = top <= 3.402823466e38f;
+        if (!finite) {
+            top = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                if (lo + g + i * groups < hi) top = fmaxf(top, fmaxf(finite_amax4(x1[i]), finite_amax4(x2[i])));
         }
         top = block_max(top, words[part]);                            // (every thread has read the old scale)
         const float scale = max_nan(old, __fmul_rn(top, kPerCode<CODE>)), near = reciprocal(scale);
+        const bool plain = finite && near == near;
         if (threadIdx.x == 0) *scale_at = scale;
         if (held && scale != old)
             for (int r = g; r < held; r += groups) {
@@ -94,13 +128,23 @@ __global__ void __launch_bounds__(kMostThreads) cache_append_kernel(const CacheA
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const int slot = lo + g + i * groups;
-            if (slot >= hi) break;
-            *reinterpret_cast<uint32_t*>(to + (int64_t)(slot - base) * sc.n) = codes4<CODE>(x1[i], scale, near);
-            *reinterpret_cast<uint32_t*>(to + (int64_t)(slot - base) * sc.n + half) = codes4<CODE>(x2[i], scale, near);
+            if (slot >= hi) continue;
+            *reinterpret_cast<uint32_t*>(to + (int64_t)(slot - base) * sc.n) = codes4<CODE>(x1[i], scale, near, plain);
+            *reinterpret_cast<uint32_t*>(to + (int64_t)(slot - base) * sc.n + half) = codes4<CODE>(x2[i], scale, near, plain);
             if (part && p.c.weight != nullptr && d == 0) p.c.weight[(at << p.c.bs_log2) + slot - base] = 0.f;
         }
     }
     if (bad) report_bad_index(p.status, p.mirror);
+}
+
+template <int CODE, bool WIDE>
+int launch_t(const CacheAppendParams& p, unsigned blocks, int threads, int touched, int per_row_log2, cudaStream_t s) {
+    const bool vec_k = rows_in_fours(p.k, p.sk, p.dtype), vec_v = rows_in_fours(p.v, p.sv, p.dtype);
+    const bool vec_t = (uintptr_t)p.s.cos % 16 == 0 && (uintptr_t)p.s.sin % 16 == 0 && p.s.rope_stride % 4 == 0;
+    count_launch();
+    if (threads <= 512) cache_append_kernel<CODE, WIDE, 512><<<blocks, threads, 0, s>>>(p, touched, per_row_log2, vec_k, vec_v, vec_t);
+    else cache_append_kernel<CODE, WIDE, 1024><<<blocks, threads, 0, s>>>(p, touched, per_row_log2, vec_k, vec_v, vec_t);
+    return (int)cudaGetLastError();
 }
 
 }  // namespace
@@ -109,16 +153,16 @@ int launch_cache_append(const CacheAppendParams& p, cudaStream_t s) {
     const int bs = 1 << p.c.bs_log2, touched = (p.T + bs - 2) / bs + 1;
     const uint64_t blocks = (uint64_t)p.s.B * p.c.Hkv * touched;
     if (blocks >= (1ull << 31)) return COROPE_ERR_TOO_LARGE;
-    const bool vec_k = rows_in_fours(p.k, p.sk, p.dtype), vec_v = rows_in_fours(p.v, p.sv, p.dtype);
-    const bool vec_t = (uintptr_t)p.s.cos % 16 == 0 && (uintptr_t)p.s.sin % 16 == 0 && p.s.rope_stride % 4 == 0;
-    // a thread for every four elements of kSteps rows: 4 * 256 rows of 16 threads are the most
+    // a thread for every four elements of kSteps rows: 1024 for 256 rows of 16 threads, the most there are
     const int per_row_log2 = p.D == 128 ? 4 : p.D == 64 ? 3 : 2, rows = p.T < bs ? p.T : bs;
     int threads = 64;
     while (threads * kSteps < rows << per_row_log2) threads *= 2;
-    count_launch();
-    if (p.code == COROPE_CODE_E4M3) cache_append_kernel<COROPE_CODE_E4M3><<<(unsigned)blocks, threads, 0, s>>>(p, touched, per_row_log2, vec_k, vec_v, vec_t);
-    else cache_append_kernel<COROPE_CODE_INT8><<<(unsigned)blocks, threads, 0, s>>>(p, touched, per_row_log2, vec_k, vec_v, vec_t);
-    return (int)cudaGetLastError();
+    const bool wide = p.dtype == COROPE_DTYPE_F32;
+    if (p.code == COROPE_CODE_E4M3)
+        return wide ? launch_t<COROPE_CODE_E4M3, true>(p, (unsigned)blocks, threads, touched, per_row_log2, s)
+                    : launch_t<COROPE_CODE_E4M3, false>(p, (unsigned)blocks, threads, touched, per_row_log2, s);
+    return wide ? launch_t<COROPE_CODE_INT8, true>(p, (unsigned)blocks, threads, touched, per_row_log2, s)
+                : launch_t<COROPE_CODE_INT8, false>(p, (unsigned)blocks, threads, touched, per_row_log2, s);
 }
 
 }  // namespace corope
