@@ -25,7 +25,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "corope_b200.h")
 DEBUG_HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "corope_b200_debug.h")
 
 SOURCES = ["abi.cu", "rope_general.cu", "rope_fp32.cu", "rope_split.cu", "rope_split_fwd_sm100.cu", "rope_split_bwd_sm100.cu", "rope_split_prepass.cu", "rope_prepass.cu", "rope_fwd_sm100.cu", "rope_bwd_sm100.cu", "corope_general.cu", "corope_fwd_mma.cu", "corope_fwd_split.cu", "corope_bwd_mma.cu", "noalloc.cu",
-           "debug.cu", "cache_abi.cu", "cache_append.cu", "cache_attn.cu", "cache_evict.cu"]
+           "debug.cu", "cache_abi.cu", "cache_append.cu", "cache_attn.cu", "cache_attn_tile.cu", "cache_evict.cu"]
 
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 OP_ROPE_FWD, OP_ROPE_BWD, OP_GQA_FWD, OP_GQA_BWD = 0, 1, 2, 3
@@ -72,7 +72,7 @@ def _build_native(force):
 def build(force=False, verbose=False):
     """Compile csrc/*.cu into libcorope_b200.so for sm_100a (cross-compiles without a GPU) and the extension module beside it."""
     srcs = [os.path.join(_CSRC, s) for s in SOURCES]
-    deps = srcs + [os.path.join(_CSRC, "common.cuh"), os.path.join(_CSRC, "corope_mma.cuh"), os.path.join(_CSRC, "rope_split.cuh"), os.path.join(_CSRC, "cache.cuh"), HEADER_PATH, DEBUG_HEADER_PATH]
+    deps = srcs + [os.path.join(_CSRC, "common.cuh"), os.path.join(_CSRC, "corope_mma.cuh"), os.path.join(_CSRC, "rope_split.cuh"), os.path.join(_CSRC, "cache.cuh"), os.path.join(_CSRC, "cache_attn.cuh"), HEADER_PATH, DEBUG_HEADER_PATH]
     if not force and _newer(LIB_PATH, deps):
         _build_native(force)
         return LIB_PATH

@@ -17,7 +17,7 @@
 
 #include <type_traits>
 
-#include "cache.cuh"
+#include "cache_attn.cuh"
 
 namespace corope {
 namespace {
@@ -25,7 +25,6 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kPiece = 16;                    // slots per step of a warp; a block of the cache holds a whole number of them
 constexpr int kUnit = kWarps * kPiece;        // slots per unit of work
-constexpr float kLowest = -1e30f;             // running maximum before any score: finite, so that differences from it are no NaN
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -54,78 +53,6 @@ template <int WORDS> __device__ __forceinline__ void load_words(uint32_t (&w)[WO
     if constexpr (WORDS == 1) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[at]) : "r"(addr));
     else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[at]), "=r"(w[at + 1]) : "r"(addr));
     else asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[at]), "=r"(w[at + 1]), "=r"(w[at + 2]), "=r"(w[at + 3]) : "r"(addr));
-}
-
-template <int CODE>
-__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint32_t& hi) {   // four codes: (0, 1), (2, 3)
-    if constexpr (CODE == COROPE_CODE_E4M3) {
-        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(word));
-    } else {   // the byte c + 128 behind the fp16 exponent of 1024 reads as 1024 + 128 + c
-        const uint32_t u = word ^ 0x80808080u, bias = 0x64806480u;
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
-        const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&bias));
-        lo = *reinterpret_cast<const uint32_t*>(&x);
-        hi = *reinterpret_cast<const uint32_t*>(&y);
-    }
-}
-
-// ------------------------------------------------------------------------------------------------ division of the work
-// Sequence b contributes items(b) = Hkv * (row tiles in use) items of units(b) units each.
-struct Load {
-    int len, n, units, items;
-};
-__device__ __forceinline__ Load load_of(const CacheAttnParams& p, int rows_per_tile, int b, bool& bad) {
-    Load l;
-    l.len = cache_len(p.s, p.c.bs_log2, b, bad);
-    l.n = cache_new(p.s, p.T, b, bad);
-    l.units = (l.len + kUnit - 1) / kUnit;
-    l.items = p.c.Hkv * ((l.n * p.G + rows_per_tile - 1) / rows_per_tile);
-    return l;
-}
-// The range of units that a block of kThreads has, as a place to start (sequence b, `off` units into its own) and a number of units; 0 of
-// them: the block is not needed.  `load(b)` tells a sequence's load.
-struct Range {
-    int b;
-    int64_t off, left;
-};
-template <typename LoadFn>
-__device__ __forceinline__ Range take_range(int B, const LoadFn& load) {
-    __shared__ int64_t words[kWarps], start_off;
-    __shared__ int start_b;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int per = (B + kThreads - 1) / kThreads, b0 = min((int)threadIdx.x * per, B), b1 = min(b0 + per, B);
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) {
-        const Load l = load(b);
-        mine += (int64_t)l.units * l.items;
-    }
-    int64_t sum = mine;
-#pragma unroll
-    for (int m = 1; m < 32; m *= 2) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, sum, m);
-        if (lane >= m) sum += up;
-    }
-    if (lane == 31) words[warp] = sum;
-    __syncthreads();
-    int64_t at = sum - mine, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) at += words[w];
-        total += words[w];
-    }
-    const int64_t ranges = min((int64_t)gridDim.x, total);
-    if (blockIdx.x >= ranges) return Range{0, 0, 0};
-    const int64_t lo = total * blockIdx.x / ranges, hi = total * (blockIdx.x + 1) / ranges;
-    if (lo >= at && lo < at + mine)
-        for (int b = b0; b < b1; ++b) {
-            const Load l = load(b);
-            const int64_t u = (int64_t)l.units * l.items;
-            if (lo >= at && lo < at + u) start_b = b, start_off = lo - at;
-            at += u;
-        }
-    __syncthreads();
-    return Range{start_b, start_off, hi - lo};
 }
 
 // ------------------------------------------------------------------------------------------------ queries
@@ -208,8 +135,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
     bool bad = false;
 
-    auto load = [&](int b) { return load_of(p, kRows, b, bad); };
-    Range range = take_range(p.s.B, load);
+    auto load = [&](int b) { return load_of(p, kRows, kUnit, b, bad); };
+    Range range = take_range<kThreads>(p.s.B, load);
     pdl_trigger();
     if (range.left == 0) {
         if (bad) report_bad_index(p.status, p.mirror);
@@ -546,14 +473,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 // added in the order of their ranges.  Rows that no unit stands for are written here: 0.
 constexpr int kJoinThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const CacheAttnParams p, int rows_per_tile, int main_blocks) {
+__global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const CacheAttnParams p, int rows_per_tile, int unit, int main_blocks) {
     __shared__ int64_t words[2][kJoinThreads / 32];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int tile = (int)(blockIdx.x % (unsigned)p.row_tiles), bh = (int)(blockIdx.x / (unsigned)p.row_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
     bool bad = false;
     int64_t before = 0, total = 0;
     for (int i = threadIdx.x; i < p.s.B; i += kJoinThreads) {
-        const Load l = load_of(p, rows_per_tile, i, bad);
+        const Load l = load_of(p, rows_per_tile, unit, i, bad);
         const int64_t u = (int64_t)l.units * l.items;
         total += u;
         if (i < b) before += u;
@@ -569,7 +496,7 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const Cac
 #pragma unroll
     for (int w = 0; w < kJoinThreads / 32; ++w) before += words[0][w], total += words[1][w];
 
-    const Load l = load_of(p, rows_per_tile, b, bad);
+    const Load l = load_of(p, rows_per_tile, unit, b, bad);
     const int tiles = l.items / p.c.Hkv;
     const bool empty = l.units == 0 || tile >= tiles;
     const int64_t ranges = min((int64_t)main_blocks, total);
@@ -629,12 +556,11 @@ template <bool FOURS>
 __global__ void __launch_bounds__(kThreads) cache_attn_sum_kernel(const CacheAttnParams p) {
     bool bad = false;
     auto load = [&](int b) {
-        Load l = load_of(p, 1, b, bad);
-        l.units = (l.len + kSumUnit - 1) / kSumUnit;
+        Load l = load_of(p, 1, kSumUnit, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     };
-    const Range range = take_range(p.s.B, load);
+    const Range range = take_range<kThreads>(p.s.B, load);
     pdl_wait();
     if (range.left == 0) return;
     int b = range.b;
@@ -684,11 +610,11 @@ __global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const Cache
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
     bool bad = false;
     auto load = [&](int b) {
-        Load l = load_of(p, kRows, b, bad);
+        Load l = load_of(p, kRows, kUnit, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     };   // items of this kernel: K / V heads
-    const Range range = take_range(p.s.B, load);
+    const Range range = take_range<kThreads>(p.s.B, load);
     if (range.left == 0) return;
     int b = range.b, had = -1;
     int64_t off = range.off;
@@ -783,12 +709,47 @@ __global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const Cache
 // rows of a tile by the number of query rows: 8 (one N extent of the MMA), 16 or 32
 int row_groups(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 int resident_blocks(int groups) { return groups == 1 ? 4 : 2; }
-unsigned main_blocks(int B, int Hkv, int row_tiles, int max_blocks, int block_size, int groups) {
-    const uint64_t units = (uint64_t)B * Hkv * row_tiles * (((uint64_t)max_blocks * block_size + kUnit - 1) / kUnit);
-    const uint64_t most = (uint64_t)sm_count() * resident_blocks(groups);
-    return (unsigned)(units < most ? units : most);
+// How a call is done and where its workspace's parts lie (the parts of joined sums come first).
+struct Layout {
+    bool tiles, two_parts;        // tcgen05 kernels; queries in two fp16 parts
+    int groups, row_tiles, rows_per_tile;
+    unsigned blocks;
+    int score_rows;               // numbers a slot in `scores`, 0 = the scores are formed again
+    size_t part_ml, lse, scores, images, total;
+};
+Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_size, int dtype, int accumulate) {
+    Layout l{};
+    const int rows = G * T;
+    const uint64_t slots = (uint64_t)max_blocks * block_size;
+    // 16-bit tensors of more than 32 rows a head: products on tcgen05 (a chunk of 1024 queries, 32 / 8 heads, over 9001 tokens: CHUNKUS us, 970 with
+    // tiles of 32 rows).  fp32 tensors stay with the kernel that splits P as well.
+    l.tiles = dtype != COROPE_DTYPE_F32 && rows > 32;
+    // one part of q is off by 2^-12 of it: next to a bf16 result's 2^-9 that is nothing, an fp16 result or a weight would feel it
+    l.two_parts = l.tiles && (dtype == COROPE_DTYPE_F16 || accumulate);
+    l.groups = row_groups(rows);
+    l.rows_per_tile = l.tiles ? kTileRows : 8 * l.groups;
+    l.row_tiles = (rows + l.rows_per_tile - 1) / l.rows_per_tile;
+    const uint64_t items = (uint64_t)B * Hkv * l.row_tiles, unit = l.tiles ? kTileRows : kUnit;
+    const uint64_t units = items * ((slots + unit - 1) / unit), most = (uint64_t)sm_count() * (l.tiles ? 1 : resident_blocks(l.groups));
+    l.blocks = (unsigned)(units < most ? units : most);
+    const size_t part_rows = (size_t)2 * l.blocks * l.rows_per_tile;
+    l.part_ml = align_up(part_rows * D * 4, 256);
+    l.lse = l.part_ml + align_up(part_rows * 8, 256);
+    l.scores = l.lse + (accumulate ? align_up((size_t)B * Hkv * rows * 4, 256) : 0);
+    // Room for the scores of every slot that the block tables could hold.  Beyond half a gigabyte (long tables that the sequences may not fill) K is
+    // read again instead: 32 sequences of up to 8192 tokens, 4 rows a head, take 88 us with the scores, 148 without.
+    const size_t bytes = (size_t)B * Hkv * slots * ((rows + 1) / 2 * 2) * 4;
+    l.score_rows = accumulate && !l.tiles && l.row_tiles == 1 && bytes <= (512u << 20) ? (rows + 1) / 2 * 2 : 0;
+    l.images = l.scores + (l.score_rows ? align_up(bytes, 256) : 0);
+    l.total = l.images + (l.tiles ? cache_tile_workspace_bytes(B, Hkv, l.row_tiles, D, l.two_parts) : 0);
+    return l;
 }
 
+template <int D>
+int launch_join(const CacheAttnParams& p, const Layout& l, int unit, cudaStream_t s) {
+    count_launch();
+    return launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles), kJoinThreads, 0, s, p, l.rows_per_tile, unit, (int)l.blocks);
+}
 template <int D, int CODE, int NT, bool EXACT_P>
 int launch_main(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
@@ -798,10 +759,9 @@ int launch_main(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
     return (int)cudaGetLastError();
 }
 template <int D, int CODE, int NT>
-int launch_all(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
-    if (int e = p.dtype == COROPE_DTYPE_F32 ? launch_main<D, CODE, NT, true>(p, blocks, s) : launch_main<D, CODE, NT, false>(p, blocks, s)) return e;
-    count_launch();
-    if (int e = launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles), kJoinThreads, 0, s, p, 8 * NT, (int)blocks)) return e;
+int launch_rows(const CacheAttnParams& p, const Layout& l, cudaStream_t s) {
+    if (int e = p.dtype == COROPE_DTYPE_F32 ? launch_main<D, CODE, NT, true>(p, l.blocks, s) : launch_main<D, CODE, NT, false>(p, l.blocks, s)) return e;
+    if (int e = launch_join<D>(p, l, kUnit, s)) return e;
     if (!p.accumulate) return COROPE_OK;
     count_launch();
     const uint64_t units = (uint64_t)p.s.B * p.c.Hkv * ((uint64_t)(p.capacity + kUnit - 1) / kUnit), most = (uint64_t)sm_count() * 8;
@@ -811,56 +771,36 @@ int launch_all(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
     return (int)cudaGetLastError();
 }
 template <int D, int CODE>
-int by_rows(const CacheAttnParams& p, int groups, unsigned blocks, cudaStream_t s) {
-    return groups == 1 ? launch_all<D, CODE, 1>(p, blocks, s) : groups == 2 ? launch_all<D, CODE, 2>(p, blocks, s) : launch_all<D, CODE, 4>(p, blocks, s);
+int by_rows(const CacheAttnParams& p, const Layout& l, cudaStream_t s) {
+    return l.groups == 1 ? launch_rows<D, CODE, 1>(p, l, s) : l.groups == 2 ? launch_rows<D, CODE, 2>(p, l, s) : launch_rows<D, CODE, 4>(p, l, s);
 }
 template <int D>
-int by_code(const CacheAttnParams& p, int groups, unsigned blocks, cudaStream_t s) {
-    return p.code == COROPE_CODE_E4M3 ? by_rows<D, COROPE_CODE_E4M3>(p, groups, blocks, s) : by_rows<D, COROPE_CODE_INT8>(p, groups, blocks, s);
-}
-
-struct Layout {
-    int groups, row_tiles;
-    unsigned blocks;
-    int score_rows;               // numbers a slot in `scores`, 0 = the scores are formed again
-    size_t part_ml, lse, scores, total;   // the parts themselves come first
-};
-Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_size, int accumulate) {
-    Layout l{};
-    const int rows = G * T;
-    l.groups = row_groups(rows);
-    l.row_tiles = (rows + 8 * l.groups - 1) / (8 * l.groups);
-    l.blocks = main_blocks(B, Hkv, l.row_tiles, max_blocks, block_size, l.groups);
-    const size_t part_rows = (size_t)2 * l.blocks * 8 * l.groups;
-    l.part_ml = align_up(part_rows * D * 4, 256);
-    l.lse = l.part_ml + align_up(part_rows * 8, 256);
-    l.scores = l.lse + (accumulate ? align_up((size_t)B * Hkv * rows * 4, 256) : 0);
-    // Room for the scores of every slot that the block tables could hold.  Beyond half a gigabyte (long tables that the sequences may not fill) K is
-    // read again instead: 32 sequences of up to 8192 tokens, 4 rows a head, take SUMUS us with the scores, 148 without.
-    const size_t bytes = (size_t)B * Hkv * max_blocks * block_size * ((rows + 1) / 2 * 2) * 4;
-    l.score_rows = accumulate && l.row_tiles == 1 && bytes <= (512u << 20) ? (rows + 1) / 2 * 2 : 0;
-    l.total = l.scores + (l.score_rows ? align_up(bytes, 256) : 0);
-    return l;
+int by_kernel(const CacheAttnParams& p, const Layout& l, void* images, cudaStream_t s) {
+    if (!l.tiles) return p.code == COROPE_CODE_E4M3 ? by_rows<D, COROPE_CODE_E4M3>(p, l, s) : by_rows<D, COROPE_CODE_INT8>(p, l, s);
+    if (int e = launch_cache_attn_tiles(p, images, l.two_parts, l.blocks, s)) return e;
+    if (int e = launch_join<D>(p, l, kTileRows, s)) return e;
+    return p.accumulate ? launch_cache_weight_tiles(p, images, s) : COROPE_OK;
 }
 
 }  // namespace
 
 size_t cache_attn_workspace_bytes(int B, int Hkv, int G, int T, int D, int max_blocks, int block_size, int dtype, int accumulate) {
-    (void)dtype;
-    return layout_of(B, Hkv, G, T, D, max_blocks, block_size, accumulate).total;
+    return layout_of(B, Hkv, G, T, D, max_blocks, block_size, dtype, accumulate).total;
 }
 
 int launch_cache_attn(CacheAttnParams p, void* ws, cudaStream_t s) {
-    const Layout l = layout_of(p.s.B, p.c.Hkv, p.G, p.T, p.D, p.s.max_blocks, 1 << p.c.bs_log2, p.accumulate);
+    const Layout l = layout_of(p.s.B, p.c.Hkv, p.G, p.T, p.D, p.s.max_blocks, 1 << p.c.bs_log2, p.dtype, p.accumulate);
+    auto part = [&](size_t at) { return reinterpret_cast<float*>(static_cast<char*>(ws) + at); };
     p.row_tiles = l.row_tiles;
-    p.part = static_cast<float*>(ws);
-    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + l.part_ml);
-    p.lse = p.accumulate ? reinterpret_cast<float*>(static_cast<char*>(ws) + l.lse) : nullptr;
+    p.part = part(0);
+    p.part_ml = part(l.part_ml);
+    p.lse = p.accumulate ? part(l.lse) : nullptr;
     p.capacity = p.s.max_blocks << p.c.bs_log2;
     p.score_rows = l.score_rows;
-    p.scores = l.score_rows ? reinterpret_cast<float*>(static_cast<char*>(ws) + l.scores) : nullptr;
+    p.scores = l.score_rows ? part(l.scores) : nullptr;
     p.vec_o = rows_in_fours(p.o, p.so, p.dtype);
-    return p.D == 128 ? by_code<128>(p, l.groups, l.blocks, s) : p.D == 64 ? by_code<64>(p, l.groups, l.blocks, s) : by_code<32>(p, l.groups, l.blocks, s);
+    void* images = part(l.images);
+    return p.D == 128 ? by_kernel<128>(p, l, images, s) : p.D == 64 ? by_kernel<64>(p, l, images, s) : by_kernel<32>(p, l, images, s);
 }
 
 }  // namespace corope

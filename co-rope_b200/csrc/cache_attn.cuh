@@ -1,0 +1,93 @@
+// What the kernels of corope_cache_attn share: codes as fp16, and the division of a batch's work among blocks.
+#pragma once
+#include "cache.cuh"
+
+namespace corope {
+
+#ifdef __CUDACC__
+constexpr float kLowest = -1e30f;             // running maximum before any score: finite, so that differences from it are no NaN
+
+// four codes as fp16: (0, 1), (2, 3)
+template <int CODE>
+__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint32_t& hi) {
+    if constexpr (CODE == COROPE_CODE_E4M3) {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(word));
+    } else {   // the byte c + 128 behind the fp16 exponent of 1024 reads as 1024 + 128 + c
+        const uint32_t u = word ^ 0x80808080u, bias = 0x64806480u;
+        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
+        const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&bias));
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ division of the work
+// Work is counted in units of `unit` slots of one item, a (K / V head, tile of query rows) of a sequence: sequence b has items(b) = Hkv * (row tiles in
+// use) items of units(b) units each, one after the other.
+struct Load {
+    int len, n, units, items;
+};
+__device__ __forceinline__ Load load_of(const CacheAttnParams& p, int rows_per_tile, int unit, int b, bool& bad) {
+    Load l;
+    l.len = cache_len(p.s, p.c.bs_log2, b, bad);
+    l.n = cache_new(p.s, p.T, b, bad);
+    l.units = (l.len + unit - 1) / unit;
+    l.items = p.c.Hkv * ((l.n * p.G + rows_per_tile - 1) / rows_per_tile);
+    return l;
+}
+// The range of units that a block has (its first THREADS threads look at the sequences), as a place to start (sequence b, `off` units into its own) and a number of units; 0 of
+// them: the block is not needed.  `load(b)` tells a sequence's load.
+struct Range {
+    int b;
+    int64_t off, left;
+};
+template <int THREADS, typename LoadFn>
+__device__ __forceinline__ Range take_range(int B, const LoadFn& load) {
+    constexpr int kWarps = THREADS / 32;
+    __shared__ int64_t words[kWarps], start_off;
+    __shared__ int start_b;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int per = (B + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * per, B), b1 = min(b0 + per, B);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        const Load l = load(b);
+        mine += (int64_t)l.units * l.items;
+    }
+    int64_t sum = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, sum, m);
+        if (lane >= m) sum += up;
+    }
+    if (lane == 31 && warp < kWarps) words[warp] = sum;
+    __syncthreads();
+    int64_t at = sum - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) at += words[w];
+        total += words[w];
+    }
+    const int64_t ranges = min((int64_t)gridDim.x, total);
+    if (blockIdx.x >= ranges) return Range{0, 0, 0};
+    const int64_t lo = total * blockIdx.x / ranges, hi = total * (blockIdx.x + 1) / ranges;
+    if (lo >= at && lo < at + mine)
+        for (int b = b0; b < b1; ++b) {
+            const Load l = load(b);
+            const int64_t u = (int64_t)l.units * l.items;
+            if (lo >= at && lo < at + u) start_b = b, start_off = lo - at;
+            at += u;
+        }
+    __syncthreads();
+    return Range{start_b, start_off, hi - lo};
+}
+
+#endif  // __CUDACC__
+
+// Attention of many query rows a K / V head on tcgen05 (16-bit types): the steps of launch_cache_attn that are its own.
+constexpr int kTileRows = 128;                // query rows, and slots of a unit
+size_t cache_tile_workspace_bytes(int B, int Hkv, int row_tiles, int D, bool two_parts);
+int launch_cache_attn_tiles(const CacheAttnParams& p, void* ws, bool two_parts, unsigned blocks, cudaStream_t s);
+int launch_cache_weight_tiles(const CacheAttnParams& p, void* ws, cudaStream_t s);
+
+}  // namespace corope

@@ -1,0 +1,917 @@
+// corope_cache_attn for many query rows a K / V head (R = G * T > 32, 16-bit types): tcgen05 MMAs on codes turned into fp16 in shared memory.
+//
+// A unit of work is 128 query rows by 128 slots; a block per SM takes a contiguous range of a batch's units (see cache_attn.cuh) and walks it
+// piece by piece, a piece being units of one tile of rows.  Warp roles (896 threads, registers divided again with setmaxnreg):
+//   warp 0        brings a piece's query tile (an image of its place in shared memory that a pre-pass has written) with bulk copies
+//   warp 2        MMA issuer and TMEM owner
+//   warps 4-7     K: loads 16 codes a lane, turns them into fp16 (exact) and stores them as the MMA wants them;  warps 8-11: V likewise
+//   warps 12-19   softmax of the even units of a piece, two threads a row (64 slots each);  warps 20-27: of the odd ones
+// TMEM: S0 [0,128) S1 [128,256) O0 [256,384) O1 [384,512); P (fp16) goes over S.  Even and odd units have sums of their own, so one group's
+// exponentials run beside the other's MMAs, and are joined when the piece is written.
+// Scales: a block of 16 slots or more has one scale of K, which multiplies the scores of its columns in fp32, and one of V, which enters the
+// exponent: P = exp2(s + log2 v_scale - M), and its sum is taken back to probabilities by the same number.
+// Queries are scaled by a power of two per row and rounded to fp16 (11 bits); with two parts (fp16 tensors, and where weights are gathered) the
+// remainder of the rounding is a second operand and scores have 22 bits.
+// Bound by the exponentials (16 a clock and SM: 1024 clocks a unit at least) and, next to that, by the MMAs (2 * 128^3 * 2 operations, 3 with two parts).
+#include "cache_attn.cuh"
+
+namespace corope {
+namespace {
+
+constexpr int kN = kTileRows;
+constexpr int kThreads = 896;
+constexpr int kMmaWarp = 2, kConvWarp0 = 4, kSmxWarp0 = 12;
+constexpr int kLaunchRegs = 72, kRegsCtl = 40, kRegsConv = 56, kRegsSmx = 88;
+static_assert(128 * (kRegsCtl + 2 * kRegsConv + 4 * kRegsSmx) <= kThreads * kLaunchRegs, "register budget");
+constexpr int kStages = 2;                    // of K and of V
+constexpr int kScaleSlots = 4;                // units whose scales are kept: one more than can be under way
+constexpr int kFlagSlots = 8;                 // pieces whose flag is kept
+
+enum Bar { Q_FULL = 0, Q_EMPTY, K_FULL, K_EMPTY = K_FULL + kStages, V_FULL = K_EMPTY + kStages, V_EMPTY = V_FULL + kStages, S_FULL = V_EMPTY + kStages,
+           P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, O_FREE = O_FULL + 2, NUM_BARS };
+
+// shared memory of head dimension D (32 is widened to 64 with zeros)
+__host__ __device__ constexpr int wide(int D) { return D == 128 ? 128 : 64; }
+__host__ __device__ constexpr size_t tile_bytes(int D) { return (size_t)kN * wide(D) * 2; }
+struct Small {
+    float k_scale[kScaleSlots][8], lift[kScaleSlots][8], drop[kScaleSlots][8];   // of each 16 slots
+    float half_max[2][2][kN];                 // exchanged between the two threads of a row
+    float end_max[2][2][kN], end_sum[2][2][2][kN];   // [piece % 2][group][half]
+    uint64_t bars[NUM_BARS];
+    int nan_v[kFlagSlots];                    // a piece has NaN in V where some rows must not see it
+    uint32_t tmem;
+    int abort;
+};
+constexpr size_t smem_bytes(int D, bool two) { return ((two ? 2 : 1) + 2 * kStages) * tile_bytes(D) + sizeof(Small) + 1024; }
+static_assert(smem_bytes(128, true) <= 232448 - 1024, "shared memory budget");
+
+// ------------------------------------------------------------------------------------------------ pieces
+struct Piece {
+    int b, h, tile, u0, u1, live;   // units [u0, u1) of the item, of which those below `live` have a slot that a row of the tile sees
+    int len, n, units;
+};
+struct Walk {
+    Range r;
+    Load l;
+    bool bad = false;
+    __device__ __forceinline__ Walk(const CacheAttnParams& p, const Range& range) : r(range) { l = load_of(p, kN, kN, r.b, bad); }
+    __device__ __forceinline__ bool next(const CacheAttnParams& p, Piece& x) {
+        if (r.left <= 0) return false;
+        while (r.off >= (int64_t)l.units * l.items) {
+            r.off -= (int64_t)l.units * l.items;
+            l = load_of(p, kN, kN, ++r.b, bad);
+        }
+        const int item = (int)(r.off / l.units), tiles = l.items / p.c.Hkv;
+        x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles;
+        x.u0 = (int)(r.off - (int64_t)item * l.units);
+        x.u1 = (int)min((int64_t)l.units, x.u0 + r.left);
+        x.len = l.len; x.n = l.n; x.units = l.units;
+        const int last = min(l.n - 1, (x.tile * kN + kN - 1) / p.G);      // the tile's last query
+        const int most = p.causal ? max(l.len - l.n + last + 1, 0) : l.len;
+        x.live = min((most + kN - 1) / kN, x.u1);
+        r.off += x.u1 - x.u0;
+        r.left -= x.u1 - x.u0;
+        return true;
+    }
+};
+__device__ __forceinline__ int least_seen(const CacheAttnParams& p, const Piece& x) { return p.causal ? x.len - x.n + x.tile * kN / p.G + 1 : x.len; }
+
+// byte offset of 16-byte run `run` (8 elements) of row r in the image of a tile: boxes of 64 columns, 128-byte swizzle
+__device__ __forceinline__ uint32_t image_at(int r, int run) { return (uint32_t)((run >> 3) * (kN * 128) + r * 128 + (((run & 7) ^ (r & 7)) << 4)); }
+
+__device__ __forceinline__ void store16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ queries
+// One block per (K / V head, tile of rows): rotates, scales and rounds the rows, and writes them as images of the tile.
+template <int D, bool TWO>
+__global__ void __launch_bounds__(256) cache_pack_kernel(const CacheAttnParams p, uint8_t* images, float* factors) {
+    constexpr int kHalf = D / 2, kPairs = kHalf / 2;
+    const int tile = (int)(blockIdx.x % (unsigned)p.row_tiles), bh = (int)(blockIdx.x / (unsigned)p.row_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    bool bad = false;
+    const int len = cache_len(p.s, p.c.bs_log2, b, bad), n = cache_new(p.s, p.T, b, bad);
+    uint8_t* image = images + (size_t)blockIdx.x * (TWO ? 2 : 1) * tile_bytes(D);
+    for (int r = warp; r < kN; r += 8) {
+        const int row = tile * kN + r, t = row / p.G;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};   // columns 2 lane, + 1, and their partners D / 2 further on
+        if (t < n && lane < kPairs) {
+            const int64_t at = (int64_t)b * p.sq.b + (int64_t)(h * p.G + row - t * p.G) * p.sq.h + (int64_t)t * p.sq.n + 2 * lane;
+            x[0] = load1(p.q, at, p.dtype); x[1] = load1(p.q, at + 1, p.dtype);
+            x[2] = load1(p.q, at + kHalf, p.dtype); x[3] = load1(p.q, at + kHalf + 1, p.dtype);
+            if (p.s.cos != nullptr) {
+                const int64_t tr = (int64_t)cache_position(p.s, b, t, len - n + t, bad) * p.s.rope_stride + 2 * lane;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float c = p.s.cos[tr + i], s = p.s.sin[tr + i], u = x[i], v = x[i + 2];
+                    x[i] = u * c - v * s;
+                    x[i + 2] = v * c + u * s;
+                }
+            }
+        }
+        float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+        for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+        const bool usual = m >= 1e-30f && m <= 1e30f;   // to [2^10, 2^11), see pack_queries of the kernel for few rows
+        const int e = usual ? (int)(__float_as_uint(m) >> 23) - 127 - 10 : 0;
+        const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
+        if (lane == 0) factors[(size_t)blockIdx.x * kN + r] = down * p.scale;
+        if (lane < kPairs) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int d = 2 * lane + i * kHalf;
+                const uint32_t at = image_at(r, d / 8) + d % 8 * 2;
+                const float u = x[2 * i] * up, v = x[2 * i + 1] * up;
+                const uint32_t hi = pack_half2(u, v);
+                *reinterpret_cast<uint32_t*>(image + at) = hi;
+                if (TWO) {
+                    const float2 back = unpack_half2(hi);
+                    *reinterpret_cast<uint32_t*>(image + tile_bytes(D) + at) = pack_half2(u - back.x, v - back.y);
+                }
+            }
+        }
+        if (D == 32 && lane < 16) {   // columns 32 .. 63
+            const uint32_t at = image_at(r, 4 + lane / 4) + lane % 4 * 4;
+            *reinterpret_cast<uint32_t*>(image + at) = 0u;
+            if (TWO) *reinterpret_cast<uint32_t*>(image + tile_bytes(D) + at) = 0u;
+        }
+    }
+    if (bad) report_bad_index(p.status, p.mirror);
+}
+
+// ------------------------------------------------------------------------------------------------ codes to operands
+// What one group of 128 threads keeps of a unit's 128 slots: lane l < 8 the block (or -1) of slots 16 l .. 16 l + 15.
+template <int D>
+struct Codes {
+    static constexpr int kLanes = D / 16, kRowsPerStep = 128 / kLanes, kSteps = kN / kRowsPerStep, kHalf = kSteps / 2;
+    uint4 x[2][kHalf];
+};
+template <typename X>
+__device__ __forceinline__ int unit_page(const CacheAttnParams& p, const X& x, int u, int lane, bool& bad) {
+    const int slot = u * kN + 16 * lane;
+    return lane < 8 && slot < x.len ? cache_page(p.s, p.c.bs_log2, p.c.num_blocks, x.b, slot, bad) : -1;
+}
+template <int D>
+__device__ __forceinline__ void load_half(Codes<D>& c, int half, const uint8_t* base, const Strides& st, const CacheAttnParams& p, const Piece& x, int u, int page, int tid) {
+    using C = Codes<D>;
+    const int rs = tid / C::kLanes, col = tid % C::kLanes * 16;
+#pragma unroll
+    for (int i = 0; i < C::kHalf; ++i) {
+        const int row = (half * C::kHalf + i) * C::kRowsPerStep + rs, pg = __shfl_sync(0xffffffffu, page, row >> 4);
+        c.x[half][i] = make_uint4(0u, 0u, 0u, 0u);
+        if (pg >= 0 && u * kN + row < x.len)
+            c.x[half][i] = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)pg * st.b + (int64_t)x.h * st.h + (int64_t)((u * kN + row) & ((1 << p.c.bs_log2) - 1)) * st.n + col));
+    }
+}
+__device__ __forceinline__ bool has_nan(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~__vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
+
+template <int D, int CODE>
+__device__ __forceinline__ void store_half(const Codes<D>& c, int half, uint32_t tile, int tid) {
+    using C = Codes<D>;
+    const int rs = tid / C::kLanes, u = tid % C::kLanes;
+    // Eight lanes that store at one time have to reach eight different runs of a 128-byte line: at D = 128 the lanes of the second box
+    // begin with their second run.
+    const int swap = D == 128 ? u >> 2 : 0;
+#pragma unroll
+    for (int i = 0; i < C::kHalf; ++i) {
+        const int row = (half * C::kHalf + i) * C::kRowsPerStep + rs;
+        const uint4 w = c.x[half][i];
+        uint32_t h[8];
+        codes_to_half<CODE>(swap ? w.z : w.x, h[0], h[1]);
+        codes_to_half<CODE>(swap ? w.w : w.y, h[2], h[3]);
+        codes_to_half<CODE>(swap ? w.x : w.z, h[4], h[5]);
+        codes_to_half<CODE>(swap ? w.y : w.w, h[6], h[7]);
+        store16(tile + image_at(row, 2 * u + swap), h[0], h[1], h[2], h[3]);
+        store16(tile + image_at(row, 2 * u + 1 - swap), h[4], h[5], h[6], h[7]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ main kernel
+template <int D, int CODE, bool TWO>
+__global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const CacheAttnParams p, const uint8_t* images, const float* factors) {
+    constexpr int kD = wide(D), kBox = kN * 128, kParts = TWO ? 2 : 1;
+    constexpr uint32_t kTile = (uint32_t)tile_bytes(D);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sQ = sm;
+    uint8_t* sK = sQ + kParts * kTile;
+    uint8_t* sV = sK + kStages * kTile;
+    Small& z = *reinterpret_cast<Small*>(sV + kStages * kTile);
+    uint64_t* bars = z.bars;
+    volatile int* abort_flag = &z.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    bool bad = false;
+    const Range range = take_range<128>(p.s.B, [&](int b) { return load_of(p, kN, kN, b, bad); });
+    pdl_trigger();
+    if (bad) report_bad_index(p.status, p.mirror);
+    // after a wait that ran out, in this launch's block or in an earlier launch, none starts anew until the host has seen it
+    const bool gave_up = p.status != nullptr && (*reinterpret_cast<volatile int*>(p.status) & COROPE_DEV_WAIT_EXPIRED);
+    if (__syncthreads_or(gave_up) || range.left == 0) {
+        if (threadIdx.x == 0 && gave_up) report_to_mirror(p.status, p.mirror);
+        pdl_wait();   // no launch ends before the one in front of it
+        return;
+    }
+    if (threadIdx.x == 0) {
+        z.abort = 0;
+        for (int i = 0; i < kFlagSlots; ++i) z.nan_v[i] = 0;
+        mbar_init(&bars[Q_FULL], 1);
+        mbar_init(&bars[Q_EMPTY], 1);
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&bars[K_FULL + i], 4);
+            mbar_init(&bars[K_EMPTY + i], 1);
+            mbar_init(&bars[V_FULL + i], 4);
+            mbar_init(&bars[V_EMPTY + i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars[S_FULL + i], 1);
+            mbar_init(&bars[P_FULL + i], 8);
+            mbar_init(&bars[O_FULL + i], 1);
+        }
+        mbar_init(&bars[O_FREE], 16);
+        fence_mbar_init();
+    }
+    if (D == 32)   // columns 32 .. 63 of K and V are never written
+        for (int i = threadIdx.x; i < (int)(2 * kStages * kTile / 16); i += kThreads) reinterpret_cast<uint4*>(sK)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tmem_alloc(&z.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = z.tmem;
+    Piece x;
+
+    if (warp < kConvWarp0) {
+        reg_dealloc<kRegsCtl>();
+        if (warp == 0) {
+            // -------------------------------------------------------------- query tiles
+            if (lane == 0) {
+                pdl_wait();
+                Walk walk(p, range);
+                int n = 0;
+                while (walk.next(p, x)) {
+                    if (x.live <= x.u0) continue;
+                    if (n > 0 && !mbar_wait(&bars[Q_EMPTY], (n - 1) & 1, p.status, Q_EMPTY, abort_flag)) break;
+                    const uint8_t* image = images + ((size_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + x.tile) * (kParts * kTile);
+                    mbar_arrive_expect_tx(&bars[Q_FULL], kParts * kTile);
+                    for (int i = 0; i < kParts; ++i) bulk_load_1d(sQ + i * kTile, image + i * kTile, kTile, &bars[Q_FULL]);
+                    ++n;
+                }
+            }
+            __syncwarp();
+        } else if (warp == kMmaWarp) {
+            // -------------------------------------------------------------- MMA issuer
+            const bool leader = elect_one();
+            const uint32_t idesc_qk = make_idesc(0, 0, 0, 0, kN, kN), idesc_pv = make_idesc(0, 0, 0, 1, kN, kD);
+            constexpr uint32_t kHi = sdesc_hi(1024);
+            const uint32_t q_lo = sdesc_lo(smem_u32(sQ), 0), k_lo = sdesc_lo(smem_u32(sK), 0), v_lo = sdesc_lo(smem_u32(sV), kBox);
+            auto issue_qk = [&](int i, int stage) {
+                const uint32_t b0 = k_lo + stage * (kTile >> 4), d = tmem + i * 128;
+#pragma unroll
+                for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                    for (int kk = 0; kk < kD / 16; ++kk) {
+                        const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
+                        // the second part first: its sum is small, and so are its truncations
+                        if (leader) umma_ss2(d, q_lo + (kParts - 1 - part) * (kTile >> 4) + off, kHi, b0 + off, kHi, idesc_qk, part + kk > 0);
+                    }
+            };
+            auto issue_pv = [&](int i, int stage, bool add) {
+                const uint32_t b0 = v_lo + stage * (kTile >> 4), d = tmem + 256 + i * 128, a = tmem + i * 128;
+#pragma unroll
+                for (int kk = 0; kk < kN / 16; ++kk)
+                    if (leader) umma_ts2(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b0 + kk * (2048 >> 4), kHi, idesc_pv, (add || kk > 0) ? 1u : 0u);
+            };
+            Walk walk(p, range);
+            int gk = 0, gv = 0, pieces = 0, done[2] = {0, 0};
+            bool ok = true;
+            while (ok && walk.next(p, x)) {
+                const int count = x.live - x.u0;
+                if (count <= 0) continue;
+                auto next_scores = [&](int j) {   // Q K^T of the piece's unit j
+                    if (!(ok = mbar_wait_warp(&bars[K_FULL + gk % kStages], (gk / kStages) & 1, p.status, K_FULL, abort_flag))) return;
+                    tc_fence_after();
+                    issue_qk(j & 1, gk % kStages);
+                    if (leader) {
+                        umma_commit(&bars[S_FULL + (j & 1)]);
+                        umma_commit(&bars[K_EMPTY + gk % kStages]);
+                        if (j + 1 == count) umma_commit(&bars[Q_EMPTY]);
+                    }
+                    ++gk;
+                };
+                if (!(ok = mbar_wait_warp(&bars[Q_FULL], pieces & 1, p.status, Q_FULL, abort_flag))) break;
+                next_scores(0);
+                if (ok && count > 1) next_scores(1);
+                for (int j = 0; ok && j < count; ++j) {
+                    const int i = j & 1, stage = gv % kStages;
+                    if (!(ok = mbar_wait_warp(&bars[V_FULL + stage], (gv / kStages) & 1, p.status, V_FULL, abort_flag))) break;
+                    if (!(ok = mbar_wait_warp(&bars[P_FULL + i], done[i] & 1, p.status, P_FULL, abort_flag))) break;
+                    if (j == 0 && pieces > 0 && !(ok = mbar_wait_warp(&bars[O_FREE], (pieces - 1) & 1, p.status, O_FREE, abort_flag))) break;
+                    tc_fence_after();
+                    issue_pv(i, stage, j > 1);
+                    if (leader) {
+                        umma_commit(&bars[O_FULL + i]);
+                        umma_commit(&bars[V_EMPTY + stage]);
+                    }
+                    ++done[i];
+                    ++gv;
+                    if (j + 2 < count) next_scores(j + 2);
+                }
+                ++pieces;
+            }
+            __syncwarp();
+        }
+    } else if (warp < kSmxWarp0) {
+        // ------------------------------------------------------------------ K and V: codes to fp16 operands
+        if constexpr (kRegsConv < kLaunchRegs) reg_dealloc<kRegsConv>();
+        const bool is_v = warp >= kConvWarp0 + 4;
+        const int tid = (threadIdx.x - kConvWarp0 * 32) & 127;
+        const uint8_t* base = is_v ? p.c.v : p.c.k;
+        const Strides st = is_v ? p.c.sv : p.c.sk;
+        const uint32_t tiles = smem_u32(is_v ? sV : sK);
+        const int full = is_v ? V_FULL : K_FULL, empty = is_v ? V_EMPTY : K_EMPTY;
+        Walk walk(p, range);
+        Codes<D> c;
+        int q = 0, pieces = 0;   // units, pieces so far
+        bool ok = true, more = false;
+        // the first piece with something to do
+        while ((more = walk.next(p, x)) && x.live <= x.u0) {}
+        int page = more ? unit_page(p, x, x.u0, lane, bad) : -1;
+        float scale = 0.f;   // V: lane l < 8 the scale of slots 16 l ..; a scale of 0 makes zeros of its codes, whatever they are
+        auto v_zero = [&](int& pg) {
+            if (!is_v) return;
+            scale = pg >= 0 ? p.c.v_scale[(int64_t)pg * p.c.Hkv + x.h] : 0.f;
+            if (scale == 0.f) pg = -1;
+        };
+        v_zero(page);
+        if (more) load_half<D>(c, 0, base, st, p, x, x.u0, page, tid);
+        while (ok && more) {
+            const int seen = least_seen(p, x);
+            for (int u = x.u0; u < x.live; ++u, ++q) {
+                const int stage = q % kStages;
+                load_half<D>(c, 1, base, st, p, x, u, page, tid);
+                if (q >= kStages && !(ok = mbar_wait_warp(&bars[empty + stage], ((q / kStages) - 1) & 1, p.status, empty, abort_flag))) break;
+                if (!is_v && tid < 8) {   // the unit's scales, for the softmax groups
+                    const int slot = q % kScaleSlots;
+                    const int64_t at = (int64_t)page * p.c.Hkv + x.h;
+                    const float ks = page >= 0 ? p.c.k_scale[at] : 0.f, vs = page >= 0 ? p.c.v_scale[at] : 0.f;
+                    const float size = vs == 0.f ? 1.f : max_nan(vs, 1e-30f);
+                    z.k_scale[slot][tid] = ks;
+                    z.lift[slot][tid] = page >= 0 ? __log2f(size) : -INFINITY;   // slots of a block that is not there count nothing
+                    z.drop[slot][tid] = 1.f / size;
+                }
+                const bool hidden = is_v && CODE == COROPE_CODE_E4M3 && (u + 1) * kN > seen;
+                const uint32_t tile = tiles + stage * kTile;
+                auto clean = [&](int half) {   // NaN that some rows must not see: left out here, put in at the end of the piece
+                    if (!hidden) return;
+                    bool nan = false;
+#pragma unroll
+                    for (int i = 0; i < Codes<D>::kHalf; ++i) {
+                        uint4& w = c.x[half][i];
+                        nan |= has_nan(w.x) || has_nan(w.y) || has_nan(w.z) || has_nan(w.w);
+                        w = make_uint4(without_nan(w.x), without_nan(w.y), without_nan(w.z), without_nan(w.w));
+                    }
+                    if (nan) z.nan_v[pieces % kFlagSlots] = 1;
+                };
+                clean(0);
+                store_half<D, CODE>(c, 0, tile, tid);
+                clean(1);
+                // the next unit's blocks and first codes are on their way while this one's second half is stored
+                if (u + 1 < x.live) {
+                    page = unit_page(p, x, u + 1, lane, bad);
+                    v_zero(page);
+                    load_half<D>(c, 0, base, st, p, x, u + 1, page, tid);
+                }
+                store_half<D, CODE>(c, 1, tile, tid);
+                fence_proxy_async();
+                mbar_arrive_warp(&bars[full + stage], lane);
+            }
+            if (!ok) break;
+            ++pieces;
+            while ((more = walk.next(p, x)) && x.live <= x.u0) {}
+            if (more) {
+                page = unit_page(p, x, x.u0, lane, bad);
+                v_zero(page);
+                load_half<D>(c, 0, base, st, p, x, x.u0, page, tid);
+            }
+        }
+        if (bad || walk.bad) report_bad_index(p.status, p.mirror);
+    } else {
+        // ------------------------------------------------------------------ softmax groups
+        reg_alloc<kRegsSmx>();
+        const int wsm = warp - kSmxWarp0, grp = wsm >> 3, half = (wsm >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
+        const int pair_bar = 1 + grp * 4 + quad;   // the two warps that hold the same 32 rows
+        const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+        const uint32_t tS = tmem + lane_base + grp * 128 + half * 64, tO = tmem + lane_base + 256;
+        pdl_wait();        // the rows' factors
+        Walk walk(p, range);
+        int q = 0, pieces = 0, gs = 0;             // units, pieces, units of this group so far
+        int ends[2] = {0, 0};                      // units of both groups at the end of the piece
+        bool ok = true;
+        // A wait that ran out is not left by: the warps of both groups meet at barriers, so each goes through all of its units, if on what happens
+        // to be there (the host learns of it), and waits for nothing more.
+        auto wait = [&](int bar, int parity) {
+            if (ok) ok = mbar_wait_warp(&bars[bar], parity, p.status, bar, abort_flag);
+            tc_fence_after();
+        };
+        while (walk.next(p, x)) {
+            const int count = max(x.live - x.u0, 0), grow = x.tile * kN + row, t = grow / p.G;
+            const int64_t item = (int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + x.tile;
+            const float factor = factors[item * kN + row];
+            const int sees = p.causal ? x.len - x.n + t + 1 : x.len, seen = least_seen(p, x);
+            float m = kLowest, l = 0.f;
+            for (int j = grp; j < count; j += 2, ++gs) {
+                const int u = x.u0 + j, slot = (q + j) % kScaleSlots;
+                wait(S_FULL + grp, gs & 1);
+                uint32_t s0[32], s1[32];
+                COROPE_TMEM_LD32(tS, s0);
+                COROPE_TMEM_LD32(tS + 32, s1);
+                const float4 ks = *reinterpret_cast<const float4*>(&z.k_scale[slot][half * 4]), up = *reinterpret_cast<const float4*>(&z.lift[slot][half * 4]);
+                tmem_wait_ld();
+                // to units of log2, the scale of V in the exponent
+                auto scale_group = [&](uint32_t* s, float k_scale, float lift) {
+                    const float f = factor * k_scale;
+                    const uint64_t f2 = f2_pack(f, f), a2 = f2_pack(lift, lift);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        float a, b;
+                        f2_unpack(f2_fma(f2_pack_bits(s[i], s[i + 1]), f2, a2), a, b);
+                        s[i] = __float_as_uint(a);
+                        s[i + 1] = __float_as_uint(b);
+                    }
+                };
+                scale_group(s0, ks.x, up.x);
+                scale_group(s0 + 16, ks.y, up.y);
+                scale_group(s1, ks.z, up.z);
+                scale_group(s1 + 16, ks.w, up.w);
+                if ((u + 1) * kN > seen) {
+                    const int last = sees - u * kN - half * 64;   // columns from here on are hidden
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (i >= last) s0[i] = 0xff800000u;
+                        if (32 + i >= last) s1[i] = 0xff800000u;
+                    }
+                }
+                float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    mx0 = fmax3(mx0, __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
+                    mx1 = fmax3(mx1, __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
+                }
+                const float top_half = fmaxf(mx0, mx1);
+                z.half_max[grp][half][row] = top_half;
+                named_bar_sync(pair_bar, 64);
+                const float top = fmaxf(m, fmaxf(top_half, z.half_max[grp][half ^ 1][row]));
+                named_bar_sync(pair_bar, 64);   // both have read before either writes again
+                const bool need = top > m + 8.f;   // exp2 of up to 8 above M fits fp16
+                const float m_old = m;
+                m = need ? top : m;
+                const uint64_t neg_m = f2_pack(-m, -m);
+                const float4 drop = *reinterpret_cast<const float4*>(&z.drop[slot][half * 4]);
+                float add = 0.f;
+                auto exp_group = [&](const uint32_t* s, float drop_g, uint32_t* pk) {
+                    uint64_t sum = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float d0, d1;
+                        f2_unpack(f2_add(f2_pack_bits(s[2 * i], s[2 * i + 1]), neg_m), d0, d1);
+                        const float p0 = fast_exp2(d0), p1 = fast_exp2(d1);
+                        pk[i] = pack_half2(p0, p1);
+                        sum = f2_add(sum, f2_pack(p0, p1));
+                    }
+                    float a, b;
+                    f2_unpack(sum, a, b);
+                    add = a + b == 0.f ? add : fmaf(a + b, drop_g, add);   // hidden slots of a block whose scale is NaN count nothing
+                };
+                {
+                    uint32_t pk[16];
+                    exp_group(s0, drop.x, pk);
+                    exp_group(s0 + 16, drop.y, pk + 8);
+                    COROPE_TMEM_ST16(tS, pk);
+                }
+                {
+                    uint32_t pk[16];
+                    exp_group(s1, drop.z, pk);
+                    exp_group(s1 + 16, drop.w, pk + 8);
+                    COROPE_TMEM_ST16(tS + 16, pk);
+                }
+                if (j > 1 && __any_sync(0xffffffffu, need)) {
+                    wait(O_FULL + grp, (gs - 1) & 1);
+                    const float shrink = fast_exp2(m_old - m);
+#pragma unroll
+                    for (int k = 0; k < kD / 64; ++k) {
+                        const uint32_t at = tO + grp * 128 + half * (kD / 2) + k * 32;
+                        uint32_t r[32];
+                        COROPE_TMEM_LD32(at, r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * shrink);
+                        COROPE_TMEM_ST32(at, r);
+                    }
+                    l *= shrink;
+                }
+                l += add;
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive_warp(&bars[P_FULL + grp], lane);
+            }
+            q += count;
+            ends[0] += (count + 1) / 2;
+            ends[1] += count / 2;
+
+            // the piece's sums: both groups' O, a quarter of the columns to each warpgroup
+            const int buf = pieces & 1;
+            if (half == 0) z.end_max[buf][grp][row] = m;
+            z.end_sum[buf][grp][half][row] = l;
+            named_bar_sync(9, 512);
+            if (count > 0) wait(O_FULL, (ends[0] - 1) & 1);
+            if (count > 1) wait(O_FULL + 1, (ends[1] - 1) & 1);
+            const float m0 = z.end_max[buf][0][row], m1 = z.end_max[buf][1][row], top = fmaxf(m0, m1);
+            const float w0 = fast_exp2(m0 - top), w1 = fast_exp2(m1 - top);
+            const float all = (z.end_sum[buf][0][0][row] + z.end_sum[buf][0][1][row]) * w0 + (z.end_sum[buf][1][0][row] + z.end_sum[buf][1][1][row]) * w1;
+            const bool whole = x.u0 == 0 && x.u1 == x.units, some = t < x.n && all != 0.f;
+            const float inv = whole ? 1.f / all : 1.f;
+            constexpr int kCols = kD / 4;
+            const int col0 = (grp * 2 + half) * kCols;
+            const int64_t part = (2 * (int64_t)blockIdx.x + (x.u0 == 0 ? 1 : 0)) * kN + row;
+            const int64_t to = (int64_t)x.b * p.so.b + (int64_t)(x.h * p.G + grow - t * p.G) * p.so.h + (int64_t)t * p.so.n;
+            const bool fix = CODE == COROPE_CODE_E4M3 && count > 0 && z.nan_v[pieces % kFlagSlots] != 0;
+#pragma unroll
+            for (int k = 0; k < kCols; k += 16) {
+                float y[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] = 0.f;
+                if (count > 0) {
+                    uint32_t r[16];
+                    COROPE_TMEM_LD16(tO + col0 + k, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(r[i]) * w0;
+                    if (count > 1) {
+                        COROPE_TMEM_LD16(tO + 128 + col0 + k, r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] = fmaf(__uint_as_float(r[i]), w1, y[i]);
+                    }
+                }
+                if (col0 + k >= D) continue;
+                if (fix) {   // NaN in V, slot by slot: to the rows that see it
+#pragma unroll 1
+                    for (int s = max(seen, x.u0 * kN) & ~(kN - 1); s < min(sees, x.live * kN); ++s) {
+                        bool far = false;
+                        const int page = cache_page(p.s, p.c.bs_log2, p.c.num_blocks, x.b, s, far);
+                        if (page < 0 || p.c.v_scale[(int64_t)page * p.c.Hkv + x.h] == 0.f) continue;
+                        const uint8_t* v = p.c.v + (int64_t)page * p.c.sv.b + (int64_t)x.h * p.c.sv.h + (int64_t)(s & ((1 << p.c.bs_log2) - 1)) * p.c.sv.n + col0 + k;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if ((v[i] & 0x7f) == 0x7f) y[i] = __int_as_float(0x7fffffff);
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(p.part + part * D + col0 + k + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                } else if (t < p.T) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4)
+                        store4(p.o, to + col0 + k + i, p.dtype, p.vec_o,
+                               some ? make_float4(y[i] * inv, y[i + 1] * inv, y[i + 2] * inv, y[i + 3] * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
+                }
+            }
+            if (grp == 0 && half == 0) {
+                if (!whole) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(top, all);
+                else if (p.lse != nullptr && t < p.T) p.lse[((int64_t)x.b * p.c.Hkv + x.h) * p.T * p.G + grow] = some ? top + log2f(all) : INFINITY;
+            }
+            if (count > 0) {
+                tc_fence_before();
+                mbar_arrive_warp(&bars[O_FREE], lane);
+                // the flag of the piece before: every thread has read it, and its place is not taken again before this thread has come by
+                if (wsm == 0 && lane == 0 && pieces > 0) z.nan_v[(pieces - 1) % kFlagSlots] = 0;
+                ++pieces;
+            } else {
+                named_bar_sync(9, 512);   // the exchange above is not overwritten while someone reads it
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) report_to_mirror(p.status, p.mirror);
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ accumulated weights
+// S^T = K Q^T with slots as rows: a thread has a slot and sums exp2(s - lse) over the columns, the query rows, so nothing crosses threads.  A unit
+// is 128 slots of a K / V head: its K stays, and the tiles of query rows (both parts) stream by.  Bound by the exponentials.
+//   warp 0  query tiles, with their rows' factors and lse;  warp 1  MMA issuer;  warps 4-7  K;  warps 8-11, 12-15  the even and odd tiles
+constexpr int kSumThreads = 512;
+enum SumBar { W_K_FULL = 0, W_K_EMPTY = 2, W_Q_FULL = 4, W_Q_EMPTY = 6, W_ROWS = 8, W_S_FULL = 10, W_S_FREE = 12, W_NUM_BARS = 14 };
+struct SumSmall {
+    float factor[2][kN], lse[2][kN], sum[2][kN];
+    float k_scale[2][8];
+    int page[2][8];
+    uint64_t bars[W_NUM_BARS];
+    uint32_t tmem;
+    int abort;
+};
+constexpr size_t sum_smem_bytes(int D) { return (2 * 2 + 2) * tile_bytes(D) + sizeof(SumSmall) + 1024; }
+static_assert(sum_smem_bytes(128) <= 232448 - 1024, "shared memory budget");
+
+struct Unit {
+    int b, h, u, len, n, tile0, tiles;   // tiles [tile0, tiles) have rows that see a slot of the unit
+};
+struct UnitWalk {
+    Range r;
+    Load l;
+    bool bad = false;
+    __device__ __forceinline__ Load load(const CacheAttnParams& p, int b) {
+        Load l = load_of(p, kN, kN, b, bad);
+        l.items = l.n > 0 ? p.c.Hkv : 0;
+        return l;
+    }
+    __device__ __forceinline__ UnitWalk(const CacheAttnParams& p, const Range& range) : r(range) { l = load(p, r.b); }
+    __device__ __forceinline__ bool next(const CacheAttnParams& p, Unit& x) {
+        for (; r.left > 0; --r.left, ++r.off) {
+            while (r.off >= (int64_t)l.units * l.items) {
+                r.off -= (int64_t)l.units * l.items;
+                l = load(p, ++r.b);
+            }
+            x.b = r.b; x.len = l.len; x.n = l.n;
+            x.h = (int)(r.off / l.units);
+            x.u = (int)(r.off - (int64_t)x.h * l.units);
+            const int64_t first = p.causal ? max((int64_t)x.u * kN - (l.len - l.n), (int64_t)0) * p.G : 0;   // the first row that sees a slot
+            x.tiles = (l.n * p.G + kN - 1) / kN;
+            x.tile0 = (int)min(first / kN, (int64_t)x.tiles);
+            if (x.tile0 < x.tiles) {
+                --r.left;
+                ++r.off;
+                return true;
+            }
+        }
+        return false;
+    }
+};
+
+template <int D, int CODE>
+__global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const CacheAttnParams p, const uint8_t* images, const float* factors) {
+    constexpr int kD = wide(D), kBox = kN * 128;
+    constexpr uint32_t kTile = (uint32_t)tile_bytes(D);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sQ = sm;                       // [stage][part]
+    uint8_t* sK = sQ + 4 * kTile;           // [stage]
+    SumSmall& z = *reinterpret_cast<SumSmall*>(sK + 2 * kTile);
+    uint64_t* bars = z.bars;
+    volatile int* abort_flag = &z.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    bool bad = false;
+    const Range range = take_range<128>(p.s.B, [&](int b) {
+        Load l = load_of(p, kN, kN, b, bad);
+        l.items = l.n > 0 ? p.c.Hkv : 0;
+        return l;
+    });
+    const bool gave_up = p.status != nullptr && (*reinterpret_cast<volatile int*>(p.status) & COROPE_DEV_WAIT_EXPIRED);
+    if (__syncthreads_or(gave_up) || range.left == 0) {
+        if (threadIdx.x == 0 && gave_up) report_to_mirror(p.status, p.mirror);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        z.abort = 0;
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars[W_K_FULL + i], 4);
+            mbar_init(&bars[W_K_EMPTY + i], 4);      // the group that ends a unit
+            mbar_init(&bars[W_Q_FULL + i], 1);
+            mbar_init(&bars[W_Q_EMPTY + i], 1);
+            mbar_init(&bars[W_ROWS + i], 1);
+            mbar_init(&bars[W_S_FULL + i], 1);
+            mbar_init(&bars[W_S_FREE + i], 4);
+        }
+        fence_mbar_init();
+    }
+    if (D == 32)
+        for (int i = threadIdx.x; i < (int)(2 * kTile / 16); i += kSumThreads) reinterpret_cast<uint4*>(sK)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async();
+    __syncthreads();
+    if (warp == 1) {
+        tmem_alloc(&z.tmem, 256);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = z.tmem;
+    UnitWalk walk(p, range);
+    Unit x;
+    bool ok = true;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ query tiles
+        int q = 0;
+        while (ok && walk.next(p, x))
+            for (int t = x.tile0; ok && t < x.tiles; ++t, ++q) {
+                const int i = q & 1;
+                if (q >= 2) {
+                    if (!(ok = mbar_wait_warp(&bars[W_Q_EMPTY + i], ((q >> 1) - 1) & 1, p.status, W_Q_EMPTY, abort_flag))) break;
+                    if (!(ok = mbar_wait_warp(&bars[W_S_FREE + i], ((q >> 1) - 1) & 1, p.status, W_S_FREE, abort_flag))) break;
+                }
+                const int64_t item = (int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + t;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&bars[W_Q_FULL + i], 2 * kTile);
+                    for (int part = 0; part < 2; ++part) bulk_load_1d(sQ + (2 * i + part) * kTile, images + ((size_t)item * 2 + part) * kTile, kTile, &bars[W_Q_FULL + i]);
+                }
+                for (int r = lane; r < kN; r += 32) {
+                    const int row = t * kN + r;
+                    z.factor[i][r] = factors[item * kN + r];
+                    z.lse[i][r] = row < x.n * p.G ? p.lse[((int64_t)x.b * p.c.Hkv + x.h) * p.T * p.G + row] : INFINITY;
+                }
+                mbar_arrive_warp(&bars[W_ROWS + i], lane);
+            }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA issuer
+        const bool leader = elect_one();
+        const uint32_t idesc = make_idesc(0, 0, 0, 0, kN, kN);
+        constexpr uint32_t kHi = sdesc_hi(1024);
+        const uint32_t q_lo = sdesc_lo(smem_u32(sQ), 0), k_lo = sdesc_lo(smem_u32(sK), 0);
+        int q = 0, units = 0;
+        while (ok && walk.next(p, x)) {
+            const int stage = units & 1;
+            if (!(ok = mbar_wait_warp(&bars[W_K_FULL + stage], (units >> 1) & 1, p.status, W_K_FULL, abort_flag))) break;
+            for (int t = x.tile0; t < x.tiles; ++t, ++q) {
+                const int i = q & 1;
+                if (!(ok = mbar_wait_warp(&bars[W_Q_FULL + i], (q >> 1) & 1, p.status, W_Q_FULL, abort_flag))) break;
+                if (q >= 2 && !(ok = mbar_wait_warp(&bars[W_S_FREE + i], ((q >> 1) - 1) & 1, p.status, W_S_FREE, abort_flag))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int part = 1; part >= 0; --part)
+#pragma unroll
+                    for (int kk = 0; kk < kD / 16; ++kk) {
+                        const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
+                        if (leader) umma_ss2(tmem + i * 128, k_lo + stage * (kTile >> 4) + off, kHi, q_lo + (2 * i + part) * (kTile >> 4) + off, kHi, idesc, part == 0 || kk > 0);
+                    }
+                if (leader) {
+                    umma_commit(&bars[W_S_FULL + i]);
+                    umma_commit(&bars[W_Q_EMPTY + i]);
+                }
+            }
+            ++units;
+        }
+        __syncwarp();
+    } else if (warp >= 4 && warp < 8) {
+        // ------------------------------------------------------------------ K
+        const int tid = threadIdx.x & 127;
+        int units = 0;
+        while (walk.next(p, x)) {
+            const int stage = units & 1;
+            Codes<D> c;
+            const int page = unit_page(p, x, x.u, lane, bad);
+            const Piece as{x.b, x.h, 0, x.u, x.u + 1, x.u + 1, x.len, x.n, 0};
+            load_half<D>(c, 0, p.c.k, p.c.sk, p, as, x.u, page, tid);
+            load_half<D>(c, 1, p.c.k, p.c.sk, p, as, x.u, page, tid);
+            if (units >= 2 && !mbar_wait_warp(&bars[W_K_EMPTY + stage], ((units >> 1) - 1) & 1, p.status, W_K_EMPTY, abort_flag)) break;
+            if (tid < 8) {
+                z.k_scale[stage][tid] = page >= 0 ? p.c.k_scale[(int64_t)page * p.c.Hkv + x.h] : 0.f;
+                z.page[stage][tid] = page;
+            }
+            store_half<D, CODE>(c, 0, smem_u32(sK) + stage * kTile, tid);
+            store_half<D, CODE>(c, 1, smem_u32(sK) + stage * kTile, tid);
+            fence_proxy_async();
+            mbar_arrive_warp(&bars[W_K_FULL + stage], lane);
+            ++units;
+        }
+    } else if (warp >= 8) {
+        // ------------------------------------------------------------------ sums
+        const int grp = (warp - 8) >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + grp * 128;
+        int q = 0, units = 0;
+        auto wait = [&](int bar, int parity) {   // as in the main kernel: nobody leaves a barrier that others come to
+            if (ok) ok = mbar_wait_warp(&bars[bar], parity, p.status, bar, abort_flag);
+        };
+        while (walk.next(p, x)) {
+            const int stage = units & 1, slot = x.u * kN + row, count = x.tiles - x.tile0;
+            wait(W_K_FULL + stage, (units >> 1) & 1);
+            const float ks = z.k_scale[stage][row >> 4];
+            const int page = z.page[stage][row >> 4];
+            const uint64_t ks2 = f2_pack(ks, ks);
+            float w = 0.f;
+            for (int j = 0; j < count; ++j, ++q) {
+                if ((q & 1) != grp) continue;
+                wait(W_ROWS + grp, (q >> 1) & 1);
+                wait(W_S_FULL + grp, (q >> 1) & 1);
+                tc_fence_after();
+                // columns that see the slot: from the first row whose query does to the last row with a query
+                const int tile = x.tile0 + j;
+                const int64_t first = p.causal ? (int64_t)max(slot - (x.len - x.n), 0) * p.G - (int64_t)tile * kN : 0;
+                const int from = (int)min(max(first, (int64_t)0), (int64_t)kN), to = min(x.n * p.G - tile * kN, kN);
+                const bool every = __all_sync(0xffffffffu, from == 0 && to == kN);
+#pragma unroll
+                for (int k = 0; k < kN; k += 32) {
+                    uint32_t s[32];
+                    COROPE_TMEM_LD32(tS + k, s);
+                    tmem_wait_ld();
+                    uint64_t sum = 0;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&z.factor[grp][k + i]), e = *reinterpret_cast<const float4*>(&z.lse[grp][k + i]);
+                        float d[4];
+                        f2_unpack(f2_fma(f2_pack_bits(s[i], s[i + 1]), f2_mul(f2_pack(f.x, f.y), ks2), f2_pack(-e.x, -e.y)), d[0], d[1]);
+                        f2_unpack(f2_fma(f2_pack_bits(s[i + 2], s[i + 3]), f2_mul(f2_pack(f.z, f.w), ks2), f2_pack(-e.z, -e.w)), d[2], d[3]);
+                        if (!every) {
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) d[y] = k + i + y >= from && k + i + y < to ? d[y] : -INFINITY;
+                        }
+                        sum = f2_add(sum, f2_pack(fast_exp2(d[0]), fast_exp2(d[1])));
+                        sum = f2_add(sum, f2_pack(fast_exp2(d[2]), fast_exp2(d[3])));
+                    }
+                    float a, b;
+                    f2_unpack(sum, a, b);
+                    w += a + b;
+                }
+                tc_fence_before();
+                mbar_arrive_warp(&bars[W_S_FREE + grp], lane);
+            }
+            z.sum[grp][row] = w;
+            named_bar_sync(1, 256);
+            if (grp == 0 && page >= 0 && slot < x.len) {   // one addition per slot and call; atomic because sequences may share blocks
+                const int bs_mask = (1 << p.c.bs_log2) - 1;
+                atomicAdd(p.c.weight + (((int64_t)page * p.c.Hkv + x.h) << p.c.bs_log2) + (slot & bs_mask), w + z.sum[1][row]);
+            }
+            named_bar_sync(1, 256);
+            // every tile of the unit has been read, so its products are complete
+            if (grp == 0) mbar_arrive_warp(&bars[W_K_EMPTY + stage], lane);
+            ++units;
+        }
+        tc_fence_before();
+    }
+    if (bad || walk.bad) report_bad_index(p.status, p.mirror);
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) report_to_mirror(p.status, p.mirror);
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 256);
+    }
+}
+
+struct TileLayout {
+    size_t factors, total;   // the images come first
+};
+TileLayout tile_layout(int B, int Hkv, int row_tiles, int D, bool two) {
+    const size_t items = (size_t)B * Hkv * row_tiles;
+    TileLayout l;
+    l.factors = items * (two ? 2 : 1) * tile_bytes(D);
+    l.total = align_up(l.factors + items * kN * 4, 256);
+    return l;
+}
+
+template <int D, int CODE, bool TWO>
+int launch_t(const CacheAttnParams& p, uint8_t* images, float* factors, unsigned blocks, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    if (int e = allow_smem(cache_attn_tile_kernel<D, CODE, TWO>, smem_bytes(D, TWO), done)) return e;
+    count_launch(2);
+    cache_pack_kernel<D, TWO><<<(unsigned)(p.s.B * p.c.Hkv * p.row_tiles), 256, 0, s>>>(p, images, factors);
+    if (int e = (int)cudaGetLastError()) return e;
+    return launch_dependent(cache_attn_tile_kernel<D, CODE, TWO>, blocks, kThreads, smem_bytes(D, TWO), s, p, (const uint8_t*)images, (const float*)factors);
+}
+template <int D, int CODE>
+int launch_weight_t(const CacheAttnParams& p, const uint8_t* images, const float* factors, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    if (int e = allow_smem(cache_weight_tile_kernel<D, CODE>, sum_smem_bytes(D), done)) return e;
+    const uint64_t units = (uint64_t)p.s.B * p.c.Hkv * ((p.capacity + kN - 1) / kN);
+    count_launch();
+    cache_weight_tile_kernel<D, CODE><<<(unsigned)(units < (uint64_t)sm_count() ? units : sm_count()), kSumThreads, sum_smem_bytes(D), s>>>(p, images, factors);
+    return (int)cudaGetLastError();
+}
+template <int D>
+int by_code(const CacheAttnParams& p, uint8_t* images, float* factors, bool two, unsigned blocks, cudaStream_t s) {
+    if (p.code == COROPE_CODE_E4M3) return two ? launch_t<D, COROPE_CODE_E4M3, true>(p, images, factors, blocks, s) : launch_t<D, COROPE_CODE_E4M3, false>(p, images, factors, blocks, s);
+    return two ? launch_t<D, COROPE_CODE_INT8, true>(p, images, factors, blocks, s) : launch_t<D, COROPE_CODE_INT8, false>(p, images, factors, blocks, s);
+}
+template <int D>
+int weight_by_code(const CacheAttnParams& p, const uint8_t* images, const float* factors, cudaStream_t s) {
+    return p.code == COROPE_CODE_E4M3 ? launch_weight_t<D, COROPE_CODE_E4M3>(p, images, factors, s) : launch_weight_t<D, COROPE_CODE_INT8>(p, images, factors, s);
+}
+
+}  // namespace
+
+size_t cache_tile_workspace_bytes(int B, int Hkv, int row_tiles, int D, bool two_parts) { return tile_layout(B, Hkv, row_tiles, D, two_parts).total; }
+
+int launch_cache_attn_tiles(const CacheAttnParams& p, void* ws, bool two_parts, unsigned blocks, cudaStream_t s) {
+    uint8_t* images = static_cast<uint8_t*>(ws);
+    float* factors = reinterpret_cast<float*>(images + tile_layout(p.s.B, p.c.Hkv, p.row_tiles, p.D, two_parts).factors);
+    return p.D == 128 ? by_code<128>(p, images, factors, two_parts, blocks, s) : p.D == 64 ? by_code<64>(p, images, factors, two_parts, blocks, s)
+                                                                                         : by_code<32>(p, images, factors, two_parts, blocks, s);
+}
+
+int launch_cache_weight_tiles(const CacheAttnParams& p, void* ws, cudaStream_t s) {
+    const uint8_t* images = static_cast<const uint8_t*>(ws);
+    const float* factors = reinterpret_cast<const float*>(images + tile_layout(p.s.B, p.c.Hkv, p.row_tiles, p.D, true).factors);
+    return p.D == 128 ? weight_by_code<128>(p, images, factors, s) : p.D == 64 ? weight_by_code<64>(p, images, factors, s) : weight_by_code<32>(p, images, factors, s);
+}
+
+}  // namespace corope
