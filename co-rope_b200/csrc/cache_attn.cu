@@ -469,14 +469,15 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 }
 
 // ------------------------------------------------------------------------------------------------ joining parts
-// One block per item, a warp per query row.  An item that one block of the main kernel did alone is finished; the parts of the others are
+// A warp per query row, a block per eight rows of an item.  An item that one block of the main kernel did alone is finished; the parts of the others are
 // added in the order of their ranges.  Rows that no unit stands for are written here: 0.
 constexpr int kJoinThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const CacheAttnParams p, int rows_per_tile, int unit, int main_blocks) {
     __shared__ int64_t words[2][kJoinThreads / 32];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int tile = (int)(blockIdx.x % (unsigned)p.row_tiles), bh = (int)(blockIdx.x / (unsigned)p.row_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
+    const unsigned blocks = (unsigned)rows_per_tile / (kJoinThreads / 32), item = blockIdx.x / blocks;
+    const int tile = (int)(item % (unsigned)p.row_tiles), bh = (int)(item / (unsigned)p.row_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
     bool bad = false;
     int64_t before = 0, total = 0;
     for (int i = threadIdx.x; i < p.s.B; i += kJoinThreads) {
@@ -508,9 +509,9 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const Cac
     }
     pdl_wait();   // by every block: the end of this kernel has to stand for the end of the one before
     if (!empty && r0 == r1) return;
-    for (int r = warp; r < rows_per_tile; r += kJoinThreads / 32) {
-        const int row = tile * rows_per_tile + r, t = row / p.G;
-        if (t >= p.T) break;
+    {
+        const int r = (int)(blockIdx.x - item * blocks) * (kJoinThreads / 32) + warp, row = tile * rows_per_tile + r, t = row / p.G;
+        if (t >= p.T) return;
         float top = kLowest, all = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         if (!empty && t < l.n) {
@@ -748,7 +749,7 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
 template <int D>
 int launch_join(const CacheAttnParams& p, const Layout& l, int unit, cudaStream_t s) {
     count_launch();
-    return launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles), kJoinThreads, 0, s, p, l.rows_per_tile, unit, (int)l.blocks);
+    return launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles * (l.rows_per_tile / 8)), kJoinThreads, 0, s, p, l.rows_per_tile, unit, (int)l.blocks);
 }
 template <int D, int CODE, int NT, bool EXACT_P>
 int launch_main(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {

@@ -4,7 +4,8 @@
 // piece by piece, a piece being units of one tile of rows.  Warp roles (896 threads, registers divided again with setmaxnreg):
 //   warp 0        brings a piece's query tile (an image of its place in shared memory that a pre-pass has written) with bulk copies
 //   warp 2        MMA issuer and TMEM owner
-//   warps 4-7     K: loads 16 codes a lane, turns them into fp16 (exact) and stores them as the MMA wants them;  warps 8-11: V likewise
+//   warp 3        scout: walks the range ahead of the others and tells them the pieces, and of each unit the addresses of its codes and their scales
+//   warps 4-7     K: 16 codes a lane and step turned into fp16 (exact) and stored as the MMA wants them;  warps 8-11: V likewise
 //   warps 12-19   softmax of the even units of a piece, two threads a row (64 slots each);  warps 20-27: of the odd ones
 // TMEM: S0 [0,128) S1 [128,256) O0 [256,384) O1 [384,512); P (fp16) goes over S.  Even and odd units have sums of their own, so one group's
 // exponentials run beside the other's MMAs, and are joined when the piece is written.
@@ -13,6 +14,8 @@
 // Queries are scaled by a power of two per row and rounded to fp16 (11 bits); with two parts (fp16 tensors, and where weights are gathered) the
 // remainder of the rounding is a second operand and scores have 22 bits.
 // Bound by the exponentials (16 a clock and SM: 1024 clocks a unit at least) and, next to that, by the MMAs (2 * 128^3 * 2 operations, 3 with two parts).
+#include <cstddef>
+
 #include "cache_attn.cuh"
 
 namespace corope {
@@ -24,57 +27,43 @@ constexpr int kMmaWarp = 2, kConvWarp0 = 4, kSmxWarp0 = 12;
 constexpr int kLaunchRegs = 72, kRegsCtl = 40, kRegsConv = 56, kRegsSmx = 88;
 static_assert(128 * (kRegsCtl + 2 * kRegsConv + 4 * kRegsSmx) <= kThreads * kLaunchRegs, "register budget");
 constexpr int kStages = 2;                    // of K and of V
-constexpr int kScaleSlots = 4;                // units whose scales are kept: one more than can be under way
+constexpr int kUnitSlots = 8, kPieceSlots = 4;   // what the scout has told and is kept
 constexpr int kFlagSlots = 8;                 // pieces whose flag is kept
 
 enum Bar { Q_FULL = 0, Q_EMPTY, K_FULL, K_EMPTY = K_FULL + kStages, V_FULL = K_EMPTY + kStages, V_EMPTY = V_FULL + kStages, S_FULL = V_EMPTY + kStages,
-           P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, O_FREE = O_FULL + 2, NUM_BARS };
+           P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, O_FREE = O_FULL + 2, UNIT_FULL = O_FREE + 1, UNIT_EMPTY = UNIT_FULL + kUnitSlots,
+           PIECE_FULL = UNIT_EMPTY + kUnitSlots, PIECE_EMPTY = PIECE_FULL + kPieceSlots, NUM_BARS = PIECE_EMPTY + kPieceSlots };
 
 // shared memory of head dimension D (32 is widened to 64 with zeros)
 __host__ __device__ constexpr int wide(int D) { return D == 128 ? 128 : 64; }
 __host__ __device__ constexpr size_t tile_bytes(int D) { return (size_t)kN * wide(D) * 2; }
-struct Small {
-    float k_scale[kScaleSlots][8], lift[kScaleSlots][8], drop[kScaleSlots][8];   // of each 16 slots
+// A unit's 16-slot groups: where their rows begin, how many there are (0: the block is not there, or its scale of V is 0), their scales.
+struct alignas(16) UnitNote {   // its floats are read four at a time
+    uint64_t k[8], v[8];
+    float k_scale[8], lift[8], drop[8];
+    int k_rows[8], v_rows[8];
+    int piece;       // number of its piece among those with units, -1: there is no unit any more
+    int hidden;      // some row of the tile does not see some slot
+};
+static_assert(sizeof(UnitNote) % 16 == 0 && offsetof(UnitNote, k_scale) % 16 == 0 && offsetof(UnitNote, lift) % 16 == 0 && offsetof(UnitNote, drop) % 16 == 0, "");
+// A piece: units [u0, u0 + count) of the item.  b < 0: there is none any more.
+struct PieceNote {
+    int b, h, tile, u0, count, len, n, whole;
+};
+struct alignas(16) Small {
+    UnitNote units[kUnitSlots];
+    PieceNote pieces[kPieceSlots];
     float half_max[2][2][kN];                 // exchanged between the two threads of a row
-    float end_max[2][2][kN], end_sum[2][2][2][kN];   // [piece % 2][group][half]
+    float end_max[2][kN], end_sum[2][2][kN];  // [group][half]
     uint64_t bars[NUM_BARS];
+    int left;                                 // the softmax warps leave
     int nan_v[kFlagSlots];                    // a piece has NaN in V where some rows must not see it
     uint32_t tmem;
     int abort;
 };
-constexpr size_t smem_bytes(int D, bool two) { return ((two ? 2 : 1) + 2 * kStages) * tile_bytes(D) + sizeof(Small) + 1024; }
-static_assert(smem_bytes(128, true) <= 232448 - 1024, "shared memory budget");
-
-// ------------------------------------------------------------------------------------------------ pieces
-struct Piece {
-    int b, h, tile, u0, u1, live;   // units [u0, u1) of the item, of which those below `live` have a slot that a row of the tile sees
-    int len, n, units;
-};
-struct Walk {
-    Range r;
-    Load l;
-    bool bad = false;
-    __device__ __forceinline__ Walk(const CacheAttnParams& p, const Range& range) : r(range) { l = load_of(p, kN, kN, r.b, bad); }
-    __device__ __forceinline__ bool next(const CacheAttnParams& p, Piece& x) {
-        if (r.left <= 0) return false;
-        while (r.off >= (int64_t)l.units * l.items) {
-            r.off -= (int64_t)l.units * l.items;
-            l = load_of(p, kN, kN, ++r.b, bad);
-        }
-        const int item = (int)(r.off / l.units), tiles = l.items / p.c.Hkv;
-        x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles;
-        x.u0 = (int)(r.off - (int64_t)item * l.units);
-        x.u1 = (int)min((int64_t)l.units, x.u0 + r.left);
-        x.len = l.len; x.n = l.n; x.units = l.units;
-        const int last = min(l.n - 1, (x.tile * kN + kN - 1) / p.G);      // the tile's last query
-        const int most = p.causal ? max(l.len - l.n + last + 1, 0) : l.len;
-        x.live = min((most + kN - 1) / kN, x.u1);
-        r.off += x.u1 - x.u0;
-        r.left -= x.u1 - x.u0;
-        return true;
-    }
-};
-__device__ __forceinline__ int least_seen(const CacheAttnParams& p, const Piece& x) { return p.causal ? x.len - x.n + x.tile * kN / p.G + 1 : x.len; }
+constexpr size_t queue_bytes(int D, bool two) { return (size_t)(D == 128 && two ? 4 : D / 16) * 16 * 128; }   // of codes on their way, per group
+constexpr size_t smem_bytes(int D, bool two) { return ((two ? 2 : 1) + 2 * kStages) * tile_bytes(D) + 2 * queue_bytes(D, two) + sizeof(Small) + 1024; }
+static_assert(smem_bytes(128, true) <= 232448 - 128 && smem_bytes(128, false) <= 232448 - 128, "shared memory budget");   // (and take_range's)
 
 // byte offset of 16-byte run `run` (8 elements) of row r in the image of a tile: boxes of 64 columns, 128-byte swizzle
 __device__ __forceinline__ uint32_t image_at(int r, int run) { return (uint32_t)((run >> 3) * (kN * 128) + r * 128 + (((run & 7) ^ (r & 7)) << 4)); }
@@ -84,16 +73,18 @@ __device__ __forceinline__ void store16(uint32_t at, uint32_t a, uint32_t b, uin
 }
 
 // ------------------------------------------------------------------------------------------------ queries
-// One block per (K / V head, tile of rows): rotates, scales and rounds the rows, and writes them as images of the tile.
+// Rotates, scales and rounds the rows, and writes them as images of their tiles: a warp per row, 16 blocks per tile.
+constexpr int kPackWarps = 8, kPackBlocks = kN / kPackWarps;
 template <int D, bool TWO>
-__global__ void __launch_bounds__(256) cache_pack_kernel(const CacheAttnParams p, uint8_t* images, float* factors) {
+__global__ void __launch_bounds__(kPackWarps * 32) cache_pack_kernel(const CacheAttnParams p, uint8_t* images, float* factors) {
     constexpr int kHalf = D / 2, kPairs = kHalf / 2;
-    const int tile = (int)(blockIdx.x % (unsigned)p.row_tiles), bh = (int)(blockIdx.x / (unsigned)p.row_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const unsigned item = blockIdx.x / (unsigned)kPackBlocks;
+    const int tile = (int)(item % (unsigned)p.row_tiles), bh = (int)(item / (unsigned)p.row_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
+    const int lane = threadIdx.x % 32, r = (int)(blockIdx.x - item * kPackBlocks) * kPackWarps + (int)threadIdx.x / 32;
     bool bad = false;
     const int len = cache_len(p.s, p.c.bs_log2, b, bad), n = cache_new(p.s, p.T, b, bad);
-    uint8_t* image = images + (size_t)blockIdx.x * (TWO ? 2 : 1) * tile_bytes(D);
-    for (int r = warp; r < kN; r += 8) {
+    uint8_t* image = images + (size_t)item * (TWO ? 2 : 1) * tile_bytes(D);
+    {
         const int row = tile * kN + r, t = row / p.G;
         float x[4] = {0.f, 0.f, 0.f, 0.f};   // columns 2 lane, + 1, and their partners D / 2 further on
         if (t < n && lane < kPairs) {
@@ -116,7 +107,7 @@ __global__ void __launch_bounds__(256) cache_pack_kernel(const CacheAttnParams p
         const bool usual = m >= 1e-30f && m <= 1e30f;   // to [2^10, 2^11), see pack_queries of the kernel for few rows
         const int e = usual ? (int)(__float_as_uint(m) >> 23) - 127 - 10 : 0;
         const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
-        if (lane == 0) factors[(size_t)blockIdx.x * kN + r] = down * p.scale;
+        if (lane == 0) factors[(size_t)item * kN + r] = down * p.scale;
         if (lane < kPairs) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -141,56 +132,50 @@ __global__ void __launch_bounds__(256) cache_pack_kernel(const CacheAttnParams p
 }
 
 // ------------------------------------------------------------------------------------------------ codes to operands
-// What one group of 128 threads keeps of a unit's 128 slots: lane l < 8 the block (or -1) of slots 16 l .. 16 l + 15.
-template <int D>
-struct Codes {
-    static constexpr int kLanes = D / 16, kRowsPerStep = 128 / kLanes, kSteps = kN / kRowsPerStep, kHalf = kSteps / 2;
-    uint4 x[2][kHalf];
+// A group of 128 threads turns a unit's 128 slots into an operand in kSteps steps, 16 codes a thread and step.  The codes wait in a queue in
+// shared memory of the thread's own (cp.async brings them, nobody else reads them), kDepth steps ahead.
+template <int D, bool TWO>
+struct Steps {
+    static constexpr int kLanes = D / 16, kRowsPerStep = 128 / kLanes, kSteps = kN / kRowsPerStep;
+    static constexpr int kDepth = D == 128 && TWO ? 4 : kSteps;
+    static constexpr int kQueueBytes = kDepth * 16 * 128;   // of one group
 };
+// the block of slots 16 lane .. of unit u, lane < 8, or -1
 template <typename X>
 __device__ __forceinline__ int unit_page(const CacheAttnParams& p, const X& x, int u, int lane, bool& bad) {
     const int slot = u * kN + 16 * lane;
     return lane < 8 && slot < x.len ? cache_page(p.s, p.c.bs_log2, p.c.num_blocks, x.b, slot, bad) : -1;
 }
-template <int D>
-__device__ __forceinline__ void load_half(Codes<D>& c, int half, const uint8_t* base, const Strides& st, const CacheAttnParams& p, const Piece& x, int u, int page, int tid) {
-    using C = Codes<D>;
-    const int rs = tid / C::kLanes, col = tid % C::kLanes * 16;
-#pragma unroll
-    for (int i = 0; i < C::kHalf; ++i) {
-        const int row = (half * C::kHalf + i) * C::kRowsPerStep + rs, pg = __shfl_sync(0xffffffffu, page, row >> 4);
-        c.x[half][i] = make_uint4(0u, 0u, 0u, 0u);
-        if (pg >= 0 && u * kN + row < x.len)
-            c.x[half][i] = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)pg * st.b + (int64_t)x.h * st.h + (int64_t)((u * kN + row) & ((1 << p.c.bs_log2) - 1)) * st.n + col));
-    }
+__device__ __forceinline__ void copy_codes(uint32_t to, const void* from, bool real) {   // zeros where not real
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 load16(uint32_t at) {
+    uint4 w;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at));
+    return w;
 }
 __device__ __forceinline__ bool has_nan(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
 __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~__vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
-template <int D, int CODE>
-__device__ __forceinline__ void store_half(const Codes<D>& c, int half, uint32_t tile, int tid) {
-    using C = Codes<D>;
-    const int rs = tid / C::kLanes, u = tid % C::kLanes;
-    // Eight lanes that store at one time have to reach eight different runs of a 128-byte line: at D = 128 the lanes of the second box
-    // begin with their second run.
-    const int swap = D == 128 ? u >> 2 : 0;
-#pragma unroll
-    for (int i = 0; i < C::kHalf; ++i) {
-        const int row = (half * C::kHalf + i) * C::kRowsPerStep + rs;
-        const uint4 w = c.x[half][i];
-        uint32_t h[8];
-        codes_to_half<CODE>(swap ? w.z : w.x, h[0], h[1]);
-        codes_to_half<CODE>(swap ? w.w : w.y, h[2], h[3]);
-        codes_to_half<CODE>(swap ? w.x : w.z, h[4], h[5]);
-        codes_to_half<CODE>(swap ? w.y : w.w, h[6], h[7]);
-        store16(tile + image_at(row, 2 * u + swap), h[0], h[1], h[2], h[3]);
-        store16(tile + image_at(row, 2 * u + 1 - swap), h[4], h[5], h[6], h[7]);
-    }
+// 16 codes to their place in the image of a tile: runs 2 u and 2 u + 1 of a row.  Eight lanes that store at one time have to reach eight different runs
+// of a 128-byte line: at D = 128 the lanes of the second box begin with their second run (swap).
+template <int CODE>
+__device__ __forceinline__ void store_codes(const uint4& w, uint32_t row_at, uint32_t run_at, int swap) {
+    uint32_t h[8];
+    codes_to_half<CODE>(swap ? w.z : w.x, h[0], h[1]);
+    codes_to_half<CODE>(swap ? w.w : w.y, h[2], h[3]);
+    codes_to_half<CODE>(swap ? w.x : w.z, h[4], h[5]);
+    codes_to_half<CODE>(swap ? w.y : w.w, h[6], h[7]);
+    store16(row_at + (run_at ^ (swap << 4)), h[0], h[1], h[2], h[3]);
+    store16(row_at + (run_at ^ ((1 - swap) << 4)), h[4], h[5], h[6], h[7]);
 }
 
 // ------------------------------------------------------------------------------------------------ main kernel
 template <int D, int CODE, bool TWO>
 __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const CacheAttnParams p, const uint8_t* images, const float* factors) {
+    using S = Steps<D, TWO>;
     constexpr int kD = wide(D), kBox = kN * 128, kParts = TWO ? 2 : 1;
     constexpr uint32_t kTile = (uint32_t)tile_bytes(D);
     extern __shared__ uint8_t smem_raw[];
@@ -198,7 +183,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
     uint8_t* sQ = sm;
     uint8_t* sK = sQ + kParts * kTile;
     uint8_t* sV = sK + kStages * kTile;
-    Small& z = *reinterpret_cast<Small*>(sV + kStages * kTile);
+    uint8_t* queues = sV + kStages * kTile;
+    Small& z = *reinterpret_cast<Small*>(queues + 2 * S::kQueueBytes);
     uint64_t* bars = z.bars;
     volatile int* abort_flag = &z.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -215,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
         return;
     }
     if (threadIdx.x == 0) {
-        z.abort = 0;
+        z.abort = z.left = 0;
         for (int i = 0; i < kFlagSlots; ++i) z.nan_v[i] = 0;
         mbar_init(&bars[Q_FULL], 1);
         mbar_init(&bars[Q_EMPTY], 1);
@@ -231,6 +217,14 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             mbar_init(&bars[O_FULL + i], 1);
         }
         mbar_init(&bars[O_FREE], 16);
+        for (int i = 0; i < kUnitSlots; ++i) {
+            mbar_init(&bars[UNIT_FULL + i], 1);
+            mbar_init(&bars[UNIT_EMPTY + i], 8);         // K and V warps
+        }
+        for (int i = 0; i < kPieceSlots; ++i) {
+            mbar_init(&bars[PIECE_FULL + i], 1);
+            mbar_init(&bars[PIECE_EMPTY + i], 1 + 1 + 16);   // query loader, MMA issuer, softmax warps
+        }
         fence_mbar_init();
     }
     if (D == 32)   // columns 32 .. 63 of K and V are never written
@@ -245,7 +239,6 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = z.tmem;
-    Piece x;
 
     if (warp < kConvWarp0) {
         reg_dealloc<kRegsCtl>();
@@ -253,14 +246,19 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             // -------------------------------------------------------------- query tiles
             if (lane == 0) {
                 pdl_wait();
-                Walk walk(p, range);
                 int n = 0;
-                while (walk.next(p, x)) {
-                    if (x.live <= x.u0) continue;
+                for (int k = 0;; ++k) {
+                    const int slot = k % kPieceSlots;
+                    if (!mbar_wait(&bars[PIECE_FULL + slot], (k / kPieceSlots) & 1, p.status, PIECE_FULL, abort_flag)) break;
+                    const PieceNote& x = z.pieces[slot];
+                    if (x.b < 0) break;
+                    const int64_t item = (int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + x.tile;
+                    const bool some = x.count > 0;
+                    mbar_arrive(&bars[PIECE_EMPTY + slot]);
+                    if (!some) continue;
                     if (n > 0 && !mbar_wait(&bars[Q_EMPTY], (n - 1) & 1, p.status, Q_EMPTY, abort_flag)) break;
-                    const uint8_t* image = images + ((size_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + x.tile) * (kParts * kTile);
                     mbar_arrive_expect_tx(&bars[Q_FULL], kParts * kTile);
-                    for (int i = 0; i < kParts; ++i) bulk_load_1d(sQ + i * kTile, image + i * kTile, kTile, &bars[Q_FULL]);
+                    for (int i = 0; i < kParts; ++i) bulk_load_1d(sQ + i * kTile, images + ((size_t)item * kParts + i) * kTile, kTile, &bars[Q_FULL]);
                     ++n;
                 }
             }
@@ -288,12 +286,15 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 for (int kk = 0; kk < kN / 16; ++kk)
                     if (leader) umma_ts2(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b0 + kk * (2048 >> 4), kHi, idesc_pv, (add || kk > 0) ? 1u : 0u);
             };
-            Walk walk(p, range);
-            int gk = 0, gv = 0, pieces = 0, done[2] = {0, 0};
+            int gk = 0, gv = 0, pieces = 0, done0 = 0, done1 = 0;
             bool ok = true;
-            while (ok && walk.next(p, x)) {
-                const int count = x.live - x.u0;
-                if (count <= 0) continue;
+            for (int k = 0; ok; ++k) {
+                const int slot = k % kPieceSlots;
+                if (!(ok = mbar_wait_warp(&bars[PIECE_FULL + slot], (k / kPieceSlots) & 1, p.status, PIECE_FULL, abort_flag))) break;
+                const int count = z.pieces[slot].b < 0 ? -1 : z.pieces[slot].count;
+                mbar_arrive_warp(&bars[PIECE_EMPTY + slot], lane);
+                if (count < 0) break;
+                if (count == 0) continue;
                 auto next_scores = [&](int j) {   // Q K^T of the piece's unit j
                     if (!(ok = mbar_wait_warp(&bars[K_FULL + gk % kStages], (gk / kStages) & 1, p.status, K_FULL, abort_flag))) return;
                     tc_fence_after();
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 for (int j = 0; ok && j < count; ++j) {
                     const int i = j & 1, stage = gv % kStages;
                     if (!(ok = mbar_wait_warp(&bars[V_FULL + stage], (gv / kStages) & 1, p.status, V_FULL, abort_flag))) break;
-                    if (!(ok = mbar_wait_warp(&bars[P_FULL + i], done[i] & 1, p.status, P_FULL, abort_flag))) break;
+                    if (!(ok = mbar_wait_warp(&bars[P_FULL + i], (i ? done1 : done0) & 1, p.status, P_FULL, abort_flag))) break;
                     if (j == 0 && pieces > 0 && !(ok = mbar_wait_warp(&bars[O_FREE], (pieces - 1) & 1, p.status, O_FREE, abort_flag))) break;
                     tc_fence_after();
                     issue_pv(i, stage, j > 1);
@@ -319,89 +320,134 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                         umma_commit(&bars[O_FULL + i]);
                         umma_commit(&bars[V_EMPTY + stage]);
                     }
-                    ++done[i];
+                    if (i) ++done1;
+                    else ++done0;
                     ++gv;
                     if (j + 2 < count) next_scores(j + 2);
                 }
                 ++pieces;
             }
             __syncwarp();
+        } else if (warp == 3) {
+            // -------------------------------------------------------------- scout
+            Range r = range;
+            Load l = load_of(p, kN, kN, r.b, bad);
+            int q = 0, told = 0, pieces = 0;   // units, pieces, pieces with units so far
+            bool ok = true;
+            const int bs_mask = (1 << p.c.bs_log2) - 1;
+            // A note may be written over when the converters are through with a unit three later than its own: then its product is issued, and the
+            // exponentials of the note's unit are done.
+            auto unit_slot_free = [&]() {
+                return q < kUnitSlots || mbar_wait_warp(&bars[UNIT_EMPTY + (q + 3) % kUnitSlots], ((q - kUnitSlots + 3) / kUnitSlots) & 1, p.status, UNIT_EMPTY, abort_flag);
+            };
+            while (ok) {
+                const int slot = told % kPieceSlots;
+                if (told >= kPieceSlots && !(ok = mbar_wait_warp(&bars[PIECE_EMPTY + slot], ((told / kPieceSlots) - 1) & 1, p.status, PIECE_EMPTY, abort_flag))) break;
+                PieceNote x{-1, 0, 0, 0, 0, 0, 0, 0};
+                int seen = 0;
+                if (r.left > 0) {
+                    while (r.off >= (int64_t)l.units * l.items) {
+                        r.off -= (int64_t)l.units * l.items;
+                        l = load_of(p, kN, kN, ++r.b, bad);
+                    }
+                    const int item = (int)(r.off / l.units), tiles = l.items / p.c.Hkv;
+                    x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles; x.len = l.len; x.n = l.n;
+                    x.u0 = (int)(r.off - (int64_t)item * l.units);
+                    const int u1 = (int)min((int64_t)l.units, x.u0 + r.left);
+                    const int last = min(l.n - 1, (x.tile * kN + kN - 1) / p.G);          // the tile's last query
+                    const int most = p.causal ? max(l.len - l.n + last + 1, 0) : l.len;   // slots that some row sees
+                    x.count = max(min((most + kN - 1) / kN, u1) - x.u0, 0);
+                    x.whole = x.u0 == 0 && u1 == l.units;
+                    seen = p.causal ? l.len - l.n + x.tile * kN / p.G + 1 : l.len;        // slots below this are seen by every row
+                    r.off += u1 - x.u0;
+                    r.left -= u1 - x.u0;
+                }
+                if (lane == 0) z.pieces[slot] = x;
+                mbar_arrive_warp(&bars[PIECE_FULL + slot], lane);
+                ++told;
+                if (x.b < 0) break;
+                for (int u = x.u0; u < x.u0 + x.count; ++u, ++q) {
+                    if (!(ok = unit_slot_free())) break;
+                    UnitNote& note = z.units[q % kUnitSlots];
+                    const int page = unit_page(p, x, u, lane, bad);
+                    if (lane < 8) {
+                        const int slot0 = u * kN + 16 * lane, rows = page >= 0 ? min(x.len - slot0, 16) : 0;
+                        const int64_t at = (int64_t)max(page, 0) * p.c.Hkv + x.h, row = slot0 & bs_mask;
+                        const float ks = p.c.k_scale[at], vs = p.c.v_scale[at], size = vs == 0.f ? 1.f : max_nan(vs, 1e-30f);
+                        note.k[lane] = (uint64_t)(p.c.k + (int64_t)max(page, 0) * p.c.sk.b + (int64_t)x.h * p.c.sk.h + row * p.c.sk.n);
+                        note.v[lane] = (uint64_t)(p.c.v + (int64_t)max(page, 0) * p.c.sv.b + (int64_t)x.h * p.c.sv.h + row * p.c.sv.n);
+                        note.k_rows[lane] = rows;
+                        note.v_rows[lane] = vs == 0.f ? 0 : rows;                    // a scale of 0 makes zeros of its codes, whatever they are
+                        note.k_scale[lane] = page >= 0 ? ks : 0.f;
+                        note.lift[lane] = page >= 0 ? __log2f(size) : -INFINITY;     // slots of a block that is not there count nothing
+                        note.drop[lane] = 1.f / size;
+                        if (lane == 0) note.piece = pieces, note.hidden = (u + 1) * kN > seen;
+                    }
+                    mbar_arrive_warp(&bars[UNIT_FULL + q % kUnitSlots], lane);
+                }
+                pieces += x.count > 0;
+            }
+            if (ok && unit_slot_free()) {
+                if (lane == 0) z.units[q % kUnitSlots].piece = -1;
+                mbar_arrive_warp(&bars[UNIT_FULL + q % kUnitSlots], lane);
+            }
+            if (bad) report_bad_index(p.status, p.mirror);
         }
     } else if (warp < kSmxWarp0) {
         // ------------------------------------------------------------------ K and V: codes to fp16 operands
         if constexpr (kRegsConv < kLaunchRegs) reg_dealloc<kRegsConv>();
         const bool is_v = warp >= kConvWarp0 + 4;
         const int tid = (threadIdx.x - kConvWarp0 * 32) & 127;
-        const uint8_t* base = is_v ? p.c.v : p.c.k;
-        const Strides st = is_v ? p.c.sv : p.c.sk;
         const uint32_t tiles = smem_u32(is_v ? sV : sK);
         const int full = is_v ? V_FULL : K_FULL, empty = is_v ? V_EMPTY : K_EMPTY;
-        Walk walk(p, range);
-        Codes<D> c;
-        int q = 0, pieces = 0;   // units, pieces so far
-        bool ok = true, more = false;
-        // the first piece with something to do
-        while ((more = walk.next(p, x)) && x.live <= x.u0) {}
-        int page = more ? unit_page(p, x, x.u0, lane, bad) : -1;
-        float scale = 0.f;   // V: lane l < 8 the scale of slots 16 l ..; a scale of 0 makes zeros of its codes, whatever they are
-        auto v_zero = [&](int& pg) {
-            if (!is_v) return;
-            scale = pg >= 0 ? p.c.v_scale[(int64_t)pg * p.c.Hkv + x.h] : 0.f;
-            if (scale == 0.f) pg = -1;
+        const int col = tid % S::kLanes * 16, row0 = tid / S::kLanes, row_in_group = row0 & 15;
+        const int64_t row_offset = (int64_t)row_in_group * (is_v ? p.c.sv.n : p.c.sk.n) + col;
+        const uint32_t queue = smem_u32(queues) + (is_v ? S::kQueueBytes : 0) + tid * 16;   // step k at queue + k * 2048
+        // rows row0 + kRowsPerStep k: the same row of a swizzle atom in every step, where steps are multiples of 8 rows
+        static_assert(S::kRowsPerStep % 16 == 0, "");
+        const int run = col / 8, swap = D == 128 ? run >> 3 : 0;
+        const uint32_t row_at = (run >> 3) * kBox + row0 * 128, run_at = ((run & 7) ^ (row0 & 7)) << 4;
+        auto copy = [&](const UnitNote& note, int step, int place) {
+            const int group = (step * S::kRowsPerStep + row0) >> 4;
+            const uint8_t* from = reinterpret_cast<const uint8_t*>(is_v ? note.v[group] : note.k[group]);
+            const bool real = row_in_group < (is_v ? note.v_rows[group] : note.k_rows[group]);
+            copy_codes(queue + place * 2048, real ? from + row_offset : from, real);
         };
-        v_zero(page);
-        if (more) load_half<D>(c, 0, base, st, p, x, x.u0, page, tid);
-        while (ok && more) {
-            const int seen = least_seen(p, x);
-            for (int u = x.u0; u < x.live; ++u, ++q) {
-                const int stage = q % kStages;
-                load_half<D>(c, 1, base, st, p, x, u, page, tid);
-                if (q >= kStages && !(ok = mbar_wait_warp(&bars[empty + stage], ((q / kStages) - 1) & 1, p.status, empty, abort_flag))) break;
-                if (!is_v && tid < 8) {   // the unit's scales, for the softmax groups
-                    const int slot = q % kScaleSlots;
-                    const int64_t at = (int64_t)page * p.c.Hkv + x.h;
-                    const float ks = page >= 0 ? p.c.k_scale[at] : 0.f, vs = page >= 0 ? p.c.v_scale[at] : 0.f;
-                    const float size = vs == 0.f ? 1.f : max_nan(vs, 1e-30f);
-                    z.k_scale[slot][tid] = ks;
-                    z.lift[slot][tid] = page >= 0 ? __log2f(size) : -INFINITY;   // slots of a block that is not there count nothing
-                    z.drop[slot][tid] = 1.f / size;
-                }
-                const bool hidden = is_v && CODE == COROPE_CODE_E4M3 && (u + 1) * kN > seen;
-                const uint32_t tile = tiles + stage * kTile;
-                auto clean = [&](int half) {   // NaN that some rows must not see: left out here, put in at the end of the piece
-                    if (!hidden) return;
-                    bool nan = false;
+        auto wait_note = [&](int q) { return mbar_wait_warp(&bars[UNIT_FULL + q % kUnitSlots], (q / kUnitSlots) & 1, p.status, UNIT_FULL, abort_flag); };
+        bool more = wait_note(0) && z.units[0].piece >= 0;
+        if (more)
 #pragma unroll
-                    for (int i = 0; i < Codes<D>::kHalf; ++i) {
-                        uint4& w = c.x[half][i];
-                        nan |= has_nan(w.x) || has_nan(w.y) || has_nan(w.z) || has_nan(w.w);
-                        w = make_uint4(without_nan(w.x), without_nan(w.y), without_nan(w.z), without_nan(w.w));
-                    }
-                    if (nan) z.nan_v[pieces % kFlagSlots] = 1;
-                };
-                clean(0);
-                store_half<D, CODE>(c, 0, tile, tid);
-                clean(1);
-                // the next unit's blocks and first codes are on their way while this one's second half is stored
-                if (u + 1 < x.live) {
-                    page = unit_page(p, x, u + 1, lane, bad);
-                    v_zero(page);
-                    load_half<D>(c, 0, base, st, p, x, u + 1, page, tid);
+            for (int k = 0; k < S::kDepth; ++k) {
+                copy(z.units[0], k, k);
+                commit_copies();
+            }
+        for (int q = 0; more; ++q) {
+            const int stage = q % kStages;
+            const UnitNote &note = z.units[q % kUnitSlots], &next = z.units[(q + 1) % kUnitSlots];
+            if (!wait_note(q + 1)) break;
+            more = next.piece >= 0;
+            if (q >= kStages && !mbar_wait_warp(&bars[empty + stage], ((q / kStages) - 1) & 1, p.status, empty, abort_flag)) break;
+            // NaN in V that some rows must not see is left out here and put in at the end of the piece
+            const bool hidden = is_v && CODE == COROPE_CODE_E4M3 && note.hidden != 0;
+            const uint32_t at = tiles + stage * kTile + row_at;
+#pragma unroll
+            for (int k = 0; k < S::kSteps; ++k) {
+                wait_copies<S::kDepth - 1>();
+                uint4 w = load16(queue + k % S::kDepth * 2048);
+                if (k + S::kDepth < S::kSteps) copy(note, k + S::kDepth, k % S::kDepth);
+                else if (more) copy(next, k + S::kDepth - S::kSteps, k % S::kDepth);
+                commit_copies();
+                if (hidden) {
+                    if (has_nan(w.x) || has_nan(w.y) || has_nan(w.z) || has_nan(w.w)) z.nan_v[note.piece % kFlagSlots] = 1;
+                    w = make_uint4(without_nan(w.x), without_nan(w.y), without_nan(w.z), without_nan(w.w));
                 }
-                store_half<D, CODE>(c, 1, tile, tid);
-                fence_proxy_async();
-                mbar_arrive_warp(&bars[full + stage], lane);
+                store_codes<CODE>(w, at + k * (S::kRowsPerStep * 128), run_at, swap);
             }
-            if (!ok) break;
-            ++pieces;
-            while ((more = walk.next(p, x)) && x.live <= x.u0) {}
-            if (more) {
-                page = unit_page(p, x, x.u0, lane, bad);
-                v_zero(page);
-                load_half<D>(c, 0, base, st, p, x, x.u0, page, tid);
-            }
+            fence_proxy_async();
+            mbar_arrive_warp(&bars[full + stage], lane);
+            if (lane == 0) mbar_arrive(&bars[UNIT_EMPTY + q % kUnitSlots]);
         }
-        if (bad || walk.bad) report_bad_index(p.status, p.mirror);
+        wait_copies<0>();
     } else {
         // ------------------------------------------------------------------ softmax groups
         reg_alloc<kRegsSmx>();
@@ -410,29 +456,34 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
         const uint32_t tS = tmem + lane_base + grp * 128 + half * 64, tO = tmem + lane_base + 256;
         pdl_wait();        // the rows' factors
-        Walk walk(p, range);
-        int q = 0, pieces = 0, gs = 0;             // units, pieces, units of this group so far
-        int ends[2] = {0, 0};                      // units of both groups at the end of the piece
+        int q = 0, pieces = 0, gs = 0;             // units, pieces with units, units of this group so far
+        int ends0 = 0, ends1 = 0;                  // units of both groups at the end of the piece
         bool ok = true;
-        // A wait that ran out is not left by: the warps of both groups meet at barriers, so each goes through all of its units, if on what happens
-        // to be there (the host learns of it), and waits for nothing more.
+        // A wait that ran out is not left by: the warps of both groups meet at barriers, so each goes through all that the scout has told, if on what
+        // happens to be there (the host learns of it), and waits for nothing more.  What is told comes from the scout's own
+        // waits; if that gave up, all 16 warps look at the same note, the one behind the last, and find the flag or the end.
         auto wait = [&](int bar, int parity) {
             if (ok) ok = mbar_wait_warp(&bars[bar], parity, p.status, bar, abort_flag);
             tc_fence_after();
         };
-        while (walk.next(p, x)) {
-            const int count = max(x.live - x.u0, 0), grow = x.tile * kN + row, t = grow / p.G;
-            const int64_t item = (int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + x.tile;
-            const float factor = factors[item * kN + row];
-            const int sees = p.causal ? x.len - x.n + t + 1 : x.len, seen = least_seen(p, x);
+        for (int k = 0;; ++k) {
+            const int place = k % kPieceSlots;
+            // all leave together: the first to find no piece in time tells the others at the barrier
+            if (!mbar_wait_warp(&bars[PIECE_FULL + place], (k / kPieceSlots) & 1, p.status, PIECE_FULL, abort_flag)) z.left = 1;
+            named_bar_sync(9, 512);
+            const PieceNote& x = z.pieces[place];
+            if (z.left != 0 || x.b < 0) break;
+            const int count = x.count, grow = x.tile * kN + row, t = grow / p.G, u0 = x.u0;
+            const float factor = factors[((int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + x.tile) * kN + row];
+            const int sees = p.causal ? x.len - x.n + t + 1 : x.len;
             float m = kLowest, l = 0.f;
             for (int j = grp; j < count; j += 2, ++gs) {
-                const int u = x.u0 + j, slot = (q + j) % kScaleSlots;
+                const UnitNote& note = z.units[(q + j) % kUnitSlots];
                 wait(S_FULL + grp, gs & 1);
                 uint32_t s0[32], s1[32];
                 COROPE_TMEM_LD32(tS, s0);
                 COROPE_TMEM_LD32(tS + 32, s1);
-                const float4 ks = *reinterpret_cast<const float4*>(&z.k_scale[slot][half * 4]), up = *reinterpret_cast<const float4*>(&z.lift[slot][half * 4]);
+                const float4 ks = *reinterpret_cast<const float4*>(&note.k_scale[half * 4]), up = *reinterpret_cast<const float4*>(&note.lift[half * 4]);
                 tmem_wait_ld();
                 // to units of log2, the scale of V in the exponent
                 auto scale_group = [&](uint32_t* s, float k_scale, float lift) {
@@ -450,8 +501,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 scale_group(s0 + 16, ks.y, up.y);
                 scale_group(s1, ks.z, up.z);
                 scale_group(s1 + 16, ks.w, up.w);
-                if ((u + 1) * kN > seen) {
-                    const int last = sees - u * kN - half * 64;   // columns from here on are hidden
+                if (note.hidden) {
+                    const int last = sees - (u0 + j) * kN - half * 64;   // columns from here on are hidden
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         if (i >= last) s0[i] = 0xff800000u;
@@ -473,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 const float m_old = m;
                 m = need ? top : m;
                 const uint64_t neg_m = f2_pack(-m, -m);
-                const float4 drop = *reinterpret_cast<const float4*>(&z.drop[slot][half * 4]);
+                const float4 drop = *reinterpret_cast<const float4*>(&note.drop[half * 4]);
                 float add = 0.f;
                 auto exp_group = [&](const uint32_t* s, float drop_g, uint32_t* pk) {
                     uint64_t sum = 0;
@@ -522,24 +573,23 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 mbar_arrive_warp(&bars[P_FULL + grp], lane);
             }
             q += count;
-            ends[0] += (count + 1) / 2;
-            ends[1] += count / 2;
+            ends0 += (count + 1) / 2;
+            ends1 += count / 2;
 
             // the piece's sums: both groups' O, a quarter of the columns to each warpgroup
-            const int buf = pieces & 1;
-            if (half == 0) z.end_max[buf][grp][row] = m;
-            z.end_sum[buf][grp][half][row] = l;
-            named_bar_sync(9, 512);
-            if (count > 0) wait(O_FULL, (ends[0] - 1) & 1);
-            if (count > 1) wait(O_FULL + 1, (ends[1] - 1) & 1);
-            const float m0 = z.end_max[buf][0][row], m1 = z.end_max[buf][1][row], top = fmaxf(m0, m1);
+            if (half == 0) z.end_max[grp][row] = m;
+            z.end_sum[grp][half][row] = l;
+            named_bar_sync(9, 512);   // (the exchange is written again behind the next piece's first barrier at the earliest)
+            if (count > 0) wait(O_FULL, (ends0 - 1) & 1);
+            if (count > 1) wait(O_FULL + 1, (ends1 - 1) & 1);
+            const float m0 = z.end_max[0][row], m1 = z.end_max[1][row], top = fmaxf(m0, m1);
             const float w0 = fast_exp2(m0 - top), w1 = fast_exp2(m1 - top);
-            const float all = (z.end_sum[buf][0][0][row] + z.end_sum[buf][0][1][row]) * w0 + (z.end_sum[buf][1][0][row] + z.end_sum[buf][1][1][row]) * w1;
-            const bool whole = x.u0 == 0 && x.u1 == x.units, some = t < x.n && all != 0.f;
+            const float all = (z.end_sum[0][0][row] + z.end_sum[0][1][row]) * w0 + (z.end_sum[1][0][row] + z.end_sum[1][1][row]) * w1;
+            const bool whole = x.whole != 0, some = t < x.n && all != 0.f;
             const float inv = whole ? 1.f / all : 1.f;
             constexpr int kCols = kD / 4;
             const int col0 = (grp * 2 + half) * kCols;
-            const int64_t part = (2 * (int64_t)blockIdx.x + (x.u0 == 0 ? 1 : 0)) * kN + row;
+            const int64_t part = (2 * (int64_t)blockIdx.x + (u0 == 0 ? 1 : 0)) * kN + row;
             const int64_t to = (int64_t)x.b * p.so.b + (int64_t)(x.h * p.G + grow - t * p.G) * p.so.h + (int64_t)t * p.so.n;
             const bool fix = CODE == COROPE_CODE_E4M3 && count > 0 && z.nan_v[pieces % kFlagSlots] != 0;
 #pragma unroll
@@ -563,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 if (col0 + k >= D) continue;
                 if (fix) {   // NaN in V, slot by slot: to the rows that see it
 #pragma unroll 1
-                    for (int s = max(seen, x.u0 * kN) & ~(kN - 1); s < min(sees, x.live * kN); ++s) {
+                    for (int s = u0 * kN; s < min(sees, (u0 + count) * kN); ++s) {
                         bool far = false;
                         const int page = cache_page(p.s, p.c.bs_log2, p.c.num_blocks, x.b, s, far);
                         if (page < 0 || p.c.v_scale[(int64_t)page * p.c.Hkv + x.h] == 0.f) continue;
@@ -593,9 +643,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 // the flag of the piece before: every thread has read it, and its place is not taken again before this thread has come by
                 if (wsm == 0 && lane == 0 && pieces > 0) z.nan_v[(pieces - 1) % kFlagSlots] = 0;
                 ++pieces;
-            } else {
-                named_bar_sync(9, 512);   // the exchange above is not overwritten while someone reads it
             }
+            mbar_arrive_warp(&bars[PIECE_EMPTY + place], lane);
         }
         tc_fence_before();
     }
@@ -612,16 +661,18 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
 // is 128 slots of a K / V head: its K stays, and the tiles of query rows (both parts) stream by.  Bound by the exponentials.
 //   warp 0  query tiles, with their rows' factors and lse;  warp 1  MMA issuer;  warps 4-7  K;  warps 8-11, 12-15  the even and odd tiles
 constexpr int kSumThreads = 512;
-enum SumBar { W_K_FULL = 0, W_K_EMPTY = 2, W_Q_FULL = 4, W_Q_EMPTY = 6, W_ROWS = 8, W_S_FULL = 10, W_S_FREE = 12, W_NUM_BARS = 14 };
-struct SumSmall {
-    float factor[2][kN], lse[2][kN], sum[2][kN];
+constexpr int kRowSlots = 4;
+__host__ __device__ constexpr int sum_stages(int D) { return D == 128 ? 2 : 4; }   // of query tiles
+enum SumBar { W_K_FULL = 0, W_K_EMPTY = 2, W_S_FULL = 4, W_S_FREE = 6, W_ROWS = 8, W_Q_FULL = W_ROWS + kRowSlots, W_Q_EMPTY = W_Q_FULL + 4, W_NUM_BARS = W_Q_EMPTY + 4 };
+struct alignas(16) SumSmall {   // factor and lse are read four at a time
+    float factor[kRowSlots][kN], lse[kRowSlots][kN], sum[2][kN];
     float k_scale[2][8];
     int page[2][8];
     uint64_t bars[W_NUM_BARS];
     uint32_t tmem;
     int abort;
 };
-constexpr size_t sum_smem_bytes(int D) { return (2 * 2 + 2) * tile_bytes(D) + sizeof(SumSmall) + 1024; }
+constexpr size_t sum_smem_bytes(int D) { return (2 * sum_stages(D) + 2) * tile_bytes(D) + sizeof(SumSmall) + 1024; }
 static_assert(sum_smem_bytes(128) <= 232448 - 1024, "shared memory budget");
 
 struct Unit {
@@ -665,8 +716,9 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
     constexpr uint32_t kTile = (uint32_t)tile_bytes(D);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t* sQ = sm;                       // [stage][part]
-    uint8_t* sK = sQ + 4 * kTile;           // [stage]
+    constexpr int kQStages = sum_stages(D);
+    uint8_t* sQ = sm;                            // [stage][part]
+    uint8_t* sK = sQ + 2 * kQStages * kTile;     // [stage]
     SumSmall& z = *reinterpret_cast<SumSmall*>(sK + 2 * kTile);
     uint64_t* bars = z.bars;
     volatile int* abort_flag = &z.abort;
@@ -687,12 +739,14 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars[W_K_FULL + i], 4);
             mbar_init(&bars[W_K_EMPTY + i], 4);      // the group that ends a unit
-            mbar_init(&bars[W_Q_FULL + i], 1);
-            mbar_init(&bars[W_Q_EMPTY + i], 1);
-            mbar_init(&bars[W_ROWS + i], 1);
             mbar_init(&bars[W_S_FULL + i], 1);
             mbar_init(&bars[W_S_FREE + i], 4);
         }
+        for (int i = 0; i < kQStages; ++i) {
+            mbar_init(&bars[W_Q_FULL + i], 1);
+            mbar_init(&bars[W_Q_EMPTY + i], 1);
+        }
+        for (int i = 0; i < kRowSlots; ++i) mbar_init(&bars[W_ROWS + i], 1);
         fence_mbar_init();
     }
     if (D == 32)
@@ -716,22 +770,25 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
         int q = 0;
         while (ok && walk.next(p, x))
             for (int t = x.tile0; ok && t < x.tiles; ++t, ++q) {
-                const int i = q & 1;
-                if (q >= 2) {
-                    if (!(ok = mbar_wait_warp(&bars[W_Q_EMPTY + i], ((q >> 1) - 1) & 1, p.status, W_Q_EMPTY, abort_flag))) break;
-                    if (!(ok = mbar_wait_warp(&bars[W_S_FREE + i], ((q >> 1) - 1) & 1, p.status, W_S_FREE, abort_flag))) break;
-                }
+                const int i = q % kQStages, slot = q % kRowSlots;
                 const int64_t item = (int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + t;
+                if (q >= kQStages && !(ok = mbar_wait_warp(&bars[W_Q_EMPTY + i], ((q / kQStages) - 1) & 1, p.status, W_Q_EMPTY, abort_flag))) break;
                 if (lane == 0) {
                     mbar_arrive_expect_tx(&bars[W_Q_FULL + i], 2 * kTile);
                     for (int part = 0; part < 2; ++part) bulk_load_1d(sQ + (2 * i + part) * kTile, images + ((size_t)item * 2 + part) * kTile, kTile, &bars[W_Q_FULL + i]);
                 }
-                for (int r = lane; r < kN; r += 32) {
-                    const int row = t * kN + r;
-                    z.factor[i][r] = factors[item * kN + r];
-                    z.lse[i][r] = row < x.n * p.G ? p.lse[((int64_t)x.b * p.c.Hkv + x.h) * p.T * p.G + row] : INFINITY;
+                float f[kN / 32], e[kN / 32];
+#pragma unroll
+                for (int k = 0; k < kN / 32; ++k) {
+                    const int row = t * kN + 32 * k + lane;
+                    f[k] = factors[item * kN + 32 * k + lane];
+                    e[k] = row < x.n * p.G ? p.lse[((int64_t)x.b * p.c.Hkv + x.h) * p.T * p.G + row] : INFINITY;
                 }
-                mbar_arrive_warp(&bars[W_ROWS + i], lane);
+                // the slot's last tile, q - 4, has been summed
+                if (q >= kRowSlots && !(ok = mbar_wait_warp(&bars[W_S_FREE + (q & 1)], ((q >> 1) - 2) & 1, p.status, W_S_FREE, abort_flag))) break;
+#pragma unroll
+                for (int k = 0; k < kN / 32; ++k) z.factor[slot][32 * k + lane] = f[k], z.lse[slot][32 * k + lane] = e[k];
+                mbar_arrive_warp(&bars[W_ROWS + slot], lane);
             }
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
@@ -745,7 +802,8 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
             if (!(ok = mbar_wait_warp(&bars[W_K_FULL + stage], (units >> 1) & 1, p.status, W_K_FULL, abort_flag))) break;
             for (int t = x.tile0; t < x.tiles; ++t, ++q) {
                 const int i = q & 1;
-                if (!(ok = mbar_wait_warp(&bars[W_Q_FULL + i], (q >> 1) & 1, p.status, W_Q_FULL, abort_flag))) break;
+                const int from = q % kQStages;
+                if (!(ok = mbar_wait_warp(&bars[W_Q_FULL + from], (q / kQStages) & 1, p.status, W_Q_FULL, abort_flag))) break;
                 if (q >= 2 && !(ok = mbar_wait_warp(&bars[W_S_FREE + i], ((q >> 1) - 1) & 1, p.status, W_S_FREE, abort_flag))) break;
                 tc_fence_after();
 #pragma unroll
@@ -753,11 +811,11 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
 #pragma unroll
                     for (int kk = 0; kk < kD / 16; ++kk) {
                         const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
-                        if (leader) umma_ss2(tmem + i * 128, k_lo + stage * (kTile >> 4) + off, kHi, q_lo + (2 * i + part) * (kTile >> 4) + off, kHi, idesc, part == 0 || kk > 0);
+                        if (leader) umma_ss2(tmem + i * 128, k_lo + stage * (kTile >> 4) + off, kHi, q_lo + (2 * from + part) * (kTile >> 4) + off, kHi, idesc, part == 0 || kk > 0);
                     }
                 if (leader) {
                     umma_commit(&bars[W_S_FULL + i]);
-                    umma_commit(&bars[W_Q_EMPTY + i]);
+                    umma_commit(&bars[W_Q_EMPTY + from]);
                 }
             }
             ++units;
@@ -765,22 +823,29 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
         __syncwarp();
     } else if (warp >= 4 && warp < 8) {
         // ------------------------------------------------------------------ K
-        const int tid = threadIdx.x & 127;
+        using S = Steps<D, true>;
+        const int tid = threadIdx.x & 127, col = tid % S::kLanes * 16, row0 = tid / S::kLanes, in_block_mask = (1 << p.c.bs_log2) - 1;
+        const int run = col / 8, swap = D == 128 ? run >> 3 : 0;
+        const uint32_t row_at = (run >> 3) * kBox + row0 * 128, run_at = ((run & 7) ^ (row0 & 7)) << 4;
         int units = 0;
         while (walk.next(p, x)) {
             const int stage = units & 1;
-            Codes<D> c;
             const int page = unit_page(p, x, x.u, lane, bad);
-            const Piece as{x.b, x.h, 0, x.u, x.u + 1, x.u + 1, x.len, x.n, 0};
-            load_half<D>(c, 0, p.c.k, p.c.sk, p, as, x.u, page, tid);
-            load_half<D>(c, 1, p.c.k, p.c.sk, p, as, x.u, page, tid);
             if (units >= 2 && !mbar_wait_warp(&bars[W_K_EMPTY + stage], ((units >> 1) - 1) & 1, p.status, W_K_EMPTY, abort_flag)) break;
             if (tid < 8) {
                 z.k_scale[stage][tid] = page >= 0 ? p.c.k_scale[(int64_t)page * p.c.Hkv + x.h] : 0.f;
                 z.page[stage][tid] = page;
             }
-            store_half<D, CODE>(c, 0, smem_u32(sK) + stage * kTile, tid);
-            store_half<D, CODE>(c, 1, smem_u32(sK) + stage * kTile, tid);
+            uint4 w[S::kSteps];
+#pragma unroll
+            for (int k = 0; k < S::kSteps; ++k) {
+                const int row = k * S::kRowsPerStep + row0, slot = x.u * kN + row, pg = __shfl_sync(0xffffffffu, page, row >> 4);
+                w[k] = make_uint4(0u, 0u, 0u, 0u);
+                if (pg >= 0 && slot < x.len)
+                    w[k] = *reinterpret_cast<const uint4*>(p.c.k + (int64_t)pg * p.c.sk.b + (int64_t)x.h * p.c.sk.h + (int64_t)(slot & in_block_mask) * p.c.sk.n + col);
+            }
+#pragma unroll
+            for (int k = 0; k < S::kSteps; ++k) store_codes<CODE>(w[k], smem_u32(sK) + stage * kTile + row_at + k * (S::kRowsPerStep * 128), run_at, swap);
             fence_proxy_async();
             mbar_arrive_warp(&bars[W_K_FULL + stage], lane);
             ++units;
@@ -802,7 +867,8 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
             float w = 0.f;
             for (int j = 0; j < count; ++j, ++q) {
                 if ((q & 1) != grp) continue;
-                wait(W_ROWS + grp, (q >> 1) & 1);
+                const int rows = q % kRowSlots;
+                wait(W_ROWS + rows, (q / kRowSlots) & 1);
                 wait(W_S_FULL + grp, (q >> 1) & 1);
                 tc_fence_after();
                 // columns that see the slot: from the first row whose query does to the last row with a query
@@ -818,7 +884,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
                     uint64_t sum = 0;
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(&z.factor[grp][k + i]), e = *reinterpret_cast<const float4*>(&z.lse[grp][k + i]);
+                        const float4 f = *reinterpret_cast<const float4*>(&z.factor[rows][k + i]), e = *reinterpret_cast<const float4*>(&z.lse[rows][k + i]);
                         float d[4];
                         f2_unpack(f2_fma(f2_pack_bits(s[i], s[i + 1]), f2_mul(f2_pack(f.x, f.y), ks2), f2_pack(-e.x, -e.y)), d[0], d[1]);
                         f2_unpack(f2_fma(f2_pack_bits(s[i + 2], s[i + 3]), f2_mul(f2_pack(f.z, f.w), ks2), f2_pack(-e.z, -e.w)), d[2], d[3]);
@@ -874,7 +940,7 @@ int launch_t(const CacheAttnParams& p, uint8_t* images, float* factors, unsigned
     static std::atomic<uint64_t> done{0};
     if (int e = allow_smem(cache_attn_tile_kernel<D, CODE, TWO>, smem_bytes(D, TWO), done)) return e;
     count_launch(2);
-    cache_pack_kernel<D, TWO><<<(unsigned)(p.s.B * p.c.Hkv * p.row_tiles), 256, 0, s>>>(p, images, factors);
+    cache_pack_kernel<D, TWO><<<(unsigned)(p.s.B * p.c.Hkv * p.row_tiles * kPackBlocks), kPackWarps * 32, 0, s>>>(p, images, factors);
     if (int e = (int)cudaGetLastError()) return e;
     return launch_dependent(cache_attn_tile_kernel<D, CODE, TWO>, blocks, kThreads, smem_bytes(D, TWO), s, p, (const uint8_t*)images, (const float*)factors);
 }

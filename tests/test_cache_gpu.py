@@ -197,6 +197,9 @@ ATTENDS = [
     ([140, 160], [130, 160], 160, 1, 4, 128, 64, BF16, E4M3, True, True, True),    # a chunk: 640 rows a head
     ([1031], None, 200, 2, 3, 64, 32, F16, INT8, True, True, False),
     ([300, 77], [65, 64], 65, 1, 2, 32, 16, F32, E4M3, True, True, True),
+    ([2500, 1900, 0], [200, 131, 0], 200, 2, 4, 64, 32, F16, E4M3, True, True, True),    # hundreds of 128 x 128 units: several a block, pieces of items
+    ([5000, 4000], [70, 300], 300, 2, 1, 128, 16, BF16, INT8, True, True, True),
+    ([1500], None, 300, 5, 2, 32, 128, F16, INT8, False, False, True),
 ]
 
 
