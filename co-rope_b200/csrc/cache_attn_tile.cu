@@ -44,6 +44,8 @@ struct alignas(16) UnitNote {   // its floats are read four at a time
     int k_rows[8], v_rows[8];
     int piece;       // number of its piece among those with units, -1: there is no unit any more
     int hidden;      // some row of the tile does not see some slot
+    int full;        // every group has 16 rows, of K and of V
+    int pad;
 };
 static_assert(sizeof(UnitNote) % 16 == 0 && offsetof(UnitNote, k_scale) % 16 == 0 && offsetof(UnitNote, lift) % 16 == 0 && offsetof(UnitNote, drop) % 16 == 0, "");
 // A piece: units [u0, u0 + count) of the item.  b < 0: there is none any more.
@@ -138,6 +140,7 @@ template <int D, bool TWO>
 struct Steps {
     static constexpr int kLanes = D / 16, kRowsPerStep = 128 / kLanes, kSteps = kN / kRowsPerStep;
     static constexpr int kDepth = D == 128 && TWO ? 4 : kSteps;
+    static constexpr int kAtOnce = kDepth >= 8 ? 4 : 2;     // steps whose loads are under way together
     static constexpr int kQueueBytes = kDepth * 16 * 128;   // of one group
 };
 // the block of slots 16 lane .. of unit u, lane < 8, or -1
@@ -146,30 +149,28 @@ __device__ __forceinline__ int unit_page(const CacheAttnParams& p, const X& x, i
     const int slot = u * kN + 16 * lane;
     return lane < 8 && slot < x.len ? cache_page(p.s, p.c.bs_log2, p.c.num_blocks, x.b, slot, bad) : -1;
 }
+__device__ __forceinline__ void copy_codes(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ void copy_codes(uint32_t to, const void* from, bool real) {   // zeros where not real
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 load16(uint32_t at) {
-    uint4 w;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at));
+__device__ __forceinline__ uint2 load8(uint32_t at) {
+    uint2 w;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(at));
     return w;
 }
 __device__ __forceinline__ bool has_nan(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
 __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~__vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
-// 16 codes to their place in the image of a tile: runs 2 u and 2 u + 1 of a row.  Eight lanes that store at one time have to reach eight different runs
-// of a 128-byte line: at D = 128 the lanes of the second box begin with their second run (swap).
+// Eight codes to a run of the image of a tile.  A thread's 16 codes make two runs of a row; eight lanes that store at one time have to reach eight
+// different runs of a 128-byte line, so at D = 128 the lanes of the second box begin with their second run (`swap`).
 template <int CODE>
-__device__ __forceinline__ void store_codes(const uint4& w, uint32_t row_at, uint32_t run_at, int swap) {
-    uint32_t h[8];
-    codes_to_half<CODE>(swap ? w.z : w.x, h[0], h[1]);
-    codes_to_half<CODE>(swap ? w.w : w.y, h[2], h[3]);
-    codes_to_half<CODE>(swap ? w.x : w.z, h[4], h[5]);
-    codes_to_half<CODE>(swap ? w.y : w.w, h[6], h[7]);
-    store16(row_at + (run_at ^ (swap << 4)), h[0], h[1], h[2], h[3]);
-    store16(row_at + (run_at ^ ((1 - swap) << 4)), h[4], h[5], h[6], h[7]);
+__device__ __forceinline__ void store_codes(const uint2& w, uint32_t at) {
+    uint32_t h[4];
+    codes_to_half<CODE>(w.x, h[0], h[1]);
+    codes_to_half<CODE>(w.y, h[2], h[3]);
+    store16(at, h[0], h[1], h[2], h[3]);
 }
 
 // ------------------------------------------------------------------------------------------------ main kernel
@@ -381,7 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                         note.k_scale[lane] = page >= 0 ? ks : 0.f;
                         note.lift[lane] = page >= 0 ? __log2f(size) : -INFINITY;     // slots of a block that is not there count nothing
                         note.drop[lane] = 1.f / size;
-                        if (lane == 0) note.piece = pieces, note.hidden = (u + 1) * kN > seen;
+                        const bool full = __all_sync(0xffu, rows == 16 && vs != 0.f);
+                        if (lane == 0) note.piece = pieces, note.hidden = (u + 1) * kN > seen, note.full = full;
                     }
                     mbar_arrive_warp(&bars[UNIT_FULL + q % kUnitSlots], lane);
                 }
@@ -406,12 +408,17 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
         // rows row0 + kRowsPerStep k: the same row of a swizzle atom in every step, where steps are multiples of 8 rows
         static_assert(S::kRowsPerStep % 16 == 0, "");
         const int run = col / 8, swap = D == 128 ? run >> 3 : 0;
-        const uint32_t row_at = (run >> 3) * kBox + row0 * 128, run_at = ((run & 7) ^ (row0 & 7)) << 4;
+        const uint32_t first_at = (run >> 3) * kBox + row0 * 128 + ((((run & 7) ^ (row0 & 7)) ^ swap) << 4), second_at = first_at ^ 16;
+        const uint32_t first_from = queue + swap * 8, second_from = queue + (1 - swap) * 8;
         auto copy = [&](const UnitNote& note, int step, int place) {
             const int group = (step * S::kRowsPerStep + row0) >> 4;
             const uint8_t* from = reinterpret_cast<const uint8_t*>(is_v ? note.v[group] : note.k[group]);
-            const bool real = row_in_group < (is_v ? note.v_rows[group] : note.k_rows[group]);
-            copy_codes(queue + place * 2048, real ? from + row_offset : from, real);
+            if (note.full) {
+                copy_codes(queue + place * 2048, from + row_offset);
+            } else {
+                const bool real = row_in_group < (is_v ? note.v_rows[group] : note.k_rows[group]);
+                copy_codes(queue + place * 2048, real ? from + row_offset : from, real);
+            }
         };
         auto wait_note = [&](int q) { return mbar_wait_warp(&bars[UNIT_FULL + q % kUnitSlots], (q / kUnitSlots) & 1, p.status, UNIT_FULL, abort_flag); };
         bool more = wait_note(0) && z.units[0].piece >= 0;
@@ -429,19 +436,38 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             if (q >= kStages && !mbar_wait_warp(&bars[empty + stage], ((q / kStages) - 1) & 1, p.status, empty, abort_flag)) break;
             // NaN in V that some rows must not see is left out here and put in at the end of the piece
             const bool hidden = is_v && CODE == COROPE_CODE_E4M3 && note.hidden != 0;
-            const uint32_t at = tiles + stage * kTile + row_at;
+            const uint32_t first = tiles + stage * kTile + first_at, second = tiles + stage * kTile + second_at;
 #pragma unroll
-            for (int k = 0; k < S::kSteps; ++k) {
-                wait_copies<S::kDepth - 1>();
-                uint4 w = load16(queue + k % S::kDepth * 2048);
-                if (k + S::kDepth < S::kSteps) copy(note, k + S::kDepth, k % S::kDepth);
-                else if (more) copy(next, k + S::kDepth - S::kSteps, k % S::kDepth);
-                commit_copies();
-                if (hidden) {
-                    if (has_nan(w.x) || has_nan(w.y) || has_nan(w.z) || has_nan(w.w)) z.nan_v[note.piece % kFlagSlots] = 1;
-                    w = make_uint4(without_nan(w.x), without_nan(w.y), without_nan(w.z), without_nan(w.w));
+            for (int k0 = 0; k0 < S::kSteps; k0 += S::kAtOnce) {
+                wait_copies<S::kDepth - S::kAtOnce>();
+                uint2 w[S::kAtOnce][2];
+#pragma unroll
+                for (int i = 0; i < S::kAtOnce; ++i) {
+                    const int place = (k0 + i) % S::kDepth * 2048;
+                    w[i][0] = load8(first_from + place);
+                    w[i][1] = load8(second_from + place);
                 }
-                store_codes<CODE>(w, at + k * (S::kRowsPerStep * 128), run_at, swap);
+#pragma unroll
+                for (int i = 0; i < S::kAtOnce; ++i) {
+                    const int k = k0 + i + S::kDepth;
+                    if (k < S::kSteps) copy(note, k, k % S::kDepth);
+                    else if (more) copy(next, k - S::kSteps, k % S::kDepth);
+                    commit_copies();
+                }
+                if (hidden) {
+#pragma unroll
+                    for (int i = 0; i < S::kAtOnce; ++i)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            if (has_nan(w[i][y].x) || has_nan(w[i][y].y)) z.nan_v[note.piece % kFlagSlots] = 1;
+                            w[i][y] = make_uint2(without_nan(w[i][y].x), without_nan(w[i][y].y));
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < S::kAtOnce; ++i) {
+                    store_codes<CODE>(w[i][0], first + (k0 + i) * (S::kRowsPerStep * 128));
+                    store_codes<CODE>(w[i][1], second + (k0 + i) * (S::kRowsPerStep * 128));
+                }
             }
             fence_proxy_async();
             mbar_arrive_warp(&bars[full + stage], lane);
@@ -826,7 +852,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
         using S = Steps<D, true>;
         const int tid = threadIdx.x & 127, col = tid % S::kLanes * 16, row0 = tid / S::kLanes, in_block_mask = (1 << p.c.bs_log2) - 1;
         const int run = col / 8, swap = D == 128 ? run >> 3 : 0;
-        const uint32_t row_at = (run >> 3) * kBox + row0 * 128, run_at = ((run & 7) ^ (row0 & 7)) << 4;
+        const uint32_t first_at = (run >> 3) * kBox + row0 * 128 + ((((run & 7) ^ (row0 & 7)) ^ swap) << 4);
         int units = 0;
         while (walk.next(p, x)) {
             const int stage = units & 1;
@@ -845,7 +871,11 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
                     w[k] = *reinterpret_cast<const uint4*>(p.c.k + (int64_t)pg * p.c.sk.b + (int64_t)x.h * p.c.sk.h + (int64_t)(slot & in_block_mask) * p.c.sk.n + col);
             }
 #pragma unroll
-            for (int k = 0; k < S::kSteps; ++k) store_codes<CODE>(w[k], smem_u32(sK) + stage * kTile + row_at + k * (S::kRowsPerStep * 128), run_at, swap);
+            for (int k = 0; k < S::kSteps; ++k) {
+                const uint32_t at = smem_u32(sK) + stage * kTile + first_at + k * (S::kRowsPerStep * 128);
+                store_codes<CODE>(swap ? make_uint2(w[k].z, w[k].w) : make_uint2(w[k].x, w[k].y), at);
+                store_codes<CODE>(swap ? make_uint2(w[k].x, w[k].y) : make_uint2(w[k].z, w[k].w), at ^ 16);
+            }
             fence_proxy_async();
             mbar_arrive_warp(&bars[W_K_FULL + stage], lane);
             ++units;
