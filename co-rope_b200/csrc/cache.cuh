@@ -36,6 +36,7 @@ struct CacheAttnParams {
     void* o;
     Strides sq, so;
     int Hq, G, T, D, code, dtype, causal, accumulate;
+    int parts;                   // blocks (a cluster) per item, 0 = ranges of the batch's units
     int row_tiles;               // tiles of query rows per K / V head (row = t * G + head of the group)
     float scale;                 // sm_scale * log2(e)
     bool vec_o;                  // rows of o take stores of four elements

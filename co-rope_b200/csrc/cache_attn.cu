@@ -4,7 +4,8 @@
 // around the reads:
 //   * Work is counted in units of 64 slots of one (sequence, K / V head, tile of query rows) and cut into equal contiguous ranges, one per resident
 //     block, from the lengths on the device: a batch of unequal lengths loads every SM alike.  A range that starts or ends inside an item leaves
-//     its part (fp32 sums, maximum, total) in the workspace, and a second kernel joins the parts in a fixed order.
+//     its part (fp32 sums, maximum, total) in the workspace, and a second kernel joins the parts in a fixed order.  Short sequences are cut
+//     evenly among the blocks of a cluster instead, which join their parts through each other's shared memory: one kernel, no workspace.
 //   * Each warp streams its own 16-slot pieces (a piece lies in one block, so one scale) through its own ring in shared memory with
 //     cp.async, without block-wide barriers.
 //   * Products on mma.sync with slots as the M extent and query rows as N = 8: S^T = K Q^T, O^T = V^T P^T.  Codes become fp16 in registers,
@@ -13,6 +14,7 @@
 //   * Rotated queries are scaled by a power of two per row and split into two fp16 numbers (22 bits), so scores have fp32 accuracy.
 //     exp2(s + log2(v scale) - M) is rounded to fp16 (11 bits) for 16-bit outputs, whose own rounding is coarser or equal, and split in two for
 //     fp32 ones; the sum of the probabilities stays fp32.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -21,6 +23,8 @@
 
 namespace corope {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kPiece = 16;                    // slots per step of a warp; a block of the cache holds a whole number of them
@@ -114,12 +118,8 @@ struct Shape {
     static constexpr int kBig = kRing > kJoin ? kRing : kJoin;
     static constexpr int kPacked = D / 16 * NT * 32 * 16;
     static constexpr int kMeta = kWarps * kStages * 16;                     // {k scale, v scale, block found} of each stage
-    static constexpr int kSmem = kBig + kPacked + kMeta + kRows * 4 + 2 * kWarps * kRows * 4;
+    static constexpr int kSmem = kBig + kPacked + kMeta + kRows * 4 + 2 * kWarps * kRows * 4 + 2 * kRows * 4;
     static constexpr int kBlocks = NT == 1 ? 4 : 2;                         // resident per SM
-};
-
-struct Piece {   // what a block does next: units [u0, u1) of an item
-    int b, h, tile, u0, u1;
 };
 
 template <int D, int CODE, int NT, bool EXACT_P>
@@ -132,18 +132,30 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     float* factor = meta + S::kMeta / 4;
     float* warp_max = factor + kRows;
     float* warp_sum = warp_max + kWarps * kRows;
+    float* part_max = warp_sum + kWarps * kRows;
+    float* part_sum = part_max + kRows;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
     bool bad = false;
 
     auto load = [&](int b) { return load_of(p, kRows, kUnit, b, bad); };
-    Range range = take_range<kThreads>(p.s.B, load);
-    pdl_trigger();
-    if (range.left == 0) {
-        if (bad) report_bad_index(p.status, p.mirror);
-        return;
+    // Either a range of the batch's units, or (p.parts) this block's share of one item, whose other shares are with the blocks of its cluster.
+    int b, part_of = 0, cluster_item = 0;
+    int64_t off = 0, left = 0;   // position in sequence b's units, units left
+    if (p.parts == 0) {
+        const Range range = take_range<kThreads>(p.s.B, load);
+        pdl_trigger();
+        if (range.left == 0) {
+            if (bad) report_bad_index(p.status, p.mirror);
+            return;
+        }
+        b = range.b;
+        off = range.off;
+        left = range.left;
+    } else {
+        cluster_item = (int)(blockIdx.x / (unsigned)p.parts);
+        part_of = (int)(blockIdx.x - (unsigned)cluster_item * p.parts);
+        b = cluster_item / (p.c.Hkv * p.row_tiles);
     }
-    int b = range.b;
-    int64_t off = range.off, left = range.left;   // position in sequence b's units, units left
     Load l = load(b);
 
     uint8_t* ring = smem + warp * (kStages * S::kStageBytes);
@@ -159,16 +171,28 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     const uint32_t k_run = (g * D + c * (D / 4)) / 16, v_run = (2 * c * D + g * (D / 8)) / 16;
     const uint32_t k_from = (k_run ^ (k_run >> 3 & 7)) * 16 + c * (D / 4) % 16, v_from = (v_run ^ (v_run >> 3 & 7)) * 16 + g * (D / 8) % 16;
 
-    while (left > 0) {
-        while (off >= (int64_t)l.units * l.items) {
-            off -= (int64_t)l.units * l.items;
-            l = load(++b);
+    do {
+        int h, tile, u0, u1;
+        if (p.parts == 0) {
+            while (off >= (int64_t)l.units * l.items) {
+                off -= (int64_t)l.units * l.items;
+                l = load(++b);
+            }
+            const int item = (int)(off / l.units), tiles = l.items / p.c.Hkv;
+            h = item / tiles;
+            tile = item % tiles;
+            u0 = (int)(off - (int64_t)item * l.units);
+            u1 = (int)min((int64_t)l.units, u0 + left);
+            off += u1 - u0;
+            left -= u1 - u0;
+        } else {
+            const int item = cluster_item - b * p.c.Hkv * p.row_tiles;
+            h = item / p.row_tiles;
+            tile = item - h * p.row_tiles;
+            const int units = tile * kRows < l.n * p.G ? l.units : 0;
+            u0 = units * part_of / p.parts;
+            u1 = units * (part_of + 1) / p.parts;
         }
-        const int item = (int)(off / l.units), tiles = l.items / p.c.Hkv;
-        const int h = item / tiles, tile = item % tiles, u0 = (int)(off - (int64_t)item * l.units);
-        const int u1 = (int)min((int64_t)l.units, u0 + left);
-        off += u1 - u0;
-        left -= u1 - u0;
         const int row0 = tile * kRows, len = l.len, n = l.n;
         // slots below least_seen are seen by every row of the tile (rows without a query see what they like)
         const int least_seen = p.causal ? len - n + row0 / p.G + 1 : len;
@@ -439,6 +463,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                 for (int x = 0; x < D / 16; ++x) to[x] = make_float2(o[nt][x][i] * shrink, o[nt][x][i + 2] * shrink);
             }
         __syncthreads();
+        auto write_row = [&](int r, int d, const float4& y, float all) {
+            const int row = row0 + r, t = row / p.G;
+            const float f = 1.f / all;
+            store4(p.o, (int64_t)b * p.so.b + (int64_t)(h * p.G + row - t * p.G) * p.so.h + (int64_t)t * p.so.n + d, p.dtype, p.vec_o,
+                   t >= n || all == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+        };
         const bool whole = u0 == 0 && u1 == l.units;
         const int64_t part = 2 * (int64_t)blockIdx.x + (u0 == 0 ? 1 : 0);
         for (int x = threadIdx.x; x < kRows * (D / 4); x += kThreads) {
@@ -454,17 +484,60 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                 const float4 z = *reinterpret_cast<const float4*>(join + (k * kRows + r) * D + d);
                 y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
             }
-            if (!whole) {
+            if (p.parts != 0) {   // for the cluster: in the place of warp 0's sums
+                *reinterpret_cast<float4*>(join + r * D + d) = y;
+                if (d == 0) part_max[r] = top, part_sum[r] = all;
+            } else if (!whole) {
                 *reinterpret_cast<float4*>(p.part + (part * kRows + r) * D + d) = y;
                 if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (part * kRows + r) * 2) = make_float2(top, all);
             } else if (t < p.T) {
-                const float f = 1.f / all;
-                y = t >= n || all == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
-                store4(p.o, (int64_t)b * p.so.b + (int64_t)(h * p.G + row - t * p.G) * p.so.h + (int64_t)t * p.so.n + d, p.dtype, p.vec_o, y);
+                write_row(r, d, y, all);
                 if (p.lse != nullptr && d == 0) p.lse[((int64_t)b * p.c.Hkv + h) * p.T * p.G + row] = t >= n || all == 0.f ? INFINITY : top + log2f(all);
             }
         }
-    }
+        if (p.parts != 0) {
+            // The blocks of the cluster have the item's parts in their shared memories: each writes its share of the output's runs of four, and adds the
+            // weights of its own slots.
+            cg::cluster_group cluster = cg::this_cluster();
+            cluster.sync();
+            auto whole_row = [&](int r, float& top, float& all) {
+                top = kLowest;
+                all = 0.f;
+                for (int q = 0; q < p.parts; ++q) top = fmaxf(top, *cluster.map_shared_rank(part_max + r, q));
+                for (int q = 0; q < p.parts; ++q) all = fmaf(*cluster.map_shared_rank(part_sum + r, q), fast_exp2(*cluster.map_shared_rank(part_max + r, q) - top), all);
+            };
+            for (int x = part_of * kThreads + threadIdx.x; x < kRows * (D / 4); x += p.parts * kThreads) {
+                const int r = x / (D / 4), d = x % (D / 4) * 4;
+                if ((row0 + r) / p.G >= p.T) break;
+                float top, all;
+                whole_row(r, top, all);
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int q = 0; q < p.parts; ++q) {
+                    const float4 z = *reinterpret_cast<const float4*>(cluster.map_shared_rank(join + r * D + d, q));
+                    const float f = fast_exp2(*cluster.map_shared_rank(part_max + r, q) - top);
+                    y.x = fmaf(z.x, f, y.x); y.y = fmaf(z.y, f, y.y); y.z = fmaf(z.z, f, y.z); y.w = fmaf(z.w, f, y.w);
+                }
+                write_row(r, d, y, all);
+            }
+            if (p.scores != nullptr) {
+                const int rows = min(kRows, n * p.G - row0);   // one tile
+                if (threadIdx.x < rows) {
+                    float top, all;
+                    whole_row(threadIdx.x, top, all);
+                    warp_max[threadIdx.x] = all == 0.f ? INFINITY : top + log2f(all);
+                }
+                __syncthreads();
+                for (int slot = u0 * kUnit + threadIdx.x; slot < min(u1 * kUnit, len); slot += kThreads) {
+                    const int page = cache_page(p.s, p.c.bs_log2, p.c.num_blocks, b, slot, bad);
+                    const float* from = p.scores + (((int64_t)b * p.c.Hkv + h) * p.capacity + slot) * p.score_rows;
+                    float w = 0.f;
+                    for (int r = 0; r < rows; ++r) w += fast_exp2(from[r] - warp_max[r]);
+                    if (page >= 0) atomicAdd(p.c.weight + (((int64_t)page * p.c.Hkv + h) << p.c.bs_log2) + (slot & in_block_mask), w);
+                }
+            }
+            cluster.sync();   // no block ends while another reads its part
+        }
+    } while (left > 0);
     if (bad) report_bad_index(p.status, p.mirror);
 }
 
@@ -708,6 +781,7 @@ __global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const Cache
 }
 
 // rows of a tile by the number of query rows: 8 (one N extent of the MMA), 16 or 32
+constexpr int kClusterUnits = 16;
 int row_groups(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 int resident_blocks(int groups) { return groups == 1 ? 4 : 2; }
 // How a call is done and where its workspace's parts lie (the parts of joined sums come first).
@@ -715,6 +789,7 @@ struct Layout {
     bool tiles, two_parts;        // tcgen05 kernels; queries in two fp16 parts
     int groups, row_tiles, rows_per_tile;
     unsigned blocks;
+    int parts;                    // blocks of a cluster per item, 0 = ranges of units
     int score_rows;               // numbers a slot in `scores`, 0 = the scores are formed again
     size_t part_ml, lse, scores, images, total;
 };
@@ -733,16 +808,27 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     const uint64_t items = (uint64_t)B * Hkv * l.row_tiles, unit = l.tiles ? kTileRows : kUnit;
     const uint64_t units = items * ((slots + unit - 1) / unit), most = (uint64_t)sm_count() * (l.tiles ? 1 : resident_blocks(l.groups));
     l.blocks = (unsigned)(units < most ? units : most);
-    const size_t part_rows = (size_t)2 * l.blocks * l.rows_per_tile;
+    // Room for the scores of every slot that the block tables could hold.  Beyond half a gigabyte (long tables that the sequences may not fill) K is
+    // read again instead: 32 sequences of up to 8192 tokens, 4 rows a head, take 88 us with the scores, 148 without.
+    const size_t score_bytes = (size_t)B * Hkv * slots * ((rows + 1) / 2 * 2) * 4;
+    l.score_rows = accumulate && !l.tiles && l.row_tiles == 1 && score_bytes <= (512u << 20) ? (rows + 1) / 2 * 2 : 0;
+    // A cluster per item where all of them are resident at once and no block has more than kClusterUnits units of the longest sequence there can be:
+    // the sequences' own lengths are not known here, so the longest sets the pace.  Ranges and a joining kernel / clusters, us, 32 / 8 heads of 128: 1 x
+    // 777 tokens 11.5 / 8.5, 1 x 4096 21.2 / 12.9, 16 x 1024 21.1 / 14.1, 16 x up to 4096 27.1 / 30.1, 64 x up to 1024 33.1 / 28.4.
+    const uint64_t item_units = (slots + unit - 1) / unit;
+    if (!l.tiles && items <= most && (!accumulate || l.score_rows)) {
+        l.parts = 1;
+        while (l.parts < 8 && items * l.parts * 2 <= most && item_units >= (uint64_t)l.parts * 2) l.parts *= 2;
+        if (item_units > (uint64_t)l.parts * kClusterUnits) l.parts = 0;
+        else l.blocks = (unsigned)(items * l.parts);
+    }
+    const size_t part_rows = l.parts ? 0 : (size_t)2 * l.blocks * l.rows_per_tile;
     l.part_ml = align_up(part_rows * D * 4, 256);
     l.lse = l.part_ml + align_up(part_rows * 8, 256);
     l.scores = l.lse + (accumulate ? align_up((size_t)B * Hkv * rows * 4, 256) : 0);
-    // Room for the scores of every slot that the block tables could hold.  Beyond half a gigabyte (long tables that the sequences may not fill) K is
-    // read again instead: 32 sequences of up to 8192 tokens, 4 rows a head, take 88 us with the scores, 148 without.
-    const size_t bytes = (size_t)B * Hkv * slots * ((rows + 1) / 2 * 2) * 4;
-    l.score_rows = accumulate && !l.tiles && l.row_tiles == 1 && bytes <= (512u << 20) ? (rows + 1) / 2 * 2 : 0;
-    l.images = l.scores + (l.score_rows ? align_up(bytes, 256) : 0);
+    l.images = l.scores + (l.score_rows ? align_up(score_bytes, 256) : 0);
     l.total = l.images + (l.tiles ? cache_tile_workspace_bytes(B, Hkv, l.row_tiles, D, l.two_parts) : 0);
+    if (l.total < 256) l.total = 256;
     return l;
 }
 
@@ -756,12 +842,27 @@ int launch_main(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     if (int e = allow_smem(cache_attn_kernel<D, CODE, NT, EXACT_P>, Shape<D, NT>::kSmem, done)) return e;
     count_launch();
-    cache_attn_kernel<D, CODE, NT, EXACT_P><<<blocks, kThreads, Shape<D, NT>::kSmem, s>>>(p);
-    return (int)cudaGetLastError();
+    if (p.parts == 0) {
+        cache_attn_kernel<D, CODE, NT, EXACT_P><<<blocks, kThreads, Shape<D, NT>::kSmem, s>>>(p);
+        return (int)cudaGetLastError();
+    }
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)p.parts;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Shape<D, NT>::kSmem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, CODE, NT, EXACT_P>, p);
 }
 template <int D, int CODE, int NT>
 int launch_rows(const CacheAttnParams& p, const Layout& l, cudaStream_t s) {
     if (int e = p.dtype == COROPE_DTYPE_F32 ? launch_main<D, CODE, NT, true>(p, l.blocks, s) : launch_main<D, CODE, NT, false>(p, l.blocks, s)) return e;
+    if (l.parts) return COROPE_OK;
     if (int e = launch_join<D>(p, l, kUnit, s)) return e;
     if (!p.accumulate) return COROPE_OK;
     count_launch();
@@ -793,6 +894,7 @@ int launch_cache_attn(CacheAttnParams p, void* ws, cudaStream_t s) {
     const Layout l = layout_of(p.s.B, p.c.Hkv, p.G, p.T, p.D, p.s.max_blocks, 1 << p.c.bs_log2, p.dtype, p.accumulate);
     auto part = [&](size_t at) { return reinterpret_cast<float*>(static_cast<char*>(ws) + at); };
     p.row_tiles = l.row_tiles;
+    p.parts = l.parts;
     p.part = part(0);
     p.part_ml = part(l.part_ml);
     p.lse = p.accumulate ? part(l.lse) : nullptr;
