@@ -40,6 +40,7 @@ struct CacheAttnParams {
     int row_tiles;               // tiles of query rows per K / V head (row = t * G + head of the group)
     float scale;                 // sm_scale * log2(e)
     bool vec_o;                  // rows of o take stores of four elements
+    bool rows_packed;            // rows of codes follow one another without gaps
     float* part;                 // partial results: two slots per block of the main kernel
     float* part_ml;              // their maxima and sums
     float* lse;                  // [B, Hkv, T * G] log2 of each row's sum (accumulate only)

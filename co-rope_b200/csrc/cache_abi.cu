@@ -10,7 +10,8 @@ Strides strides_of(const int64_t* a) { return Strides{a[0], a[1], a[2]}; }
 
 // rows of codes move in 16-byte runs
 bool cache_rows_ok(const void* ptr, const Strides& st, int D) {
-    return (uintptr_t)ptr % 16 == 0 && st.b % 16 == 0 && st.h % 16 == 0 && st.n % 16 == 0 && st.n >= D && st.b >= 0 && st.h >= 0;
+    return (uintptr_t)ptr % 16 == 0 && st.b % 16 == 0 && st.h % 16 == 0 && st.n % 16 == 0 && st.n >= D && st.b >= 0 && st.h >= 0 &&
+           st.b < (1ll << 32) && st.n < (1ll << 32);   // (strides are 32-bit numbers in the kernels)
 }
 
 int view_of(CacheView& v, const corope_kv_cache_t* c) {

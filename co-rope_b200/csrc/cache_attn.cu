@@ -17,8 +17,6 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
-#include <type_traits>
-
 #include "cache_attn.cuh"
 
 namespace corope {
@@ -34,6 +32,16 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float fast_log2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float fast_reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     uint32_t d;
@@ -119,7 +127,7 @@ struct Shape {
     static constexpr int kPacked = D / 16 * NT * 32 * 16;
     static constexpr int kMeta = kWarps * kStages * 16;                     // {k scale, v scale, block found} of each stage
     static constexpr int kSmem = kBig + kPacked + kMeta + kRows * 4 + 2 * kWarps * kRows * 4 + 2 * kRows * 4;
-    static constexpr int kBlocks = NT == 1 ? 4 : 2;                         // resident per SM
+    static constexpr int kBlocks = NT == 1 ? 4 : NT == 2 ? 3 : 2;                         // resident per SM
 };
 
 template <int D, int CODE, int NT, bool EXACT_P>
@@ -138,6 +146,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     bool bad = false;
 
     auto load = [&](int b) { return load_of(p, kRows, kUnit, b, bad); };
+    __shared__ int nan_v;   // NaN in V where some rows must not see it
     // Either a range of the batch's units, or (p.parts) this block's share of one item, whose other shares are with the blocks of its cluster.
     int b, part_of = 0, cluster_item = 0;
     int64_t off = 0, left = 0;   // position in sequence b's units, units left
@@ -160,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 
     uint8_t* ring = smem + warp * (kStages * S::kStageBytes);
     float* my_meta = meta + warp * kStages * 4;
-    const uint32_t ring_at = smem_u32(ring), meta_at = smem_u32(my_meta);
+    const uint32_t ring_at = smem_u32(ring), meta_at = smem_u32(my_meta), packed_at = smem_u32(packed) + lane * 16;
     // A stage holds 16 rows of K, then of V; the 16-byte run x of a tile sits at run x ^ (x / 8 % 8), which keeps the reads below off one
     // another's banks.  Lane's share of a copy: runs lane + 32 i, rows copy_row + kCopyRows i.
     constexpr int kCopyRows = 512 / D;
@@ -197,6 +206,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
         // slots below least_seen are seen by every row of the tile (rows without a query see what they like)
         const int least_seen = p.causal ? len - n + row0 / p.G + 1 : len;
         __syncthreads();   // the tile before is written out
+        if (threadIdx.x == 0) nan_v = 0;
         // pieces first, first + 4, .. of this warp
         const int first = u0 * kWarps + warp, end = min(u1 * kWarps, (len + kPiece - 1) / kPiece);
         const int count = end > first ? (end - first + kWarps - 1) / kWarps : 0;
@@ -205,43 +215,48 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
         const uint8_t* k_lane = p.c.k + (int64_t)h * p.c.sk.h + (int64_t)copy_row * p.c.sk.n + copy_col;
         const uint8_t* v_lane = p.c.v + (int64_t)h * p.c.sv.h + (int64_t)copy_row * p.c.sv.n + copy_col;
         const float* scale_lane = (lane ? p.c.v_scale : p.c.k_scale) + h;
-        int next_page = count > 0 ? table[first >> shift] : 0;
-        uint32_t fill = ring_at;         // stage that the next piece is copied to
-        int fill_stage = 0;
+        const uint32_t k_block = (uint32_t)p.c.sk.b, v_block = (uint32_t)p.c.sv.b, k_row = (uint32_t)p.c.sk.n, v_row = (uint32_t)p.c.sv.n;   // below 2^32
+        const int* entry = table + (first >> shift);   // of the next piece to be copied
+        int next_page = count > 0 ? *entry : 0;
+        uint32_t fill = ring_at + copy_to, fill_meta = meta_at + lane * 4;   // where its copy goes
+        int next_piece = first;
         auto issue = [&](int j) {
             if (j < count) {
-                const int piece = first + j * kWarps;
                 const bool found = (unsigned)next_page < (unsigned)p.c.num_blocks;
-                const int page = found ? next_page : 0;
-                bad |= !found;
-                if (j + 1 < count) next_page = table[(piece + kWarps) >> shift];
-                const int in_block = (piece << 4) & in_block_mask, rows = found ? len - (piece << 4) : 0;
-                const uint8_t* kb = k_lane + (int64_t)page * p.c.sk.b + (int64_t)in_block * p.c.sk.n;
-                const uint8_t* vb = v_lane + (int64_t)page * p.c.sv.b + (int64_t)in_block * p.c.sv.n;
-                const uint32_t dst = fill + copy_to;
-                if (rows >= kPiece) {
+                const uint32_t page = found ? (uint32_t)next_page : 0u, in_block = (uint32_t)(next_piece << 4) & (uint32_t)in_block_mask;
+                const int rows = len - (next_piece << 4);
+                next_piece += kWarps;
+                if (j + 1 < count) next_page = table[next_piece >> shift];
+                const uint8_t* kb = k_lane + (uint64_t)page * k_block + (uint64_t)in_block * k_row;
+                const uint8_t* vb = v_lane + (uint64_t)page * v_block + (uint64_t)in_block * v_row;
+                const uint32_t other = fill ^ 64;
+                if (found && rows >= kPiece && p.rows_packed) {
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i) {
-                        const uint32_t to = (dst ^ (i % 2 * 64)) + 512 * i;
-                        copy16_async(to, kb + (int64_t)i * kCopyRows * p.c.sk.n);
-                        copy16_async(to + kPiece * D, vb + (int64_t)i * kCopyRows * p.c.sv.n);
+                        copy16_async((i % 2 ? other : fill) + 512 * i, kb + i * 512);
+                        copy16_async((i % 2 ? other : fill) + 512 * i + kPiece * D, vb + i * 512);
                     }
-                } else {   // slots behind the last one become zeros
+                } else {   // slots behind the last one, and those of a block that is not there, become zeros
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i) {
-                        const uint32_t to = (dst ^ (i % 2 * 64)) + 512 * i;
-                        const bool real = copy_row + i * kCopyRows < rows;
-                        copy16_async(to, real ? kb + (int64_t)i * kCopyRows * p.c.sk.n : p.c.k, real);
-                        copy16_async(to + kPiece * D, real ? vb + (int64_t)i * kCopyRows * p.c.sv.n : p.c.v, real);
+                        const bool real = found && copy_row + i * kCopyRows < rows;
+                        copy16_async((i % 2 ? other : fill) + 512 * i, real ? kb + (uint64_t)(i * kCopyRows) * k_row : p.c.k, real);
+                        copy16_async((i % 2 ? other : fill) + 512 * i + kPiece * D, real ? vb + (uint64_t)(i * kCopyRows) * v_row : p.c.v, real);
+                    }
+                    if (!found) {
+                        bad = true;
+                        if (lane == 2) my_meta[j % kStages * 4 + 2] = 0.f;   // (1 otherwise)
                     }
                 }
-                if (lane < 2) copy4_async(meta_at + fill_stage * 16 + lane * 4, scale_lane + (int64_t)page * p.c.Hkv);
-                if (lane == 2) my_meta[fill_stage * 4 + 2] = found ? 1.f : 0.f;
+                if (lane < 2) copy4_async(fill_meta, scale_lane + (uint64_t)page * (uint32_t)p.c.Hkv);
             }
             commit_copies();
             fill += S::kStageBytes;
-            if (++fill_stage == kStages) fill_stage = 0, fill = ring_at;
+            fill_meta += 16;
+            if (fill == ring_at + copy_to + kStages * S::kStageBytes) fill = ring_at + copy_to, fill_meta = meta_at + lane * 4;
         };
+        if (lane < kStages) my_meta[lane * 4 + 2] = 1.f;
+        __syncwarp();
 #pragma unroll
         for (int j = 0; j < kStages - 1; ++j) issue(j);   // on their way while the queries are made ready
 
@@ -255,20 +270,16 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             for (int i = 0; i < 2; ++i) fac[nt][i] = factor[8 * nt + 2 * c + i];
         // slots below this are seen by the row
         auto sees = [&](int nt, int i) { return p.causal ? len - n + (row0 + 8 * nt + 2 * c + i) / p.G + 1 : len; };
-        uint4 qf[NT == 1 ? kKSteps : 1];
-        if constexpr (NT == 1) {
-#pragma unroll
-            for (int w = 0; w < kKSteps; ++w) qf[w] = reinterpret_cast<const uint4*>(packed)[w * 32 + lane];
-        }
-
-        float o[NT][D / 16][4], m[NT][2], sum[NT][2];
+        // m: reference of the exponents, which are at most 8 (exp2 of that fits fp16): it moves when one is beyond `most`, -infinity before the first
+        float o[NT][D / 16][4], m[NT][2], most[NT][2], sum[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int x = 0; x < D / 16; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[nt][x][i] = 0.f;
-            m[nt][0] = m[nt][1] = kLowest;
+            m[nt][0] = m[nt][1] = 0.f;
+            most[nt][0] = most[nt][1] = -INFINITY;
             sum[nt][0] = sum[nt][1] = 0.f;
         }
 
@@ -280,8 +291,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             __syncwarp();
             const int slot0 = (first + j * kWarps) * kPiece;
             const uint32_t k_at = stage_at + k_from, v_at = stage_at + kPiece * D + v_from;
-            const float k_scale = my_meta[stage * 4], v_scale = my_meta[stage * 4 + 1];
-            const bool found = my_meta[stage * 4 + 2] != 0.f;
+            const float4 said = *reinterpret_cast<const float4*>(my_meta + stage * 4);
+            const float k_scale = said.x, v_scale = said.y;
+            const bool found = said.z != 0.f;
 
             // S^T: slots g and g + 8 by rows 2 c and 2 c + 1
             float s[NT][4];
@@ -303,29 +315,41 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                 codes_to_half<CODE>(k1[w], a[1], a[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const uint4 q = NT == 1 ? qf[NT == 1 ? w : 0] : reinterpret_cast<const uint4*>(packed)[(w * NT + nt) * 32 + lane];
-                    mma16816(s[nt], a, q.x, q.y);
-                    mma16816(rest[nt], a, q.z, q.w);
+                    uint32_t q[4];   // read each time: held in registers they would cost more than they save
+                    load_words(q, 0, packed_at + (w * NT + nt) * 512);
+                    mma16816(s[nt], a, q[0], q[1]);
+                    mma16816(rest[nt], a, q[2], q[3]);
                 }
             }
 
             // scores in units of log2, the scale of V folded into the exponent: O = sum of exp2(s + log2 v_scale - M) * code
             // (a scale of 0 is left out of the exponent, and its slots out of O)
-            const float v_size = v_scale == 0.f ? 1.f : max_nan(v_scale, 1e-30f), lift = __log2f(v_size), drop = __fdividef(1.f, v_size);
+            const float v_size = v_scale == 0.f ? 1.f : max_nan(v_scale, 1e-30f), lift = fast_log2(v_size), drop = fast_reciprocal(v_size);
             bool higher = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float f0 = fac[nt][0] * k_scale, f1 = fac[nt][1] * k_scale;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + rest[nt][i]) * (i % 2 ? f1 : f0);
-            }
-            if (!found || slot0 + kPiece > least_seen) {
+            const bool masked = !found || slot0 + kPiece > least_seen;
+            auto hide = [&]() {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[nt][i] = found && slot0 + g + 8 * (i / 2) < sees(nt, i % 2) ? s[nt][i] : -INFINITY;
-            }
-            if (p.scores != nullptr) {   // for the weights: whole rows of `score_rows` numbers a slot
+            };
+            // s becomes the exponent, relative to m
+            if (p.scores == nullptr) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float f0 = fac[nt][0] * k_scale, f1 = fac[nt][1] * k_scale, a0 = lift - m[nt][0], a1 = lift - m[nt][1];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nt][i] = fmaf(s[nt][i] + rest[nt][i], i % 2 ? f1 : f0, i % 2 ? a1 : a0);
+                }
+                if (masked) hide();
+            } else {   // the scores are kept for the weights: whole rows of `score_rows` numbers a slot
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float f0 = fac[nt][0] * k_scale, f1 = fac[nt][1] * k_scale;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + rest[nt][i]) * (i % 2 ? f1 : f0);
+                }
+                if (masked) hide();
                 float* to = p.scores + (((int64_t)b * p.c.Hkv + h) * p.capacity + slot0 + g) * p.score_rows + 2 * c;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -333,26 +357,31 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                         if (slot0 + g < len) *reinterpret_cast<float2*>(to + 8 * nt) = make_float2(s[nt][0], s[nt][1]);
                         if (slot0 + g + 8 < len) *reinterpret_cast<float2*>(to + 8 * p.score_rows + 8 * nt) = make_float2(s[nt][2], s[nt][3]);
                     }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nt][i] += lift - m[nt][i % 2];
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[nt][i] += lift;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) higher |= fmaxf(s[nt][i], s[nt][i + 2]) > m[nt][i] + 8.f;
-            if (__any_sync(0xffffffffu, higher)) {   // exp2 of up to 8 above M fits fp16: M moves only when a score is beyond that
+                for (int i = 0; i < 2; ++i) higher |= fmaxf(s[nt][i], s[nt][i + 2]) > most[nt][i];
+            if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float top = fmaxf(s[nt][i], s[nt][i + 2]);
+                        float up = fmaxf(s[nt][i], s[nt][i + 2]);
 #pragma unroll
-                        for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                        top = fmaxf(top, m[nt][i]);
-                        const float shrink = fast_exp2(m[nt][i] - top);
-                        m[nt][i] = top;
+                        for (int k = 4; k < 32; k *= 2) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, k));
+                        const bool begins = most[nt][i] < 0.f;
+                        if (begins && up == -INFINITY) continue;   // no score yet
+                        if (!begins) up = fmaxf(up, 0.f);
+                        const float shrink = begins ? 0.f : fast_exp2(-up);
+                        m[nt][i] += up;
+                        most[nt][i] = 8.f;
+                        s[nt][i] -= up;
+                        s[nt][i + 2] -= up;
                         sum[nt][i] *= shrink;
 #pragma unroll
                         for (int x = 0; x < D / 16; ++x) o[nt][x][i] *= shrink, o[nt][x][i + 2] *= shrink;
@@ -363,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             for (int nt = 0; nt < NT; ++nt) {
                 float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = fast_exp2(s[nt][i] - m[nt][i % 2]);
+                for (int i = 0; i < 4; ++i) w[i] = fast_exp2(s[nt][i]);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float both = w[i] + w[i + 2];
@@ -385,49 +414,38 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 #pragma unroll
             for (int i = 0; i < 4; ++i)   // slots 2 c, 2 c + 1, and 8 further on
                 load_words(v[i], 0, (v_at ^ (i % 2 * kNextXor) ^ (i / 2 * kNext8Xor)) + i % 2 * kNextAdd + i / 2 * (kPiece * D / 2));
-            auto add_values = [&](auto per_slot, int only) {   // only: the one slot of the piece to add, to the rows that see it
-                constexpr bool kPerSlot = decltype(per_slot)::value;
-#pragma unroll
-                for (int w = 0; w < kVWords; ++w) {
-                    uint32_t x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = !kPerSlot || only == 2 * c + i % 2 + 8 * (i / 2) ? v[i][w] : 0u;
-                    uint32_t a[2][4];
-                    codes_to_half<CODE>(__byte_perm(x[0], x[1], 0x5140), a[0][0], a[0][1]);
-                    codes_to_half<CODE>(__byte_perm(x[2], x[3], 0x5140), a[0][2], a[0][3]);
-                    codes_to_half<CODE>(__byte_perm(x[0], x[1], 0x7362), a[1][0], a[1][1]);
-                    codes_to_half<CODE>(__byte_perm(x[2], x[3], 0x7362), a[1][2], a[1][3]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            if constexpr (EXACT_P || kPerSlot) {   // EXACT_P: the long sum in fp32 additions, as MMA accumulation truncates
-                                float t[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma16816(t, a[y], pb[nt][0], pb[nt][1]);
-                                if constexpr (EXACT_P) mma16816(t, a[y], pl[nt][0], pl[nt][1]);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (!kPerSlot || slot0 + only < sees(nt, i % 2)) o[nt][2 * w + y][i] += t[i];
-                            } else {
-                                mma16816(o[nt][2 * w + y], a[y], pb[nt][0], pb[nt][1]);
-                            }
-                        }
-                }
-            };
-            // A NaN in V reaches the rows that see its slot, and 0 * NaN would bring it to the others: such a piece goes slot by slot
-            bool nan = false;
+            // NaN in V reaches the rows that see its slot, and 0 * NaN would bring it to the others: it is left out here and put in when the rows are written
             if (CODE == COROPE_CODE_E4M3 && slot0 + kPiece > least_seen) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int w = 0; w < kVWords; ++w) nan |= __vcmpeq4(v[i][w] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
-                nan = __any_sync(0xffffffffu, nan);
+                    for (int w = 0; w < kVWords; ++w) {
+                        const uint32_t where = __vcmpeq4(v[i][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        if (where) nan_v = 1;
+                        v[i][w] &= ~where;
+                    }
             }
-            if (CODE == COROPE_CODE_E4M3 && nan) {
-#pragma unroll 1
-                for (int only = 0; only < kPiece; ++only) add_values(std::true_type{}, only);
-            } else {
-                add_values(std::false_type{}, 0);
+#pragma unroll
+            for (int w = 0; w < kVWords; ++w) {
+                uint32_t a[2][4];
+                codes_to_half<CODE>(__byte_perm(v[0][w], v[1][w], 0x5140), a[0][0], a[0][1]);
+                codes_to_half<CODE>(__byte_perm(v[2][w], v[3][w], 0x5140), a[0][2], a[0][3]);
+                codes_to_half<CODE>(__byte_perm(v[0][w], v[1][w], 0x7362), a[1][0], a[1][1]);
+                codes_to_half<CODE>(__byte_perm(v[2][w], v[3][w], 0x7362), a[1][2], a[1][3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        if constexpr (EXACT_P) {   // the long sum in fp32 additions, as MMA accumulation truncates
+                            float t[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma16816(t, a[y], pb[nt][0], pb[nt][1]);
+                            mma16816(t, a[y], pl[nt][0], pl[nt][1]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[nt][2 * w + y][i] += t[i];
+                        } else {
+                            mma16816(o[nt][2 * w + y], a[y], pb[nt][0], pb[nt][1]);
+                        }
+                    }
             }
             stage_at += S::kStageBytes;
             if (++stage == kStages) stage = 0, stage_at = ring_at;
@@ -440,6 +458,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
+                if (most[nt][i] < 0.f) m[nt][i] = kLowest;
 #pragma unroll
                 for (int k = 4; k < 32; k *= 2) sum[nt][i] += __shfl_xor_sync(0xffffffffu, sum[nt][i], k);
                 if (g == 0) {
@@ -483,6 +502,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             for (int k = 0; k < kWarps; ++k) {
                 const float4 z = *reinterpret_cast<const float4*>(join + (k * kRows + r) * D + d);
                 y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+            }
+            if (CODE == COROPE_CODE_E4M3 && nan_v != 0) {
+                const int sees_row = p.causal ? len - n + t + 1 : len;
+#pragma unroll 1
+                for (int slot = u0 * kUnit; slot < min(sees_row, u1 * kUnit); ++slot) {
+                    const int page = table[slot >> p.c.bs_log2];
+                    if ((unsigned)page >= (unsigned)p.c.num_blocks || p.c.v_scale[(int64_t)page * p.c.Hkv + h] == 0.f) continue;
+                    const uint32_t word = *reinterpret_cast<const uint32_t*>(p.c.v + (int64_t)page * p.c.sv.b + (int64_t)h * p.c.sv.h + (int64_t)(slot & in_block_mask) * p.c.sv.n + d);
+                    if ((word & 0x7fu) == 0x7fu) y.x = __int_as_float(0x7fffffff);
+                    if ((word >> 8 & 0x7fu) == 0x7fu) y.y = __int_as_float(0x7fffffff);
+                    if ((word >> 16 & 0x7fu) == 0x7fu) y.z = __int_as_float(0x7fffffff);
+                    if ((word >> 24 & 0x7fu) == 0x7fu) y.w = __int_as_float(0x7fffffff);
+                }
             }
             if (p.parts != 0) {   // for the cluster: in the place of warp 0's sums
                 *reinterpret_cast<float4*>(join + r * D + d) = y;
@@ -783,7 +815,7 @@ __global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const Cache
 // rows of a tile by the number of query rows: 8 (one N extent of the MMA), 16 or 32
 constexpr int kClusterUnits = 16;
 int row_groups(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
-int resident_blocks(int groups) { return groups == 1 ? 4 : 2; }
+int resident_blocks(int groups) { return groups == 1 ? 4 : groups == 2 ? 3 : 2; }
 // How a call is done and where its workspace's parts lie (the parts of joined sums come first).
 struct Layout {
     bool tiles, two_parts;        // tcgen05 kernels; queries in two fp16 parts
@@ -902,6 +934,7 @@ int launch_cache_attn(CacheAttnParams p, void* ws, cudaStream_t s) {
     p.score_rows = l.score_rows;
     p.scores = l.score_rows ? part(l.scores) : nullptr;
     p.vec_o = rows_in_fours(p.o, p.so, p.dtype);
+    p.rows_packed = p.c.sk.n == p.D && p.c.sv.n == p.D;
     void* images = part(l.images);
     return p.D == 128 ? by_kernel<128>(p, l, images, s) : p.D == 64 ? by_kernel<64>(p, l, images, s) : by_kernel<32>(p, l, images, s);
 }
