@@ -54,6 +54,7 @@ struct CacheEvictParams {
     const int* out_table;
     int64_t out_stride;
     int out_blocks, budget, recent, D, code;
+    bool vec_weight;             // weights take loads of four
     int *new_lens, *kept;
     int *status, *mirror;
 };
@@ -160,13 +161,26 @@ __device__ __forceinline__ void from_codes4(uint32_t w, float (&x)[4]) {
 template <int CODE>
 __device__ __forceinline__ uint32_t rescale4(uint32_t codes, float old, float scale, float near) {
     const bool plain = near == near && old < scale;   // not NaN, either
-    uint32_t w;
-    float x[4], y[4];
-    from_codes4<CODE>(codes, x);
     const float ratio = old * near;
+    uint32_t w;
+    float x[4];
+    if constexpr (CODE == COROPE_CODE_INT8) {
+        // c * ratio in units of 2^-24: u * r + (2^23 - 128 r) with u = c + 128 has the rounded product in its top byte.  r is off by 3 at most, the product
+        // by 400, the fp32 quotient by as much: not within 1024 of a tie, it has the quotient's code.
+        const uint32_t r = __float2uint_rn(ratio * 16777216.f), shift = 8388608u - 128u * r, u = codes ^ 0x80808080u;
+        uint32_t t[4], least = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = x[i] * ratio;
-    if (codes4_near<CODE>(y, w) && plain) return w;
+        for (int i = 0; i < 4; ++i) {
+            t[i] = __byte_perm(u, 0u, 0x4440 + i) * r + shift;
+            least = min(least, t[i] * 256u + 1024u * 256u);
+        }
+        if (least >= 2048u * 256u && plain) return __byte_perm(__byte_perm(t[0], t[1], 0x0073), __byte_perm(t[2], t[3], 0x0073), 0x5410);
+        from_codes4<CODE>(codes, x);
+    } else {
+        from_codes4<CODE>(codes, x);
+        const float y[4] = {x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio};
+        if (codes4_near<CODE>(y, w) && plain) return w;
+    }
     return divided4<CODE>(__fmul_rn(x[0], old), __fmul_rn(x[1], old), __fmul_rn(x[2], old), __fmul_rn(x[3], old), scale);
 }
 // max(a, b), NaN if one of them is

@@ -49,7 +49,7 @@ __device__ __forceinline__ unsigned sum_before(unsigned x, unsigned* words, unsi
 
 // `parts` blocks (a cluster) per item; `held`: slots a block has shared memory for
 __global__ void __launch_bounds__(kSelectThreads, 1) cache_select_kernel(const CacheEvictParams p, int parts, int held) {
-    extern __shared__ uint32_t keys[];
+    extern __shared__ __align__(16) uint32_t keys[];
     __shared__ unsigned counts[3][kBins];
     __shared__ unsigned words[6][32];
     __shared__ unsigned chosen[3], above[3], found[2];
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) cache_select_kernel(const C
         return;
     }
     // this block's slots, and the consecutive ones of each thread among them (an odd number: neighbours' words lie in different banks)
-    const int share = (open + parts - 1) / parts, lo = min(part * share, open), n = min(share, open - lo);
+    const int share = ((open + parts - 1) / parts + 3) & ~3, lo = min(part * share, open), n = min(share, open - lo);
     const int each = ((share + kSelectThreads - 1) / kSelectThreads) | 1;
     const bool in_smem = n <= held;
     auto weight_key = [&](int slot) -> uint32_t {
@@ -80,11 +80,29 @@ __global__ void __launch_bounds__(kSelectThreads, 1) cache_select_kernel(const C
     };
     auto key = [&](int i) -> uint32_t { return in_smem ? keys[i] : weight_key(lo + i); };
     for (int i = threadIdx.x; i < 3 * kBins; i += kSelectThreads) (&counts[0][0])[i] = 0;
-    if (in_smem) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += kSelectThreads) keys[i] = weight_key(lo + i);
-    }
     __syncthreads();
+    if (in_smem) {   // patterns to shared memory, the first digit counted on the way; four slots at a time: they lie in one block
+#pragma unroll 2
+        for (int i = 4 * threadIdx.x; i < n; i += 4 * kSelectThreads) {
+            const int slot = lo + i, page = cache_page(p.s, p.c.bs_log2, p.c.num_blocks, b, slot, bad);
+            const float* from = p.c.weight + (((int64_t)max(page, 0) * p.c.Hkv + h) << p.c.bs_log2) + (slot & bs_mask);
+            float w[4];
+            if (p.vec_weight) {
+                const float4 x = *reinterpret_cast<const float4*>(from);   // (what lies behind the share is not used)
+                w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+            } else {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) w[y] = from[y];
+            }
+            uint32_t k[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                k[y] = page < 0 ? 0u : ordered(w[y]);
+                if (i + y < n) atomicAdd(&counts[0][k[y] >> 21], 1u);
+            }
+            *reinterpret_cast<uint4*>(keys + i) = make_uint4(k[0], k[1], k[2], k[3]);
+        }
+    }
 
     uint32_t prefix = 0, mask = 0;   // the digits of the last kept key that are known
     unsigned rest = need;            // slots to keep among those that share them
@@ -92,9 +110,19 @@ __global__ void __launch_bounds__(kSelectThreads, 1) cache_select_kernel(const C
     for (int round = 0; round < 3; ++round) {
         const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
         const uint32_t digit_mask = round == 2 ? 1023u : 2047u;
-        for (int i = threadIdx.x; i < n; i += kSelectThreads) {
-            const uint32_t k = key(i);
-            if ((k & mask) == prefix) atomicAdd(&counts[round][(k >> shift) & digit_mask], 1u);
+        if (!in_smem) {
+            for (int i = threadIdx.x; i < n; i += kSelectThreads) {
+                const uint32_t k = key(i);
+                if ((k & mask) == prefix) atomicAdd(&counts[round][(k >> shift) & digit_mask], 1u);
+            }
+        } else if (round > 0) {
+            for (int i = 4 * threadIdx.x; i < n; i += 4 * kSelectThreads) {
+                const uint4 x = *reinterpret_cast<const uint4*>(keys + i);
+                const uint32_t k[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    if ((k[y] & mask) == prefix && i + y < n) atomicAdd(&counts[round][(k[y] >> shift) & digit_mask], 1u);
+            }
         }
         if (parts > 1) cluster.sync();
         else __syncthreads();
@@ -230,7 +258,7 @@ int launch_cache_evict(const CacheEvictParams& p, cudaStream_t s) {
     const int64_t most = (int64_t)p.s.max_blocks << p.c.bs_log2;
     int parts = 1;
     while (parts < 8 && items * parts * 2 <= (uint64_t)sm_count() && most / (parts * 2) >= 4096) parts *= 2;
-    const int64_t share = (most + parts - 1) / parts;
+    const int64_t share = ((most + parts - 1) / parts + 3) / 4 * 4;
     const int held = (int)(share < kHeldSlots ? share : kHeldSlots);
     static std::atomic<uint64_t> done{0};
     if (int e = allow_smem(cache_select_kernel, kHeldSlots * 4, done)) return e;
@@ -246,7 +274,9 @@ int launch_cache_evict(const CacheEvictParams& p, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (int e = (int)cudaLaunchKernelEx(&cfg, cache_select_kernel, p, parts, held)) return e;
+    CacheEvictParams q = p;
+    q.vec_weight = (uintptr_t)p.c.weight % 16 == 0;
+    if (int e = (int)cudaLaunchKernelEx(&cfg, cache_select_kernel, q, parts, held)) return e;
     const unsigned blocks = (unsigned)(items * out_used);
     if (p.code == COROPE_CODE_E4M3) return launch_dependent(cache_move_kernel<COROPE_CODE_E4M3>, blocks, kMoveThreads, 0, s, p, out_used);
     return launch_dependent(cache_move_kernel<COROPE_CODE_INT8>, blocks, kMoveThreads, 0, s, p, out_used);
