@@ -1,13 +1,12 @@
 // corope_cache_append: keys rotated, keys and values quantised into the blocks of the 8-bit cache.
 //
 // One thread block per (cache block with new tokens, K / V head): a block's scale is known once all its new rows have been seen, so they wait in
-// registers (up to four rows a thread, as fp32) for the block-wide maximum.  Keys first, then values.  Bound by the reads of k and v.
+// registers (two rows a thread where that takes no more than 1024 threads, else four) for the block-wide maxima.  Bound by the reads of k and v.
 #include "cache.cuh"
 
 namespace corope {
 namespace {
 
-constexpr int kSteps = 4;        // rows a thread holds
 
 // x1' = x1 c - x2 s, x2' = x2 c + x1 s, each operation rounded by itself: the codes are those of that formula in fp32
 __device__ __forceinline__ void rotate4(float4& a, float4& b, const float4& c, const float4& s) {
@@ -42,22 +41,21 @@ template <> struct Raw<false> {
     }
 };
 
-// largest value of the thread block, in every thread; `words`: 32 floats, a different array for each use
-__device__ __forceinline__ float block_max(float x, float* words) {
-#pragma unroll
-    for (int m = 16; m; m >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
-    if (threadIdx.x % 32 == 0) words[threadIdx.x / 32] = x;
+// Largest values (none negative: their bits are in the same order) of the thread block, in every thread; `words`: 64 words.
+__device__ __forceinline__ void block_max(float& k, float& v, uint32_t* words) {
+    const uint32_t a = __reduce_max_sync(0xffffffffu, __float_as_uint(k)), b = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+    const int lane = threadIdx.x % 32;
+    if (lane == 0) words[threadIdx.x / 32] = a, words[32 + threadIdx.x / 32] = b;
     __syncthreads();
-    x = threadIdx.x % 32 < blockDim.x / 32 ? words[threadIdx.x % 32] : 0.f;
-#pragma unroll
-    for (int m = 16; m; m >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
-    return x;
+    const bool there = lane < (int)blockDim.x / 32;
+    k = __uint_as_float(__reduce_max_sync(0xffffffffu, there ? words[lane] : 0u));
+    v = __uint_as_float(__reduce_max_sync(0xffffffffu, there ? words[32 + lane] : 0u));
 }
 
-// WIDE: fp32 rows.  MOST: threads of the largest block launched.
-template <int CODE, bool WIDE, int MOST>
-__global__ void __launch_bounds__(MOST) cache_append_kernel(const CacheAppendParams p, int touched, int per_row_log2, bool vec_k, bool vec_v, bool vec_t) {
-    __shared__ float words[2][32];
+// WIDE: fp32 rows.  kSteps: rows a thread holds.  MOST: threads of the largest block launched.
+template <int CODE, bool WIDE, int kSteps, int MOST>
+__global__ void __launch_bounds__(MOST, 1024 / MOST) cache_append_kernel(const CacheAppendParams p, int touched, int per_row_log2, bool vec_k, bool vec_v, bool vec_t) {
+    __shared__ uint32_t words[64];
     const unsigned item = blockIdx.x / (unsigned)touched;
     const int j = (int)(blockIdx.x - item * (unsigned)touched), b = (int)(item / (unsigned)p.c.Hkv), h = (int)(item - (unsigned)b * (unsigned)p.c.Hkv);
     const int bs = 1 << p.c.bs_log2, half = p.D / 2;
@@ -88,37 +86,43 @@ __global__ void __launch_bounds__(MOST) cache_append_kernel(const CacheAppendPar
         }
     const int64_t at = (int64_t)page * p.c.Hkv + h;
     const int held = lo - base;                                       // older tokens of the block
+    const float old_k = held ? p.c.k_scale[at] : 0.f, old_v = held ? p.c.v_scale[at] : 0.f;
+    float4 x[2][kSteps][2];
+    float top[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const int slot = lo + g + i * groups;
+        if (slot >= hi) continue;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            x[part][i][0] = raw[part][i][0].get(p.dtype);
+            x[part][i][1] = raw[part][i][1].get(p.dtype);
+        }
+        if (p.s.cos != nullptr) {
+            const int64_t row = (int64_t)cache_position(p.s, b, slot - first, slot, bad) * p.s.rope_stride + d;
+            rotate4(x[0][i][0], x[0][i][1], load4(p.s.cos, row, COROPE_DTYPE_F32, vec_t), load4(p.s.sin, row, COROPE_DTYPE_F32, vec_t));
+        }
+#pragma unroll
+        for (int part = 0; part < 2; ++part) top[part] = amax4(amax4(top[part], x[part][i][0]), x[part][i][1]);
+    }
+    bool finite[2];
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        finite[part] = top[part] <= 3.402823466e38f;
+        if (finite[part]) continue;
+        top[part] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+            if (lo + g + i * groups < hi) top[part] = fmaxf(top[part], fmaxf(finite_amax4(x[part][i][0]), finite_amax4(x[part][i][1])));
+    }
+    block_max(top[0], top[1], words);                                 // (every thread has read the old scales)
 #pragma unroll
     for (int part = 0; part < 2; ++part) {                            // keys, values
         const Strides sc = part ? p.c.sv : p.c.sk;
         uint8_t* to = (part ? p.c.v : p.c.k) + (int64_t)page * sc.b + (int64_t)h * sc.h + d;
-        float* scale_at = (part ? p.c.v_scale : p.c.k_scale) + at;
-        const float old = held ? *scale_at : 0.f;
-        float4 x1[kSteps], x2[kSteps];
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const int slot = lo + g + i * groups;
-            if (slot >= hi) continue;
-            x1[i] = raw[part][i][0].get(p.dtype);
-            x2[i] = raw[part][i][1].get(p.dtype);
-            if (part == 0 && p.s.cos != nullptr) {
-                const int64_t row = (int64_t)cache_position(p.s, b, slot - first, slot, bad) * p.s.rope_stride + d;
-                rotate4(x1[i], x2[i], load4(p.s.cos, row, COROPE_DTYPE_F32, vec_t), load4(p.s.sin, row, COROPE_DTYPE_F32, vec_t));
-            }
-            top = amax4(amax4(top, x1[i]), x2[i]);
-        }
-        const bool finite = top <= 3.402823466e38f;
-        if (!finite) {
-            top = 0.f;
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-                if (lo + g + i * groups < hi) top = fmaxf(top, fmaxf(finite_amax4(x1[i]), finite_amax4(x2[i])));
-        }
-        top = block_max(top, words[part]);                            // (every thread has read the old scale)
-        const float scale = max_nan(old, __fmul_rn(top, kPerCode<CODE>)), near = reciprocal(scale);
-        const bool plain = finite && near == near;
-        if (threadIdx.x == 0) *scale_at = scale;
+        const float old = part ? old_v : old_k, scale = max_nan(old, __fmul_rn(top[part], kPerCode<CODE>)), near = reciprocal(scale);
+        const bool plain = finite[part] && near == near;
+        if (threadIdx.x == 0) (part ? p.c.v_scale : p.c.k_scale)[at] = scale;
         if (held && scale != old)
             for (int r = g; r < held; r += groups) {
                 uint32_t *w1 = reinterpret_cast<uint32_t*>(to + (int64_t)r * sc.n), *w2 = reinterpret_cast<uint32_t*>(to + (int64_t)r * sc.n + half);
@@ -129,8 +133,8 @@ __global__ void __launch_bounds__(MOST) cache_append_kernel(const CacheAppendPar
         for (int i = 0; i < kSteps; ++i) {
             const int slot = lo + g + i * groups;
             if (slot >= hi) continue;
-            *reinterpret_cast<uint32_t*>(to + (int64_t)(slot - base) * sc.n) = codes4<CODE>(x1[i], scale, near, plain);
-            *reinterpret_cast<uint32_t*>(to + (int64_t)(slot - base) * sc.n + half) = codes4<CODE>(x2[i], scale, near, plain);
+            *reinterpret_cast<uint32_t*>(to + (int64_t)(slot - base) * sc.n) = codes4<CODE>(x[part][i][0], scale, near, plain);
+            *reinterpret_cast<uint32_t*>(to + (int64_t)(slot - base) * sc.n + half) = codes4<CODE>(x[part][i][1], scale, near, plain);
             if (part && p.c.weight != nullptr && d == 0) p.c.weight[(at << p.c.bs_log2) + slot - base] = 0.f;
         }
     }
@@ -138,12 +142,19 @@ __global__ void __launch_bounds__(MOST) cache_append_kernel(const CacheAppendPar
 }
 
 template <int CODE, bool WIDE>
-int launch_t(const CacheAppendParams& p, unsigned blocks, int threads, int touched, int per_row_log2, cudaStream_t s) {
+int launch_t(const CacheAppendParams& p, unsigned blocks, int rows, int touched, int per_row_log2, cudaStream_t s) {
     const bool vec_k = rows_in_fours(p.k, p.sk, p.dtype), vec_v = rows_in_fours(p.v, p.sv, p.dtype);
     const bool vec_t = (uintptr_t)p.s.cos % 16 == 0 && (uintptr_t)p.s.sin % 16 == 0 && p.s.rope_stride % 4 == 0;
     count_launch();
-    if (threads <= 512) cache_append_kernel<CODE, WIDE, 512><<<blocks, threads, 0, s>>>(p, touched, per_row_log2, vec_k, vec_v, vec_t);
-    else cache_append_kernel<CODE, WIDE, 1024><<<blocks, threads, 0, s>>>(p, touched, per_row_log2, vec_k, vec_v, vec_t);
+    const int wanted = rows << per_row_log2;   // threads, with a row each
+    auto threads = [&](int steps) {
+        int t = 64;
+        while (t * steps < wanted) t *= 2;
+        return t;
+    };
+    if (threads(2) <= 512) cache_append_kernel<CODE, WIDE, 2, 512><<<blocks, threads(2), 0, s>>>(p, touched, per_row_log2, vec_k, vec_v, vec_t);
+    else if (threads(2) <= 1024) cache_append_kernel<CODE, WIDE, 2, 1024><<<blocks, threads(2), 0, s>>>(p, touched, per_row_log2, vec_k, vec_v, vec_t);
+    else cache_append_kernel<CODE, WIDE, 4, 1024><<<blocks, threads(4), 0, s>>>(p, touched, per_row_log2, vec_k, vec_v, vec_t);   // 256 rows of 16 threads, the most there are
     return (int)cudaGetLastError();
 }
 
@@ -153,16 +164,13 @@ int launch_cache_append(const CacheAppendParams& p, cudaStream_t s) {
     const int bs = 1 << p.c.bs_log2, touched = (p.T + bs - 2) / bs + 1;
     const uint64_t blocks = (uint64_t)p.s.B * p.c.Hkv * touched;
     if (blocks >= (1ull << 31)) return COROPE_ERR_TOO_LARGE;
-    // a thread for every four elements of kSteps rows: 1024 for 256 rows of 16 threads, the most there are
     const int per_row_log2 = p.D == 128 ? 4 : p.D == 64 ? 3 : 2, rows = p.T < bs ? p.T : bs;
-    int threads = 64;
-    while (threads * kSteps < rows << per_row_log2) threads *= 2;
     const bool wide = p.dtype == COROPE_DTYPE_F32;
     if (p.code == COROPE_CODE_E4M3)
-        return wide ? launch_t<COROPE_CODE_E4M3, true>(p, (unsigned)blocks, threads, touched, per_row_log2, s)
-                    : launch_t<COROPE_CODE_E4M3, false>(p, (unsigned)blocks, threads, touched, per_row_log2, s);
-    return wide ? launch_t<COROPE_CODE_INT8, true>(p, (unsigned)blocks, threads, touched, per_row_log2, s)
-                : launch_t<COROPE_CODE_INT8, false>(p, (unsigned)blocks, threads, touched, per_row_log2, s);
+        return wide ? launch_t<COROPE_CODE_E4M3, true>(p, (unsigned)blocks, rows, touched, per_row_log2, s)
+                    : launch_t<COROPE_CODE_E4M3, false>(p, (unsigned)blocks, rows, touched, per_row_log2, s);
+    return wide ? launch_t<COROPE_CODE_INT8, true>(p, (unsigned)blocks, rows, touched, per_row_log2, s)
+                : launch_t<COROPE_CODE_INT8, false>(p, (unsigned)blocks, rows, touched, per_row_log2, s);
 }
 
 }  // namespace corope
