@@ -818,7 +818,7 @@ int row_groups(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 int resident_blocks(int groups) { return groups == 1 ? 4 : groups == 2 ? 3 : 2; }
 // How a call is done and where its workspace's parts lie (the parts of joined sums come first).
 struct Layout {
-    bool tiles, two_parts;        // tcgen05 kernels; queries in two fp16 parts
+    bool tiles, two_parts, pair;  // tcgen05 kernels; queries in two fp16 parts; two tiles of 128 rows an item
     int groups, row_tiles, rows_per_tile;
     unsigned blocks;
     int parts;                    // blocks of a cluster per item, 0 = ranges of units
@@ -834,8 +834,9 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     l.tiles = dtype != COROPE_DTYPE_F32 && rows > 32;
     // one part of q is off by 2^-12 of it: next to a bf16 result's 2^-9 that is nothing, an fp16 result or a weight would feel it
     l.two_parts = l.tiles && (dtype == COROPE_DTYPE_F16 || accumulate);
+    l.pair = l.tiles && cache_tile_pairs(rows, D, l.two_parts);
     l.groups = row_groups(rows);
-    l.rows_per_tile = l.tiles ? kTileRows : 8 * l.groups;
+    l.rows_per_tile = l.tiles ? kTileRows * (l.pair ? 2 : 1) : 8 * l.groups;
     l.row_tiles = (rows + l.rows_per_tile - 1) / l.rows_per_tile;
     const uint64_t items = (uint64_t)B * Hkv * l.row_tiles, unit = l.tiles ? kTileRows : kUnit;
     const uint64_t units = items * ((slots + unit - 1) / unit), most = (uint64_t)sm_count() * (l.tiles ? 1 : resident_blocks(l.groups));
@@ -859,7 +860,7 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     l.lse = l.part_ml + align_up(part_rows * 8, 256);
     l.scores = l.lse + (accumulate ? align_up((size_t)B * Hkv * rows * 4, 256) : 0);
     l.images = l.scores + (l.score_rows ? align_up(score_bytes, 256) : 0);
-    l.total = l.images + (l.tiles ? cache_tile_workspace_bytes(B, Hkv, l.row_tiles, D, l.two_parts) : 0);
+    l.total = l.images + (l.tiles ? cache_tile_workspace_bytes(B, Hkv, l.row_tiles * (l.pair ? 2 : 1), D, l.two_parts) : 0);
     if (l.total < 256) l.total = 256;
     return l;
 }
@@ -911,9 +912,9 @@ int by_rows(const CacheAttnParams& p, const Layout& l, cudaStream_t s) {
 template <int D>
 int by_kernel(const CacheAttnParams& p, const Layout& l, void* images, cudaStream_t s) {
     if (!l.tiles) return p.code == COROPE_CODE_E4M3 ? by_rows<D, COROPE_CODE_E4M3>(p, l, s) : by_rows<D, COROPE_CODE_INT8>(p, l, s);
-    if (int e = launch_cache_attn_tiles(p, images, l.two_parts, l.blocks, s)) return e;
+    if (int e = launch_cache_attn_tiles(p, images, l.two_parts, l.pair, l.blocks, s)) return e;
     if (int e = launch_join<D>(p, l, kTileRows, s)) return e;
-    return p.accumulate ? launch_cache_weight_tiles(p, images, s) : COROPE_OK;
+    return p.accumulate ? launch_cache_weight_tiles(p, images, l.pair, s) : COROPE_OK;
 }
 
 }  // namespace

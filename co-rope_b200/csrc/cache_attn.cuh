@@ -85,9 +85,10 @@ __device__ __forceinline__ Range take_range(int B, const LoadFn& load) {
 #endif  // __CUDACC__
 
 // Attention of many query rows a K / V head on tcgen05 (16-bit types): the steps of launch_cache_attn that are its own.
-constexpr int kTileRows = 128;                // query rows, and slots of a unit
-size_t cache_tile_workspace_bytes(int B, int Hkv, int row_tiles, int D, bool two_parts);
-int launch_cache_attn_tiles(const CacheAttnParams& p, void* ws, bool two_parts, unsigned blocks, cudaStream_t s);
-int launch_cache_weight_tiles(const CacheAttnParams& p, void* ws, cudaStream_t s);
+constexpr int kTileRows = 128;                // query rows of a tile, and slots of a unit
+bool cache_tile_pairs(int rows, int D, bool two_parts);   // items of two tiles of rows
+size_t cache_tile_workspace_bytes(int B, int Hkv, int image_tiles, int D, bool two_parts);
+int launch_cache_attn_tiles(const CacheAttnParams& p, void* ws, bool two_parts, bool pair, unsigned blocks, cudaStream_t s);
+int launch_cache_weight_tiles(const CacheAttnParams& p, void* ws, bool pair, cudaStream_t s);
 
 }  // namespace corope

@@ -9,6 +9,8 @@
 //   warps 12-19   softmax of the even units of a piece, two threads a row (64 slots each);  warps 20-27: of the odd ones
 // TMEM: S0 [0,128) S1 [128,256) O0 [256,384) O1 [384,512); P (fp16) goes over S.  Even and odd units have sums of their own, so one group's
 // exponentials run beside the other's MMAs, and are joined when the piece is written.
+// With more than 128 rows a head (PAIR) an item is two tiles of rows, a group to each: K and V are turned into operands once for both, which halves
+// that work and the reads from L2.  Not for D = 128 with two parts, whose four query tiles leave no room for two stages of K and V.
 // Scales: a block of 16 slots or more has one scale of K, which multiplies the scores of its columns in fp32, and one of V, which enters the
 // exponent: P = exp2(s + log2 v_scale - M), and its sum is taken back to probabilities by the same number.
 // Queries are scaled by a power of two per row and rounded to fp16 (11 bits); with two parts (fp16 tensors, and where weights are gathered) the
@@ -63,9 +65,11 @@ struct alignas(16) Small {
     uint32_t tmem;
     int abort;
 };
-constexpr size_t queue_bytes(int D, bool two) { return (size_t)(D == 128 && two ? 4 : D / 16) * 16 * 128; }   // of codes on their way, per group
-constexpr size_t smem_bytes(int D, bool two) { return ((two ? 2 : 1) + 2 * kStages) * tile_bytes(D) + 2 * queue_bytes(D, two) + sizeof(Small) + 1024; }
-static_assert(smem_bytes(128, true) <= 232448 - 128 && smem_bytes(128, false) <= 232448 - 128, "shared memory budget");   // (and take_range's)
+constexpr size_t queue_bytes(int D, bool two, bool pair) { return (size_t)(D == 128 && (two || pair) ? 4 : D / 16) * 16 * 128; }   // of codes on their way, per group
+constexpr size_t smem_bytes(int D, bool two, bool pair) {
+    return ((two ? 2 : 1) * (pair ? 2 : 1) + 2 * kStages) * tile_bytes(D) + 2 * queue_bytes(D, two, pair) + sizeof(Small) + 1024;
+}
+static_assert(smem_bytes(128, true, false) <= 232448 - 128 && smem_bytes(128, false, false) <= 232448 - 128 && smem_bytes(128, false, true) <= 232448 - 128, "shared memory budget");   // (and take_range's)
 
 // byte offset of 16-byte run `run` (8 elements) of row r in the image of a tile: boxes of 64 columns, 128-byte swizzle
 __device__ __forceinline__ uint32_t image_at(int r, int run) { return (uint32_t)((run >> 3) * (kN * 128) + r * 128 + (((run & 7) ^ (r & 7)) << 4)); }
@@ -78,10 +82,10 @@ __device__ __forceinline__ void store16(uint32_t at, uint32_t a, uint32_t b, uin
 // Rotates, scales and rounds the rows, and writes them as images of their tiles: a warp per row, 16 blocks per tile.
 constexpr int kPackWarps = 8, kPackBlocks = kN / kPackWarps;
 template <int D, bool TWO>
-__global__ void __launch_bounds__(kPackWarps * 32) cache_pack_kernel(const CacheAttnParams p, uint8_t* images, float* factors) {
+__global__ void __launch_bounds__(kPackWarps * 32) cache_pack_kernel(const CacheAttnParams p, int image_tiles, uint8_t* images, float* factors) {
     constexpr int kHalf = D / 2, kPairs = kHalf / 2;
     const unsigned item = blockIdx.x / (unsigned)kPackBlocks;
-    const int tile = (int)(item % (unsigned)p.row_tiles), bh = (int)(item / (unsigned)p.row_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
+    const int tile = (int)(item % (unsigned)image_tiles), bh = (int)(item / (unsigned)image_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
     const int lane = threadIdx.x % 32, r = (int)(blockIdx.x - item * kPackBlocks) * kPackWarps + (int)threadIdx.x / 32;
     bool bad = false;
     const int len = cache_len(p.s, p.c.bs_log2, b, bad), n = cache_new(p.s, p.T, b, bad);
@@ -136,10 +140,10 @@ __global__ void __launch_bounds__(kPackWarps * 32) cache_pack_kernel(const Cache
 // ------------------------------------------------------------------------------------------------ codes to operands
 // A group of 128 threads turns a unit's 128 slots into an operand in kSteps steps, 16 codes a thread and step.  The codes wait in a queue in
 // shared memory of the thread's own (cp.async brings them, nobody else reads them), kDepth steps ahead.
-template <int D, bool TWO>
+template <int D, bool TWO, bool PAIR>
 struct Steps {
     static constexpr int kLanes = D / 16, kRowsPerStep = 128 / kLanes, kSteps = kN / kRowsPerStep;
-    static constexpr int kDepth = D == 128 && TWO ? 4 : kSteps;
+    static constexpr int kDepth = D == 128 && (TWO || PAIR) ? 4 : kSteps;
     static constexpr int kAtOnce = kDepth >= 8 ? 4 : 2;     // steps whose loads are under way together
     static constexpr int kQueueBytes = kDepth * 16 * 128;   // of one group
 };
@@ -174,15 +178,15 @@ __device__ __forceinline__ void store_codes(const uint2& w, uint32_t at) {
 }
 
 // ------------------------------------------------------------------------------------------------ main kernel
-template <int D, int CODE, bool TWO>
+template <int D, int CODE, bool TWO, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const CacheAttnParams p, const uint8_t* images, const float* factors) {
-    using S = Steps<D, TWO>;
-    constexpr int kD = wide(D), kBox = kN * 128, kParts = TWO ? 2 : 1;
+    using S = Steps<D, TWO, PAIR>;
+    constexpr int kD = wide(D), kBox = kN * 128, kParts = TWO ? 2 : 1, kQTiles = PAIR ? 2 : 1, kItemRows = kQTiles * kN;
     constexpr uint32_t kTile = (uint32_t)tile_bytes(D);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sQ = sm;
-    uint8_t* sK = sQ + kParts * kTile;
+    uint8_t* sK = sQ + kQTiles * kParts * kTile;   // (queries: [tile][part])
     uint8_t* sV = sK + kStages * kTile;
     uint8_t* queues = sV + kStages * kTile;
     Small& z = *reinterpret_cast<Small*>(queues + 2 * S::kQueueBytes);
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     bool bad = false;
-    const Range range = take_range<128>(p.s.B, [&](int b) { return load_of(p, kN, kN, b, bad); });
+    const Range range = take_range<128>(p.s.B, [&](int b) { return load_of(p, kItemRows, kN, b, bad); });
     pdl_trigger();
     if (bad) report_bad_index(p.status, p.mirror);
     // after a wait that ran out, in this launch's block or in an earlier launch, none starts anew until the host has seen it
@@ -258,8 +262,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                     mbar_arrive(&bars[PIECE_EMPTY + slot]);
                     if (!some) continue;
                     if (n > 0 && !mbar_wait(&bars[Q_EMPTY], (n - 1) & 1, p.status, Q_EMPTY, abort_flag)) break;
-                    mbar_arrive_expect_tx(&bars[Q_FULL], kParts * kTile);
-                    for (int i = 0; i < kParts; ++i) bulk_load_1d(sQ + i * kTile, images + ((size_t)item * kParts + i) * kTile, kTile, &bars[Q_FULL]);
+                    mbar_arrive_expect_tx(&bars[Q_FULL], kQTiles * kParts * kTile);
+                    for (int i = 0; i < kQTiles * kParts; ++i)
+                        bulk_load_1d(sQ + i * kTile, images + ((size_t)item * (kQTiles * kParts) + i) * kTile, kTile, &bars[Q_FULL]);
                     ++n;
                 }
             }
@@ -278,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                     for (int kk = 0; kk < kD / 16; ++kk) {
                         const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
                         // the second part first: its sum is small, and so are its truncations
-                        if (leader) umma_ss2(d, q_lo + (kParts - 1 - part) * (kTile >> 4) + off, kHi, b0 + off, kHi, idesc_qk, part + kk > 0);
+                        if (leader) umma_ss2(d, q_lo + ((PAIR ? i * kParts : 0) + kParts - 1 - part) * (kTile >> 4) + off, kHi, b0 + off, kHi, idesc_qk, part + kk > 0);
                     }
             };
             auto issue_pv = [&](int i, int stage, bool add) {
@@ -296,35 +301,73 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 mbar_arrive_warp(&bars[PIECE_EMPTY + slot], lane);
                 if (count < 0) break;
                 if (count == 0) continue;
-                auto next_scores = [&](int j) {   // Q K^T of the piece's unit j
-                    if (!(ok = mbar_wait_warp(&bars[K_FULL + gk % kStages], (gk / kStages) & 1, p.status, K_FULL, abort_flag))) return;
-                    tc_fence_after();
-                    issue_qk(j & 1, gk % kStages);
-                    if (leader) {
-                        umma_commit(&bars[S_FULL + (j & 1)]);
-                        umma_commit(&bars[K_EMPTY + gk % kStages]);
-                        if (j + 1 == count) umma_commit(&bars[Q_EMPTY]);
-                    }
-                    ++gk;
-                };
                 if (!(ok = mbar_wait_warp(&bars[Q_FULL], pieces & 1, p.status, Q_FULL, abort_flag))) break;
-                next_scores(0);
-                if (ok && count > 1) next_scores(1);
-                for (int j = 0; ok && j < count; ++j) {
-                    const int i = j & 1, stage = gv % kStages;
-                    if (!(ok = mbar_wait_warp(&bars[V_FULL + stage], (gv / kStages) & 1, p.status, V_FULL, abort_flag))) break;
-                    if (!(ok = mbar_wait_warp(&bars[P_FULL + i], (i ? done1 : done0) & 1, p.status, P_FULL, abort_flag))) break;
-                    if (j == 0 && pieces > 0 && !(ok = mbar_wait_warp(&bars[O_FREE], (pieces - 1) & 1, p.status, O_FREE, abort_flag))) break;
-                    tc_fence_after();
-                    issue_pv(i, stage, j > 1);
-                    if (leader) {
-                        umma_commit(&bars[O_FULL + i]);
-                        umma_commit(&bars[V_EMPTY + stage]);
+                if constexpr (PAIR) {
+                    // PV0(j) QK0(j + 1) | PV1(j) QK1(j + 1); j = -1 forms the scores of unit 0
+                    for (int j = -1; ok && j < count; ++j) {
+                        const bool have_next = j + 1 < count;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            if (j >= 0) {
+                                const int stage = gv % kStages;
+                                if (i == 0 && !(ok = mbar_wait_warp(&bars[V_FULL + stage], (gv / kStages) & 1, p.status, V_FULL, abort_flag))) break;
+                                if (!(ok = mbar_wait_warp(&bars[P_FULL + i], (i ? done1 : done0) & 1, p.status, P_FULL, abort_flag))) break;
+                                if (i == 0 && j == 0 && pieces > 0 && !(ok = mbar_wait_warp(&bars[O_FREE], (pieces - 1) & 1, p.status, O_FREE, abort_flag))) break;
+                                tc_fence_after();
+                                issue_pv(i, stage, j > 0);
+                                if (leader) umma_commit(&bars[O_FULL + i]);
+                                if (i == 0) {
+                                    ++done0;
+                                } else {
+                                    if (leader) umma_commit(&bars[V_EMPTY + stage]);
+                                    ++done1;
+                                    ++gv;
+                                }
+                            }
+                            if (have_next) {
+                                const int stage = gk % kStages;
+                                if (i == 0 && !(ok = mbar_wait_warp(&bars[K_FULL + stage], (gk / kStages) & 1, p.status, K_FULL, abort_flag))) break;
+                                tc_fence_after();
+                                issue_qk(i, stage);
+                                if (leader) umma_commit(&bars[S_FULL + i]);
+                                if (i == 1) {
+                                    if (leader) umma_commit(&bars[K_EMPTY + stage]);
+                                    if (j + 2 == count && leader) umma_commit(&bars[Q_EMPTY]);
+                                    ++gk;
+                                }
+                            }
+                        }
                     }
-                    if (i) ++done1;
-                    else ++done0;
-                    ++gv;
-                    if (j + 2 < count) next_scores(j + 2);
+                } else {
+                    auto next_scores = [&](int j) {   // Q K^T of the piece's unit j
+                        if (!(ok = mbar_wait_warp(&bars[K_FULL + gk % kStages], (gk / kStages) & 1, p.status, K_FULL, abort_flag))) return;
+                        tc_fence_after();
+                        issue_qk(j & 1, gk % kStages);
+                        if (leader) {
+                            umma_commit(&bars[S_FULL + (j & 1)]);
+                            umma_commit(&bars[K_EMPTY + gk % kStages]);
+                            if (j + 1 == count) umma_commit(&bars[Q_EMPTY]);
+                        }
+                        ++gk;
+                    };
+                    next_scores(0);
+                    if (ok && count > 1) next_scores(1);
+                    for (int j = 0; ok && j < count; ++j) {
+                        const int i = j & 1, stage = gv % kStages;
+                        if (!(ok = mbar_wait_warp(&bars[V_FULL + stage], (gv / kStages) & 1, p.status, V_FULL, abort_flag))) break;
+                        if (!(ok = mbar_wait_warp(&bars[P_FULL + i], (i ? done1 : done0) & 1, p.status, P_FULL, abort_flag))) break;
+                        if (j == 0 && pieces > 0 && !(ok = mbar_wait_warp(&bars[O_FREE], (pieces - 1) & 1, p.status, O_FREE, abort_flag))) break;
+                        tc_fence_after();
+                        issue_pv(i, stage, j > 1);
+                        if (leader) {
+                            umma_commit(&bars[O_FULL + i]);
+                            umma_commit(&bars[V_EMPTY + stage]);
+                        }
+                        if (i) ++done1;
+                        else ++done0;
+                        ++gv;
+                        if (j + 2 < count) next_scores(j + 2);
+                    }
                 }
                 ++pieces;
             }
@@ -332,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
         } else if (warp == 3) {
             // -------------------------------------------------------------- scout
             Range r = range;
-            Load l = load_of(p, kN, kN, r.b, bad);
+            Load l = load_of(p, kItemRows, kN, r.b, bad);
             int q = 0, told = 0, pieces = 0;   // units, pieces, pieces with units so far
             bool ok = true;
             const int bs_mask = (1 << p.c.bs_log2) - 1;
@@ -349,17 +392,17 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 if (r.left > 0) {
                     while (r.off >= (int64_t)l.units * l.items) {
                         r.off -= (int64_t)l.units * l.items;
-                        l = load_of(p, kN, kN, ++r.b, bad);
+                        l = load_of(p, kItemRows, kN, ++r.b, bad);
                     }
                     const int item = (int)(r.off / l.units), tiles = l.items / p.c.Hkv;
                     x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles; x.len = l.len; x.n = l.n;
                     x.u0 = (int)(r.off - (int64_t)item * l.units);
                     const int u1 = (int)min((int64_t)l.units, x.u0 + r.left);
-                    const int last = min(l.n - 1, (x.tile * kN + kN - 1) / p.G);          // the tile's last query
+                    const int last = min(l.n - 1, (x.tile * kItemRows + kItemRows - 1) / p.G);   // the item's last query
                     const int most = p.causal ? max(l.len - l.n + last + 1, 0) : l.len;   // slots that some row sees
                     x.count = max(min((most + kN - 1) / kN, u1) - x.u0, 0);
                     x.whole = x.u0 == 0 && u1 == l.units;
-                    seen = p.causal ? l.len - l.n + x.tile * kN / p.G + 1 : l.len;        // slots below this are seen by every row
+                    seen = p.causal ? l.len - l.n + x.tile * kItemRows / p.G + 1 : l.len;   // slots below this are seen by every row
                     r.off += u1 - x.u0;
                     r.left -= u1 - x.u0;
                 }
@@ -499,11 +542,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             named_bar_sync(9, 512);
             const PieceNote& x = z.pieces[place];
             if (z.left != 0 || x.b < 0) break;
-            const int count = x.count, grow = x.tile * kN + row, t = grow / p.G, u0 = x.u0;
-            const float factor = factors[((int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + x.tile) * kN + row];
+            const int count = x.count, item_row = PAIR ? grp * kN + row : row, grow = x.tile * kItemRows + item_row, t = grow / p.G, u0 = x.u0;
+            const float factor = factors[((int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + x.tile) * kItemRows + item_row];
             const int sees = p.causal ? x.len - x.n + t + 1 : x.len;
             float m = kLowest, l = 0.f;
-            for (int j = grp; j < count; j += 2, ++gs) {
+            for (int j = PAIR ? 0 : grp; j < count; j += PAIR ? 1 : 2, ++gs) {
                 const UnitNote& note = z.units[(q + j) % kUnitSlots];
                 wait(S_FULL + grp, gs & 1);
                 uint32_t s0[32], s1[32];
@@ -578,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                     exp_group(s1 + 16, drop.w, pk + 8);
                     COROPE_TMEM_ST16(tS + 16, pk);
                 }
-                if (j > 1 && __any_sync(0xffffffffu, need)) {
+                if (j > (PAIR ? 0 : 1) && __any_sync(0xffffffffu, need)) {
                     wait(O_FULL + grp, (gs - 1) & 1);
                     const float shrink = fast_exp2(m_old - m);
 #pragma unroll
@@ -602,20 +645,27 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             ends0 += (count + 1) / 2;
             ends1 += count / 2;
 
-            // the piece's sums: both groups' O, a quarter of the columns to each warpgroup
+            // The piece's sums.  PAIR: the group's O, half of the columns to each warpgroup.  Else both groups' O, a quarter of them to each.
             if (half == 0) z.end_max[grp][row] = m;
             z.end_sum[grp][half][row] = l;
             named_bar_sync(9, 512);   // (the exchange is written again behind the next piece's first barrier at the earliest)
-            if (count > 0) wait(O_FULL, (ends0 - 1) & 1);
-            if (count > 1) wait(O_FULL + 1, (ends1 - 1) & 1);
-            const float m0 = z.end_max[0][row], m1 = z.end_max[1][row], top = fmaxf(m0, m1);
-            const float w0 = fast_exp2(m0 - top), w1 = fast_exp2(m1 - top);
-            const float all = (z.end_sum[0][0][row] + z.end_sum[0][1][row]) * w0 + (z.end_sum[1][0][row] + z.end_sum[1][1][row]) * w1;
+            if (PAIR) {
+                if (count > 0) wait(O_FULL + grp, (gs - 1) & 1);
+            } else {
+                if (count > 0) wait(O_FULL, (ends0 - 1) & 1);
+                if (count > 1) wait(O_FULL + 1, (ends1 - 1) & 1);
+            }
+            const int other = PAIR ? grp : 0;
+            const float m0 = PAIR ? m : z.end_max[0][row], m1 = PAIR ? kLowest : z.end_max[1][row], top = fmaxf(m0, m1);
+            const float w0 = PAIR ? 1.f : fast_exp2(m0 - top), w1 = fast_exp2(m1 - top);
+            const float own = z.end_sum[other][0][row] + z.end_sum[other][1][row];
+            const float all = PAIR ? own : own * w0 + (z.end_sum[1][0][row] + z.end_sum[1][1][row]) * w1;
             const bool whole = x.whole != 0, some = t < x.n && all != 0.f;
             const float inv = whole ? 1.f / all : 1.f;
-            constexpr int kCols = kD / 4;
-            const int col0 = (grp * 2 + half) * kCols;
-            const int64_t part = (2 * (int64_t)blockIdx.x + (u0 == 0 ? 1 : 0)) * kN + row;
+            constexpr int kCols = PAIR ? kD / 2 : kD / 4;
+            const int col0 = (PAIR ? half : grp * 2 + half) * kCols;
+            const uint32_t tO0 = tO + other * 128;
+            const int64_t part = (2 * (int64_t)blockIdx.x + (u0 == 0 ? 1 : 0)) * kItemRows + item_row;
             const int64_t to = (int64_t)x.b * p.so.b + (int64_t)(x.h * p.G + grow - t * p.G) * p.so.h + (int64_t)t * p.so.n;
             const bool fix = CODE == COROPE_CODE_E4M3 && count > 0 && z.nan_v[pieces % kFlagSlots] != 0;
 #pragma unroll
@@ -625,11 +675,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 for (int i = 0; i < 16; ++i) y[i] = 0.f;
                 if (count > 0) {
                     uint32_t r[16];
-                    COROPE_TMEM_LD16(tO + col0 + k, r);
+                    COROPE_TMEM_LD16(tO0 + col0 + k, r);
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(r[i]) * w0;
-                    if (count > 1) {
+                    if (!PAIR && count > 1) {
                         COROPE_TMEM_LD16(tO + 128 + col0 + k, r);
                         tmem_wait_ld();
 #pragma unroll
@@ -659,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                                some ? make_float4(y[i] * inv, y[i + 1] * inv, y[i + 2] * inv, y[i + 3] * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
                 }
             }
-            if (grp == 0 && half == 0) {
+            if ((PAIR || grp == 0) && half == 0) {
                 if (!whole) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(top, all);
                 else if (p.lse != nullptr && t < p.T) p.lse[((int64_t)x.b * p.c.Hkv + x.h) * p.T * p.G + grow] = some ? top + log2f(all) : INFINITY;
             }
@@ -737,7 +787,7 @@ struct UnitWalk {
 };
 
 template <int D, int CODE>
-__global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const CacheAttnParams p, const uint8_t* images, const float* factors) {
+__global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const CacheAttnParams p, int image_tiles, const uint8_t* images, const float* factors) {
     constexpr int kD = wide(D), kBox = kN * 128;
     constexpr uint32_t kTile = (uint32_t)tile_bytes(D);
     extern __shared__ uint8_t smem_raw[];
@@ -797,7 +847,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
         while (ok && walk.next(p, x))
             for (int t = x.tile0; ok && t < x.tiles; ++t, ++q) {
                 const int i = q % kQStages, slot = q % kRowSlots;
-                const int64_t item = (int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + t;
+                const int64_t item = (int64_t)(x.b * p.c.Hkv + x.h) * image_tiles + t;
                 if (q >= kQStages && !(ok = mbar_wait_warp(&bars[W_Q_EMPTY + i], ((q / kQStages) - 1) & 1, p.status, W_Q_EMPTY, abort_flag))) break;
                 if (lane == 0) {
                     mbar_arrive_expect_tx(&bars[W_Q_FULL + i], 2 * kTile);
@@ -849,7 +899,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
         __syncwarp();
     } else if (warp >= 4 && warp < 8) {
         // ------------------------------------------------------------------ K
-        using S = Steps<D, true>;
+        using S = Steps<D, true, false>;
         const int tid = threadIdx.x & 127, col = tid % S::kLanes * 16, row0 = tid / S::kLanes, in_block_mask = (1 << p.c.bs_log2) - 1;
         const int run = col / 8, swap = D == 128 ? run >> 3 : 0;
         const uint32_t first_at = (run >> 3) * kBox + row0 * 128 + ((((run & 7) ^ (row0 & 7)) ^ swap) << 4);
@@ -957,57 +1007,70 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
 struct TileLayout {
     size_t factors, total;   // the images come first
 };
-TileLayout tile_layout(int B, int Hkv, int row_tiles, int D, bool two) {
-    const size_t items = (size_t)B * Hkv * row_tiles;
+TileLayout tile_layout(int B, int Hkv, int image_tiles, int D, bool two) {
+    const size_t items = (size_t)B * Hkv * image_tiles;
     TileLayout l;
     l.factors = items * (two ? 2 : 1) * tile_bytes(D);
     l.total = align_up(l.factors + items * kN * 4, 256);
     return l;
 }
 
-template <int D, int CODE, bool TWO>
+template <int D, int CODE, bool TWO, bool PAIR>
 int launch_t(const CacheAttnParams& p, uint8_t* images, float* factors, unsigned blocks, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    if (int e = allow_smem(cache_attn_tile_kernel<D, CODE, TWO>, smem_bytes(D, TWO), done)) return e;
+    if (int e = allow_smem(cache_attn_tile_kernel<D, CODE, TWO, PAIR>, smem_bytes(D, TWO, PAIR), done)) return e;
+    const int image_tiles = p.row_tiles * (PAIR ? 2 : 1);
     count_launch(2);
-    cache_pack_kernel<D, TWO><<<(unsigned)(p.s.B * p.c.Hkv * p.row_tiles * kPackBlocks), kPackWarps * 32, 0, s>>>(p, images, factors);
+    cache_pack_kernel<D, TWO><<<(unsigned)(p.s.B * p.c.Hkv * image_tiles * kPackBlocks), kPackWarps * 32, 0, s>>>(p, image_tiles, images, factors);
     if (int e = (int)cudaGetLastError()) return e;
-    return launch_dependent(cache_attn_tile_kernel<D, CODE, TWO>, blocks, kThreads, smem_bytes(D, TWO), s, p, (const uint8_t*)images, (const float*)factors);
+    return launch_dependent(cache_attn_tile_kernel<D, CODE, TWO, PAIR>, blocks, kThreads, smem_bytes(D, TWO, PAIR), s, p, (const uint8_t*)images, (const float*)factors);
 }
 template <int D, int CODE>
-int launch_weight_t(const CacheAttnParams& p, const uint8_t* images, const float* factors, cudaStream_t s) {
+int by_shape(const CacheAttnParams& p, uint8_t* images, float* factors, bool two, bool pair, unsigned blocks, cudaStream_t s) {
+    if constexpr (D != 128)
+        if (two && pair) return launch_t<D, CODE, true, true>(p, images, factors, blocks, s);
+    if (pair) return launch_t<D, CODE, false, true>(p, images, factors, blocks, s);
+    return two ? launch_t<D, CODE, true, false>(p, images, factors, blocks, s) : launch_t<D, CODE, false, false>(p, images, factors, blocks, s);
+}
+template <int D>
+int by_code(const CacheAttnParams& p, uint8_t* images, float* factors, bool two, bool pair, unsigned blocks, cudaStream_t s) {
+    return p.code == COROPE_CODE_E4M3 ? by_shape<D, COROPE_CODE_E4M3>(p, images, factors, two, pair, blocks, s)
+                                      : by_shape<D, COROPE_CODE_INT8>(p, images, factors, two, pair, blocks, s);
+}
+template <int D, int CODE>
+int launch_weight_t(const CacheAttnParams& p, int image_tiles, const uint8_t* images, const float* factors, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     if (int e = allow_smem(cache_weight_tile_kernel<D, CODE>, sum_smem_bytes(D), done)) return e;
     const uint64_t units = (uint64_t)p.s.B * p.c.Hkv * ((p.capacity + kN - 1) / kN);
     count_launch();
-    cache_weight_tile_kernel<D, CODE><<<(unsigned)(units < (uint64_t)sm_count() ? units : sm_count()), kSumThreads, sum_smem_bytes(D), s>>>(p, images, factors);
+    cache_weight_tile_kernel<D, CODE><<<(unsigned)(units < (uint64_t)sm_count() ? units : sm_count()), kSumThreads, sum_smem_bytes(D), s>>>(p, image_tiles, images, factors);
     return (int)cudaGetLastError();
 }
 template <int D>
-int by_code(const CacheAttnParams& p, uint8_t* images, float* factors, bool two, unsigned blocks, cudaStream_t s) {
-    if (p.code == COROPE_CODE_E4M3) return two ? launch_t<D, COROPE_CODE_E4M3, true>(p, images, factors, blocks, s) : launch_t<D, COROPE_CODE_E4M3, false>(p, images, factors, blocks, s);
-    return two ? launch_t<D, COROPE_CODE_INT8, true>(p, images, factors, blocks, s) : launch_t<D, COROPE_CODE_INT8, false>(p, images, factors, blocks, s);
-}
-template <int D>
-int weight_by_code(const CacheAttnParams& p, const uint8_t* images, const float* factors, cudaStream_t s) {
-    return p.code == COROPE_CODE_E4M3 ? launch_weight_t<D, COROPE_CODE_E4M3>(p, images, factors, s) : launch_weight_t<D, COROPE_CODE_INT8>(p, images, factors, s);
+int weight_by_code(const CacheAttnParams& p, int image_tiles, const uint8_t* images, const float* factors, cudaStream_t s) {
+    return p.code == COROPE_CODE_E4M3 ? launch_weight_t<D, COROPE_CODE_E4M3>(p, image_tiles, images, factors, s)
+                                      : launch_weight_t<D, COROPE_CODE_INT8>(p, image_tiles, images, factors, s);
 }
 
 }  // namespace
 
-size_t cache_tile_workspace_bytes(int B, int Hkv, int row_tiles, int D, bool two_parts) { return tile_layout(B, Hkv, row_tiles, D, two_parts).total; }
+bool cache_tile_pairs(int rows, int D, bool two_parts) { return rows > kN && !(D == 128 && two_parts); }
 
-int launch_cache_attn_tiles(const CacheAttnParams& p, void* ws, bool two_parts, unsigned blocks, cudaStream_t s) {
+size_t cache_tile_workspace_bytes(int B, int Hkv, int image_tiles, int D, bool two_parts) { return tile_layout(B, Hkv, image_tiles, D, two_parts).total; }
+
+int launch_cache_attn_tiles(const CacheAttnParams& p, void* ws, bool two_parts, bool pair, unsigned blocks, cudaStream_t s) {
     uint8_t* images = static_cast<uint8_t*>(ws);
-    float* factors = reinterpret_cast<float*>(images + tile_layout(p.s.B, p.c.Hkv, p.row_tiles, p.D, two_parts).factors);
-    return p.D == 128 ? by_code<128>(p, images, factors, two_parts, blocks, s) : p.D == 64 ? by_code<64>(p, images, factors, two_parts, blocks, s)
-                                                                                         : by_code<32>(p, images, factors, two_parts, blocks, s);
+    float* factors = reinterpret_cast<float*>(images + tile_layout(p.s.B, p.c.Hkv, p.row_tiles * (pair ? 2 : 1), p.D, two_parts).factors);
+    return p.D == 128 ? by_code<128>(p, images, factors, two_parts, pair, blocks, s) : p.D == 64 ? by_code<64>(p, images, factors, two_parts, pair, blocks, s)
+                                                                                               : by_code<32>(p, images, factors, two_parts, pair, blocks, s);
 }
 
-int launch_cache_weight_tiles(const CacheAttnParams& p, void* ws, cudaStream_t s) {
+int launch_cache_weight_tiles(const CacheAttnParams& p, void* ws, bool pair, cudaStream_t s) {
+    const int image_tiles = p.row_tiles * (pair ? 2 : 1);
     const uint8_t* images = static_cast<const uint8_t*>(ws);
-    const float* factors = reinterpret_cast<const float*>(images + tile_layout(p.s.B, p.c.Hkv, p.row_tiles, p.D, true).factors);
-    return p.D == 128 ? weight_by_code<128>(p, images, factors, s) : p.D == 64 ? weight_by_code<64>(p, images, factors, s) : weight_by_code<32>(p, images, factors, s);
+    const float* factors = reinterpret_cast<const float*>(images + tile_layout(p.s.B, p.c.Hkv, image_tiles, p.D, true).factors);
+    return p.D == 128 ? weight_by_code<128>(p, image_tiles, images, factors, s) : p.D == 64 ? weight_by_code<64>(p, image_tiles, images, factors, s)
+                                                                                          : weight_by_code<32>(p, image_tiles, images, factors, s);
 }
 
 }  // namespace corope
