@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 // added in the order of their ranges.  Rows that no unit stands for are written here: 0.
 constexpr int kJoinThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const CacheAttnParams p, int rows_per_tile, int unit, int main_blocks) {
+__global__ void __launch_bounds__(kJoinThreads, 6) cache_attn_join_kernel(const CacheAttnParams p, int rows_per_tile, int unit, int main_blocks) {
     __shared__ int64_t words[2][kJoinThreads / 32];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const unsigned blocks = (unsigned)rows_per_tile / (kJoinThreads / 32), item = blockIdx.x / blocks;
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const Cac
                 for (int m = 16; m; m >>= 1) add += __shfl_xor_sync(0xffffffffu, add, m);
                 all = fmaf(all, shrink, add);
                 y = make_float4(y.x * shrink, y.y * shrink, y.z * shrink, y.w * shrink);
-#pragma unroll 8
+#pragma unroll 4
                 for (int k = 0; k < here; ++k) {
                     const float fk = __shfl_sync(0xffffffffu, f, k);
                     if (lane < D / 4) {
@@ -657,9 +657,9 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attn_join_kernel(const Cac
 // ------------------------------------------------------------------------------------------------ accumulated weights
 // Few query rows (one tile): the main kernel has left the scores, 4 bytes a row and slot, and a thread sums a slot's exp2(s - lse).  K is not read
 // again, which would be D bytes a slot and all of its products.
-constexpr int kSumUnit = kThreads;
+constexpr int kSumUnit = kThreads, kSumBlocks = 16;   // blocks an SM: a unit is a chain of two loads, what is beside it hides them
 template <bool FOURS>
-__global__ void __launch_bounds__(kThreads) cache_attn_sum_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(kThreads, kSumBlocks) cache_attn_sum_kernel(const CacheAttnParams p) {
     bool bad = false;
     auto load = [&](int b) {
         Load l = load_of(p, 1, kSumUnit, b, bad);
@@ -899,7 +899,8 @@ int launch_rows(const CacheAttnParams& p, const Layout& l, cudaStream_t s) {
     if (int e = launch_join<D>(p, l, kUnit, s)) return e;
     if (!p.accumulate) return COROPE_OK;
     count_launch();
-    const uint64_t units = (uint64_t)p.s.B * p.c.Hkv * ((uint64_t)(p.capacity + kUnit - 1) / kUnit), most = (uint64_t)sm_count() * 8;
+    const int unit = p.scores != nullptr ? kSumUnit : kUnit;
+    const uint64_t units = (uint64_t)p.s.B * p.c.Hkv * ((uint64_t)(p.capacity + unit - 1) / unit), most = (uint64_t)sm_count() * (p.scores != nullptr ? kSumBlocks : 8);
     const unsigned grid = (unsigned)(units < most ? units : most);
     if (p.scores != nullptr) return launch_dependent(p.score_rows % 4 == 0 ? cache_attn_sum_kernel<true> : cache_attn_sum_kernel<false>, grid, kThreads, 0, s, p);
     cache_attn_weight_kernel<D, CODE, NT><<<grid, kThreads, 0, s>>>(p);
