@@ -296,8 +296,10 @@ int corope_gqa_bwd_strided(const void* q, const void* k, const void* v, const vo
  *
  * All index arrays are device memory and are never read on the host.  An entry that points outside its tensor (a block id outside
  * [0, num_blocks), a length beyond the block table or below 0, a position beyond the tables) is not followed: the tokens concerned are
- * left out (a position is clamped) and COROPE_DEV_BAD_INDEX is written to the status word.  These kernels run on whatever an earlier kernel left in
- * the word.  They take fp32 / bf16 / fp16 tensors, hold scores, sums and scales in fp32 and have no backward pass.
+ * left out (a position is clamped) and COROPE_DEV_BAD_INDEX is written to the status word.  These kernels run whatever an earlier kernel left in
+ * the word, but for those of corope_cache_attn with waits of their own (16-bit tensors, more than 32 query rows a K / V head), which do not after
+ * COROPE_DEV_WAIT_EXPIRED.  They take fp32 / bf16 / fp16 tensors, hold scores, sums and scales in fp32 and have no backward pass.  Scales are
+ * not negative.
  */
 #define COROPE_CODE_E4M3 0   /* 8-bit floats, largest finite value 448 */
 #define COROPE_CODE_INT8 1   /* whole numbers -127 .. 127 */
@@ -338,7 +340,10 @@ int corope_cache_append(const corope_kv_cache_t* cache, const corope_cache_seqs_
  * Attention of q [B, Hq, T, D] over the cache: query t < n of sequence b (its last n tokens) sees slots below
  * seq_lens[b] - n + t + 1 (causal) or all seq_lens[b].  Query head h reads K / V head h / (Hq / Hkv), any group size.  o [B, Hq, T, D] in
  * `dtype`; rows without a visible slot and rows t >= n are 0.  accumulate: weight[slot] += the slot's probabilities summed over
- * the queries and the heads of its group.
+ * the queries and the heads of its group.  Scores have fp32 accuracy; for bf16 tensors of more than 32 query rows a K / V head without `accumulate`
+ * the rotated queries are rounded to 11 bits first.  Probabilities are rounded to 11 bits for 16-bit tensors, to 22 for fp32 ones.
+ * The workspace (ask with the call's own arguments and the same current device): parts of results, with `accumulate` also 4 bytes per slot of the
+ * block tables and query row (where that is at most 512 MiB), for more than 32 rows fp16 copies of q.
  */
 size_t corope_cache_attn_workspace_bytes(const corope_kv_cache_t* cache, const corope_cache_seqs_t* seqs, int Hq, int T, int dtype, int accumulate);
 int corope_cache_attn(const corope_kv_cache_t* cache, const corope_cache_seqs_t* seqs, const void* q, void* o, const int64_t q_strides[3],
