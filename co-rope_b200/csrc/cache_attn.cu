@@ -27,6 +27,9 @@ namespace cg = cooperative_groups;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kPiece = 16;                    // slots per step of a warp; a block of the cache holds a whole number of them
 constexpr int kUnit = kWarps * kPiece;        // slots per unit of work
+// Units that an item counts beside its own in sharing out the work.  0 / 4 / 6 / 12, us, 32 / 8 heads of 128: 64 x up to 4096 tokens 68.1 / 62.6 /
+// 60.5 / 63.1, 256 x up to 1000 97.6 / 80.3 / 80.6 / 81.8, 8 x 16384 58.0 / 56.4 / 56.5 / 57.6.
+constexpr int kItemCost = 6;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
     bool bad = false;
 
-    auto load = [&](int b) { return load_of(p, kRows, kUnit, b, bad); };
+    auto load = [&](int b) { return load_of(p, kRows, kUnit, kItemCost, b, bad); };
     __shared__ int nan_v;   // NaN in V where some rows must not see it
     // Either a range of the batch's units, or (p.parts) this block's share of one item, whose other shares are with the blocks of its cluster.
     int b, part_of = 0, cluster_item = 0;
@@ -183,17 +186,20 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     do {
         int h, tile, u0, u1;
         if (p.parts == 0) {
-            while (off >= (int64_t)l.units * l.items) {
-                off -= (int64_t)l.units * l.items;
+            while (off >= (int64_t)l.cost * l.items) {
+                off -= (int64_t)l.cost * l.items;
                 l = load(++b);
             }
-            const int item = (int)(off / l.units), tiles = l.items / p.c.Hkv;
+            const int item = (int)(off / l.cost), tiles = l.items / p.c.Hkv;
             h = item / tiles;
             tile = item % tiles;
-            u0 = (int)(off - (int64_t)item * l.units);
-            u1 = (int)min((int64_t)l.units, u0 + left);
+            u0 = (int)(off - (int64_t)item * l.cost);
+            u1 = (int)min((int64_t)l.cost, u0 + left);
             off += u1 - u0;
             left -= u1 - u0;
+            u0 = max(u0 - kItemCost, 0);
+            u1 -= kItemCost;
+            if (u1 <= 0) continue;   // the range ends before the item's first unit
         } else {
             const int item = cluster_item - b * p.c.Hkv * p.row_tiles;
             h = item / p.row_tiles;
@@ -578,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 // added in the order of their ranges.  Rows that no unit stands for are written here: 0.
 constexpr int kJoinThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads, 6) cache_attn_join_kernel(const CacheAttnParams p, int rows_per_tile, int unit, int main_blocks) {
+__global__ void __launch_bounds__(kJoinThreads, 6) cache_attn_join_kernel(const CacheAttnParams p, int rows_per_tile, int unit, int extra, int main_blocks) {
     __shared__ int64_t words[2][kJoinThreads / 32];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const unsigned blocks = (unsigned)rows_per_tile / (kJoinThreads / 32), item = blockIdx.x / blocks;
@@ -586,8 +592,8 @@ __global__ void __launch_bounds__(kJoinThreads, 6) cache_attn_join_kernel(const 
     bool bad = false;
     int64_t before = 0, total = 0;
     for (int i = threadIdx.x; i < p.s.B; i += kJoinThreads) {
-        const Load l = load_of(p, rows_per_tile, unit, i, bad);
-        const int64_t u = (int64_t)l.units * l.items;
+        const Load l = load_of(p, rows_per_tile, unit, extra, i, bad);
+        const int64_t u = (int64_t)l.cost * l.items;
         total += u;
         if (i < b) before += u;
     }
@@ -602,13 +608,13 @@ __global__ void __launch_bounds__(kJoinThreads, 6) cache_attn_join_kernel(const 
 #pragma unroll
     for (int w = 0; w < kJoinThreads / 32; ++w) before += words[0][w], total += words[1][w];
 
-    const Load l = load_of(p, rows_per_tile, unit, b, bad);
+    const Load l = load_of(p, rows_per_tile, unit, extra, b, bad);
     const int tiles = l.items / p.c.Hkv;
     const bool empty = l.units == 0 || tile >= tiles;
     const int64_t ranges = min((int64_t)main_blocks, total);
     int64_t r0 = 0, r1 = 0;
     if (!empty) {
-        const int64_t u0 = before + (int64_t)(h * tiles + tile) * l.units, u1 = u0 + l.units - 1;
+        const int64_t u0 = before + (int64_t)(h * tiles + tile) * l.cost + extra, u1 = u0 + l.units - 1;
         r0 = ((u0 + 1) * ranges - 1) / total;   // the range that holds a unit
         r1 = ((u1 + 1) * ranges - 1) / total;
     }
@@ -662,7 +668,7 @@ template <bool FOURS>
 __global__ void __launch_bounds__(kThreads, kSumBlocks) cache_attn_sum_kernel(const CacheAttnParams p) {
     bool bad = false;
     auto load = [&](int b) {
-        Load l = load_of(p, 1, kSumUnit, b, bad);
+        Load l = load_of(p, 1, kSumUnit, 0, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     };
@@ -716,7 +722,7 @@ __global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const Cache
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
     bool bad = false;
     auto load = [&](int b) {
-        Load l = load_of(p, kRows, kUnit, b, bad);
+        Load l = load_of(p, kRows, kUnit, 0, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     };   // items of this kernel: K / V heads
@@ -829,7 +835,7 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     Layout l{};
     const int rows = G * T;
     const uint64_t slots = (uint64_t)max_blocks * block_size;
-    // 16-bit tensors of more than 32 rows a head: products on tcgen05 (a chunk of 1024 queries, 32 / 8 heads, over 9001 tokens: 224 us, 970 with
+    // 16-bit tensors of more than 32 rows a head: products on tcgen05 (a chunk of 1024 queries, 32 / 8 heads, over 9001 tokens: 217 us, 970 with
     // tiles of 32 rows).  fp32 tensors stay with the kernel that splits P as well.
     l.tiles = dtype != COROPE_DTYPE_F32 && rows > 32;
     // one part of q is off by 2^-12 of it: next to a bf16 result's 2^-9 that is nothing, an fp16 result or a weight would feel it
@@ -839,7 +845,7 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     l.rows_per_tile = l.tiles ? kTileRows * (l.pair ? 2 : 1) : 8 * l.groups;
     l.row_tiles = (rows + l.rows_per_tile - 1) / l.rows_per_tile;
     const uint64_t items = (uint64_t)B * Hkv * l.row_tiles, unit = l.tiles ? kTileRows : kUnit;
-    const uint64_t units = items * ((slots + unit - 1) / unit), most = (uint64_t)sm_count() * (l.tiles ? 1 : resident_blocks(l.groups));
+    const uint64_t item_units = (slots + unit - 1) / unit, units = items * (item_units + (l.tiles ? kTileItemCost : kItemCost)), most = (uint64_t)sm_count() * (l.tiles ? 1 : resident_blocks(l.groups));
     l.blocks = (unsigned)(units < most ? units : most);
     // Room for the scores of every slot that the block tables could hold.  Beyond half a gigabyte (long tables that the sequences may not fill) K is
     // read again instead: 32 sequences of up to 8192 tokens, 4 rows a head, take 88 us with the scores, 148 without.
@@ -847,8 +853,7 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     l.score_rows = accumulate && !l.tiles && l.row_tiles == 1 && score_bytes <= (512u << 20) ? (rows + 1) / 2 * 2 : 0;
     // A cluster per item where all of them are resident at once and no block has more than kClusterUnits units of the longest sequence there can be:
     // the sequences' own lengths are not known here, so the longest sets the pace.  Ranges and a joining kernel / clusters, us, 32 / 8 heads of 128: 1 x
-    // 777 tokens 11.5 / 8.5, 1 x 4096 21.2 / 12.9, 16 x 1024 21.1 / 14.1, 16 x up to 4096 27.1 / 30.1, 64 x up to 1024 33.1 / 28.4.
-    const uint64_t item_units = (slots + unit - 1) / unit;
+    // 777 tokens 11.5 / 8.5, 1 x 4096 27.2 / 11.5, 16 x 1024 17.3 / 13.6, 16 x up to 4096 24.2 / 25.9, 64 x up to 1024 26.5 / 24.7.
     if (!l.tiles && items <= most && (!accumulate || l.score_rows)) {
         l.parts = 1;
         while (l.parts < 8 && items * l.parts * 2 <= most && item_units >= (uint64_t)l.parts * 2) l.parts *= 2;
@@ -866,9 +871,9 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
 }
 
 template <int D>
-int launch_join(const CacheAttnParams& p, const Layout& l, int unit, cudaStream_t s) {
+int launch_join(const CacheAttnParams& p, const Layout& l, int unit, int extra, cudaStream_t s) {
     count_launch();
-    return launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles * (l.rows_per_tile / 8)), kJoinThreads, 0, s, p, l.rows_per_tile, unit, (int)l.blocks);
+    return launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles * (l.rows_per_tile / 8)), kJoinThreads, 0, s, p, l.rows_per_tile, unit, extra, (int)l.blocks);
 }
 template <int D, int CODE, int NT, bool EXACT_P>
 int launch_main(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
@@ -896,7 +901,7 @@ template <int D, int CODE, int NT>
 int launch_rows(const CacheAttnParams& p, const Layout& l, cudaStream_t s) {
     if (int e = p.dtype == COROPE_DTYPE_F32 ? launch_main<D, CODE, NT, true>(p, l.blocks, s) : launch_main<D, CODE, NT, false>(p, l.blocks, s)) return e;
     if (l.parts) return COROPE_OK;
-    if (int e = launch_join<D>(p, l, kUnit, s)) return e;
+    if (int e = launch_join<D>(p, l, kUnit, kItemCost, s)) return e;
     if (!p.accumulate) return COROPE_OK;
     count_launch();
     const int unit = p.scores != nullptr ? kSumUnit : kUnit;
@@ -914,7 +919,7 @@ template <int D>
 int by_kernel(const CacheAttnParams& p, const Layout& l, void* images, cudaStream_t s) {
     if (!l.tiles) return p.code == COROPE_CODE_E4M3 ? by_rows<D, COROPE_CODE_E4M3>(p, l, s) : by_rows<D, COROPE_CODE_INT8>(p, l, s);
     if (int e = launch_cache_attn_tiles(p, images, l.two_parts, l.pair, l.blocks, s)) return e;
-    if (int e = launch_join<D>(p, l, kTileRows, s)) return e;
+    if (int e = launch_join<D>(p, l, kTileRows, kTileItemCost, s)) return e;
     return p.accumulate ? launch_cache_weight_tiles(p, images, l.pair, s) : COROPE_OK;
 }
 

@@ -25,18 +25,21 @@ __device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint3
 // ------------------------------------------------------------------------------------------------ division of the work
 // Work is counted in units of `unit` slots of one item, a (K / V head, tile of query rows) of a sequence: sequence b has items(b) = Hkv * (row tiles in
 // use) items of units(b) units each, one after the other.
+// What an item costs beside its units (queries made ready, parts joined and written) is counted as `extra` units in front of them, so that a block
+// with the ends of several items has as long to do as one with the middle of one.
 struct Load {
-    int len, n, units, items;
+    int len, n, units, items, cost;   // cost: of an item, extra units included
 };
-__device__ __forceinline__ Load load_of(const CacheAttnParams& p, int rows_per_tile, int unit, int b, bool& bad) {
+__device__ __forceinline__ Load load_of(const CacheAttnParams& p, int rows_per_tile, int unit, int extra, int b, bool& bad) {
     Load l;
     l.len = cache_len(p.s, p.c.bs_log2, b, bad);
     l.n = cache_new(p.s, p.T, b, bad);
     l.units = (l.len + unit - 1) / unit;
     l.items = p.c.Hkv * ((l.n * p.G + rows_per_tile - 1) / rows_per_tile);
+    l.cost = l.units > 0 ? l.units + extra : 0;
     return l;
 }
-// The range of units that a block has (its first THREADS threads look at the sequences), as a place to start (sequence b, `off` units into its own) and a number of units; 0 of
+// The range of units that a block has (its first THREADS threads look at the sequences), as a place to start (sequence b, `off` into its own) and a number of units; 0 of
 // them: the block is not needed.  `load(b)` tells a sequence's load.
 struct Range {
     int b;
@@ -52,7 +55,7 @@ __device__ __forceinline__ Range take_range(int B, const LoadFn& load) {
     int64_t mine = 0;
     for (int b = b0; b < b1; ++b) {
         const Load l = load(b);
-        mine += (int64_t)l.units * l.items;
+        mine += (int64_t)l.cost * l.items;
     }
     int64_t sum = mine;
 #pragma unroll
@@ -74,7 +77,7 @@ __device__ __forceinline__ Range take_range(int B, const LoadFn& load) {
     if (lo >= at && lo < at + mine)
         for (int b = b0; b < b1; ++b) {
             const Load l = load(b);
-            const int64_t u = (int64_t)l.units * l.items;
+            const int64_t u = (int64_t)l.cost * l.items;
             if (lo >= at && lo < at + u) start_b = b, start_off = lo - at;
             at += u;
         }
@@ -86,6 +89,10 @@ __device__ __forceinline__ Range take_range(int B, const LoadFn& load) {
 
 // Attention of many query rows a K / V head on tcgen05 (16-bit types): the steps of launch_cache_attn that are its own.
 constexpr int kTileRows = 128;                // query rows of a tile, and slots of a unit
+// Units that an item counts beside its own in sharing out the work (queries loaded, parts written).  0 / 2 / 4 / 8, us, 32 / 8 heads of 128: 32
+// sequences of up to 4096 tokens with 16 queries each 137 / 116 / 109 / 109, one of 4096 with 256 59.4 / 53.8 / 51.5 / 53.3, one of 9001 with 1024
+// 216 / 216 / 217 / 226.
+constexpr int kTileItemCost = 4;
 bool cache_tile_pairs(int rows, int D, bool two_parts);   // items of two tiles of rows
 size_t cache_tile_workspace_bytes(int B, int Hkv, int image_tiles, int D, bool two_parts);
 int launch_cache_attn_tiles(const CacheAttnParams& p, void* ws, bool two_parts, bool pair, unsigned blocks, cudaStream_t s);

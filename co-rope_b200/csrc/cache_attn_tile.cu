@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     bool bad = false;
-    const Range range = take_range<128>(p.s.B, [&](int b) { return load_of(p, kItemRows, kN, b, bad); });
+    const Range range = take_range<128>(p.s.B, [&](int b) { return load_of(p, kItemRows, kN, kTileItemCost, b, bad); });
     pdl_trigger();
     if (bad) report_bad_index(p.status, p.mirror);
     // after a wait that ran out, in this launch's block or in an earlier launch, none starts anew until the host has seen it
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
         } else if (warp == 3) {
             // -------------------------------------------------------------- scout
             Range r = range;
-            Load l = load_of(p, kItemRows, kN, r.b, bad);
+            Load l = load_of(p, kItemRows, kN, kTileItemCost, r.b, bad);
             int q = 0, told = 0, pieces = 0;   // units, pieces, pieces with units so far
             bool ok = true;
             const int bs_mask = (1 << p.c.bs_log2) - 1;
@@ -389,22 +389,24 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 if (told >= kPieceSlots && !(ok = mbar_wait_warp(&bars[PIECE_EMPTY + slot], ((told / kPieceSlots) - 1) & 1, p.status, PIECE_EMPTY, abort_flag))) break;
                 PieceNote x{-1, 0, 0, 0, 0, 0, 0, 0};
                 int seen = 0;
-                if (r.left > 0) {
-                    while (r.off >= (int64_t)l.units * l.items) {
-                        r.off -= (int64_t)l.units * l.items;
-                        l = load_of(p, kItemRows, kN, ++r.b, bad);
+                while (r.left > 0 && x.b < 0) {
+                    while (r.off >= (int64_t)l.cost * l.items) {
+                        r.off -= (int64_t)l.cost * l.items;
+                        l = load_of(p, kItemRows, kN, kTileItemCost, ++r.b, bad);
                     }
-                    const int item = (int)(r.off / l.units), tiles = l.items / p.c.Hkv;
+                    const int item = (int)(r.off / l.cost), tiles = l.items / p.c.Hkv;
+                    const int at = (int)(r.off - (int64_t)item * l.cost), end = (int)min((int64_t)l.cost, at + r.left);
+                    r.off += end - at;
+                    r.left -= end - at;
+                    const int u1 = end - kTileItemCost;
+                    if (u1 <= 0) continue;   // the range ends before the item's first unit
                     x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles; x.len = l.len; x.n = l.n;
-                    x.u0 = (int)(r.off - (int64_t)item * l.units);
-                    const int u1 = (int)min((int64_t)l.units, x.u0 + r.left);
+                    x.u0 = max(at - kTileItemCost, 0);
                     const int last = min(l.n - 1, (x.tile * kItemRows + kItemRows - 1) / p.G);   // the item's last query
                     const int most = p.causal ? max(l.len - l.n + last + 1, 0) : l.len;   // slots that some row sees
                     x.count = max(min((most + kN - 1) / kN, u1) - x.u0, 0);
                     x.whole = x.u0 == 0 && u1 == l.units;
                     seen = p.causal ? l.len - l.n + x.tile * kItemRows / p.G + 1 : l.len;   // slots below this are seen by every row
-                    r.off += u1 - x.u0;
-                    r.left -= u1 - x.u0;
                 }
                 if (lane == 0) z.pieces[slot] = x;
                 mbar_arrive_warp(&bars[PIECE_FULL + slot], lane);
@@ -759,7 +761,7 @@ struct UnitWalk {
     Load l;
     bool bad = false;
     __device__ __forceinline__ Load load(const CacheAttnParams& p, int b) {
-        Load l = load_of(p, kN, kN, b, bad);
+        Load l = load_of(p, kN, kN, 0, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     }
@@ -801,7 +803,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     bool bad = false;
     const Range range = take_range<128>(p.s.B, [&](int b) {
-        Load l = load_of(p, kN, kN, b, bad);
+        Load l = load_of(p, kN, kN, 0, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     });
