@@ -81,7 +81,7 @@ __device__ __forceinline__ void pack_queries(const CacheAttnParams& p, int b, in
     for (int r = warp; r < 8 * NT; r += kWarps) {
         const int row = row0 + r, t = row / p.G;
         float x[4] = {0.f, 0.f, 0.f, 0.f};   // columns 2 lane, + 1, and their partners D / 2 further on
-        if (t < n && lane < kPairLanes) {
+        if (t < n && sees_something(p, len, n, t) && lane < kPairLanes) {
             const int64_t at = (int64_t)b * p.sq.b + (int64_t)(h * p.G + row - t * p.G) * p.sq.h + (int64_t)t * p.sq.n + 2 * lane;
             x[0] = load1(p.q, at, p.dtype); x[1] = load1(p.q, at + 1, p.dtype);
             x[2] = load1(p.q, at + kHalf, p.dtype); x[3] = load1(p.q, at + kHalf + 1, p.dtype);

@@ -22,6 +22,9 @@ __device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint3
     }
 }
 
+// A query that sees no slot (an empty place of a padded batch) is not read: its position need not be in the tables.
+__device__ __forceinline__ bool sees_something(const CacheAttnParams& p, int len, int n, int t) { return (p.causal ? len - n + t + 1 : len) > 0; }
+
 // ------------------------------------------------------------------------------------------------ division of the work
 // Work is counted in units of `unit` slots of one item, a (K / V head, tile of query rows) of a sequence: sequence b has items(b) = Hkv * (row tiles in
 // use) items of units(b) units each, one after the other.

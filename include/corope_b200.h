@@ -331,7 +331,7 @@ typedef struct corope_cache_seqs_t {
  *   scale of a block: max(its scale so far, if it holds older tokens; largest |finite new element| * r), r = the fp32 number next to 1/448 or 1/127
  *   code = x / scale rounded to nearest even, saturated; NaN stays NaN (e4m3) or becomes 0 (int8); a scale of 0 has codes 0
  * Older codes of a block whose scale grows are written again for the new one.  weight (if any) of the new slots becomes 0.
- * A block that a token is written to must belong to one sequence only.
+ * A block that a token is written to must stand in one place of the block table only.
  */
 int corope_cache_append(const corope_kv_cache_t* cache, const corope_cache_seqs_t* seqs, const void* k, const void* v, const int64_t k_strides[3],
                         const int64_t v_strides[3], int T, int dtype, int* status_word, void* stream);
@@ -339,7 +339,7 @@ int corope_cache_append(const corope_kv_cache_t* cache, const corope_cache_seqs_
 /*
  * Attention of q [B, Hq, T, D] over the cache: query t < n of sequence b (its last n tokens) sees slots below
  * seq_lens[b] - n + t + 1 (causal) or all seq_lens[b].  Query head h reads K / V head h / (Hq / Hkv), any group size.  o [B, Hq, T, D] in
- * `dtype`; rows without a visible slot and rows t >= n are 0.  accumulate: weight[slot] += the slot's probabilities summed over
+ * `dtype`; rows without a visible slot and rows t >= n are 0, whatever their query and position.  accumulate: weight[slot] += the slot's probabilities summed over
  * the queries and the heads of its group.  Scores have fp32 accuracy; for bf16 tensors of more than 32 query rows a K / V head without `accumulate`
  * the rotated queries are rounded to 11 bits first.  Probabilities are rounded to 11 bits for 16-bit tensors, to 22 for fp32 ones.
  * The workspace (ask with the call's own arguments and the same current device): parts of results, with `accumulate` also 4 bytes per slot of the

@@ -282,6 +282,18 @@ def test_rows_behind_the_last_query_are_zero_and_others_untouched():
     assert all(torch.equal(getattr(cache, x).view(torch.uint8), y) for x, y in zip(("k", "v"), before))
 
 
+@pytest.mark.parametrize("T", [1, 3, 20])
+@pytest.mark.parametrize("causal", [True, False])
+def test_empty_places_have_no_position(T, causal):
+    """Sequences of no tokens, and queries without a slot, beside a table of positions: their slots are below its first row."""
+    D, bs, lens = 64, 16, [0, 37, 2 if causal else 0, 0]
+    cache, host = make_cache(12, 2, bs, D, E4M3)
+    table = make_table(4, 3, 12, lens, bs)
+    cos, sin = precompute_freqs_cis(D, 50, 10000.0)
+    check_attention(cache, host, draw((4, 4, T, D), 1, F16), table, lens, causal, 0.3, cos, sin, accumulate=True)
+    check_attention(cache, host | {"weight": cache.weight.cpu()}, draw((4, 4, T, D), 1, F32), table, lens, causal, 0.3, cos, sin, new_lens=[T, 1, T, T])
+
+
 def test_many_sequences():
     """More sequences than a block has threads, most of them short or empty."""
     B, D, bs = 300, 32, 16
@@ -290,6 +302,42 @@ def test_many_sequences():
     table = make_table(B, 3, 3 * B, lens, bs)
     check_attention(cache, host, draw((B, 2, 1, D), 1, F16), table, lens, True, 0.3, accumulate=True)
     check_attention(cache, host | {"weight": cache.weight.cpu()}, draw((B, 2, 20, D), 2, BF16), table, lens, True, 0.3, new_lens=[i % 21 for i in range(B)], accumulate=True)
+
+
+@pytest.mark.parametrize("B,Hkv,T,dtype,wide,most", [
+    (60, 12, 1, BF16, 32, 500),      # more heads than resident blocks: several items a block
+    (3, 2, 1, F16, 600, 9600),       # tables too long for clusters
+    (3, 2, 1, BF16, 600, 200),       # .. and hardly filled: most blocks have no slot to read
+    (5, 2, 7, F32, 600, 1500),
+    (5, 3, 20, F32, 300, 900),       # two tiles of rows
+    (7, 3, 20, BF16, 300, 900),
+    (6, 2, 70, BF16, 100, 1500),
+    (2, 3, 70, F16, 12, 190),
+])
+def test_work_shared_out(B, Hkv, T, dtype, wide, most):
+    """Ranges that begin and end everywhere in an item: in its slots, between two items, in what an item costs beside its slots."""
+    D, bs = 32, 16
+    lens = torch.randint(0, most + 1, (B,), generator=torch.Generator().manual_seed(B * T)).tolist()
+    lens[B // 2], lens[-1] = 1, most
+    needed = sum(-(-n // bs) for n in lens)
+    cache, host = make_cache(needed + 1, Hkv, bs, D, INT8)
+    table, at = torch.full((B, wide), -1, dtype=torch.int32), 0
+    for b, n in enumerate(lens):
+        table[b, :-(-n // bs)] = torch.arange(at, at + -(-n // bs), dtype=torch.int32)
+        at += -(-n // bs)
+    check_attention(cache, host, draw((B, 2 * Hkv, T, D), 1, dtype), table, lens, True, 0.3, accumulate=True)
+
+
+@pytest.mark.parametrize("T", [1, 5, 40])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_scales_of_any_sign(T, dtype):
+    """A score times a negative number is that of the negated query, bit for bit; times 0 all slots count the same."""
+    D, bs, lens = 64, 16, [70, 45]
+    cache, host = make_cache(12, 2, bs, D, E4M3, weights=False)
+    table, q = make_table(2, 5, 12, lens, bs), draw((2, 4, T, D), 1, dtype)
+    got = [pkg.cache_attention(x.cuda(), cache, *gpu(table, ints(lens)), True, s) for x, s in ((q, -0.4), (-q, 0.4))]
+    assert torch.equal(*got)
+    check_attention(cache, host, q, table, lens, True, 0.0)
 
 
 def test_weights_without_room_for_scores():
