@@ -112,6 +112,7 @@ int corope_cache_evict(const corope_kv_cache_t* cache, const corope_cache_seqs_t
     if (int e = view_of(p.s, seqs, p.c, cache->D)) return e;
     if (!cache->weight) return COROPE_ERR_NULL_POINTER;
     if (budget <= 0 || recent < 0 || recent > budget) return COROPE_ERR_BAD_SHAPE;
+    if (budget >= (1 << 30)) return COROPE_ERR_TOO_LARGE;
     if (out_blocks <= 0 || ((int64_t)out_blocks << p.c.bs_log2) < budget) return COROPE_ERR_BAD_SHAPE;
     if (out_table_stride < (seqs->B > 1 ? out_blocks : 0)) return COROPE_ERR_BAD_STRIDE;
     p.out_table = out_table; p.out_stride = out_table_stride; p.out_blocks = out_blocks;

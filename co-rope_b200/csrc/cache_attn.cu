@@ -848,7 +848,7 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     const uint64_t item_units = (slots + unit - 1) / unit, units = items * (item_units + (l.tiles ? kTileItemCost : kItemCost)), most = (uint64_t)sm_count() * (l.tiles ? 1 : resident_blocks(l.groups));
     l.blocks = (unsigned)(units < most ? units : most);
     // Room for the scores of every slot that the block tables could hold.  Beyond half a gigabyte (long tables that the sequences may not fill) K is
-    // read again instead: 32 sequences of up to 8192 tokens, 4 rows a head, take 88 us with the scores, 148 without.
+    // read again instead: 32 sequences of up to 8192 tokens, 4 rows a head, take 80 us with the scores, 137 without.
     const size_t score_bytes = (size_t)B * Hkv * slots * ((rows + 1) / 2 * 2) * 4;
     l.score_rows = accumulate && !l.tiles && l.row_tiles == 1 && score_bytes <= (512u << 20) ? (rows + 1) / 2 * 2 : 0;
     // A cluster per item where all of them are resident at once and no block has more than kClusterUnits units of the longest sequence there can be:

@@ -403,14 +403,14 @@ const int* index_ptr(const Tensor& t, int64_t B, const Tensor& like, const char*
 }
 void table_checks(const Tensor& t, int64_t B, const Tensor& like, const char* name) {
     require_cuda(t);
-    require_value(t.dim() == 2 && t.size(0) == B && t.size(1) > 0 && t.scalar_type() == at::kInt && t.device() == like.device(),
+    require_value(t.dim() == 2 && t.size(0) == B && t.size(1) > 0 && t.size(1) < (1ll << 30) && t.scalar_type() == at::kInt && t.device() == like.device(),
                   std::string(name) + " must be an int32 tensor [B, blocks] on the cache's device");
     require_value((t.size(1) == 1 || t.stride(1) == 1) && (B == 1 || t.stride(0) >= t.size(1)), std::string(name) + " must have rows without gaps that do not overlap");
 }
 // `keep` holds what the tables were converted to
 corope_cache_seqs_t seqs_view(const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, const Optional& cos, const Optional& sin,
                               const Optional& positions, const Optional& new_lens, Tables& keep) {
-    require_value(seq_lens.dim() == 1 && seq_lens.size(0) > 0, "seq_lens must be a tensor [B]");
+    require_value(seq_lens.dim() == 1 && seq_lens.size(0) > 0 && seq_lens.size(0) < (1ll << 24), "seq_lens must be a tensor [B], of fewer than 2^24 sequences");
     const int64_t B = seq_lens.size(0), D = c.k.size(3);
     corope_cache_seqs_t r{};
     table_checks(block_table, B, c.k, "block_table");
@@ -493,7 +493,7 @@ std::tuple<Tensor, Tensor> cache_evict(const CacheTensors& c, const Tensor& bloc
     Tables keep;
     const corope_cache_seqs_t seqs = seqs_view(c, block_table, seq_lens, {}, {}, {}, {}, keep);
     table_checks(out_table, seqs.B, c.k, "out_table");
-    require_value(budget > 0 && recent >= 0 && recent <= budget, "budget must be positive and recent between 0 and budget");
+    require_value(budget > 0 && budget < (1ll << 30) && recent >= 0 && recent <= budget, "budget must be positive (below 2^30) and recent between 0 and budget");
     require_value(out_table.size(1) * cache.block_size >= budget, "out_table's blocks must hold budget tokens");
     const auto ints = seq_lens.options();
     Tensor lens = at::empty({seqs.B}, ints), kept = at::empty({seqs.B, cache.Hkv, budget}, ints);

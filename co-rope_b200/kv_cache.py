@@ -13,8 +13,9 @@ flash_attn_v2_triton.py: what was trained through them is served through these. 
 A code c of block p and head h stands for c * scale[p, h].  Sequence b's slot s is in block block_table[b, s // block_size].
 block_table [B, blocks], seq_lens, new_lens and positions [B] are int32 CUDA tensors; they are read on the device only, so a step
 captured into a CUDA graph follows what they hold at replay.  An entry that points outside its tensor is not followed: the tokens
-concerned are left out and the next call on the device raises RuntimeError.  Block table entries behind a sequence's last block
-are not read.  No operator has a backward pass: tensors that require a gradient are refused outside torch.no_grad().
+concerned are left out (a position is brought into the tables) and the next call on the device raises RuntimeError.  Block table
+entries behind a sequence's last block are not read.  A place of a padded batch that holds no sequence has a length of 0.  No
+operator has a backward pass: k, v and q that require a gradient are refused outside torch.no_grad().
 """
 
 import torch
@@ -44,8 +45,8 @@ def cache_append(k, v, cache, block_table, seq_lens, freqs_cos=None, freqs_sin=N
     freqs_cos / freqs_sin [N, D] or [N, D/2]: keys are rotated by row positions[b] + t of the tables (default: by the slot).
     A block's scale is the largest finite element it holds times 1 / 448 (e4m3) or 1 / 127 (int8), one for k and one for v; when a
     new token raises it, the block's older codes are written again.  Codes are x / scale rounded to nearest even; infinities
-    saturate, NaN stays NaN in e4m3 and becomes 0 in int8.  cache.weight of the new slots becomes 0.  Blocks that are written to
-    must belong to one sequence; full blocks may be shared."""
+    saturate, NaN stays NaN in e4m3 and becomes 0 in int8; a scale of 0 has codes 0.  cache.weight of the new slots becomes 0.
+    Blocks that are written to must stand in one place of block_table; full blocks may be shared."""
     _ext.native().cache_append(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.weight, block_table, seq_lens, freqs_cos, freqs_sin, positions, new_lens)
 
 

@@ -105,6 +105,12 @@ def test_codes_stand_for_what_was_stored(code, worst):
             assert ((got - v[b, h].double()).abs() <= 1.0001 * step).all()
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    assert _evict(budget=1 << 30, out_blocks=1 << 26, stride=1 << 26) == -10
+    for wide in ([1 << 32, 1024, 64], [1 << 40, 1024, 1 << 32]):
+        assert _append(k_stride=wide) == -12 and _attend(v_stride=wide) == -12 and _evict(k_stride=wide) == -12
+
+
 def test_eviction_order():
     """Largest weights first, lowest slots among equal ones, NaN before everything, the last slots always."""
     bs = 16

@@ -636,3 +636,12 @@ def test_refusals():
         with pytest.raises(ValueError):
             pkg.cache_evict(cache, table, lens, *args)
     pkg.check_status()
+
+
+def test_budgets_of_32_bits():
+    """A table of 2^28 + 1 blocks of 16 has room for a budget beyond 32 bits; 2^32 + 8 is not taken for 8."""
+    cache = pkg.KVCache(6, 2, 16, 64, weights=True)
+    table, lens, wide = *gpu(ints([[0, 1]]), ints([20])), torch.zeros(1, 2 ** 28 + 1, dtype=torch.int32, device="cuda")
+    for budget in (2 ** 30, 2 ** 32 + 8):
+        with pytest.raises(ValueError, match="budget"):
+            pkg.cache_evict(cache, table, lens, wide, budget)
