@@ -27,9 +27,11 @@ namespace cg = cooperative_groups;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kPiece = 16;                    // slots per step of a warp; a block of the cache holds a whole number of them
 constexpr int kUnit = kWarps * kPiece;        // slots per unit of work
-// Units that an item counts beside its own in sharing out the work.  0 / 4 / 6 / 12, us, 32 / 8 heads of 128: 64 x up to 4096 tokens 68.1 / 62.6 /
+// Units that an item counts beside its own in sharing out the work.  With 8 rows 0 / 4 / 6 / 12, us, 32 / 8 heads of 128: 64 x up to 4096 tokens 68.1 / 62.6 /
 // 60.5 / 63.1, 256 x up to 1000 97.6 / 80.3 / 80.6 / 81.8, 8 x 16384 58.0 / 56.4 / 56.5 / 57.6.
-constexpr int kItemCost = 6;
+// Two more for each further eight rows: 6 / 8 with 16 rows, 16 x up to 4000 tokens and their weights, 45.4 / 43.7; 6 / 12 / 20 with 32 rows, 64 x up to
+// 4000, 157.6 / 152.7 / 161.2.
+__host__ __device__ constexpr int item_cost(int groups) { return 4 + 2 * groups; }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -136,6 +138,7 @@ struct Shape {
 template <int D, int CODE, int NT, bool EXACT_P>
 __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_kernel(const CacheAttnParams p) {
     using S = Shape<D, NT>;
+    constexpr int kItemCost = item_cost(NT);
     constexpr int kRows = S::kRows, kKSteps = D / 16, kVWords = D / 32, kStages = S::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
     uint32_t* packed = reinterpret_cast<uint32_t*>(smem + S::kBig);
@@ -845,7 +848,7 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     l.rows_per_tile = l.tiles ? kTileRows * (l.pair ? 2 : 1) : 8 * l.groups;
     l.row_tiles = (rows + l.rows_per_tile - 1) / l.rows_per_tile;
     const uint64_t items = (uint64_t)B * Hkv * l.row_tiles, unit = l.tiles ? kTileRows : kUnit;
-    const uint64_t item_units = (slots + unit - 1) / unit, units = items * (item_units + (l.tiles ? kTileItemCost : kItemCost)), most = (uint64_t)sm_count() * (l.tiles ? 1 : resident_blocks(l.groups));
+    const uint64_t item_units = (slots + unit - 1) / unit, units = items * (item_units + (l.tiles ? kTileItemCost : item_cost(l.groups))), most = (uint64_t)sm_count() * (l.tiles ? 1 : resident_blocks(l.groups));
     l.blocks = (unsigned)(units < most ? units : most);
     // Room for the scores of every slot that the block tables could hold.  Beyond half a gigabyte (long tables that the sequences may not fill) K is
     // read again instead: 32 sequences of up to 8192 tokens, 4 rows a head, take 80 us with the scores, 137 without.
@@ -901,7 +904,7 @@ template <int D, int CODE, int NT>
 int launch_rows(const CacheAttnParams& p, const Layout& l, cudaStream_t s) {
     if (int e = p.dtype == COROPE_DTYPE_F32 ? launch_main<D, CODE, NT, true>(p, l.blocks, s) : launch_main<D, CODE, NT, false>(p, l.blocks, s)) return e;
     if (l.parts) return COROPE_OK;
-    if (int e = launch_join<D>(p, l, kUnit, kItemCost, s)) return e;
+    if (int e = launch_join<D>(p, l, kUnit, item_cost(NT), s)) return e;
     if (!p.accumulate) return COROPE_OK;
     count_launch();
     const int unit = p.scores != nullptr ? kSumUnit : kUnit;
