@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             }
             const int item = (int)(off / l.cost), tiles = l.items / p.c.Hkv;
             h = item / tiles;
-            tile = item % tiles;
+            tile = item % tiles + first_tile(p, kRows, l.len, l.n);
             u0 = (int)(off - (int64_t)item * l.cost);
             u1 = (int)min((int64_t)l.cost, u0 + left);
             off += u1 - u0;
@@ -612,12 +612,12 @@ __global__ void __launch_bounds__(kJoinThreads, 6) cache_attn_join_kernel(const 
     for (int w = 0; w < kJoinThreads / 32; ++w) before += words[0][w], total += words[1][w];
 
     const Load l = load_of(p, rows_per_tile, unit, extra, b, bad);
-    const int tiles = l.items / p.c.Hkv;
-    const bool empty = l.units == 0 || tile >= tiles;
+    const int tiles = l.items / p.c.Hkv, tile0 = first_tile(p, rows_per_tile, l.len, l.n);
+    const bool empty = l.units == 0 || tile < tile0 || tile >= tile0 + tiles;
     const int64_t ranges = min((int64_t)main_blocks, total);
     int64_t r0 = 0, r1 = 0;
     if (!empty) {
-        const int64_t u0 = before + (int64_t)(h * tiles + tile) * l.cost + extra, u1 = u0 + l.units - 1;
+        const int64_t u0 = before + (int64_t)(h * tiles + tile - tile0) * l.cost + extra, u1 = u0 + l.units - 1;
         r0 = ((u0 + 1) * ranges - 1) / total;   // the range that holds a unit
         r1 = ((u1 + 1) * ranges - 1) / total;
     }

@@ -27,18 +27,21 @@ __device__ __forceinline__ bool sees_something(const CacheAttnParams& p, int len
 
 // ------------------------------------------------------------------------------------------------ division of the work
 // Work is counted in units of `unit` slots of one item, a (K / V head, tile of query rows) of a sequence: sequence b has items(b) = Hkv * (row tiles in
-// use) items of units(b) units each, one after the other.
+// use) items of units(b) units each, one after the other.  Tiles whose rows all come before slot 0 (causal, more queries than tokens) are no
+// items: the joining kernel writes their zeros.
 // What an item costs beside its units (queries made ready, parts joined and written) is counted as `extra` units in front of them, so that a block
 // with the ends of several items has as long to do as one with the middle of one.
 struct Load {
     int len, n, units, items, cost;   // cost: of an item, extra units included
 };
+// the first tile with a row that sees a slot (of a sequence that has slots)
+__device__ __forceinline__ int first_tile(const CacheAttnParams& p, int rows_per_tile, int len, int n) { return p.causal ? max(n - len, 0) * p.G / rows_per_tile : 0; }
 __device__ __forceinline__ Load load_of(const CacheAttnParams& p, int rows_per_tile, int unit, int extra, int b, bool& bad) {
     Load l;
     l.len = cache_len(p.s, p.c.bs_log2, b, bad);
     l.n = cache_new(p.s, p.T, b, bad);
     l.units = (l.len + unit - 1) / unit;
-    l.items = p.c.Hkv * ((l.n * p.G + rows_per_tile - 1) / rows_per_tile);
+    l.items = p.c.Hkv * ((l.n * p.G + rows_per_tile - 1) / rows_per_tile - first_tile(p, rows_per_tile, l.len, l.n));
     l.cost = l.units > 0 ? l.units + extra : 0;
     return l;
 }

@@ -374,6 +374,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             __syncwarp();
         } else if (warp == 3) {
             // -------------------------------------------------------------- scout
+            // A unit is finished by its converters when the next one has been told, and a piece by the softmax warps when its last unit has.  So the note of
+            // a piece's first unit must not wait for the end of the piece before: no more pieces without units may follow one another than notes
+            // are kept.  There is one at most, the first of the range (the end of an item whose rows see none of the last slots): a tile of rows that
+            // sees nothing is no item, and every item's first unit is seen by some row.
             Range r = range;
             Load l = load_of(p, kItemRows, kN, kTileItemCost, r.b, bad);
             int q = 0, told = 0, pieces = 0;   // units, pieces, pieces with units so far
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                     r.left -= end - at;
                     const int u1 = end - kTileItemCost;
                     if (u1 <= 0) continue;   // the range ends before the item's first unit
-                    x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles; x.len = l.len; x.n = l.n;
+                    x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles + first_tile(p, kItemRows, l.len, l.n); x.len = l.len; x.n = l.n;
                     x.u0 = max(at - kTileItemCost, 0);
                     const int last = min(l.n - 1, (x.tile * kItemRows + kItemRows - 1) / p.G);   // the item's last query
                     const int most = p.causal ? max(l.len - l.n + last + 1, 0) : l.len;   // slots that some row sees

@@ -294,6 +294,27 @@ def test_empty_places_have_no_position(T, causal):
     check_attention(cache, host | {"weight": cache.weight.cpu()}, draw((4, 4, T, D), 1, F32), table, lens, causal, 0.3, cos, sin, new_lens=[T, 1, T, T])
 
 
+@pytest.mark.parametrize("B,Hkv,G,T,D,dtype,accumulate", [
+    (8, 8, 4, 600, 128, BF16, False),     # two tiles of 128 rows an item: most items in front of slot 0, several of them a block
+    (8, 8, 4, 600, 64, F16, False),
+    (6, 8, 4, 600, 128, F16, False),      # one tile an item
+    (40, 4, 1, 300, 32, BF16, False),
+    (3, 3, 2, 200, 32, F32, True),        # tiles of 32 rows
+])
+def test_tiles_of_rows_before_the_first_slot(B, Hkv, G, T, D, dtype, accumulate):
+    """Far more queries than tokens: whole tiles of rows see nothing, many in a row, between ones that see some slots."""
+    bs, lens = 16, [(29 * i) % 41 for i in range(B)]
+    lens[0], lens[-1] = 150, 3
+    cache, host = make_cache(10 + 3 * B, Hkv, bs, D, E4M3)
+    table = torch.full((B, 10), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(lens):
+        table[b, :-(-n // bs)] = torch.arange(at, at + -(-n // bs), dtype=torch.int32)
+        at += -(-n // bs)
+    got = check_attention(cache, host, draw((B, Hkv * G, T, D), 1, dtype), table, lens, True, 0.2, accumulate=accumulate)
+    assert (got[-1, :, :T - 3] == 0).all()
+
+
 def test_many_sequences():
     """More sequences than a block has threads, most of them short or empty."""
     B, D, bs = 300, 32, 16
