@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
 constexpr int kSumThreads = 512;
 constexpr int kRowSlots = 4;
 __host__ __device__ constexpr int sum_stages(int D) { return D == 128 ? 2 : 4; }   // of query tiles
-enum SumBar { W_K_FULL = 0, W_K_EMPTY = 2, W_S_FULL = 4, W_S_FREE = 6, W_ROWS = 8, W_Q_FULL = W_ROWS + kRowSlots, W_Q_EMPTY = W_Q_FULL + 4, W_NUM_BARS = W_Q_EMPTY + 4 };
+enum SumBar { W_K_FULL = 0, W_K_EMPTY = 2, W_S_FULL = 4, W_S_FREE = 6, W_ROWS = 8, W_Q_FULL = W_ROWS + kRowSlots, W_Q_EMPTY = W_Q_FULL + 4, W_ROWS_FREE = W_Q_EMPTY + 4, W_NUM_BARS = W_ROWS_FREE + kRowSlots };
 struct alignas(16) SumSmall {   // factor and lse are read four at a time
     float factor[kRowSlots][kN], lse[kRowSlots][kN], sum[2][kN];
     float k_scale[2][8];
@@ -828,7 +828,10 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
             mbar_init(&bars[W_Q_FULL + i], 1);
             mbar_init(&bars[W_Q_EMPTY + i], 1);
         }
-        for (int i = 0; i < kRowSlots; ++i) mbar_init(&bars[W_ROWS + i], 1);
+        for (int i = 0; i < kRowSlots; ++i) {
+            mbar_init(&bars[W_ROWS + i], 1);
+            mbar_init(&bars[W_ROWS_FREE + i], 4);    // the group whose tile it is
+        }
         fence_mbar_init();
     }
     if (D == 32)
@@ -866,8 +869,9 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
                     f[k] = factors[item * kN + 32 * k + lane];
                     e[k] = row < x.n * p.G ? p.lse[((int64_t)x.b * p.c.Hkv + x.h) * p.T * p.G + row] : INFINITY;
                 }
-                // the slot's last tile, q - 4, has been summed
-                if (q >= kRowSlots && !(ok = mbar_wait_warp(&bars[W_S_FREE + (q & 1)], ((q >> 1) - 2) & 1, p.status, W_S_FREE, abort_flag))) break;
+                // The slot's last tile has been summed.  A barrier of the slot's own: its next phase needs the rows that are posted here, so the parity is never
+                // that of two phases back (the group's W_S_FREE can be one tile further on).
+                if (q >= kRowSlots && !(ok = mbar_wait_warp(&bars[W_ROWS_FREE + slot], ((q / kRowSlots) - 1) & 1, p.status, W_ROWS_FREE, abort_flag))) break;
 #pragma unroll
                 for (int k = 0; k < kN / 32; ++k) z.factor[slot][32 * k + lane] = f[k], z.lse[slot][32 * k + lane] = e[k];
                 mbar_arrive_warp(&bars[W_ROWS + slot], lane);
@@ -987,6 +991,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
                 }
                 tc_fence_before();
                 mbar_arrive_warp(&bars[W_S_FREE + grp], lane);
+                if (lane == 0) mbar_arrive(&bars[W_ROWS_FREE + rows]);
             }
             z.sum[grp][row] = w;
             named_bar_sync(1, 256);

@@ -300,6 +300,8 @@ def test_empty_places_have_no_position(T, causal):
     (6, 8, 4, 600, 128, F16, False),      # one tile an item
     (40, 4, 1, 300, 32, BF16, False),
     (3, 3, 2, 200, 32, F32, True),        # tiles of 32 rows
+    (8, 8, 4, 600, 64, F16, True),
+    (6, 8, 4, 600, 128, F16, True),
 ])
 def test_tiles_of_rows_before_the_first_slot(B, Hkv, G, T, D, dtype, accumulate):
     """Far more queries than tokens: whole tiles of rows see nothing, many in a row, between ones that see some slots."""
@@ -313,6 +315,18 @@ def test_tiles_of_rows_before_the_first_slot(B, Hkv, G, T, D, dtype, accumulate)
         at += -(-n // bs)
     got = check_attention(cache, host, draw((B, Hkv * G, T, D), 1, dtype), table, lens, True, 0.2, accumulate=accumulate)
     assert (got[-1, :, :T - 3] == 0).all()
+
+
+@pytest.mark.parametrize("D,Hkv,T,long,empty", [(128, 2, 320, 12900, 150), (32, 1, 700, 26000, 300), (64, 3, 256, 10000, 40)])
+def test_weights_of_sequences_far_apart(D, Hkv, T, long, empty):
+    """Five and more tiles of rows a head, weights, and empty places between two long sequences: a block looks for its next unit while its sums go on."""
+    bs, lens = 64, [long] + [0] * empty + [long - 77, 5]
+    wide = -(-long // bs)
+    cache, host = make_cache(2 * wide + 1, Hkv, bs, D, E4M3)
+    table = torch.full((len(lens), wide), -1, dtype=torch.int32)
+    for i, b in enumerate((0, empty + 1, empty + 2)):
+        table[b, :-(-lens[b] // bs)] = torch.arange(i * wide, i * wide + -(-lens[b] // bs), dtype=torch.int32)
+    check_attention(cache, host, draw((len(lens), 2 * Hkv, T, D), 1, F16), table, lens, True, 0.1, accumulate=True)
 
 
 def test_many_sequences():
