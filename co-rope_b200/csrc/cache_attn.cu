@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                 y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
             }
             if (CODE == COROPE_CODE_E4M3 && nan_v != 0) {
-                const int sees_row = p.causal ? len - n + t + 1 : len;
+                const int sees_row = t >= n ? 0 : p.causal ? len - n + t + 1 : len;   // (never behind the last slot, whose block the table still has)
 #pragma unroll 1
                 for (int slot = u0 * kUnit; slot < min(sees_row, u1 * kUnit); ++slot) {
                     const int page = table[slot >> p.c.bs_log2];

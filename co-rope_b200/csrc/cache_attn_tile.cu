@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 if (col0 + k >= D) continue;
                 if (fix) {   // NaN in V, slot by slot: to the rows that see it
 #pragma unroll 1
-                    for (int s = u0 * kN; s < min(sees, (u0 + count) * kN); ++s) {
+                    for (int s = u0 * kN; s < (t < x.n ? min(sees, (u0 + count) * kN) : 0); ++s) {   // (never behind the last slot, whose block the table still has)
                         bool far = false;
                         const int page = cache_page(p.s, p.c.bs_log2, p.c.num_blocks, x.b, s, far);
                         if (page < 0 || p.c.v_scale[(int64_t)page * p.c.Hkv + x.h] == 0.f) continue;

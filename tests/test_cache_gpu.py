@@ -272,6 +272,26 @@ def test_hidden_numbers_stay_hidden(T, G, dtype):
     assert not (excess[seen] > 0).any() and not got.cpu()[seen].isnan().any()
 
 
+@pytest.mark.parametrize("T,G,dtype,new", [(4, 1, BF16, [1, 3]), (7, 3, F32, [2, 7]), (90, 2, BF16, [3, 70]), (300, 1, F16, [10, 299])])
+def test_hidden_nan_with_a_table_that_ends_with_the_sequence(T, G, dtype, new):
+    """Rows without a query stand behind the last one: they must not make anyone look behind the last block of the table."""
+    D, bs, lens = 64, 16, [16 * (T // 16) + 32, 16 * (T // 16) + 32]
+    wide = lens[0] // bs
+    cache, host = make_cache(2 * wide, 1, bs, D, E4M3)
+    table = make_table(2, wide, 2 * wide, lens, bs)
+    for b in range(2):      # the last token
+        host["v"].view(torch.uint8)[int(table[b, -1]), 0, bs - 1] = 0x7F
+    cache.v.view(torch.uint8).copy_(host["v"].view(torch.uint8).cuda())
+    q = draw((2, G, T, D), 4, dtype)
+    o, bulk, slack, _ = ref.attention(host, q, table, lens, True, 0.125, new_lens=new)
+    got = pkg.cache_attention(q.cuda(), cache, *gpu(table, ints(lens)), True, 0.125, new_lens=ints(new).cuda()).double().cpu()
+    pkg.check_status()
+    assert torch.equal(got.isnan(), o.isnan())
+    assert all(o[b, :, new[b] - 1].isnan().all() and not o[b, :, :new[b] - 1].isnan().any() and (got[b, :, new[b]:] == 0).all() for b in range(2))
+    excess = (got - o).abs() - tolerance(dtype, o, bulk, slack, dtype == BF16 and T * G > 32)
+    assert not (excess > 0).any()
+
+
 def test_rows_behind_the_last_query_are_zero_and_others_untouched():
     D, bs, lens, new = 32, 16, [20, 9], [2, 0]
     cache, host = make_cache(6, 2, bs, D, INT8, weights=False)
