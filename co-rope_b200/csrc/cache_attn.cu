@@ -252,11 +252,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                         copy16_async((i % 2 ? other : fill) + 512 * i, real ? kb + (uint64_t)(i * kCopyRows) * k_row : p.c.k, real);
                         copy16_async((i % 2 ? other : fill) + 512 * i + kPiece * D, real ? vb + (uint64_t)(i * kCopyRows) * v_row : p.c.v, real);
                     }
-                    if (!found) {
-                        bad = true;
-                        if (lane == 2) my_meta[j % kStages * 4 + 2] = 0.f;   // (1 otherwise)
-                    }
                 }
+                bad |= !found;
+                if (bad && lane == 2) my_meta[j % kStages * 4 + 2] = found ? 1.f : 0.f;   // (1 before the first bad one)
                 if (lane < 2) copy4_async(fill_meta, scale_lane + (uint64_t)page * (uint32_t)p.c.Hkv);
             }
             commit_copies();

@@ -650,6 +650,32 @@ def test_bad_indices_are_not_followed():
     pkg.flash_attention(k, k, k, True, 0.2)
 
 
+@pytest.mark.parametrize("wide,bs,accumulate", [(63, 16, True), (63, 16, False), (16, 64, True), (1000, 16, True), (300, 64, False)])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_a_bad_block_hides_no_other(D, wide, bs, accumulate):
+    """Bad entries near the start, hundreds of good slots behind them in the same block of threads: only the tokens of the bad blocks are left out."""
+    length, Hkv = 1000, 300
+    blocks = -(-length // bs) + 2
+    cache, host = make_cache(blocks, Hkv, bs, D, INT8)
+    whole = torch.arange(wide, dtype=torch.int32) % blocks
+    good = [i for i in range(-(-length // bs)) if i not in (1, 6)]
+    for T, dtype, bad in ((1, F16, -1), (4, F32, 2 ** 30)):
+        q = draw((1, Hkv, T, D), T, dtype)
+        table = whole.clone()
+        table[[1, 6]] = bad
+        some = torch.tensor([0, 1, 137, 200, 299])                        # heads that are compared
+        few = {x: t.view(torch.uint8)[:, some].view(t.dtype) if x in ("k", "v") else t[:, some] for x, t in host.items()}
+        o, bulk, slack, weight = ref.attention(few, q[:, some], whole[good][None], [length - 2 * bs], True, 0.2)
+        cache.weight.copy_(host["weight"].cuda())
+        got = pkg.cache_attention(q.cuda(), cache, *gpu(table[None], ints([length])), True, 0.2, accumulate=accumulate)
+        with pytest.raises(RuntimeError, match="0x4000"):
+            pkg.check_status()
+        assert not ((got[:, some.cuda()].double().cpu() - o).abs() > tolerance(dtype, o, bulk, slack)).any()
+        if accumulate:
+            off = (cache.weight.cpu()[:, some].double() - few["weight"].double() - weight).abs()
+            assert not (off > 2 * 2.0 ** -17 * slack.max() * weight + (T + 2) * 2.0 ** -23 * (few["weight"].double() + weight)).any()
+
+
 # ---------------------------------------------------------------------------------------------------------------- refusals
 def test_refusals():
     D, bs = 64, 16
