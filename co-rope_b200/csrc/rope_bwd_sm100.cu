@@ -152,12 +152,12 @@ rope_bwd_sm100_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
         pdl_wait();   // no launch ends before the one in front of it
         return;
     }
-    // A non-zero status word means an earlier CTA (of this or a previous launch) gave up on a wait: do not pile up
-    // more timeouts behind it.  The word stays set until the host reads and clears it; the mirror may already be clear (the host resets it
+    // An earlier CTA (of this or a previous launch) gave up on a wait: do not pile up more timeouts behind it.  (What else the word may hold, a
+    // clamped gradient or a bad index of a cache operator, concerns only the call that met it.)  The word stays set until the host reads and clears it; the mirror may already be clear (the host resets it
     // at once, the word in stream order), so this launch reports too.
     if (p.status != nullptr) {
         // one answer for the whole block: a launch beside this one may set the word while its threads read it
-        if (__syncthreads_or(*reinterpret_cast<volatile int*>(p.status))) {
+        if (__syncthreads_or(*reinterpret_cast<volatile int*>(p.status) & COROPE_DEV_WAIT_EXPIRED)) {
             if (threadIdx.x == 0) report_to_mirror(p.status, p.status_mirror);
             pdl_wait();
             return;

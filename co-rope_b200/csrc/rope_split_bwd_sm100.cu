@@ -117,7 +117,7 @@ rope_bwd_split_sm100_kernel(const __grid_constant__ CUtensorMap mapOwn, const __
     }
     if (p.status != nullptr) {   // an earlier launch gave up on a wait: see rope_fwd_sm100_kernel
         // one answer for the whole block: a launch beside this one may set the word while its threads read it
-        if (__syncthreads_or(*reinterpret_cast<volatile int*>(p.status))) {
+        if (__syncthreads_or(*reinterpret_cast<volatile int*>(p.status) & COROPE_DEV_WAIT_EXPIRED)) {
             if (threadIdx.x == 0) report_to_mirror(p.status, p.status_mirror);
             pdl_wait();
             return;

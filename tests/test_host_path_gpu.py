@@ -113,3 +113,32 @@ def test_other_threads_run_while_launches_wait(entry):
         torch.cuda.synchronize()
     assert took > 0.3          # the queue did fill up
     assert longest[0] < 0.25, longest   # half of what a held lock shows
+
+
+@pytest.mark.parametrize("code", [0x2000, 0x4000])
+@pytest.mark.parametrize("D,N,dtype", [(64, 256, torch.bfloat16), (128, 256, torch.float16), (64, 200, torch.bfloat16), (128, 333, torch.float16), (128, 256, torch.float32)])
+def test_what_one_call_met_does_not_stop_another(code, D, N, dtype):
+    # The word holds a clamped gradient or a bad index of an earlier call that the host has not seen yet: calls behind it compute all the same.
+    dev = torch.device("cuda", 0)
+    ext.check_status(dev)
+    q, k, v, do = (draw((1, 2, N, D), 10 + i, dtype).cuda() for i in range(4))
+    cos, sin = (t.cuda() for t in oracle.precompute_freqs_cis(D, N, 10000.0))
+    rope, word = pkg.fused_rope_attn, ext.status_word(dev)
+
+    def both():
+        saved = rope._forward(q, k, v, True, D ** -0.5, cos, sin)
+        return [saved[3]] + list(rope._backward(*saved, do, True, D ** -0.5))
+
+    want = both()
+    torch.use_deterministic_algorithms(True, warn_only=True)   # memory that nobody has written holds NaN
+    try:
+        word.fill_(code)
+        got = both()
+    finally:
+        torch.use_deterministic_algorithms(False)
+    torch.cuda.synchronize()
+    assert int(word.item()) == code
+    with pytest.raises(RuntimeError, match="0x%x" % code):
+        ext.check_status(dev)
+    for x, y in zip(got, want):    # (dQ's sums are added in any order: a step of the result's type, and of fp32 in sums of a size of 4)
+        assert x.shape == y.shape and ((x.float() - y.float()).abs() <= torch.finfo(dtype).eps * y.float().abs() + 2.0 ** -18).all()
