@@ -260,12 +260,15 @@ def status_word(device):
     return _status(device).word
 
 
+_STATUS_BITS = (
+    (0x1000, "a bounded device-side wait expired (results of that call and of later calls are undefined)"),
+    (0x2000, "a gradient term left the value range of the 16-bit Co-RoPE backward and was clamped (results of that call are inaccurate)"),
+    (0x4000, "a block table entry, length or position of a cache operator pointed outside its tensor (it was not followed; the tokens concerned were left out)"),
+)
+
+
 def _status_message(v):
-    if v == 0x4000:
-        return "a block table entry, length or position of a cache operator pointed outside its tensor (it was not followed; the tokens concerned were left out)"
-    if v & 0x2000:
-        return "a gradient term left the value range of the 16-bit Co-RoPE backward and was clamped (results of that call are inaccurate)"
-    return "a bounded device-side wait expired (results of that call and of later calls are undefined)"
+    return "; ".join(text for bit, text in _STATUS_BITS if v & bit)
 
 
 def pre_call(device):

@@ -67,8 +67,8 @@ int launch_cache_evict(const CacheEvictParams& p, cudaStream_t s);
 #ifdef __CUDACC__
 __device__ __forceinline__ void report_bad_index(int* status, int* mirror) {
     if (status == nullptr) return;
-    atomicCAS(status, 0, COROPE_DEV_BAD_INDEX);
-    report_to_mirror(COROPE_DEV_BAD_INDEX, mirror);
+    atomicOr(status, COROPE_DEV_BAD_INDEX);
+    report_to_mirror(status, mirror);
 }
 // A sequence's length and its new tokens, brought into range.  A new token count above the length is one whose first tokens have no
 // slot: not an error (an empty place in a padded batch).

@@ -192,6 +192,15 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
+// The status word gains bits until the host clears it: what one kernel meets does not cover up what another met.  Of expired waits the first one's id stays.
+__device__ __forceinline__ void note_expired_wait(int* status, int id) {
+    if (status == nullptr) return;
+    int held = *reinterpret_cast<volatile int*>(status);
+    for (int seen; !(held & COROPE_DEV_WAIT_EXPIRED); held = seen) {
+        seen = atomicCAS(status, held, held | COROPE_DEV_WAIT_EXPIRED | id);
+        if (seen == held) break;
+    }
+}
 // Bounded wait.  Returns false (after recording `id` in *status) when the limit is hit; callers
 // then leave their loops and fall through to the common exit path.  try_wait itself blocks for
 // a hardware-defined slice, so the limit corresponds to well over a second.
@@ -203,18 +212,22 @@ __device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity
         if ((it & 1023u) == 1023u && *abort_flag) return false;
     }
     *abort_flag = 1;
-    if (status) atomicCAS(status, 0, COROPE_DEV_WAIT_EXPIRED | id);
+    note_expired_wait(status, id);
     return false;
 }
-// A kernel that gave up, or that did not start because an earlier one had, leaves the code in the host mirror too: the host learns of
-// every launch that did not compute without a copy or a synchronisation.
-__device__ __forceinline__ void report_to_mirror(int code, int* mirror) {
-    if (code == 0 || mirror == nullptr) return;
-    *reinterpret_cast<volatile int*>(mirror) = code;
-    __threadfence_system();
-}
+// A kernel that gave up, or that did not start because an earlier one had, leaves the word in the host mirror too: the host learns of
+// every launch that did not compute without a copy or a synchronisation.  Written again if the word has gained a bit meanwhile: a kernel beside this one
+// may have written it before (the word has three flags, so a few rounds are enough).
 __device__ __forceinline__ void report_to_mirror(const int* status, int* mirror) {
-    if (status != nullptr) report_to_mirror(*reinterpret_cast<const volatile int*>(status), mirror);
+    if (status == nullptr || mirror == nullptr) return;
+    const volatile int* word = reinterpret_cast<const volatile int*>(status);
+    for (int v = *word, round = 0; v != 0 && round < 4; ++round) {
+        *reinterpret_cast<volatile int*>(mirror) = v;
+        __threadfence_system();
+        const int now = *word;
+        if (now == v) return;
+        v = now;
+    }
 }
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* status, int id, volatile int* abort_flag) {
     return mbar_wait_limited(bar, parity, status, id, abort_flag, kWaitLimit);
@@ -251,7 +264,7 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
         if ((it & 1023u) == 1023u && __any_sync(0xffffffffu, *abort_flag)) return false;
     }
     *abort_flag = 1;
-    if (status) atomicCAS(status, 0, COROPE_DEV_WAIT_EXPIRED | id);
+    note_expired_wait(status, id);
     return false;
 }
 

@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) corope_bwd_mma_kernel(GqaParams p
         }
     }
     if (__any_sync(0xffffffffu, range_clamped) && lane == 0 && p.status) {
-        atomicCAS(p.status, 0, COROPE_DEV_RANGE);
+        atomicOr(p.status, COROPE_DEV_RANGE);
         report_to_mirror(p.status, p.status_mirror);
     }
 #pragma unroll

@@ -146,8 +146,8 @@ rope_bwd_sm100_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
 
     if (reinterpret_cast<uintptr_t>(sm) - reinterpret_cast<uintptr_t>(smem_raw) > kSmemSlack) {   // base less aligned than assumed
         if (threadIdx.x == 0 && p.status) {
-            atomicCAS(p.status, 0, COROPE_DEV_WAIT_EXPIRED | 0xfff);
-            report_to_mirror(COROPE_DEV_WAIT_EXPIRED | 0xfff, p.status_mirror);
+            note_expired_wait(p.status, 0xfff);
+            report_to_mirror(p.status, p.status_mirror);
         }
         pdl_wait();   // no launch ends before the one in front of it
         return;

@@ -87,8 +87,8 @@ rope_fwd_split_sm100_kernel(const __grid_constant__ CUtensorMap mapK, const __gr
 
     if (reinterpret_cast<uintptr_t>(sm) - reinterpret_cast<uintptr_t>(smem_raw) > F::kSlack) {   // base less aligned than assumed
         if (threadIdx.x == 0 && p.status) {
-            atomicCAS(p.status, 0, COROPE_DEV_WAIT_EXPIRED | 0xfff);
-            report_to_mirror(COROPE_DEV_WAIT_EXPIRED | 0xfff, p.status_mirror);
+            note_expired_wait(p.status, 0xfff);
+            report_to_mirror(p.status, p.status_mirror);
         }
         pdl_wait();   // no launch ends before the one in front of it
         return;

@@ -59,12 +59,15 @@ DeviceStatus& device_status(int index) {
     return g_status[index];
 }
 
-std::string status_message(int v) {
-    if (v == COROPE_DEV_BAD_INDEX)
-        return "a block table entry, length or position of a cache operator pointed outside its tensor (it was not followed; the tokens concerned were left out)";
-    if (v & 0x2000)
-        return "a gradient term left the value range of the 16-bit Co-RoPE backward and was clamped (results of that call are inaccurate)";
-    return "a bounded device-side wait expired (results of that call and of later calls are undefined)";
+std::string status_message(int v) {   // as _ext._status_message
+    std::string text;
+    auto add = [&](int bit, const char* what) {
+        if (v & bit) text += (text.empty() ? "" : "; ") + std::string(what);
+    };
+    add(COROPE_DEV_WAIT_EXPIRED, "a bounded device-side wait expired (results of that call and of later calls are undefined)");
+    add(COROPE_DEV_RANGE, "a gradient term left the value range of the 16-bit Co-RoPE backward and was clamped (results of that call are inaccurate)");
+    add(COROPE_DEV_BAD_INDEX, "a block table entry, length or position of a cache operator pointed outside its tensor (it was not followed; the tokens concerned were left out)");
+    return text;
 }
 
 // Raises if an earlier call on this device left the status word set; clears it first.

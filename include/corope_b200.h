@@ -63,7 +63,7 @@ extern "C" {
 #define COROPE_ERR_BAD_STRIDE (-11)    /* row stride below D, or a negative stride */
 #define COROPE_ERR_BAD_CACHE (-12)     /* code type, block size or strides that the cache operators do not take */
 
-/* device-side status codes written to *status_word */
+/* device-side status codes: bits of *status_word, which stay until the host clears them (of several expired waits the first one's id) */
 #define COROPE_DEV_OK 0
 #define COROPE_DEV_WAIT_EXPIRED 0x1000 /* | barrier id: a bounded mbarrier wait ran out */
 #define COROPE_DEV_RANGE 0x2000        /* a gradient term left the range of the 16-bit Co-RoPE backward and was clamped */

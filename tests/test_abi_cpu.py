@@ -150,3 +150,9 @@ def test_the_extension_module_of_another_torch_version_is_not_loaded(monkeypatch
     monkeypatch.setattr(ext, "NATIVE_PATH", ext.NATIVE_PATH.replace(torch.__version__, "0.0.0"))
     with pytest.raises(RuntimeError, match="missing"):
         ext.native()
+
+
+def test_every_bit_of_the_status_word_has_its_message():
+    wait, clamped, index = (ext._status_message(v) for v in (0x107e, 0x2000, 0x4000))
+    assert "wait expired" in wait and "clamped" in clamped and "block table entry" in index
+    assert ext._status_message(0x707e) == "; ".join((wait, clamped, index)) and ext._status_message(0x5001) == wait + "; " + index

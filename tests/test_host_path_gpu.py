@@ -142,3 +142,30 @@ def test_what_one_call_met_does_not_stop_another(code, D, N, dtype):
         ext.check_status(dev)
     for x, y in zip(got, want):    # (dQ's sums are added in any order: a step of the result's type, and of fp32 in sums of a size of 4)
         assert x.shape == y.shape and ((x.float() - y.float()).abs() <= torch.finfo(dtype).eps * y.float().abs() + 2.0 ** -18).all()
+
+
+def _cache_call_with_a_bad_block():
+    cache = pkg.KVCache(2, 1, 16, 32)
+    table, lens = torch.full((1, 1), 7, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    pkg.cache_append(*(torch.ones(1, 1, 1, 32, device="cuda") for _ in range(2)), cache, table, lens)
+
+
+@pytest.mark.parametrize("wait_first", [True, False])
+def test_an_expired_wait_and_a_bad_index_do_not_cover_each_other_up(wait_first):
+    dev = torch.device("cuda", 0)
+    ext.check_status(dev)
+    word, mirror = ext.status_word(dev), ext._status(dev).mirror_view
+
+    def expire():
+        assert ext.lib().corope_debug_expire_wait(word.data_ptr(), 100, torch.cuda.current_stream(dev).cuda_stream) == 0
+
+    for step in ((expire, _cache_call_with_a_bad_block) if wait_first else (_cache_call_with_a_bad_block, expire)):
+        mirror[0] = 0               # (else the second call would raise for the first)
+        step()
+        torch.cuda.synchronize()
+    assert int(word.item()) == 0x507e and mirror[0] == 0x507e
+    with pytest.raises(RuntimeError, match="0x507e: a bounded device-side wait expired.*; a block table entry"):
+        _cache_call_with_a_bad_block()
+    torch.cuda.synchronize()
+    assert int(word.item()) == 0
+    ext.check_status(dev)
