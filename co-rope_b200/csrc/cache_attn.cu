@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             if (CODE == COROPE_CODE_E4M3 && nan_v != 0) {
                 const int sees_row = t >= n ? 0 : p.causal ? len - n + t + 1 : len;   // (never behind the last slot, whose block the table still has)
 #pragma unroll 1
-                for (int slot = u0 * kUnit; slot < min(sees_row, u1 * kUnit); ++slot) {
+                for (int slot = max(u0 * kUnit, least_seen / kPiece * kPiece); slot < min(sees_row, u1 * kUnit); ++slot) {   // from where it was left out
                     const int page = table[slot >> p.c.bs_log2];
                     if ((unsigned)page >= (unsigned)p.c.num_blocks || p.c.v_scale[(int64_t)page * p.c.Hkv + h] == 0.f) continue;
                     const uint32_t word = *reinterpret_cast<const uint32_t*>(p.c.v + (int64_t)page * p.c.sv.b + (int64_t)h * p.c.sv.h + (int64_t)(slot & in_block_mask) * p.c.sv.n + d);

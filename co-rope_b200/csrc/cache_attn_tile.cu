@@ -674,6 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             const int64_t part = (2 * (int64_t)blockIdx.x + (u0 == 0 ? 1 : 0)) * kItemRows + item_row;
             const int64_t to = (int64_t)x.b * p.so.b + (int64_t)(x.h * p.G + grow - t * p.G) * p.so.h + (int64_t)t * p.so.n;
             const bool fix = CODE == COROPE_CODE_E4M3 && count > 0 && z.nan_v[pieces % kFlagSlots] != 0;
+            const int seen = p.causal ? max(x.len - x.n + x.tile * kItemRows / p.G + 1, 0) : x.len;   // as the scout's: NaN is left out of units that reach beyond
 #pragma unroll
             for (int k = 0; k < kCols; k += 16) {
                 float y[16];
@@ -695,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 if (col0 + k >= D) continue;
                 if (fix) {   // NaN in V, slot by slot: to the rows that see it
 #pragma unroll 1
-                    for (int s = u0 * kN; s < (t < x.n ? min(sees, (u0 + count) * kN) : 0); ++s) {   // (never behind the last slot, whose block the table still has)
+                    for (int s = max(u0, seen / kN) * kN; s < (t < x.n ? min(sees, (u0 + count) * kN) : 0); ++s) {   // (never behind the last slot, whose block the table still has)
                         bool far = false;
                         const int page = cache_page(p.s, p.c.bs_log2, p.c.num_blocks, x.b, s, far);
                         if (page < 0 || p.c.v_scale[(int64_t)page * p.c.Hkv + x.h] == 0.f) continue;

@@ -292,6 +292,37 @@ def test_hidden_nan_with_a_table_that_ends_with_the_sequence(T, G, dtype, new):
     assert not (excess > 0).any()
 
 
+@pytest.mark.parametrize("T,G,dtype", [(2, 2, BF16), (2, 2, F32), (64, 2, BF16)])
+def test_hidden_nan_costs_little_behind_a_long_context(T, G, dtype):
+    """A NaN that some queries must not see is looked for where it can be, not through all of the context."""
+    D, bs, length = 128, 256, 400000
+    wide = -(-length // bs)
+    cache = pkg.KVCache(wide, 4, bs, D)
+    cache.k_scale.fill_(1.0)
+    cache.v_scale.fill_(1.0)
+    table, lens = torch.arange(wide, dtype=torch.int32, device="cuda")[None], ints([length]).cuda()
+    q = draw((1, 4 * G, T, D), 4, dtype).cuda()
+
+    def fastest():
+        times = []
+        for _ in range(6):
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            got = pkg.cache_attention(q, cache, table, lens, True, 0.1)
+            end.record()
+            end.synchronize()
+            times.append(begin.elapsed_time(end))
+        return min(times), got
+
+    clean, zeros = fastest()
+    assert (zeros == 0).all()
+    cache.v.view(torch.uint8)[-1, :, (length - 1) % bs, 5] = 0x7F       # the last token
+    once, got = fastest()
+    pkg.check_status()
+    assert got[:, :, -1, 5].isnan().all() and (got[:, :, :-1] == 0).all() and got.isnan().sum() == 4 * G
+    assert once < 3 * clean, (once, clean)
+
+
 def test_rows_behind_the_last_query_are_zero_and_others_untouched():
     D, bs, lens, new = 32, 16, [20, 9], [2, 0]
     cache, host = make_cache(6, 2, bs, D, INT8, weights=False)
