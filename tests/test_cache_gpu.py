@@ -292,6 +292,25 @@ def test_hidden_nan_with_a_table_that_ends_with_the_sequence(T, G, dtype, new):
     assert not (excess > 0).any()
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf")])
+@pytest.mark.parametrize("T,G,dtype,wide", [(4, 2, BF16, 9), (4, 2, F16, 400), (6, 3, F32, 9), (70, 2, F16, 9)])
+def test_hidden_scales_stay_hidden(T, G, dtype, wide, scale, accumulate):
+    """A block whose scales are no finite numbers, of which the first queries see nothing, in every way that scores are kept."""
+    D, bs = 64, 16
+    length = -(-(T + 20) // bs) * bs + 2        # the last two tokens begin a block
+    cache, host = make_cache(20, 2, bs, D, INT8)
+    table = make_table(1, 9, 20, [length], bs)
+    table = torch.cat((table, torch.full((1, wide - 9), -1, dtype=torch.int32)), dim=1)
+    q = draw((1, 2 * G, T, D), 4, dtype)
+    o, bulk, slack, _ = ref.attention(host, q, table, [length], True, 0.125)
+    for x in ("k_scale", "v_scale"):
+        getattr(cache, x)[int(table[0, length // bs])] = scale
+    got = pkg.cache_attention(q.cuda(), cache, *gpu(table, ints([length])), True, 0.125, accumulate=accumulate)[:, :, :T - 2].double().cpu()
+    pkg.check_status()
+    assert not got.isnan().any() and not ((got - o[:, :, :T - 2]).abs() > tolerance(dtype, o, bulk, slack)[:, :, :T - 2]).any()
+
+
 @pytest.mark.parametrize("T,G,dtype", [(2, 2, BF16), (2, 2, F32), (64, 2, BF16)])
 def test_hidden_nan_costs_little_behind_a_long_context(T, G, dtype):
     """A NaN that some queries must not see is looked for where it can be, not through all of the context."""
