@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(MOST, 1024 / MOST) cache_append_kernel(const C
     const int first = len - n;                                        // slot of token 0; negative: the tokens before slot 0 are left out
     const int block = (max(first, 0) >> p.c.bs_log2) + j, base = block << p.c.bs_log2;
     const int lo = max(first, base), hi = min(len, base + bs);        // the block's new slots
-    const int page = n > 0 && lo < hi ? cache_page(p.s, p.c.bs_log2, p.c.num_blocks, b, base, bad) : -1;
+    // a length or a number of new tokens out of range does not tell where the tokens belong: none is stored
+    const int page = !bad && n > 0 && lo < hi ? cache_page(p.s, p.c.bs_log2, p.c.num_blocks, b, base, bad) : -1;
     // 2^per_row_log2 threads share a row, each has four elements of its first half and their partners in the second
     const int d = ((int)threadIdx.x & ((1 << per_row_log2) - 1)) * 4, g = (int)threadIdx.x >> per_row_log2, groups = (int)blockDim.x >> per_row_log2;
     if (bad && threadIdx.x == 0) report_bad_index(p.status, p.mirror);

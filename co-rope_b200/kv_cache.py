@@ -13,7 +13,8 @@ flash_attn_v2_triton.py: what was trained through them is served through these. 
 A code c of block p and head h stands for c * scale[p, h].  Sequence b's slot s is in block block_table[b, s // block_size].
 block_table [B, blocks], seq_lens, new_lens and positions [B] are int32 CUDA tensors; they are read on the device only, so a step
 captured into a CUDA graph follows what they hold at replay.  An entry that points outside its tensor is not followed: the tokens
-concerned are left out (a position is brought into the tables) and the next call on the device raises RuntimeError.  Block table
+concerned are left out and the next call on the device raises RuntimeError.  (A length or a number of new tokens out of range: nothing
+of the sequence is stored; attention and eviction take the nearest number in range, and so does a position.)  Block table
 entries behind a sequence's last block are not read.  A place of a padded batch that holds no sequence has a length of 0.  No
 operator has a backward pass: k, v and q that require a gradient are refused outside torch.no_grad().
 """

@@ -296,7 +296,8 @@ int corope_gqa_bwd_strided(const void* q, const void* k, const void* v, const vo
  *
  * All index arrays are device memory and are never read on the host.  An entry that points outside its tensor (a block id outside
  * [0, num_blocks), a length beyond the block table or below 0, a position beyond the tables) is not followed: the tokens concerned are
- * left out (a position is clamped) and COROPE_DEV_BAD_INDEX is written to the status word.  These kernels run whatever an earlier kernel left in
+ * left out (a position is clamped; a sequence whose length or number of new tokens is out of range stores nothing, while attention and
+ * eviction clamp the number) and COROPE_DEV_BAD_INDEX is added to the status word.  These kernels run whatever an earlier kernel left in
  * the word, but for those of corope_cache_attn with waits of their own (16-bit tensors, more than 32 query rows a K / V head), which do not after
  * COROPE_DEV_WAIT_EXPIRED.  They take fp32 / bf16 / fp16 tensors, hold scores, sums and scales in fp32 and have no backward pass.  Scales are
  * not negative.

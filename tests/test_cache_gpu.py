@@ -700,6 +700,25 @@ def test_bad_indices_are_not_followed():
     pkg.flash_attention(k, k, k, True, 0.2)
 
 
+@pytest.mark.parametrize("what,value", [("length", 49), ("length", 60), ("length", 2 ** 31 - 1), ("length", -1), ("new", 3), ("new", 2 ** 31 - 1), ("new", -1)])
+def test_tokens_of_a_sequence_out_of_range_are_not_stored_elsewhere(what, value):
+    """A length beyond the table, or more new tokens than there are: older slots stay as they were, and the other sequences get theirs."""
+    D, bs, T = 32, 16, 2
+    cache, host = make_cache(10, 2, bs, D, E4M3)
+    table, lens, new = make_table(3, 3, 10, [48, 48, 48], bs), [20, 48, 33], [2, 2, 1]
+    k, v = (draw((3, 2, T, D), i, BF16) for i in range(2))
+    for b in (0, 2):
+        ref.append(host, k[b:b + 1], v[b:b + 1], table[b:b + 1], lens[b:b + 1], new_lens=new[b:b + 1])
+    if what == "length":
+        lens[1] = value
+    else:
+        new[1] = value
+    pkg.cache_append(*gpu(k, v), cache, *gpu(table, ints(lens)), new_lens=ints(new).cuda())
+    with pytest.raises(RuntimeError, match="0x4000"):
+        pkg.check_status()
+    same_cache(cache, host)
+
+
 @pytest.mark.parametrize("wide,bs,accumulate", [(63, 16, True), (63, 16, False), (16, 64, True), (1000, 16, True), (300, 64, False)])
 @pytest.mark.parametrize("D", [32, 64, 128])
 def test_a_bad_block_hides_no_other(D, wide, bs, accumulate):
