@@ -100,10 +100,8 @@ __device__ __forceinline__ void pack_queries(const CacheAttnParams& p, int b, in
         float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
         for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-        // brings the row's largest element to [2^10, 2^11): then the second part is a normal fp16 number too
-        const bool usual = m >= 1e-30f && m <= 1e30f;
-        const int e = usual ? (int)(__float_as_uint(m) >> 23) - 127 - 10 : 0;
-        const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
+        float up, down;
+        row_scaling(m, up, down);
         if (lane == 0) factor[r] = down * p.scale;
         if (lane < kPairLanes) {
 #pragma unroll

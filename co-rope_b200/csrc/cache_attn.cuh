@@ -7,6 +7,15 @@ namespace corope {
 #ifdef __CUDACC__
 constexpr float kLowest = -1e30f;             // running maximum before any score: finite, so that differences from it are no NaN
 
+// The power of two 2^-e that brings a row whose largest element is m to [2^10, 2^11), so that the second of two fp16 parts is a normal number too; as `up` =
+// 2^-e and `down` = 2^e.  Rows below 2^-100 stay below 2^10; rows with infinities or NaN are left as they are.
+__device__ __forceinline__ void row_scaling(float m, float& up, float& down) {
+    const bool finite = m > 0.f && m <= 3.402823466e38f;
+    const int e = finite ? max((int)(__float_as_uint(m) >> 23) - 127 - 10, -110) : 0;
+    up = __uint_as_float((uint32_t)(127 - e) << 23);
+    down = __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
 // four codes as fp16: (0, 1), (2, 3)
 template <int CODE>
 __device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint32_t& hi) {

@@ -110,9 +110,8 @@ __global__ void __launch_bounds__(kPackWarps * 32) cache_pack_kernel(const Cache
         float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
         for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-        const bool usual = m >= 1e-30f && m <= 1e30f;   // to [2^10, 2^11), see pack_queries of the kernel for few rows
-        const int e = usual ? (int)(__float_as_uint(m) >> 23) - 127 - 10 : 0;
-        const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
+        float up, down;
+        row_scaling(m, up, down);
         if (lane == 0) factors[(size_t)item * kN + r] = down * p.scale;
         if (lane < kPairs) {
 #pragma unroll

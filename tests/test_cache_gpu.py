@@ -272,6 +272,18 @@ def test_hidden_numbers_stay_hidden(T, G, dtype):
     assert not (excess[seen] > 0).any() and not got.cpu()[seen].isnan().any()
 
 
+@pytest.mark.parametrize("T,G,dtype", [(1, 4, BF16), (3, 4, F32), (50, 3, BF16), (30, 2, F32)])
+def test_queries_of_any_size(T, G, dtype):
+    """Queries of 2^110 and 2^-115 beside an sm_scale that makes their scores ordinary ones."""
+    D, bs, lens = 64, 16, [90 + T, 33 + T]
+    cache, host = make_cache(30, 2, bs, D, E4M3)
+    table, q = make_table(2, 12, 30, lens, bs), draw((2, 2 * G, T, D), 4, dtype)
+    usual = pkg.cache_attention(q.cuda(), cache, *gpu(table, ints(lens)), True, 0.125)
+    assert torch.equal(usual, pkg.cache_attention(q.cuda() * 2.0 ** 110, cache, *gpu(table, ints(lens)), True, 0.125 * 2.0 ** -110))
+    check_attention(cache, host, q * 2.0 ** -115, table, lens, True, 0.125 * 2.0 ** 115)
+    check_attention(cache, host, q * 2.0 ** 110, table, lens, True, 0.125 * 2.0 ** -110, accumulate=True)
+
+
 @pytest.mark.parametrize("T,G,dtype,new", [(4, 1, BF16, [1, 3]), (7, 3, F32, [2, 7]), (90, 2, BF16, [3, 70]), (300, 1, F16, [10, 299])])
 def test_hidden_nan_with_a_table_that_ends_with_the_sequence(T, G, dtype, new):
     """Rows without a query stand behind the last one: they must not make anyone look behind the last block of the table."""
