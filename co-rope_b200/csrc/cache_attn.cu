@@ -328,8 +328,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             }
 
             // scores in units of log2, the scale of V folded into the exponent: O = sum of exp2(s + log2 v_scale - M) * code
-            // (a scale of 0 is left out of the exponent, and its slots out of O)
-            const float v_size = v_scale == 0.f ? 1.f : max_nan(v_scale, 1e-30f), lift = fast_log2(v_size), drop = fast_reciprocal(v_size);
+            // (a scale without values is left out of the exponent, and its slots out of O)
+            const bool no_v = no_values(v_scale);
+            const float v_size = no_v ? 1.f : v_scale, lift = fast_log2(v_size), drop = fast_reciprocal(v_size);
             bool higher = false;
             const bool masked = !found || slot0 + kPiece > least_seen;
             auto hide = [&]() {
@@ -406,11 +407,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const uint32_t hi = v_scale == 0.f ? 0u : pack_half2(w[2 * i], w[2 * i + 1]);
+                    const uint32_t hi = no_v ? 0u : pack_half2(w[2 * i], w[2 * i + 1]);
                     pb[nt][i] = transpose8x8(hi);
                     if constexpr (EXACT_P) {
                         const float2 back = unpack_half2(hi);
-                        pl[nt][i] = transpose8x8(v_scale == 0.f ? 0u : pack_half2(w[2 * i] - back.x, w[2 * i + 1] - back.y));
+                        pl[nt][i] = transpose8x8(no_v ? 0u : pack_half2(w[2 * i] - back.x, w[2 * i + 1] - back.y));
                     }
                 }
             }
@@ -514,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 #pragma unroll 1
                 for (int slot = max(u0 * kUnit, least_seen / kPiece * kPiece); slot < min(sees_row, u1 * kUnit); ++slot) {   // from where it was left out
                     const int page = table[slot >> p.c.bs_log2];
-                    if ((unsigned)page >= (unsigned)p.c.num_blocks || p.c.v_scale[(int64_t)page * p.c.Hkv + h] == 0.f) continue;
+                    if ((unsigned)page >= (unsigned)p.c.num_blocks || no_values(p.c.v_scale[(int64_t)page * p.c.Hkv + h])) continue;
                     const uint32_t word = *reinterpret_cast<const uint32_t*>(p.c.v + (int64_t)page * p.c.sv.b + (int64_t)h * p.c.sv.h + (int64_t)(slot & in_block_mask) * p.c.sv.n + d);
                     if ((word & 0x7fu) == 0x7fu) y.x = __int_as_float(0x7fffffff);
                     if ((word >> 8 & 0x7fu) == 0x7fu) y.y = __int_as_float(0x7fffffff);

@@ -7,6 +7,11 @@ namespace corope {
 #ifdef __CUDACC__
 constexpr float kLowest = -1e30f;             // running maximum before any score: finite, so that differences from it are no NaN
 
+// Values of a block whose scale of V is below this count as 0 (as those of a scale of 0 do): the scale enters the exponents, and its reciprocal the sums
+// of fp32 probabilities, which 2^27 slots of the largest exponent then still fit.
+constexpr float kLeastScale = 1e-30f;
+__device__ __forceinline__ bool no_values(float v_scale) { return v_scale < kLeastScale; }
+
 // The power of two 2^-e that brings a row whose largest element is m to [2^10, 2^11), so that the second of two fp16 parts is a normal number too; as `up` =
 // 2^-e and `down` = 2^e.  Rows below 2^-100 stay below 2^10; rows with infinities or NaN are left as they are.
 __device__ __forceinline__ void row_scaling(float m, float& up, float& down) {

@@ -39,7 +39,7 @@ enum Bar { Q_FULL = 0, Q_EMPTY, K_FULL, K_EMPTY = K_FULL + kStages, V_FULL = K_E
 // shared memory of head dimension D (32 is widened to 64 with zeros)
 __host__ __device__ constexpr int wide(int D) { return D == 128 ? 128 : 64; }
 __host__ __device__ constexpr size_t tile_bytes(int D) { return (size_t)kN * wide(D) * 2; }
-// A unit's 16-slot groups: where their rows begin, how many there are (0: the block is not there, or its scale of V is 0), their scales.
+// A unit's 16-slot groups: where their rows begin, how many there are (0: the block is not there, or has no values), their scales.
 struct alignas(16) UnitNote {   // its floats are read four at a time
     uint64_t k[8], v[8];
     float k_scale[8], lift[8], drop[8];
@@ -422,15 +422,15 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                     if (lane < 8) {
                         const int slot0 = u * kN + 16 * lane, rows = page >= 0 ? min(x.len - slot0, 16) : 0;
                         const int64_t at = (int64_t)max(page, 0) * p.c.Hkv + x.h, row = slot0 & bs_mask;
-                        const float ks = p.c.k_scale[at], vs = p.c.v_scale[at], size = vs == 0.f ? 1.f : max_nan(vs, 1e-30f);
+                        const float ks = p.c.k_scale[at], vs = p.c.v_scale[at], size = no_values(vs) ? 1.f : vs;
                         note.k[lane] = (uint64_t)(p.c.k + (int64_t)max(page, 0) * p.c.sk.b + (int64_t)x.h * p.c.sk.h + row * p.c.sk.n);
                         note.v[lane] = (uint64_t)(p.c.v + (int64_t)max(page, 0) * p.c.sv.b + (int64_t)x.h * p.c.sv.h + row * p.c.sv.n);
                         note.k_rows[lane] = rows;
-                        note.v_rows[lane] = vs == 0.f ? 0 : rows;                    // a scale of 0 makes zeros of its codes, whatever they are
+                        note.v_rows[lane] = no_values(vs) ? 0 : rows;                // zeros, whatever the codes are
                         note.k_scale[lane] = page >= 0 ? ks : 0.f;
                         note.lift[lane] = page >= 0 ? __log2f(size) : -INFINITY;     // slots of a block that is not there count nothing
                         note.drop[lane] = 1.f / size;
-                        const bool full = __all_sync(0xffu, rows == 16 && vs != 0.f);
+                        const bool full = __all_sync(0xffu, rows == 16 && !no_values(vs));
                         if (lane == 0) note.piece = pieces, note.hidden = (u + 1) * kN > seen, note.full = full;
                     }
                     mbar_arrive_warp(&bars[UNIT_FULL + q % kUnitSlots], lane);
@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                     for (int s = max(u0, seen / kN) * kN; s < (t < x.n ? min(sees, (u0 + count) * kN) : 0); ++s) {   // (never behind the last slot, whose block the table still has)
                         bool far = false;
                         const int page = cache_page(p.s, p.c.bs_log2, p.c.num_blocks, x.b, s, far);
-                        if (page < 0 || p.c.v_scale[(int64_t)page * p.c.Hkv + x.h] == 0.f) continue;
+                        if (page < 0 || no_values(p.c.v_scale[(int64_t)page * p.c.Hkv + x.h])) continue;
                         const uint8_t* v = p.c.v + (int64_t)page * p.c.sv.b + (int64_t)x.h * p.c.sv.h + (int64_t)(s & ((1 << p.c.bs_log2) - 1)) * p.c.sv.n + col0 + k;
 #pragma unroll
                         for (int i = 0; i < 16; ++i)

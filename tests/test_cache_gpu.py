@@ -284,6 +284,21 @@ def test_queries_of_any_size(T, G, dtype):
     check_attention(cache, host, q * 2.0 ** 110, table, lens, True, 0.125 * 2.0 ** -110, accumulate=True)
 
 
+@pytest.mark.parametrize("T,G,dtype", [(1, 4, BF16), (3, 4, F32), (50, 3, BF16), (30, 2, F32)])
+@pytest.mark.parametrize("code", [E4M3, INT8])
+def test_values_below_the_least_scale_are_zeros(T, G, dtype, code):
+    """Blocks of scale 2^-120 are not read as ones of a larger scale: alone they give zeros, beside others nothing."""
+    D, bs, lens = 64, 16, [90 + T, 33 + T]
+    cache, host = make_cache(30, 1, bs, D, code)
+    table, q = make_table(2, 12, 30, lens, bs), draw((2, G, T, D), 4, dtype)
+    cache.v_scale.fill_(2.0 ** -120)
+    got = pkg.cache_attention(q.cuda(), cache, *gpu(table, ints(lens)), True, 0.125)
+    assert (got == 0).all()
+    host["v_scale"][table[:, 1].long()] = 2.0 ** -120
+    cache.v_scale.copy_(host["v_scale"].cuda())
+    check_attention(cache, host, q, table, lens, True, 0.125, accumulate=True)
+
+
 @pytest.mark.parametrize("T,G,dtype,new", [(4, 1, BF16, [1, 3]), (7, 3, F32, [2, 7]), (90, 2, BF16, [3, 70]), (300, 1, F16, [10, 299])])
 def test_hidden_nan_with_a_table_that_ends_with_the_sequence(T, G, dtype, new):
     """Rows without a query stand behind the last one: they must not make anyone look behind the last block of the table."""
