@@ -474,8 +474,10 @@ Tensor cache_attention(const Tensor& q_in, const CacheTensors& c, const Tensor& 
     require_value(q_in.size(1) > 0 && q_in.size(1) % cache.Hkv == 0, "Number of query heads must be divisible by KV heads.");
     require_value(!accumulate || cache.weight != nullptr, "accumulate needs a cache with weights");
     const Tensor q = readable_rows(q_in);
-    // o is laid out like q, whose heads or batch entries may share memory; o's may not
+    // o is laid out like q, whose heads, tokens or batch entries may share memory; o's may not, and where q's overlap that can put the head dimension
+    // somewhere else than last
     Tensor o = at::empty_like(q);
+    if (o.stride(3) != 1) o = at::empty(q.sizes(), q.options());
     const int Hq = (int)q.size(1), T = (int)q.size(2), dt = dtype_code(q);
     const size_t bytes = corope_cache_attn_workspace_bytes(&cache, &seqs, Hq, T, dt, accumulate ? 1 : 0);
     const Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 256)}, q.options().dtype(at::kByte));

@@ -233,6 +233,18 @@ def test_attention_layouts(layout, kind):
     check_attention(cache, host, q, table, lens, True, 0.2, accumulate=True, q_gpu=q_gpu)
 
 
+@pytest.mark.parametrize("strides", [(1000, 300, 1, 1), (1, 1, 1, 1), (64, 1, 2, 1), (0, 0, 1, 1), (0, 1, 0, 1), (7, 1, 3, 1)])
+@pytest.mark.parametrize("T,dtype", [(1, F32), (3, BF16), (20, F16)])
+def test_queries_that_overlap(T, dtype, strides):
+    """Windows that slide over one row: what lies next to what in q says nothing about o."""
+    B, Hq, D, bs, lens = 2, 4, 64, 16, [50, 30]
+    cache, host = make_cache(9, 2, bs, D, INT8)
+    table = make_table(B, 4, 9, lens, bs)
+    row = draw((4000,), 4, dtype)
+    q = row.as_strided((B, Hq, T, D), strides)
+    check_attention(cache, host, q.contiguous(), table, lens, True, 0.2, q_gpu=row.cuda().as_strided((B, Hq, T, D), strides))
+
+
 @pytest.mark.parametrize("dtype,T,G", [(BF16, 1, 4), (F32, 1, 4), (F16, 100, 4)])
 def test_attention_extremes(dtype, T, G):
     """Scores of some hundred (one slot has all the weight), equal scores, blocks whose scales differ by 2^20, scales of 0."""
