@@ -359,11 +359,16 @@ void require_shape(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, 
         throw ValueError(os.str());
     }
 }
-// no gradient flows through the cache: a caller who expects one learns it here
-void require_no_grad(std::initializer_list<const Tensor*> ts) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor* t : ts)
-        if (t->requires_grad()) throw std::runtime_error("corope_b200: the cache operators have no backward pass; call them under torch.no_grad()");
+// no gradient flows through the cache, backwards or forwards: a caller who expects one learns it here
+void require_no_grad(std::initializer_list<const Tensor*> ts, const CacheTensors& c) {
+    auto check = [](const Tensor& t) {
+        if (at::GradMode::is_enabled() && t.requires_grad())
+            throw std::runtime_error("corope_b200: the cache operators have no backward pass; call them under torch.no_grad()");
+        if (t._fw_grad(0).defined()) throw std::runtime_error("corope_b200: the cache operators have no derivatives; a tensor of the call is a forward-mode dual");
+    };
+    for (const Tensor* t : ts) check(*t);
+    for (const Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale}) check(*t);
+    if (c.weight.has_value()) check(*c.weight);
 }
 
 corope_kv_cache_t cache_view(const CacheTensors& c) {
@@ -447,7 +452,7 @@ void check_tokens(const Tensor& t, const CacheTensors& c, int64_t B, const char*
 
 void cache_append(const Tensor& k_in, const Tensor& v_in, const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, const Optional& cos,
                   const Optional& sin, const Optional& positions, const Optional& new_lens) {
-    require_no_grad({&k_in, &v_in});
+    require_no_grad({&k_in, &v_in}, c);
     const corope_kv_cache_t cache = cache_view(c);
     Call call(c.k);
     Tables keep;
@@ -465,7 +470,7 @@ void cache_append(const Tensor& k_in, const Tensor& v_in, const CacheTensors& c,
 
 Tensor cache_attention(const Tensor& q_in, const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, bool causal, double sm_scale,
                        const Optional& cos, const Optional& sin, const Optional& positions, const Optional& new_lens, bool accumulate) {
-    require_no_grad({&q_in});
+    require_no_grad({&q_in}, c);
     const corope_kv_cache_t cache = cache_view(c);
     Call call(c.k);
     Tables keep;
@@ -492,6 +497,7 @@ Tensor cache_attention(const Tensor& q_in, const CacheTensors& c, const Tensor& 
 
 std::tuple<Tensor, Tensor> cache_evict(const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, const Tensor& out_table, int64_t budget,
                                        int64_t recent) {
+    require_no_grad({}, c);
     const corope_kv_cache_t cache = cache_view(c);
     require_value(cache.weight != nullptr, "eviction needs a cache with weights");
     Call call(c.k);

@@ -16,7 +16,7 @@ captured into a CUDA graph follows what they hold at replay.  An entry that poin
 concerned are left out and the next call on the device raises RuntimeError.  (A length or a number of new tokens out of range: nothing
 of the sequence is stored; attention and eviction take the nearest number in range, and so does a position.)  Block table
 entries behind a sequence's last block are not read.  A place of a padded batch that holds no sequence has a length of 0.  No
-operator has a backward pass: k, v and q that require a gradient are refused outside torch.no_grad().
+operator has a backward pass: tensors that require a gradient are refused outside torch.no_grad(), duals of forward mode everywhere.
 """
 
 import torch

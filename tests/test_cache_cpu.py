@@ -88,6 +88,43 @@ def test_entry_points_refuse_cpu_tensors():
             call()
 
 
+def test_entry_points_refuse_what_expects_a_derivative():
+    """Tensors of the cache count as well; forward-mode duals are refused whatever the grad mode."""
+    import torch.autograd.forward_ad as fwd
+
+    table, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    x = draw((1, 2, 1, 64), 0, torch.float32)
+
+    def calls(cache, k):
+        return (lambda: pkg.cache_append(k, x, cache, table, lens), lambda: pkg.cache_append(x, k, cache, table, lens),
+                lambda: pkg.cache_attention(k, cache, table, lens, True, 0.1), lambda: pkg.cache_evict(cache, table, lens, table, 16))
+
+    cache = pkg.KVCache(4, 2, 16, 64, device="cpu", weights=True)
+    for call in calls(cache, x.clone().requires_grad_(True))[:3]:
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+    for name in ("k_scale", "v_scale", "weight"):
+        cache = pkg.KVCache(4, 2, 16, 64, device="cpu", weights=True)
+        getattr(cache, name).requires_grad_(True)
+        for call in calls(cache, x):
+            with pytest.raises(RuntimeError, match="no backward"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors only"):
+                call()
+    cache = pkg.KVCache(4, 2, 16, 64, device="cpu", weights=True)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in calls(cache, dual)[:3]:
+            with pytest.raises(RuntimeError, match="dual"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="dual"):
+                call()
+        cache.weight = fwd.make_dual(cache.weight, torch.ones_like(cache.weight))
+        for call in calls(cache, x):
+            with pytest.raises(RuntimeError, match="dual"):
+                call()
+
+
 @pytest.mark.parametrize("code,worst", [(torch.float8_e4m3fn, 2.0 ** -4), (torch.int8, 0.5 / 127)])
 def test_codes_stand_for_what_was_stored(code, worst):
     """The oracle's codes: within half a step of the element (e4m3: 2^-4 of it, or of the smallest normal code; int8: of the block's largest)."""
