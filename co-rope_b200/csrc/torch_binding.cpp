@@ -370,6 +370,15 @@ void require_no_grad(std::initializer_list<const Tensor*> ts, const CacheTensors
     for (const Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale}) check(*t);
     if (c.weight.has_value()) check(*c.weight);
 }
+// Tensors that a call has written to in place: a backward pass that saved one of them has to find out.
+void written(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+void whole_cache_written(const CacheTensors& c) {
+    written({&c.k, &c.v, &c.k_scale, &c.v_scale});
+    if (c.weight.has_value()) written({&*c.weight});
+}
 
 corope_kv_cache_t cache_view(const CacheTensors& c) {
     for (const Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale}) require_cuda(*t);
@@ -466,6 +475,7 @@ void cache_append(const Tensor& k_in, const Tensor& v_in, const CacheTensors& c,
     set_strides(sv, v);
     raise_for_status(corope_cache_append(&cache, &seqs, k.data_ptr(), v.data_ptr(), sk, sv, (int)k.size(2), dtype_code(k), call.status.word_ptr, call.stream),
                      "corope_cache_append");
+    whole_cache_written(c);
 }
 
 Tensor cache_attention(const Tensor& q_in, const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, bool causal, double sm_scale,
@@ -492,6 +502,7 @@ Tensor cache_attention(const Tensor& q_in, const CacheTensors& c, const Tensor& 
     raise_for_status(corope_cache_attn(&cache, &seqs, q.data_ptr(), o.data_ptr(), sq, so, Hq, T, dt, causal ? 1 : 0, (float)sm_scale, accumulate ? 1 : 0,
                                        ws.data_ptr(), bytes, call.status.word_ptr, call.stream),
                      "corope_cache_attn");
+    if (accumulate) written({&*c.weight});
     return o;
 }
 
@@ -511,6 +522,7 @@ std::tuple<Tensor, Tensor> cache_evict(const CacheTensors& c, const Tensor& bloc
     raise_for_status(corope_cache_evict(&cache, &seqs, out_table.data_ptr<int>(), out_table.stride(0), (int)out_table.size(1), (int)budget, (int)recent,
                                         lens.data_ptr<int>(), kept.data_ptr<int>(), call.status.word_ptr, call.stream),
                      "corope_cache_evict");
+    whole_cache_written(c);
     return {lens, kept};
 }
 

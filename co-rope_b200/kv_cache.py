@@ -17,6 +17,7 @@ concerned are left out and the next call on the device raises RuntimeError.  (A 
 of the sequence is stored; attention and eviction take the nearest number in range, and so does a position.)  Block table
 entries behind a sequence's last block are not read.  A place of a padded batch that holds no sequence has a length of 0.  No
 operator has a backward pass: tensors that require a gradient are refused outside torch.no_grad(), duals of forward mode everywhere.
+What an operator writes to in place counts as modified for autograd.
 """
 
 import torch

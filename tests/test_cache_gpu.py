@@ -678,6 +678,35 @@ def test_calls_on_two_streams_and_twice_are_the_same(T, dtype):
     assert all(torch.equal(want, x) for x in got)
 
 
+def test_writes_in_place_are_known_to_autograd():
+    """A tensor of the cache that a backward pass has saved cannot be written to unnoticed; inference tensors are taken as they are."""
+    cache = pkg.KVCache(6, 1, 16, 32, weights=True)
+    names = ("k", "v", "k_scale", "v_scale", "weight")
+    table, out, lens = gpu(ints([[0, 1]]), ints([[2]]), ints([20]))
+    x = draw((1, 1, 20, 32), 1, BF16).cuda()
+
+    def bumped(call):
+        before = [getattr(cache, n)._version for n in names]
+        call()
+        return [n for n, was in zip(names, before) if getattr(cache, n)._version > was]
+
+    assert bumped(lambda: pkg.cache_append(x, x, cache, table, lens)) == list(names)
+    assert bumped(lambda: pkg.cache_attention(x, cache, table, lens, True, 0.1)) == []
+    assert bumped(lambda: pkg.cache_attention(x, cache, table, lens, True, 0.1, accumulate=True)) == ["weight"]
+    assert bumped(lambda: pkg.cache_evict(cache, table, lens, out, 16)) == list(names)
+    y = torch.ones(6, 1, 16, device="cuda", requires_grad=True)
+    loss = (cache.weight * y).sum()
+    pkg.cache_attention(x, cache, table, lens, True, 0.1, accumulate=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        cache = pkg.KVCache(6, 1, 16, 32, weights=True)
+        pkg.cache_append(x, x, cache, table, lens)
+    pkg.cache_append(x, x, cache, table, lens)
+    pkg.cache_attention(x, cache, table, lens, True, 0.1, accumulate=True)
+    pkg.check_status()
+
+
 def test_sequences_may_share_blocks():
     """A common prefix: reads are shared, and each sequence's weights are added."""
     D, bs, lens = 64, 16, [40, 36]
