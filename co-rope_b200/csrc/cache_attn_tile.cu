@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
         tc_fence_before();
     }
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_flag) report_to_mirror(p.status, p.mirror);
+    if (threadIdx.x == 0 && *abort_flag) report_expired_wait(p.status, *abort_flag, p.mirror);
     if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -1008,7 +1008,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
     }
     if (bad || walk.bad) report_bad_index(p.status, p.mirror);
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_flag) report_to_mirror(p.status, p.mirror);
+    if (threadIdx.x == 0 && *abort_flag) report_expired_wait(p.status, *abort_flag, p.mirror);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 256);

@@ -192,15 +192,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
-// The status word gains bits until the host clears it: what one kernel meets does not cover up what another met.  Of expired waits the first one's id stays.
-__device__ __forceinline__ void note_expired_wait(int* status, int id) {
-    if (status == nullptr) return;
-    int held = *reinterpret_cast<volatile int*>(status);
-    for (int seen; !(held & COROPE_DEV_WAIT_EXPIRED); held = seen) {
-        seen = atomicCAS(status, held, held | COROPE_DEV_WAIT_EXPIRED | id);
-        if (seen == held) break;
-    }
-}
 // Bounded wait.  Returns false (after recording `id` in *status) when the limit is hit; callers
 // then leave their loops and fall through to the common exit path.  try_wait itself blocks for
 // a hardware-defined slice, so the limit corresponds to well over a second.
@@ -211,8 +202,8 @@ __device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity
         if (mbar_try_wait(bar, parity)) return true;
         if ((it & 1023u) == 1023u && *abort_flag) return false;
     }
-    *abort_flag = 1;
-    note_expired_wait(status, id);
+    *abort_flag = COROPE_DEV_WAIT_EXPIRED | id;
+    if (status) atomicCAS(status, 0, COROPE_DEV_WAIT_EXPIRED | id);   // (where the word holds something else, at the kernel's end)
     return false;
 }
 // A kernel that gave up, or that did not start because an earlier one had, leaves the word in the host mirror too: the host learns of
@@ -228,6 +219,12 @@ __device__ __forceinline__ void report_to_mirror(const int* status, int* mirror)
         if (now == v) return;
         v = now;
     }
+}
+// The end of a kernel in which a wait ran out, `what` = COROPE_DEV_WAIT_EXPIRED | id.  The word gains bits until the host clears it, so that what one kernel
+// meets does not cover up what another met; of expired waits the first one's id stays.
+__device__ __forceinline__ void report_expired_wait(int* status, int what, int* mirror) {
+    if (status != nullptr && !(atomicOr(status, COROPE_DEV_WAIT_EXPIRED) & COROPE_DEV_WAIT_EXPIRED)) atomicOr(status, what);
+    report_to_mirror(status, mirror);
 }
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* status, int id, volatile int* abort_flag) {
     return mbar_wait_limited(bar, parity, status, id, abort_flag, kWaitLimit);
@@ -263,8 +260,8 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
         if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
         if ((it & 1023u) == 1023u && __any_sync(0xffffffffu, *abort_flag)) return false;
     }
-    *abort_flag = 1;
-    note_expired_wait(status, id);
+    *abort_flag = COROPE_DEV_WAIT_EXPIRED | id;
+    if (status) atomicCAS(status, 0, COROPE_DEV_WAIT_EXPIRED | id);   // (where the word holds something else, at the kernel's end)
     return false;
 }
 

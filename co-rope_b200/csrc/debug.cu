@@ -17,7 +17,7 @@ __global__ void expire_wait_kernel(int* status, int* status_mirror, unsigned max
     }
     __syncthreads();
     const bool ok = mbar_wait_limited(&bar, 0, status, 0x7e, &abort_flag, max_polls);
-    if (!ok && threadIdx.x == 0) report_to_mirror(status, status_mirror);   // the phase never completes
+    if (!ok && threadIdx.x == 0) report_expired_wait(status, abort_flag, status_mirror);   // the phase never completes
 }
 
 }  // namespace

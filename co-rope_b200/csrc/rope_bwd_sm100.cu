@@ -145,10 +145,7 @@ rope_bwd_sm100_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
     auto step_row = [&](int bh, int q_first, int spg, int s) { return (bh * G + step_head(spg, s)) * N + step_q0(q_first, spg, s); };
 
     if (reinterpret_cast<uintptr_t>(sm) - reinterpret_cast<uintptr_t>(smem_raw) > kSmemSlack) {   // base less aligned than assumed
-        if (threadIdx.x == 0 && p.status) {
-            note_expired_wait(p.status, 0xfff);
-            report_to_mirror(p.status, p.status_mirror);
-        }
+        if (threadIdx.x == 0) report_expired_wait(p.status, COROPE_DEV_WAIT_EXPIRED | 0xfff, p.status_mirror);
         pdl_wait();   // no launch ends before the one in front of it
         return;
     }
@@ -577,7 +574,7 @@ rope_bwd_sm100_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
         if (threadIdx.x == kDrainWarp0 * 32) bulk_wait_group0();   // all reduces have landed before the CTA exits
     }
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_flag) report_to_mirror(p.status, p.status_mirror);
+    if (threadIdx.x == 0 && *abort_flag) report_expired_wait(p.status, *abort_flag, p.status_mirror);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);

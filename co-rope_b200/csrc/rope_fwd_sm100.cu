@@ -156,10 +156,7 @@ rope_fwd_sm100_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
     // item's last tiles are still in the MMAs and its output is being written.
 
     if (reinterpret_cast<uintptr_t>(sm) - reinterpret_cast<uintptr_t>(smem_raw) > kSmemSlack) {   // base less aligned than assumed
-        if (threadIdx.x == 0 && p.status) {
-            note_expired_wait(p.status, 0xfff);
-            report_to_mirror(p.status, p.status_mirror);
-        }
+        if (threadIdx.x == 0) report_expired_wait(p.status, COROPE_DEV_WAIT_EXPIRED | 0xfff, p.status_mirror);
         pdl_wait();   // no launch ends before the one in front of it
         return;
     }
@@ -537,7 +534,7 @@ rope_fwd_sm100_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
         tc_fence_before();
     }
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_flag) report_to_mirror(p.status, p.status_mirror);
+    if (threadIdx.x == 0 && *abort_flag) report_expired_wait(p.status, *abort_flag, p.status_mirror);
     if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);

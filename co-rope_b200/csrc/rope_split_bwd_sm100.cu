@@ -108,10 +108,7 @@ rope_bwd_split_sm100_kernel(const __grid_constant__ CUtensorMap mapOwn, const __
     auto steps_of = [&](int t) { return KV ? nb_all - first_of(t) : causal ? min(nb_all, 2 * t + 2) : nb_all; };   // streamed blocks (KV: of each query head)
 
     if (reinterpret_cast<uintptr_t>(sm) - reinterpret_cast<uintptr_t>(smem_raw) > W::kSlack) {   // base less aligned than assumed
-        if (threadIdx.x == 0 && p.status) {
-            note_expired_wait(p.status, 0xfff);
-            report_to_mirror(p.status, p.status_mirror);
-        }
+        if (threadIdx.x == 0) report_expired_wait(p.status, COROPE_DEV_WAIT_EXPIRED | 0xfff, p.status_mirror);
         pdl_wait();
         return;
     }
@@ -607,7 +604,7 @@ rope_bwd_split_sm100_kernel(const __grid_constant__ CUtensorMap mapOwn, const __
         tc_fence_before();
     }
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_flag) report_to_mirror(p.status, p.status_mirror);
+    if (threadIdx.x == 0 && *abort_flag) report_expired_wait(p.status, *abort_flag, p.status_mirror);
     if (!KV) pdl_wait();
     if (warp == 1) {
         tc_fence_after();

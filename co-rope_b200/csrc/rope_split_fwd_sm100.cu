@@ -86,10 +86,7 @@ rope_fwd_split_sm100_kernel(const __grid_constant__ CUtensorMap mapK, const __gr
     auto blocks_of = [&](int t) { return causal ? min(nb_all, 2 * t + 2) : nb_all; };
 
     if (reinterpret_cast<uintptr_t>(sm) - reinterpret_cast<uintptr_t>(smem_raw) > F::kSlack) {   // base less aligned than assumed
-        if (threadIdx.x == 0 && p.status) {
-            note_expired_wait(p.status, 0xfff);
-            report_to_mirror(p.status, p.status_mirror);
-        }
+        if (threadIdx.x == 0) report_expired_wait(p.status, COROPE_DEV_WAIT_EXPIRED | 0xfff, p.status_mirror);
         pdl_wait();   // no launch ends before the one in front of it
         return;
     }
@@ -452,7 +449,7 @@ rope_fwd_split_sm100_kernel(const __grid_constant__ CUtensorMap mapK, const __gr
         tc_fence_before();
     }
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_flag) report_to_mirror(p.status, p.status_mirror);
+    if (threadIdx.x == 0 && *abort_flag) report_expired_wait(p.status, *abort_flag, p.status_mirror);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
