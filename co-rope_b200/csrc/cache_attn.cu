@@ -26,7 +26,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kPiece = 16;                    // slots per step of a warp; a block of the cache holds a whole number of them
-constexpr int kUnit = kWarps * kPiece;        // slots per unit of work
+constexpr int kUnit = kWarps * kPiece, kUnitLog2 = log2_of(kUnit);        // slots per unit of work
 // Units that an item counts beside its own in sharing out the work.  With 8 rows 0 / 4 / 6 / 12, us, 32 / 8 heads of 128: 64 x up to 4096 tokens 68.1 / 62.6 /
 // 60.5 / 63.1, 256 x up to 1000 97.6 / 80.3 / 80.6 / 81.8, 8 x 16384 58.0 / 56.4 / 56.5 / 57.6.
 // Two more for each further eight rows: 6 / 8 with 16 rows, 16 x up to 4000 tokens and their weights, 45.4 / 43.7; 6 / 12 / 20 with 32 rows, 64 x up to
@@ -137,7 +137,7 @@ template <int D, int CODE, int NT, bool EXACT_P>
 __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_kernel(const CacheAttnParams p) {
     using S = Shape<D, NT>;
     constexpr int kItemCost = item_cost(NT);
-    constexpr int kRows = S::kRows, kKSteps = D / 16, kVWords = D / 32, kStages = S::kStages;
+    constexpr int kRows = S::kRows, kRowsLog2 = log2_of(kRows), kKSteps = D / 16, kVWords = D / 32, kStages = S::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
     uint32_t* packed = reinterpret_cast<uint32_t*>(smem + S::kBig);
     float* meta = reinterpret_cast<float*>(smem + S::kBig + S::kPacked);
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
     bool bad = false;
 
-    auto load = [&](int b) { return load_of(p, kRows, kUnit, kItemCost, b, bad); };
+    auto load = [&](int b) { return load_of(p, kRowsLog2, kUnitLog2, kItemCost, b, bad); };
     __shared__ int nan_v;   // NaN in V where some rows must not see it
     // Either a range of the batch's units, or (p.parts) this block's share of one item, whose other shares are with the blocks of its cluster.
     int b, part_of = 0, cluster_item = 0;
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             }
             const int item = (int)(off / l.cost), tiles = l.items / p.c.Hkv;
             h = item / tiles;
-            tile = item % tiles + first_tile(p, kRows, l.len, l.n);
+            tile = item % tiles + first_tile(p, kRowsLog2, l.len, l.n);
             u0 = (int)(off - (int64_t)item * l.cost);
             u1 = (int)min((int64_t)l.cost, u0 + left);
             off += u1 - u0;
@@ -585,15 +585,16 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 // added in the order of their ranges.  Rows that no unit stands for are written here: 0.
 constexpr int kJoinThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads, 6) cache_attn_join_kernel(const CacheAttnParams p, int rows_per_tile, int unit, int extra, int main_blocks) {
+__global__ void __launch_bounds__(kJoinThreads, 6) cache_attn_join_kernel(const CacheAttnParams p, int rows_log2, int unit_log2, int extra, int main_blocks) {
     __shared__ int64_t words[2][kJoinThreads / 32];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const unsigned blocks = (unsigned)rows_per_tile / (kJoinThreads / 32), item = blockIdx.x / blocks;
+    const int rows_per_tile = 1 << rows_log2;
+    const unsigned blocks_log2 = rows_log2 - log2_of(kJoinThreads / 32), item = blockIdx.x >> blocks_log2;
     const int tile = (int)(item % (unsigned)p.row_tiles), bh = (int)(item / (unsigned)p.row_tiles), b = bh / p.c.Hkv, h = bh - b * p.c.Hkv;
     bool bad = false;
     int64_t before = 0, total = 0;
     for (int i = threadIdx.x; i < p.s.B; i += kJoinThreads) {
-        const Load l = load_of(p, rows_per_tile, unit, extra, i, bad);
+        const Load l = load_of(p, rows_log2, unit_log2, extra, i, bad);
         const int64_t u = (int64_t)l.cost * l.items;
         total += u;
         if (i < b) before += u;
@@ -609,28 +610,28 @@ __global__ void __launch_bounds__(kJoinThreads, 6) cache_attn_join_kernel(const 
 #pragma unroll
     for (int w = 0; w < kJoinThreads / 32; ++w) before += words[0][w], total += words[1][w];
 
-    const Load l = load_of(p, rows_per_tile, unit, extra, b, bad);
-    const int tiles = l.items / p.c.Hkv, tile0 = first_tile(p, rows_per_tile, l.len, l.n);
+    const Load l = load_of(p, rows_log2, unit_log2, extra, b, bad);
+    const int tiles = tiles_in_use(p, rows_log2, l.len, l.n), tile0 = first_tile(p, rows_log2, l.len, l.n);
     const bool empty = l.units == 0 || tile < tile0 || tile >= tile0 + tiles;
     const int64_t ranges = min((int64_t)main_blocks, total);
-    int64_t r0 = 0, r1 = 0;
+    int r0 = 0, r1 = 0;
     if (!empty) {
         const int64_t u0 = before + (int64_t)(h * tiles + tile - tile0) * l.cost + extra, u1 = u0 + l.units - 1;
-        r0 = ((u0 + 1) * ranges - 1) / total;   // the range that holds a unit
-        r1 = ((u1 + 1) * ranges - 1) / total;
+        r0 = (int)(((u0 + 1) * ranges - 1) / total);   // the range that holds a unit
+        r1 = (int)(((u1 + 1) * ranges - 1) / total);
     }
     pdl_wait();   // by every block: the end of this kernel has to stand for the end of the one before
     if (!empty && r0 == r1) return;
     {
-        const int r = (int)(blockIdx.x - item * blocks) * (kJoinThreads / 32) + warp, row = tile * rows_per_tile + r, t = row / p.G;
+        const int r = (int)(blockIdx.x - (item << blocks_log2)) * (kJoinThreads / 32) + warp, row = tile * rows_per_tile + r, t = row / p.G;
         if (t >= p.T) return;
         float top = kLowest, all = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         if (!empty && t < l.n) {
             // a part that starts its item is in the second slot of its block, the others are in the first; 32 parts at a time, a lane each
-            for (int64_t base = r0; base <= r1; base += 32) {
-                const int here = (int)min(r1 - base + 1, (int64_t)32);
-                auto row_of = [&](int k) { return (2 * (base + k) + (base + k == r0 ? 1 : 0)) * rows_per_tile + r; };
+            for (int base = r0; base <= r1; base += 32) {
+                const int here = min(r1 - base + 1, 32);
+                auto row_of = [&](int k) { return (int64_t)((2 * (base + k) + (base + k == r0 ? 1 : 0)) * rows_per_tile + r); };
                 const float2 ml = lane < here ? *reinterpret_cast<const float2*>(p.part_ml + row_of(lane) * 2) : make_float2(kLowest, 0.f);
                 float best = ml.x;
 #pragma unroll
@@ -669,7 +670,7 @@ template <bool FOURS>
 __global__ void __launch_bounds__(kThreads, kSumBlocks) cache_attn_sum_kernel(const CacheAttnParams p) {
     bool bad = false;
     auto load = [&](int b) {
-        Load l = load_of(p, 1, kSumUnit, 0, b, bad);
+        Load l = load_of(p, 0, log2_of(kSumUnit), 0, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     };
@@ -723,7 +724,7 @@ __global__ void __launch_bounds__(kThreads) cache_attn_weight_kernel(const Cache
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
     bool bad = false;
     auto load = [&](int b) {
-        Load l = load_of(p, kRows, kUnit, 0, b, bad);
+        Load l = load_of(p, log2_of(kRows), kUnitLog2, 0, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     };   // items of this kernel: K / V heads
@@ -872,9 +873,9 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
 }
 
 template <int D>
-int launch_join(const CacheAttnParams& p, const Layout& l, int unit, int extra, cudaStream_t s) {
+int launch_join(const CacheAttnParams& p, const Layout& l, int unit_log2, int extra, cudaStream_t s) {
     count_launch();
-    return launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles * (l.rows_per_tile / 8)), kJoinThreads, 0, s, p, l.rows_per_tile, unit, extra, (int)l.blocks);
+    return launch_dependent(cache_attn_join_kernel<D>, (unsigned)(p.s.B * p.c.Hkv * p.row_tiles * (l.rows_per_tile / 8)), kJoinThreads, 0, s, p, log2_of(l.rows_per_tile), unit_log2, extra, (int)l.blocks);
 }
 template <int D, int CODE, int NT, bool EXACT_P>
 int launch_main(const CacheAttnParams& p, unsigned blocks, cudaStream_t s) {
@@ -902,7 +903,7 @@ template <int D, int CODE, int NT>
 int launch_rows(const CacheAttnParams& p, const Layout& l, cudaStream_t s) {
     if (int e = p.dtype == COROPE_DTYPE_F32 ? launch_main<D, CODE, NT, true>(p, l.blocks, s) : launch_main<D, CODE, NT, false>(p, l.blocks, s)) return e;
     if (l.parts) return COROPE_OK;
-    if (int e = launch_join<D>(p, l, kUnit, item_cost(NT), s)) return e;
+    if (int e = launch_join<D>(p, l, kUnitLog2, item_cost(NT), s)) return e;
     if (!p.accumulate) return COROPE_OK;
     count_launch();
     const int unit = p.scores != nullptr ? kSumUnit : kUnit;
@@ -920,7 +921,7 @@ template <int D>
 int by_kernel(const CacheAttnParams& p, const Layout& l, void* images, cudaStream_t s) {
     if (!l.tiles) return p.code == COROPE_CODE_E4M3 ? by_rows<D, COROPE_CODE_E4M3>(p, l, s) : by_rows<D, COROPE_CODE_INT8>(p, l, s);
     if (int e = launch_cache_attn_tiles(p, images, l.two_parts, l.pair, l.blocks, s)) return e;
-    if (int e = launch_join<D>(p, l, kTileRows, kTileItemCost, s)) return e;
+    if (int e = launch_join<D>(p, l, log2_of(kTileRows), kTileItemCost, s)) return e;
     return p.accumulate ? launch_cache_weight_tiles(p, images, l.pair, s) : COROPE_OK;
 }
 

@@ -5,6 +5,8 @@
 namespace corope {
 
 #ifdef __CUDACC__
+__host__ __device__ constexpr int log2_of(int x) { return x > 1 ? 1 + log2_of(x / 2) : 0; }
+
 constexpr float kLowest = -1e30f;             // running maximum before any score: finite, so that differences from it are no NaN
 
 // Values of a block whose scale of V is below this count as 0 (as those of a scale of 0 do): the scale enters the exponents, and its reciprocal the sums
@@ -48,14 +50,18 @@ __device__ __forceinline__ bool sees_something(const CacheAttnParams& p, int len
 struct Load {
     int len, n, units, items, cost;   // cost: of an item, extra units included
 };
-// the first tile with a row that sees a slot (of a sequence that has slots)
-__device__ __forceinline__ int first_tile(const CacheAttnParams& p, int rows_per_tile, int len, int n) { return p.causal ? max(n - len, 0) * p.G / rows_per_tile : 0; }
-__device__ __forceinline__ Load load_of(const CacheAttnParams& p, int rows_per_tile, int unit, int extra, int b, bool& bad) {
+// Rows of a tile and slots of a unit are powers of two, given by their logarithms: the joining kernel has them as arguments and would divide.
+// The first tile with a row that sees a slot (of a sequence that has slots):
+__device__ __forceinline__ int first_tile(const CacheAttnParams& p, int rows_log2, int len, int n) { return p.causal ? max(n - len, 0) * p.G >> rows_log2 : 0; }
+__device__ __forceinline__ int tiles_in_use(const CacheAttnParams& p, int rows_log2, int len, int n) {
+    return ((n * p.G + (1 << rows_log2) - 1) >> rows_log2) - first_tile(p, rows_log2, len, n);
+}
+__device__ __forceinline__ Load load_of(const CacheAttnParams& p, int rows_log2, int unit_log2, int extra, int b, bool& bad) {
     Load l;
     l.len = cache_len(p.s, p.c.bs_log2, b, bad);
     l.n = cache_new(p.s, p.T, b, bad);
-    l.units = (l.len + unit - 1) / unit;
-    l.items = p.c.Hkv * ((l.n * p.G + rows_per_tile - 1) / rows_per_tile - first_tile(p, rows_per_tile, l.len, l.n));
+    l.units = (l.len + (1 << unit_log2) - 1) >> unit_log2;
+    l.items = p.c.Hkv * tiles_in_use(p, rows_log2, l.len, l.n);
     l.cost = l.units > 0 ? l.units + extra : 0;
     return l;
 }

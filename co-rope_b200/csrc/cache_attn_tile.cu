@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     bool bad = false;
-    const Range range = take_range<128>(p.s.B, [&](int b) { return load_of(p, kItemRows, kN, kTileItemCost, b, bad); });
+    const Range range = take_range<128>(p.s.B, [&](int b) { return load_of(p, log2_of(kItemRows), log2_of(kN), kTileItemCost, b, bad); });
     pdl_trigger();
     if (bad) report_bad_index(p.status, p.mirror);
     // after a wait that ran out, in this launch's block or in an earlier launch, none starts anew until the host has seen it
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             // are kept.  There is one at most, the first of the range (the end of an item whose rows see none of the last slots): a tile of rows that
             // sees nothing is no item, and every item's first unit is seen by some row.
             Range r = range;
-            Load l = load_of(p, kItemRows, kN, kTileItemCost, r.b, bad);
+            Load l = load_of(p, log2_of(kItemRows), log2_of(kN), kTileItemCost, r.b, bad);
             int q = 0, told = 0, pieces = 0;   // units, pieces, pieces with units so far
             bool ok = true;
             const int bs_mask = (1 << p.c.bs_log2) - 1;
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 while (r.left > 0 && x.b < 0) {
                     while (r.off >= (int64_t)l.cost * l.items) {
                         r.off -= (int64_t)l.cost * l.items;
-                        l = load_of(p, kItemRows, kN, kTileItemCost, ++r.b, bad);
+                        l = load_of(p, log2_of(kItemRows), log2_of(kN), kTileItemCost, ++r.b, bad);
                     }
                     const int item = (int)(r.off / l.cost), tiles = l.items / p.c.Hkv;
                     const int at = (int)(r.off - (int64_t)item * l.cost), end = (int)min((int64_t)l.cost, at + r.left);
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                     r.left -= end - at;
                     const int u1 = end - kTileItemCost;
                     if (u1 <= 0) continue;   // the range ends before the item's first unit
-                    x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles + first_tile(p, kItemRows, l.len, l.n); x.len = l.len; x.n = l.n;
+                    x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles + first_tile(p, log2_of(kItemRows), l.len, l.n); x.len = l.len; x.n = l.n;
                     x.u0 = max(at - kTileItemCost, 0);
                     const int last = min(l.n - 1, (x.tile * kItemRows + kItemRows - 1) / p.G);   // the item's last query
                     const int most = p.causal ? max(l.len - l.n + last + 1, 0) : l.len;   // slots that some row sees
@@ -765,7 +765,7 @@ struct UnitWalk {
     Load l;
     bool bad = false;
     __device__ __forceinline__ Load load(const CacheAttnParams& p, int b) {
-        Load l = load_of(p, kN, kN, 0, b, bad);
+        Load l = load_of(p, log2_of(kN), log2_of(kN), 0, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     }
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) cache_weight_tile_kernel(const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     bool bad = false;
     const Range range = take_range<128>(p.s.B, [&](int b) {
-        Load l = load_of(p, kN, kN, 0, b, bad);
+        Load l = load_of(p, log2_of(kN), log2_of(kN), 0, b, bad);
         l.items = l.n > 0 ? p.c.Hkv : 0;
         return l;
     });
