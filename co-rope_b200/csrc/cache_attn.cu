@@ -366,8 +366,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nt][i] += lift - m[nt][i % 2];
-                if (masked) hide();   // (once more: the lift of a block whose scale is no finite number)
+                    for (int i = 0; i < 4; ++i) s[nt][i] = s[nt][i] == -INFINITY ? s[nt][i] : s[nt][i] + (lift - m[nt][i % 2]);   // (hidden whatever the lift)
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
