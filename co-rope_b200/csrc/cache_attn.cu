@@ -27,6 +27,10 @@ namespace cg = cooperative_groups;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kPiece = 16;                    // slots per step of a warp; a block of the cache holds a whole number of them
 constexpr int kUnit = kWarps * kPiece, kUnitLog2 = log2_of(kUnit);        // slots per unit of work
+// Tensor cores truncate where they add to their sums, by up to 2^-23 of the sum in each step, and always towards 0.  So the sums of a block's units of an
+// item are added in fp32 after this many of them (a step each; 2^-13 of the result at most).  With one sum for all of 2^20 slots fp16 results came out
+// 1.8e-3 too small.
+constexpr int kMostUnits = 1024;
 // Units that an item counts beside its own in sharing out the work.  With 8 rows 0 / 4 / 6 / 12, us, 32 / 8 heads of 128: 64 x up to 4096 tokens 68.1 / 62.6 /
 // 60.5 / 63.1, 256 x up to 1000 97.6 / 80.3 / 80.6 / 81.8, 8 x 16384 58.0 / 56.4 / 56.5 / 57.6.
 // Two more for each further eight rows: 6 / 8 with 16 rows, 16 x up to 4000 tokens and their weights, 45.4 / 43.7; 6 / 12 / 20 with 32 rows, 64 x up to
@@ -151,6 +155,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 
     auto load = [&](int b) { return load_of(p, kRowsLog2, kUnitLog2, kItemCost, b, bad); };
     __shared__ int nan_v;   // NaN in V where some rows must not see it
+    // The block's share of the item at work: its first unit, whether sums of earlier units wait in the block's part, and whether units are still to come.
+    // (Not in registers, of which there are none left.)
+    __shared__ int share0, carried, more;
+    if (p.parts == 0 && threadIdx.x == 0) more = 0;
     // Either a range of the batch's units, or (p.parts) this block's share of one item, whose other shares are with the blocks of its cluster.
     int b, part_of = 0, cluster_item = 0;
     int64_t off = 0, left = 0;   // position in sequence b's units, units left
@@ -186,6 +194,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
 
     do {
         int h, tile, u0, u1;
+        bool goes_on = false;
         if (p.parts == 0) {
             while (off >= (int64_t)l.cost * l.items) {
                 off -= (int64_t)l.cost * l.items;
@@ -195,9 +204,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             h = item / tiles;
             tile = item % tiles + first_tile(p, kRowsLog2, l.len, l.n);
             u0 = (int)(off - (int64_t)item * l.cost);
-            u1 = (int)min((int64_t)l.cost, u0 + left);
+            const int end = (int)min((int64_t)l.cost, u0 + left);
+            u1 = min(end, max(u0, kItemCost) + kMostUnits);
             off += u1 - u0;
             left -= u1 - u0;
+            goes_on = u1 < end;
             u0 = max(u0 - kItemCost, 0);
             u1 -= kItemCost;
             if (u1 <= 0) continue;   // the range ends before the item's first unit
@@ -213,7 +224,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
         // slots below least_seen are seen by every row of the tile (rows without a query see what they like)
         const int least_seen = p.causal ? len - n + row0 / p.G + 1 : len;
         __syncthreads();   // the tile before is written out
-        if (threadIdx.x == 0) nan_v = 0;
+        if (threadIdx.x == 0) {
+            nan_v = 0;
+            if (p.parts == 0) {
+                carried = more;
+                more = goes_on;
+                if (!carried) share0 = u0;
+            }
+        }
         // pieces first, first + 4, .. of this warp
         const int first = u0 * kWarps + warp, end = min(u1 * kWarps, (len + kPiece - 1) / kPiece);
         const int count = end > first ? (end - first + kWarps - 1) / kWarps : 0;
@@ -237,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                 const uint8_t* kb = k_lane + (uint64_t)page * k_block + (uint64_t)in_block * k_row;
                 const uint8_t* vb = v_lane + (uint64_t)page * v_block + (uint64_t)in_block * v_row;
                 const uint32_t other = fill ^ 64;
-                if (found && rows >= kPiece && p.rows_packed) {
+                if (found && rows >= kPiece && p.rows_packed && !bad) {
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i) {
                         copy16_async((i % 2 ? other : fill) + 512 * i, kb + i * 512);
@@ -250,9 +268,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
                         copy16_async((i % 2 ? other : fill) + 512 * i, real ? kb + (uint64_t)(i * kCopyRows) * k_row : p.c.k, real);
                         copy16_async((i % 2 ? other : fill) + 512 * i + kPiece * D, real ? vb + (uint64_t)(i * kCopyRows) * v_row : p.c.v, real);
                     }
+                    bad |= !found;
+                    if (lane == 2) my_meta[j % kStages * 4 + 2] = found ? 1.f : 0.f;   // (1 before the first bad one)
                 }
-                bad |= !found;
-                if (bad && lane == 2) my_meta[j % kStages * 4 + 2] = found ? 1.f : 0.f;   // (1 before the first bad one)
                 if (lane < 2) copy4_async(fill_meta, scale_lane + (uint64_t)page * (uint32_t)p.c.Hkv);
             }
             commit_copies();
@@ -494,8 +512,21 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             store4(p.o, (int64_t)b * p.so.b + (int64_t)(h * p.G + row - t * p.G) * p.so.h + (int64_t)t * p.so.n + d, p.dtype, p.vec_o,
                    t >= n || all == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
         };
-        const bool whole = u0 == 0 && u1 == l.units;
-        const int64_t part = 2 * (int64_t)blockIdx.x + (u0 == 0 ? 1 : 0);
+        bool whole = false, add = false;   // the block has all of the item; its part holds sums to be added
+        int64_t part = 0;
+        if (p.parts == 0) {
+            whole = share0 == 0 && u1 == l.units;
+            add = carried != 0;
+            part = 2 * (int64_t)blockIdx.x + (share0 == 0 ? 1 : 0);
+            if (add) {
+                if (threadIdx.x < kRows) {
+                    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (part * kRows + threadIdx.x) * 2);
+                    part_max[threadIdx.x] = ml.x;
+                    part_sum[threadIdx.x] = ml.y;
+                }
+                __syncthreads();
+            }
+        }
         for (int x = threadIdx.x; x < kRows * (D / 4); x += kThreads) {
             const int r = x / (D / 4), d = x % (D / 4) * 4, row = row0 + r, t = row / p.G;
             float top = warp_max[r], all = 0.f;
@@ -525,7 +556,16 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kBlocks) cache_attn_ke
             if (p.parts != 0) {   // for the cluster: in the place of warp 0's sums
                 *reinterpret_cast<float4*>(join + r * D + d) = y;
                 if (d == 0) part_max[r] = top, part_sum[r] = all;
-            } else if (!whole) {
+                continue;
+            }
+            if (add) {   // (this thread has written them)
+                const float best = fmaxf(top, part_max[r]), now = fast_exp2(top - best), then = fast_exp2(part_max[r] - best);
+                const float4 was = *reinterpret_cast<const float4*>(p.part + (part * kRows + r) * D + d);
+                y = make_float4(fmaf(was.x, then, y.x * now), fmaf(was.y, then, y.y * now), fmaf(was.z, then, y.z * now), fmaf(was.w, then, y.w * now));
+                all = fmaf(part_sum[r], then, all * now);
+                top = best;
+            }
+            if (!whole) {
                 *reinterpret_cast<float4*>(p.part + (part * kRows + r) * D + d) = y;
                 if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (part * kRows + r) * 2) = make_float2(top, all);
             } else if (t < p.T) {

@@ -53,7 +53,13 @@ static_assert(sizeof(UnitNote) % 16 == 0 && offsetof(UnitNote, k_scale) % 16 == 
 // A piece: units [u0, u0 + count) of the item.  b < 0: there is none any more.
 struct PieceNote {
     int b, h, tile, u0, count, len, n, whole;
+    int seen;           // slots below this are seen by every row
+    int share0;         // the block's first unit of the item
+    int carried, more;  // the sums of the block's earlier units of the item wait in its part; units are still to come
 };
+// Units of a piece at most: tensor cores truncate where they add to their sums (see the kernel for few rows), 8 steps a unit, so longer shares of an item are
+// added piece by piece in fp32.  With one sum for 2^17 / 2^20 slots fp16 results came out 8e-4 / 8e-3 too small.  (Without PAIR a piece has two sums.)
+__host__ __device__ constexpr int most_units(bool pair) { return pair ? 128 : 256; }
 struct alignas(16) Small {
     UnitNote units[kUnitSlots];
     PieceNote pieces[kPieceSlots];
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                     const PieceNote& x = z.pieces[slot];
                     if (x.b < 0) break;
                     const int64_t item = (int64_t)(x.b * p.c.Hkv + x.h) * p.row_tiles + x.tile;
-                    const bool some = x.count > 0;
+                    const bool some = x.count > 0 && !x.carried;   // (the tile of a piece that goes on is there)
                     mbar_arrive(&bars[PIECE_EMPTY + slot]);
                     if (!some) continue;
                     if (n > 0 && !mbar_wait(&bars[Q_EMPTY], (n - 1) & 1, p.status, Q_EMPTY, abort_flag)) break;
@@ -291,16 +297,17 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 for (int kk = 0; kk < kN / 16; ++kk)
                     if (leader) umma_ts2(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b0 + kk * (2048 >> 4), kHi, idesc_pv, (add || kk > 0) ? 1u : 0u);
             };
-            int gk = 0, gv = 0, pieces = 0, done0 = 0, done1 = 0;
+            int gk = 0, gv = 0, pieces = 0, query_tiles = 0, done0 = 0, done1 = 0;
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 const int slot = k % kPieceSlots;
                 if (!(ok = mbar_wait_warp(&bars[PIECE_FULL + slot], (k / kPieceSlots) & 1, p.status, PIECE_FULL, abort_flag))) break;
                 const int count = z.pieces[slot].b < 0 ? -1 : z.pieces[slot].count;
+                const bool new_tile = !z.pieces[slot].carried, last_use = !z.pieces[slot].more;
                 mbar_arrive_warp(&bars[PIECE_EMPTY + slot], lane);
                 if (count < 0) break;
                 if (count == 0) continue;
-                if (!(ok = mbar_wait_warp(&bars[Q_FULL], pieces & 1, p.status, Q_FULL, abort_flag))) break;
+                if (new_tile && !(ok = mbar_wait_warp(&bars[Q_FULL], query_tiles++ & 1, p.status, Q_FULL, abort_flag))) break;
                 if constexpr (PAIR) {
                     // PV0(j) QK0(j + 1) | PV1(j) QK1(j + 1); j = -1 forms the scores of unit 0
                     for (int j = -1; ok && j < count; ++j) {
@@ -331,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                                 if (leader) umma_commit(&bars[S_FULL + i]);
                                 if (i == 1) {
                                     if (leader) umma_commit(&bars[K_EMPTY + stage]);
-                                    if (j + 2 == count && leader) umma_commit(&bars[Q_EMPTY]);
+                                    if (j + 2 == count && last_use && leader) umma_commit(&bars[Q_EMPTY]);
                                     ++gk;
                                 }
                             }
@@ -345,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                         if (leader) {
                             umma_commit(&bars[S_FULL + (j & 1)]);
                             umma_commit(&bars[K_EMPTY + gk % kStages]);
-                            if (j + 1 == count) umma_commit(&bars[Q_EMPTY]);
+                            if (j + 1 == count && last_use) umma_commit(&bars[Q_EMPTY]);
                         }
                         ++gk;
                     };
@@ -380,6 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             Range r = range;
             Load l = load_of(p, log2_of(kItemRows), log2_of(kN), kTileItemCost, r.b, bad);
             int q = 0, told = 0, pieces = 0;   // units, pieces, pieces with units so far
+            int share0 = 0, carried = 0;
             bool ok = true;
             const int bs_mask = (1 << p.c.bs_log2) - 1;
             // A note may be written over when the converters are through with a unit three later than its own: then its product is issued, and the
@@ -390,26 +398,33 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             while (ok) {
                 const int slot = told % kPieceSlots;
                 if (told >= kPieceSlots && !(ok = mbar_wait_warp(&bars[PIECE_EMPTY + slot], ((told / kPieceSlots) - 1) & 1, p.status, PIECE_EMPTY, abort_flag))) break;
-                PieceNote x{-1, 0, 0, 0, 0, 0, 0, 0};
-                int seen = 0;
+                PieceNote x{-1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
                 while (r.left > 0 && x.b < 0) {
                     while (r.off >= (int64_t)l.cost * l.items) {
                         r.off -= (int64_t)l.cost * l.items;
                         l = load_of(p, log2_of(kItemRows), log2_of(kN), kTileItemCost, ++r.b, bad);
                     }
                     const int item = (int)(r.off / l.cost), tiles = l.items / p.c.Hkv;
-                    const int at = (int)(r.off - (int64_t)item * l.cost), end = (int)min((int64_t)l.cost, at + r.left);
-                    r.off += end - at;
-                    r.left -= end - at;
-                    const int u1 = end - kTileItemCost;
-                    if (u1 <= 0) continue;   // the range ends before the item's first unit
-                    x.b = r.b; x.h = item / tiles; x.tile = item - x.h * tiles + first_tile(p, log2_of(kItemRows), l.len, l.n); x.len = l.len; x.n = l.n;
-                    x.u0 = max(at - kTileItemCost, 0);
+                    x.h = item / tiles; x.tile = item - x.h * tiles + first_tile(p, log2_of(kItemRows), l.len, l.n); x.len = l.len; x.n = l.n;
                     const int last = min(l.n - 1, (x.tile * kItemRows + kItemRows - 1) / p.G);   // the item's last query
                     const int most = p.causal ? max(l.len - l.n + last + 1, 0) : l.len;   // slots that some row sees
-                    x.count = max(min((most + kN - 1) / kN, u1) - x.u0, 0);
-                    x.whole = x.u0 == 0 && u1 == l.units;
-                    seen = p.causal ? l.len - l.n + x.tile * kItemRows / p.G + 1 : l.len;   // slots below this are seen by every row
+                    const int seen_units = (most + kN - 1) / kN;
+                    const int at = (int)(r.off - (int64_t)item * l.cost), end = (int)min((int64_t)l.cost, at + r.left);
+                    int stop = min(end, max(at, kTileItemCost) + most_units(PAIR));
+                    if (stop - kTileItemCost >= seen_units) stop = end;   // the rest is hidden from all rows: no piece of its own
+                    r.off += stop - at;
+                    r.left -= stop - at;
+                    const int u1 = stop - kTileItemCost;
+                    if (u1 <= 0) continue;   // the range ends before the item's first unit
+                    x.b = r.b;
+                    x.u0 = max(at - kTileItemCost, 0);
+                    x.count = max(min(seen_units, u1) - x.u0, 0);
+                    x.carried = carried;
+                    x.more = carried = stop < end;
+                    if (!x.carried) share0 = x.u0;
+                    x.share0 = share0;
+                    x.whole = share0 == 0 && u1 == l.units;
+                    x.seen = p.causal ? max(l.len - l.n + x.tile * kItemRows / p.G + 1, 0) : l.len;
                 }
                 if (lane == 0) z.pieces[slot] = x;
                 mbar_arrive_warp(&bars[PIECE_FULL + slot], lane);
@@ -431,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                         note.lift[lane] = page >= 0 ? __log2f(size) : -INFINITY;     // slots of a block that is not there count nothing
                         note.drop[lane] = 1.f / size;
                         const bool full = __all_sync(0xffu, rows == 16 && !no_values(vs));
-                        if (lane == 0) note.piece = pieces, note.hidden = (u + 1) * kN > seen, note.full = full;
+                        if (lane == 0) note.piece = pieces, note.hidden = (u + 1) * kN > x.seen, note.full = full;
                     }
                     mbar_arrive_warp(&bars[UNIT_FULL + q % kUnitSlots], lane);
                 }
@@ -651,6 +666,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
             ends1 += count / 2;
 
             // The piece's sums.  PAIR: the group's O, half of the columns to each warpgroup.  Else both groups' O, a quarter of them to each.
+            const int64_t part = (2 * (int64_t)blockIdx.x + (x.share0 == 0 ? 1 : 0)) * kItemRows + item_row;
+            // what waits in the block's part: read before the barrier, as one thread of the row writes it again behind it
+            const bool carried = x.carried != 0;
+            const float2 had = carried ? *reinterpret_cast<const float2*>(p.part_ml + part * 2) : make_float2(kLowest, 0.f);
             if (half == 0) z.end_max[grp][row] = m;
             z.end_sum[grp][half][row] = l;
             named_bar_sync(9, 512);   // (the exchange is written again behind the next piece's first barrier at the earliest)
@@ -661,19 +680,18 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                 if (count > 1) wait(O_FULL + 1, (ends1 - 1) & 1);
             }
             const int other = PAIR ? grp : 0;
-            const float m0 = PAIR ? m : z.end_max[0][row], m1 = PAIR ? kLowest : z.end_max[1][row], top = fmaxf(m0, m1);
-            const float w0 = PAIR ? 1.f : fast_exp2(m0 - top), w1 = fast_exp2(m1 - top);
+            const bool whole = x.whole != 0;
+            const float m0 = PAIR ? m : z.end_max[0][row], m1 = PAIR ? kLowest : z.end_max[1][row], top = fmaxf(fmaxf(m0, m1), had.x);
+            const float w0 = fast_exp2(m0 - top), w1 = fast_exp2(m1 - top), w_old = fast_exp2(had.x - top);
             const float own = z.end_sum[other][0][row] + z.end_sum[other][1][row];
-            const float all = PAIR ? own : own * w0 + (z.end_sum[1][0][row] + z.end_sum[1][1][row]) * w1;
-            const bool whole = x.whole != 0, some = t < x.n && all != 0.f;
+            const float all = fmaf(had.y, w_old, PAIR ? own * w0 : own * w0 + (z.end_sum[1][0][row] + z.end_sum[1][1][row]) * w1);
+            const bool some = t < x.n && all != 0.f;
             const float inv = whole ? 1.f / all : 1.f;
             constexpr int kCols = PAIR ? kD / 2 : kD / 4;
             const int col0 = (PAIR ? half : grp * 2 + half) * kCols;
             const uint32_t tO0 = tO + other * 128;
-            const int64_t part = (2 * (int64_t)blockIdx.x + (u0 == 0 ? 1 : 0)) * kItemRows + item_row;
             const int64_t to = (int64_t)x.b * p.so.b + (int64_t)(x.h * p.G + grow - t * p.G) * p.so.h + (int64_t)t * p.so.n;
             const bool fix = CODE == COROPE_CODE_E4M3 && count > 0 && z.nan_v[pieces % kFlagSlots] != 0;
-            const int seen = p.causal ? max(x.len - x.n + x.tile * kItemRows / p.G + 1, 0) : x.len;   // as the scout's: NaN is left out of units that reach beyond
 #pragma unroll
             for (int k = 0; k < kCols; k += 16) {
                 float y[16];
@@ -693,9 +711,16 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tile_kernel(const Cach
                     }
                 }
                 if (col0 + k >= D) continue;
+                if (carried) {   // (this thread has written them)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 was = *reinterpret_cast<const float4*>(p.part + part * D + col0 + k + i);
+                        y[i] = fmaf(was.x, w_old, y[i]); y[i + 1] = fmaf(was.y, w_old, y[i + 1]); y[i + 2] = fmaf(was.z, w_old, y[i + 2]); y[i + 3] = fmaf(was.w, w_old, y[i + 3]);
+                    }
+                }
                 if (fix) {   // NaN in V, slot by slot: to the rows that see it
 #pragma unroll 1
-                    for (int s = max(u0, seen / kN) * kN; s < (t < x.n ? min(sees, (u0 + count) * kN) : 0); ++s) {   // (never behind the last slot, whose block the table still has)
+                    for (int s = max(u0, x.seen / kN) * kN; s < (t < x.n ? min(sees, (u0 + count) * kN) : 0); ++s) {   // (never behind the last slot, whose block the table still has)
                         bool far = false;
                         const int page = cache_page(p.s, p.c.bs_log2, p.c.num_blocks, x.b, s, far);
                         if (page < 0 || no_values(p.c.v_scale[(int64_t)page * p.c.Hkv + x.h])) continue;

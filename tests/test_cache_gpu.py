@@ -245,6 +245,74 @@ def test_queries_that_overlap(T, dtype, strides):
     check_attention(cache, host, q.contiguous(), table, lens, True, 0.2, q_gpu=row.cuda().as_strided((B, Hq, T, D), strides))
 
 
+def shared_context(B, S, D, code, bs=256):
+    """A cache of one sequence of S tokens that B sequences read, with their table."""
+    cache, host = make_cache(S // bs, 1, bs, D, code)
+    return cache, host, torch.arange(S // bs, dtype=torch.int32)[None].expand(B, -1).contiguous()
+
+
+def long_attention(host, q, rows, length, causal, sm_scale):
+    """(o, bulk, slack) as the oracle's, of rows `rows` of one sequence's q [Hq, T, D] over the first `length` tokens of the one K / V head, in 64 bits on the GPU."""
+    k, v = ((host[x].view(torch.uint8).cuda().view(host[x].dtype).double() * host[x + "_scale"].cuda().double()[:, :, None, None])[:, 0].flatten(0, 1)[:length] for x in ("k", "v"))
+    T, q = q.shape[1], q[:, rows].double()
+    sees = torch.tensor([length - T + t + 1 if causal else length for t in rows], device="cuda")[:, None]
+    hidden = torch.arange(length, device="cuda") >= sees
+    p = torch.softmax((q @ k.T * sm_scale).masked_fill(hidden, float("-inf")), dim=-1).nan_to_num(0.0)
+    return p @ v, p @ v.abs(), (q.abs() @ k.abs().T * sm_scale).masked_fill(hidden, 0.0).amax(dim=-1, keepdim=True)
+
+
+@pytest.mark.parametrize("B,G,T,dtype,S,causal", [
+    (600, 1, 1, F16, 2 ** 20, False), (600, 1, 1, BF16, 2 ** 20, False), (150, 2, 64, F16, 2 ** 19, False), (150, 1, 33, F16, 2 ** 19, True), (150, 2, 65, BF16, 2 ** 19, True),
+])
+def test_long_sums_are_not_truncated(B, G, T, dtype, S, causal):
+    """Values of one sign and equal weights over a context that one block of threads goes through: rounding errors of single results go up and down,
+    so the mean of many shows what is lost in adding.  Allowed are 2^-13 (1024 additions that truncate by up to 2^-23 each, at all lengths) and for the mean
+    of over 64 roundings by up to eps / 2 each five of its standard deviations, 5 * eps / 2 / sqrt(3 * 64) < 0.37 * eps / 2."""
+    D = 64
+    cache, host, table = shared_context(B, S, D, INT8)
+    gen = torch.Generator().manual_seed(7)
+    host["v"] = torch.randint(64, 128, host["v"].shape, generator=gen, dtype=torch.int8)
+    host["v_scale"] = torch.full_like(host["v_scale"], 1 / 127)
+    cache.v.copy_(host["v"].cuda())
+    cache.v_scale.copy_(host["v_scale"].cuda())
+    q = (draw((B, G, T, D), 1, F32) / 100).to(dtype).cuda()
+    got = pkg.cache_attention(q, cache, table.cuda(), torch.full((B,), S, dtype=torch.int32, device="cuda"), causal, 0.1)
+    pkg.check_status()
+    for b in (0, B // 2, B - 1):
+        o, _, _ = long_attention(host, q[b], [T - 1], S, causal, 0.1)
+        off = ((got[b, :, -1:].double() - o) / o).mean().abs()
+        assert off < 2.0 ** -13 + 0.37 * torch.finfo(dtype).eps / 2, off
+
+
+@pytest.mark.parametrize("B,G,T,D,dtype,code,most,causal", [
+    (700, 2, 1, 64, F16, E4M3, 150000, True), (700, 1, 3, 32, F32, INT8, 140000, True), (160, 5, 4, 32, BF16, E4M3, 700000, False), (300, 4, 8, 32, F32, INT8, 150000, True),
+    (160, 1, 64, 32, F16, INT8, 60000, True), (160, 1, 140, 64, BF16, E4M3, 50000, True), (150, 2, 200, 32, F16, E4M3, 60000, True), (160, 1, 40, 128, F16, INT8, 50000, False),
+    (40, 1, 3000, 32, BF16, INT8, 40000, True),
+])
+def test_shares_in_several_pieces(B, G, T, D, dtype, code, most, causal):
+    """Blocks of threads that go through more of an item than is added in one sum: whole items, ends, beginnings and middles of them."""
+    S = -(-most // 256) * 256
+    cache, host, table = shared_context(B, S, D, code)
+    lens = torch.randint(most // 2, most + 1, (B,), generator=torch.Generator().manual_seed(B + T), dtype=torch.int32)
+    lens[0], lens[1], lens[-1] = most, 5, most - 300
+    q = draw((B, G, T, D), 1, dtype).cuda()
+    cache.weight.zero_()
+    accumulate = T <= 4
+    got = pkg.cache_attention(q, cache, *gpu(table, lens), causal, 0.2, accumulate=accumulate)
+    pkg.check_status()
+    one_part = dtype == BF16 and not accumulate and G * T > 32
+    # beside the usual: 1024 truncating additions, or (fp32) 2^12 that round, which go up and down: 5 * 2^-24 * sqrt(2^12 / 3) < 2^-16
+    adding = 2.0 ** -16 if dtype == F32 else 2.0 ** -13
+    for b in [0, 1, B - 1] + list(range(2, B - 1, max(B // 9, 1))):
+        rows = sorted({0, T // 2, T - 1})
+        o, bulk, slack = long_attention(host, q[b], rows, int(lens[b]), causal, 0.2)
+        x = got[b][:, rows].double()
+        assert not ((x - o).abs() > tolerance(dtype, o, bulk, slack, one_part) + adding * bulk).any() and not x.isnan().any(), b
+    if accumulate:   # every row that sees something has probabilities of 1 in all; 2^-10 of it covers 2 * 2^-17 of a score of below 60
+        rows = sum(min(T, int(n)) if causal else T for n in lens) * G
+        assert abs(cache.weight.double().sum().item() / rows - 1) < 2.0 ** -10
+
+
 @pytest.mark.parametrize("dtype,T,G", [(BF16, 1, 4), (F32, 1, 4), (F16, 100, 4)])
 def test_attention_extremes(dtype, T, G):
     """Scores of some hundred (one slot has all the weight), equal scores, blocks whose scales differ by 2^20, scales of 0."""
