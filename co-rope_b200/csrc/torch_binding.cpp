@@ -361,8 +361,10 @@ void require_shape(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, 
 }
 // no gradient flows through the cache, backwards or forwards: a caller who expects one learns it here
 void require_no_grad(std::initializer_list<const Tensor*> ts, const CacheTensors& c) {
-    auto check = [](const Tensor& t) {
-        if (at::GradMode::is_enabled() && t.requires_grad())
+    const bool grad_mode = at::GradMode::is_enabled();
+    auto check = [grad_mode](const Tensor& t) {
+        if (t.unsafeGetTensorImpl()->autograd_meta() == nullptr) return;   // neither
+        if (grad_mode && t.requires_grad())
             throw std::runtime_error("corope_b200: the cache operators have no backward pass; call them under torch.no_grad()");
         if (t._fw_grad(0).defined()) throw std::runtime_error("corope_b200: the cache operators have no derivatives; a tensor of the call is a forward-mode dual");
     };
