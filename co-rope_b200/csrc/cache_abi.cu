@@ -14,7 +14,10 @@ bool cache_rows_ok(const void* ptr, const Strides& st, int D) {
            st.b < (1ll << 32) && st.n < (1ll << 32);   // (strides are 32-bit numbers in the kernels)
 }
 
-int view_of(CacheView& v, const corope_kv_cache_t* c) {
+// blocks and heads have codes of their own, as who writes them needs
+bool cache_rows_apart(const corope_kv_cache_t* c, const int64_t* st) { return (c->num_blocks == 1 || st[0] > 0) && (c->Hkv == 1 || st[1] > 0); }
+
+int view_of(CacheView& v, const corope_kv_cache_t* c, bool written) {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return COROPE_ERR_NULL_POINTER;
     if (c->num_blocks <= 0 || c->Hkv <= 0) return COROPE_ERR_BAD_SHAPE;
     if (c->D != 32 && c->D != 64 && c->D != 128) return COROPE_ERR_BAD_HEAD_DIM;
@@ -27,6 +30,7 @@ int view_of(CacheView& v, const corope_kv_cache_t* c) {
     v.sk = bytes_of(c->k_stride); v.sv = bytes_of(c->v_stride);
     v.num_blocks = c->num_blocks; v.Hkv = c->Hkv; v.bs_log2 = log2;
     if (!cache_rows_ok(c->k, v.sk, c->D) || !cache_rows_ok(c->v, v.sv, c->D)) return COROPE_ERR_BAD_CACHE;
+    if (written && !(cache_rows_apart(c, c->k_stride) && cache_rows_apart(c, c->v_stride))) return COROPE_ERR_BAD_CACHE;
     return COROPE_OK;
 }
 
@@ -66,7 +70,7 @@ int corope_cache_append(const corope_kv_cache_t* cache, const corope_cache_seqs_
                         const int64_t v_strides[3], int T, int dtype, int* status_word, void* stream) {
     if (!k || !v || !k_strides || !v_strides) return COROPE_ERR_NULL_POINTER;
     CacheAppendParams p{};
-    if (int e = view_of(p.c, cache)) return e;
+    if (int e = view_of(p.c, cache, true)) return e;
     if (int e = view_of(p.s, seqs, p.c, cache->D)) return e;
     if (int e = tokens_ok(T)) return e;
     if (!dtype_ok(dtype)) return COROPE_ERR_BAD_DTYPE;
@@ -79,7 +83,7 @@ int corope_cache_append(const corope_kv_cache_t* cache, const corope_cache_seqs_
 
 size_t corope_cache_attn_workspace_bytes(const corope_kv_cache_t* cache, const corope_cache_seqs_t* seqs, int Hq, int T, int dtype, int accumulate) {
     CacheAttnParams p{};
-    if (view_of(p.c, cache) || view_of(p.s, seqs, p.c, cache->D) || attn_sizes(cache, seqs, Hq, T)) return 0;
+    if (view_of(p.c, cache, false) || view_of(p.s, seqs, p.c, cache->D) || attn_sizes(cache, seqs, Hq, T)) return 0;
     return cache_attn_workspace_bytes(seqs->B, cache->Hkv, Hq / cache->Hkv, T, cache->D, seqs->max_blocks, cache->block_size, dtype, accumulate);
 }
 
@@ -88,7 +92,7 @@ int corope_cache_attn(const corope_kv_cache_t* cache, const corope_cache_seqs_t*
                       size_t workspace_bytes, int* status_word, void* stream) {
     if (!q || !o || !q_strides || !o_strides) return COROPE_ERR_NULL_POINTER;
     CacheAttnParams p{};
-    if (int e = view_of(p.c, cache)) return e;
+    if (int e = view_of(p.c, cache, false)) return e;
     if (int e = view_of(p.s, seqs, p.c, cache->D)) return e;
     if (int e = attn_sizes(cache, seqs, Hq, T)) return e;
     if (!dtype_ok(dtype)) return COROPE_ERR_BAD_DTYPE;
@@ -108,7 +112,7 @@ int corope_cache_evict(const corope_kv_cache_t* cache, const corope_cache_seqs_t
                        int budget, int recent, int* new_lens, int* kept, int* status_word, void* stream) {
     if (!out_table || !new_lens || !kept) return COROPE_ERR_NULL_POINTER;
     CacheEvictParams p{};
-    if (int e = view_of(p.c, cache)) return e;
+    if (int e = view_of(p.c, cache, true)) return e;
     if (int e = view_of(p.s, seqs, p.c, cache->D)) return e;
     if (!cache->weight) return COROPE_ERR_NULL_POINTER;
     if (budget <= 0 || recent < 0 || recent > budget) return COROPE_ERR_BAD_SHAPE;

@@ -382,7 +382,7 @@ void whole_cache_written(const CacheTensors& c) {
     if (c.weight.has_value()) written({&*c.weight});
 }
 
-corope_kv_cache_t cache_view(const CacheTensors& c) {
+corope_kv_cache_t cache_view(const CacheTensors& c, bool written) {
     for (const Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale}) require_cuda(*t);
     require_value(c.k.dim() == 4 && c.k.sizes() == c.v.sizes() && c.k.scalar_type() == c.v.scalar_type() && c.k.device() == c.v.device(),
                   "cache.k and cache.v must be [num_blocks, Hkv, block_size, D] tensors of one shape, type and device");
@@ -405,6 +405,7 @@ corope_kv_cache_t cache_view(const CacheTensors& c) {
         bool ok = st[3] == 1 && st[2] >= D && (uintptr_t)t->data_ptr() % 16 == 0;
         for (int i = 0; i < 3; ++i) ok = ok && st[i] >= 0 && st[i] % 16 == 0;
         require_value(ok, "rows of cache.k and cache.v must be contiguous and start at multiples of 16 bytes");
+        require_value(!written || ((N == 1 || st[0] > 0) && (H == 1 || st[1] > 0)), "blocks and heads of cache.k and cache.v that are written to must not share memory");
     }
     r.k = c.k.data_ptr(); r.v = c.v.data_ptr();
     r.k_scale = c.k_scale.data_ptr<float>(); r.v_scale = c.v_scale.data_ptr<float>();
@@ -464,7 +465,7 @@ void check_tokens(const Tensor& t, const CacheTensors& c, int64_t B, const char*
 void cache_append(const Tensor& k_in, const Tensor& v_in, const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, const Optional& cos,
                   const Optional& sin, const Optional& positions, const Optional& new_lens) {
     require_no_grad({&k_in, &v_in}, c);
-    const corope_kv_cache_t cache = cache_view(c);
+    const corope_kv_cache_t cache = cache_view(c, true);
     Call call(c.k);
     Tables keep;
     const corope_cache_seqs_t seqs = seqs_view(c, block_table, seq_lens, cos, sin, positions, new_lens, keep);
@@ -483,7 +484,7 @@ void cache_append(const Tensor& k_in, const Tensor& v_in, const CacheTensors& c,
 Tensor cache_attention(const Tensor& q_in, const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, bool causal, double sm_scale,
                        const Optional& cos, const Optional& sin, const Optional& positions, const Optional& new_lens, bool accumulate) {
     require_no_grad({&q_in}, c);
-    const corope_kv_cache_t cache = cache_view(c);
+    const corope_kv_cache_t cache = cache_view(c, false);
     Call call(c.k);
     Tables keep;
     const corope_cache_seqs_t seqs = seqs_view(c, block_table, seq_lens, cos, sin, positions, new_lens, keep);
@@ -511,7 +512,7 @@ Tensor cache_attention(const Tensor& q_in, const CacheTensors& c, const Tensor& 
 std::tuple<Tensor, Tensor> cache_evict(const CacheTensors& c, const Tensor& block_table, const Tensor& seq_lens, const Tensor& out_table, int64_t budget,
                                        int64_t recent) {
     require_no_grad({}, c);
-    const corope_kv_cache_t cache = cache_view(c);
+    const corope_kv_cache_t cache = cache_view(c, true);
     require_value(cache.weight != nullptr, "eviction needs a cache with weights");
     Call call(c.k);
     Tables keep;

@@ -32,7 +32,8 @@ class KVCache:
     """Holds k, v [num_blocks, num_heads, block_size, head_dim] codes (float8_e4m3fn or int8), k_scale, v_scale [num_blocks,
     num_heads] fp32 and, with weights=True, weight [num_blocks, num_heads, block_size] fp32, the attention weight that each
     slot has gathered.  The operators take any object with these attributes (weight may be None), so that a program can
-    keep them as views of its own buffers: rows need 16-byte alignment, the scales and weights have to be contiguous."""
+    keep them as views of its own buffers: rows need 16-byte alignment (and memory of their own where they are written to), the
+    scales and weights have to be contiguous."""
 
     def __init__(self, num_blocks, num_heads, block_size, head_dim, dtype=torch.float8_e4m3fn, device="cuda", weights=False):
         shape = (num_blocks, num_heads, block_size, head_dim)

@@ -309,7 +309,7 @@ typedef struct corope_kv_cache_t {
     void *k, *v;                   /* codes [num_blocks, Hkv, block_size, D], 16-byte aligned */
     float *k_scale, *v_scale;      /* [num_blocks, Hkv] contiguous */
     float* weight;                 /* [num_blocks, Hkv, block_size] contiguous, accumulated attention weight of each slot, or NULL */
-    int64_t k_stride[3], v_stride[3];   /* {block, head, row} in elements, multiples of 16 */
+    int64_t k_stride[3], v_stride[3];   /* {block, head, row} in elements, multiples of 16; 0 for blocks or heads only where nothing is written */
     int num_blocks, Hkv, block_size, D; /* block_size 16, 32, 64, 128 or 256; D 32, 64 or 128 */
     int code;                      /* COROPE_CODE_* */
 } corope_kv_cache_t;

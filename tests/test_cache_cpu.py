@@ -148,6 +148,14 @@ def test_sizes_beyond_32_bits_are_refused():
         assert _append(k_stride=wide) == -12 and _attend(v_stride=wide) == -12 and _evict(k_stride=wide) == -12
 
 
+def test_codes_that_share_memory_are_not_written():
+    for shared in ([0, 1024, 64], [2048, 0, 64]):
+        for name in ("k_stride", "v_stride"):
+            assert _append(**{name: shared}) == -12 and _evict(**{name: shared}) == -12
+            assert _attend(**{name: shared}) == -5      # (reads them; the workspace is missing)
+    assert _append(num_blocks=1, Hkv=1, k_stride=[0, 0, 64], T=0) == -2
+
+
 def test_eviction_order():
     """Largest weights first, lowest slots among equal ones, NaN before everything, the last slots always."""
     bs = 16

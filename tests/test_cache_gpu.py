@@ -924,6 +924,24 @@ def test_refusals():
     pkg.check_status()
 
 
+def test_one_block_read_as_many_heads():
+    """Heads that share their codes are read; append and eviction refuse them."""
+    D, bs, lens = 64, 16, [30]
+    cache, host = make_cache(3, 1, bs, D, INT8)
+    wide = pkg.KVCache(3, 4, bs, D, dtype=INT8, weights=True)
+    for x in ("k", "v", "k_scale", "v_scale"):
+        t = getattr(cache, x).expand((3, 4) + getattr(cache, x).shape[2:])
+        setattr(wide, x, t if x in ("k", "v") else t.contiguous())
+    table, q = ints([[0, 1]]), draw((1, 4, 1, D), 1, F32)
+    got = pkg.cache_attention(q.cuda(), wide, *gpu(table, ints(lens)), True, 0.2)
+    assert torch.equal(got, pkg.cache_attention(q.cuda(), cache, *gpu(table, ints(lens)), True, 0.2))
+    with pytest.raises(ValueError, match="share memory"):
+        pkg.cache_append(q.cuda(), q.cuda(), wide, *gpu(table, ints(lens)))
+    with pytest.raises(ValueError, match="share memory"):
+        pkg.cache_evict(wide, *gpu(table, ints(lens), ints([[2]])), 8)
+    pkg.check_status()
+
+
 def test_budgets_of_32_bits():
     """A table of 2^28 + 1 blocks of 16 has room for a budget beyond 32 bits; 2^32 + 8 is not taken for 8."""
     cache = pkg.KVCache(6, 2, 16, 64, weights=True)
