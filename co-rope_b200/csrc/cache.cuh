@@ -107,7 +107,8 @@ __device__ __forceinline__ uint32_t to_code(float x, float scale) {
     else return (uint32_t)(int)fminf(fmaxf(rintf(y != y ? 0.f : y), -127.f), 127.f) & 0xffu;
 }
 // Four codes of x / scale without a division.  x times a reciprocal is within 4 units of 2^-24 of the fp32 quotient, so it has the quotient's code
-// unless a tie lies that near (one number in 10^4): then, and where the scale has no usable reciprocal, all four are divided.
+// unless a tie lies that near (one number in 10^4 for e4m3; for int8, whose band is 2^-12 of a step on either side, one in 2000, so one call in 500 and
+// one warp in 16): then, and where the scale has no usable reciprocal, all four are divided.
 // `near` = reciprocal(scale); |x| <= (1 + 2^-22) * scale * largest code, or `plain` is false.
 __device__ __forceinline__ float reciprocal(float scale) { return scale > 1e-30f && scale < 1e30f ? __frcp_rn(scale) : __int_as_float(0x7fffffff); }
 template <int CODE>
@@ -127,7 +128,7 @@ __device__ __forceinline__ bool codes4_near(const float (&y)[4], uint32_t& w) {
         const uint32_t lo = (uint32_t)r[0] | (uint32_t)r[2] << 16, hi = (uint32_t)r[1] | (uint32_t)r[3] << 16;
         w = lo;
         return lo == hi;
-    } else {   // rounded by the addition of 1.5 * 2^23, and not within 2^-12 of a tie (2^-24 * 4 * 127 = 2^-15)
+    } else {   // rounded by the addition of 1.5 * 2^23, and not within 2^-12 of a tie (the error is 2^-24 * 4 * 127 = 2^-15 at most)
         float r[4], off = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

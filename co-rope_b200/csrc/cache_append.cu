@@ -1,7 +1,8 @@
 // corope_cache_append: keys rotated, keys and values quantised into the blocks of the 8-bit cache.
 //
 // One thread block per (cache block with new tokens, K / V head): a block's scale is known once all its new rows have been seen, so they wait in
-// registers (two rows a thread where that takes no more than 1024 threads, else four) for the block-wide maxima.  Bound by the reads of k and v.
+// registers (two rows a thread where that takes no more than 1024 threads, else four) for the block-wide maxima.  Bound by instruction issue (62 % of the slots at
+// 4 prompts of up to 4096 tokens, 33 instructions a code), not by the reads of k and v (a third of the time).
 #include "cache.cuh"
 
 namespace corope {

@@ -876,8 +876,11 @@ Layout layout_of(int B, int Hkv, int G, int T, int D, int max_blocks, int block_
     Layout l{};
     const int rows = G * T;
     const uint64_t slots = (uint64_t)max_blocks * block_size;
-    // 16-bit tensors of more than 32 rows a head: products on tcgen05 (a chunk of 1024 queries, 32 / 8 heads, over 9001 tokens: 217 us, 970 with
-    // tiles of 32 rows).  fp32 tensors stay with the kernel that splits P as well.
+    // 16-bit tensors of more than 32 rows a head: products on tcgen05.  This kernel with tiles of 32 rows / tcgen05, us on the GPU, bf16, 32 / 8 heads of
+    // 128, sequences x tokens: 36 rows 1 x 300 18.9 / 22.6, 8 x 1024 33.2 / 33.8, 8 x 4096 68 / 52, 64 x 4096 416 / 275; 64 rows 1 x 1024 20.0 / 23.7,
+    // 8 x 300 25.5 / 28.7, 64 x 300 103 / 95.5; 256 rows 1 x 300 22.4 / 25.9, 1 x 4096 44 / 34.5, 8 x 1024 89 / 50; 1024 rows 1 x 300 35.7 / 34.4,
+    // 8 x 4096 866 / 236.  With weights 64 rows 8 x 1024 80 / 56.5.  So calls of little work lose up to 5 us by the rule: what they would take depends on
+    // lengths that the host does not know.  fp32 tensors stay with the kernel that splits P as well.
     l.tiles = dtype != COROPE_DTYPE_F32 && rows > 32;
     // one part of q is off by 2^-12 of it: next to a bf16 result's 2^-9 that is nothing, an fp16 result or a weight would feel it
     l.two_parts = l.tiles && (dtype == COROPE_DTYPE_F16 || accumulate);

@@ -1,8 +1,8 @@
 // corope_cache_attn for many query rows a K / V head (R = G * T > 32, 16-bit types): tcgen05 MMAs on codes turned into fp16 in shared memory.
 //
 // A unit of work is 128 query rows by 128 slots; a block per SM takes a contiguous range of a batch's units (see cache_attn.cuh) and walks it
-// piece by piece, a piece being units of one tile of rows.  Warp roles (896 threads, registers divided again with setmaxnreg):
-//   warp 0        brings a piece's query tile (an image of its place in shared memory that a pre-pass has written) with bulk copies
+// piece by piece, a piece being units of one tile of rows (a long share of an item is several pieces, see most_units).  Warp roles (896 threads, registers divided again with setmaxnreg):
+//   warp 0        brings the query tile of an item's first piece (an image of its place in shared memory that a pre-pass has written) with bulk copies
 //   warp 2        MMA issuer and TMEM owner
 //   warp 3        scout: walks the range ahead of the others and tells them the pieces, and of each unit the addresses of its codes and their scales
 //   warps 4-7     K: 16 codes a lane and step turned into fp16 (exact) and stored as the MMA wants them;  warps 8-11: V likewise
@@ -15,7 +15,8 @@
 // exponent: P = exp2(s + log2 v_scale - M), and its sum is taken back to probabilities by the same number.
 // Queries are scaled by a power of two per row and rounded to fp16 (11 bits); with two parts (fp16 tensors, and where weights are gathered) the
 // remainder of the rounding is a second operand and scores have 22 bits.
-// Bound by the exponentials (16 a clock and SM: 1024 clocks a unit at least) and, next to that, by the MMAs (2 * 128^3 * 2 operations, 3 with two parts).
+// Bound by the chain scores ready -> exponentials -> P ready -> P V and the next Q K^T of a tile, as P stands over S: a unit of 256 x 128 takes 5300 cycles,
+// of which the exponentials (16 a clock and SM) and the MMAs have 2048 each (XU and tensor pipe at 37 %, 1024 queries over 9001 tokens).
 #include <cstddef>
 
 #include "cache_attn.cuh"

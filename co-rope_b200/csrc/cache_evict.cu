@@ -25,7 +25,7 @@ __device__ __forceinline__ uint32_t ordered(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the threads before this one, and over all; `words`: 33 words, not in use by an earlier call that a thread may still be in.
+// Sum over the threads before this one, and over all; `words`: 32 words, not in use by an earlier call that a thread may still be in.
 __device__ __forceinline__ unsigned sum_before(unsigned x, unsigned* words, unsigned& all) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     unsigned up = x;
@@ -51,7 +51,7 @@ __device__ __forceinline__ unsigned sum_before(unsigned x, unsigned* words, unsi
 __global__ void __launch_bounds__(kSelectThreads, 1) cache_select_kernel(const CacheEvictParams p, int parts, int held) {
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ unsigned counts[3][kBins];
-    __shared__ unsigned words[6][32];
+    __shared__ unsigned words[5][32];   // of the three rounds, and of the two sums behind them
     __shared__ unsigned chosen[3], above[3], found[2];
     cg::cluster_group cluster = cg::this_cluster();
     const int part = (int)(blockIdx.x % (unsigned)parts), item = (int)(blockIdx.x / (unsigned)parts), b = item / p.c.Hkv, h = item - b * p.c.Hkv;

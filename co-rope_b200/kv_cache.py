@@ -59,7 +59,7 @@ def cache_attention(q, cache, block_table, seq_lens, causal, sm_scale, freqs_cos
     Queries t < n = new_lens[b] (default T) belong to the last n tokens of sequence b: with `causal` query t sees slots below
     seq_lens[b] - n + t + 1, without it all of them.  Queries are rotated like the keys of cache_append.  Rows t >= n and rows that
     see nothing are 0.  V of a block whose scale is below 1e-30 counts as 0.  accumulate: cache.weight[slot] += the slot's probabilities, summed over the queries and the query heads of
-    its K / V head (of sequences that share a block both add to it)."""
+    its K / V head (sequences that share a block all add to it, in any order)."""
     return _ext.native().cache_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.weight, block_table, seq_lens, causal, sm_scale, freqs_cos, freqs_sin,
                                          positions, new_lens, accumulate)
 

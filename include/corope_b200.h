@@ -342,7 +342,8 @@ int corope_cache_append(const corope_kv_cache_t* cache, const corope_cache_seqs_
  * seq_lens[b] - n + t + 1 (causal) or all seq_lens[b].  Query head h reads K / V head h / (Hq / Hkv), any group size.  o [B, Hq, T, D] in
  * `dtype`; rows without a visible slot and rows t >= n are 0, whatever their query and position.  accumulate: weight[slot] += the slot's probabilities summed over
  * the queries and the heads of its group.  Scores have fp32 accuracy; for bf16 tensors of more than 32 query rows a K / V head without `accumulate`
- * the rotated queries are rounded to 11 bits first.  Probabilities are rounded to 11 bits for 16-bit tensors, to 22 for fp32 ones.
+ * the rotated queries are rounded to 11 bits first.  Probabilities are rounded to 11 bits for 16-bit tensors, to 22 for fp32 ones, and where they are
+ * far below a row's largest to 2^-25 of it.  Sums over long contexts are added in fp32, in pieces of 1024 steps of the tensor cores (which truncate).
  * Values of a block whose scale of V is below 1e-30 (the largest is then below 4.5e-28) count as 0.
  * The workspace (ask with the call's own arguments and the same current device): parts of results, with `accumulate` also 4 bytes per slot of the
  * block tables and query row (where that is at most 512 MiB), for more than 32 rows fp16 copies of q.
